@@ -18,6 +18,9 @@ MODE_NAMES = ["CUBLAS", "FP16TCEC", "TF32TCEC", "FP16TC", "TF32TC", "CUBLAS_SIMT
 # hipblasStatus_t
 STATUS_SUCCESS, STATUS_INVALID_VALUE = 0, 3
 
+# hipDataType
+R_32F, R_16F, R_8I, R_16BF = 0, 2, 3, 14
+
 _u64 = ctypes.c_uint64
 _u32 = ctypes.c_uint
 _ptr = ctypes.c_void_p
@@ -111,6 +114,13 @@ def _declare(L):
                      ("cuMpSGEMM_sgemm_2xNx2", f32p), ("cuMpSGEMM_cgemm_2xNx2", c2p)):
         getattr(L, name).argtypes = [_ptr, _int, _int, _u64, sp, _ptr, _u64, _u64, _ptr, _u64, _u64,
                                      sp, _ptr, _u64, _u64, _u64]
+    L.cuMpSGEMM_gemm_grouped.argtypes = [_ptr, _int] + gemm_tail + [
+        f32p, _ptr, _u64, _u64, _ptr, _u64, f32p, _ptr, _u64, _ptr, _u64, _int, _int, _int]
+    L.cuMpSGEMM_gemm_grouped_k.argtypes = [_ptr] + gemm_tail + [
+        f32p, _ptr, _u64, _ptr, _u64, f32p, _ptr, _u64, _u64, _ptr, _u64, _int, _int, _int]
+    L.cuMpSGEMM_gemm_i8.argtypes = [_ptr] + gemm_tail + [
+        _ptr, _u64, _u64, _ptr, _ptr, _u64, _ptr, _ptr, _u64, _int, _ptr, _u64]
+    L.cuMpSGEMM_quantize_i8.argtypes = [_ptr, _u64, _u64, _ptr, _u64, _int, _ptr, _u64, _ptr]
     L.cuMpSGEMM_get_workspace_size.argtypes = [_ptr]
     L.cuMpSGEMM_get_workspace_size.restype = ctypes.c_size_t
     L.cuMpSGEMM_get_workspace_pointer.argtypes = [_ptr]
@@ -306,6 +316,30 @@ class Handle:
         fn = self._L.cuMpSGEMM_cgemm_2xNx2 if cplx else self._L.cuMpSGEMM_sgemm_2xNx2
         return fn(self._h, op_a, op_b, n, _scalar(alpha, cplx), _dptr(a), lda, stridea, _dptr(b),
                   ldb, strideb, _scalar(beta, cplx), _dptr(c), ldc, stridec, batch)
+
+    # ---- products of experts' layers ----
+    def gemm_grouped(self, op_a, m, n, k, alpha, a, lda, stridea, b, ldb, beta, c, ldc, offsets, groups, mode,
+                     type_ab=R_32F, type_c=R_32F):
+        """Tokens (the columns of b, n of them) times their group's matrix; offsets: groups + 1 int32 on the device."""
+        return self._L.cuMpSGEMM_gemm_grouped(self._h, op_a, m, n, k, _scalar(alpha, False), _dptr(a), lda, stridea,
+                                              _dptr(b), ldb, _scalar(beta, False), _dptr(c), ldc, _dptr(offsets),
+                                              groups, int(mode), int(type_ab), int(type_c))
+
+    def gemm_grouped_k(self, m, n, k, alpha, a, lda, b, ldb, beta, c, ldc, stridec, offsets, groups, mode,
+                       type_ab=R_32F, type_c=R_32F):
+        """For each group, the product over its tokens (k in all): the gradient of the groups' matrices."""
+        return self._L.cuMpSGEMM_gemm_grouped_k(self._h, m, n, k, _scalar(alpha, False), _dptr(a), lda, _dptr(b), ldb,
+                                                _scalar(beta, False), _dptr(c), ldc, stridec, _dptr(offsets), groups,
+                                                int(mode), int(type_ab), int(type_c))
+
+    def gemm_i8(self, m, n, k, a, lda, stridea, scale_a, b, ldb, scale_b, c, ldc, type_c=R_32F, offsets=None, groups=1):
+        """8-bit integers with a scale for each channel of a and each token (column of b); grouped with offsets."""
+        return self._L.cuMpSGEMM_gemm_i8(self._h, m, n, k, _dptr(a), lda, stridea, _dptr(scale_a), _dptr(b), ldb,
+                                         _dptr(scale_b), _dptr(c), ldc, int(type_c), _dptr(offsets), groups)
+
+    def quantize_i8(self, k, n, x, ldx, type_x, q, ldq, scale):
+        """The n columns of x as 8-bit integers with a scale each."""
+        return self._L.cuMpSGEMM_quantize_i8(self._h, k, n, _dptr(x), ldx, int(type_x), _dptr(q), ldq, _dptr(scale))
 
     # ---- exponent statistics ----
     def exp_stats_ext(self, m, n, ptr, ld, batch=1, stride=0, cplx=False):

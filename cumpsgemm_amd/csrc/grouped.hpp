@@ -1,0 +1,52 @@
+// Products of experts' layers: what the kernels take, and who launches them.
+//
+//   ragged columns (gemm_grouped, gemm_i8): C[:, j] = alpha op(A_g) B[:, j] + beta C[:, j]   for j in group g
+//   ragged K (gemm_grouped_k):              C_g     = alpha A[:, g] B[:, g]^T + beta C_g
+//
+// Column-major throughout.  Where a group begins and ends is read from device memory by the kernels themselves
+// (offsets[g], offsets[g + 1], brought into [0, count] and into order there, so that no value of them leads out of
+// the operands): a call waits for nothing and can be captured into a graph.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace cumpsgemm_amd {
+
+// What a kernel multiplies: FP32 in one of the four splits (gemm_kernel.hpp), FP16, BF16 or 8-bit integers.
+enum class Elem : int { F32_FP16TCEC = 0, F32_FP16TC = 1, F32_BF16X3 = 2, F32_BF16X2 = 3, F16 = 4, BF16 = 5, I8 = 6 };
+constexpr int kNumElems = 7;
+
+enum GroupedOut : uint32_t { OUT_F32 = 0, OUT_F16 = 1, OUT_BF16 = 2 };
+
+struct GroupedArgs {
+  uint32_t m, n, k;         // n (ragged K: k) counts the tokens of all groups
+  uint32_t groups;
+  const int *offsets;       // [groups + 1] in device memory; null: one group of everything
+  const char *a, *b;
+  char *c;
+  uint64_t lda, ldb, ldc;   // in elements
+  uint64_t stride_a;        // between the groups' A (ragged K: unused)
+  uint64_t stride_c;        // between the groups' C (ragged K only)
+  float alpha, beta;
+  uint32_t out;             // GroupedOut
+  uint32_t vec_c;           // four results of a column can be stored at once
+  const float *scale_a;     // 8-bit integers: [groups][m] and [n]
+  const float *scale_b;
+};
+
+struct GroupedKernel {
+  void (*launch)(const GroupedArgs &, uint32_t workgroups, hipStream_t);
+  int bm, bn;
+};
+
+// Tiles of the tiled kernels, from the largest.
+enum TileClass : int { TILE_256 = 0, TILE_128 = 1, TILE_NARROW = 2, kGroupedClasses = 3 };
+
+// Which of the two ways an operand comes into LDS (grouped_kernel.hpp): straight from memory (16-bit and 8-bit
+// elements in rows of whole, aligned 16-byte chunks), or through registers (anything).
+const GroupedKernel *lookup_grouped(Elem e, bool a_kc, bool ragged_k, bool direct, int cls);
+
+// The kernels of few tokens to a group (grouped_stream.hpp).
+const GroupedKernel *lookup_grouped_stream(Elem e, bool a_kc, bool aligned);
+
+} // namespace cumpsgemm_amd

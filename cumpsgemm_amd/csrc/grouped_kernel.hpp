@@ -1,0 +1,564 @@
+// Tiled kernels of the experts' products (gfx950, wave64).
+//
+// One workgroup computes a BM x BN tile of one group's result.  A K-step of both operands lies in LDS, in NSTAGE
+// buffers; fragments are read from there and multiplied with 16-row MFMAs, whose rows are rows of C (m) and whose
+// columns are tokens (n), so that a lane holds four results next to each other in memory.
+//
+// LDS images of an operand's K-step (ROWS rows of C or tokens):
+//   K-contiguous: ROWS rows of ROW_BYTES bytes.  128 bytes of 16-bit or 8-bit values; 64 bytes (32 values) in each
+//     plane of a split FP32 operand.  The 16-byte chunks of a row are exchanged (chunk ^ f(row)) so that the sixteen
+//     rows that one part of a ds_read_b128 touches fall on sixteen different bank groups.
+//   row-contiguous (16-bit operands whose rows, not K, are contiguous: op N weights, and both operands of the
+//     weights' gradient): BK lines of ROWS values, as they come from memory.  ds_read_b64_tr_b16 reads four lines of
+//     sixteen rows and hands each lane one row's four K-values, so nothing is transposed by vector instructions.
+//     The 32-byte pieces of a line are exchanged by two line bits and one of the eight-line bits: the sixteen lines of
+//     one read cover all banks twice, the least that 512 bytes can.
+// FP32 operands are split while they are staged, whatever their layout: a thread reads eight K-values of one row and
+// writes one chunk to each plane.
+#pragma once
+#include "gemm_kernel.hpp"
+#include "grouped.hpp"
+#include "gemm_table.hpp"
+
+namespace cumpsgemm_amd {
+
+typedef int i4_t __attribute__((ext_vector_type(4)));
+
+template <Elem E> struct elem_traits {
+  static constexpr bool F32 = (int)E <= 3;
+  static constexpr bool I8 = E == Elem::I8;
+  static constexpr Prec P = F32 ? (Prec)(int)E : Prec::FP16TC;
+  static constexpr bool IS_BF16 = F32 ? prec_traits<P>::IS_BF16 : E == Elem::BF16;
+  static constexpr int BYTES = F32 ? 4 : I8 ? 1 : 2; // of an element in memory
+  static constexpr int NP = F32 ? prec_traits<P>::NP : 1;
+  static constexpr int NPROD = F32 ? prec_traits<P>::NPROD : 1;
+  static constexpr int NACC = F32 ? prec_traits<P>::NACC : 1;
+  static constexpr int CHUNK = I8 ? 16 : 8;         // K-values of a 16-byte chunk in LDS
+  static constexpr int ROW_BYTES = F32 ? 64 : 128;  // of a K-contiguous row in LDS
+  static constexpr int BK = ROW_BYTES / 16 * CHUNK; // K-values of a step
+  static constexpr int SLICES = ROW_BYTES / 64;     // MFMAs deep
+  typedef typename std::conditional<I8, i4_t, f4v_t>::type acc_t;
+};
+
+// 16 zero bytes: where a lane reads that has nothing to read (a K-value past the end)
+static __device__ const u4_t g_grouped_zeros = {0, 0, 0, 0};
+
+// offset of a 16-byte chunk in a K-contiguous image
+template <int ROW_BYTES> __device__ inline int chunk_offset(int row, int chunk) {
+  if constexpr (ROW_BYTES == 64) return lds_offset(row, chunk);
+  else return row * 128 + ((chunk ^ ((row >> 1) & 7)) << 4);
+}
+// which 32-byte piece of line k holds piece p of a row-contiguous image
+__device__ inline int line_swizzle(int k) { return (k & 3) | (((k >> 3) & 1) << 2); }
+
+// A tile's place: its group, and where that begins and ends.
+struct TilePlace {
+  uint32_t group, tm, tn;
+  uint32_t lo, hi; // tokens of the group
+};
+
+// One group's tokens, brought into [0, count] and into order.
+__device__ inline void group_span(const int *offsets, uint32_t g, uint32_t count, uint32_t &lo, uint32_t &hi) {
+  const int a = offsets[g], b = offsets[g + 1], c = (int)count;
+  const int l = a < 0 ? 0 : a > c ? c : a;
+  lo = (uint32_t)l;
+  hi = (uint32_t)(b < l ? l : b > c ? c : b);
+}
+
+__device__ inline uint32_t wave_inclusive_sum(uint32_t x, int lane) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t y = __shfl_up(x, d, 64);
+    if (lane >= d) x += y;
+  }
+  return x;
+}
+
+// Workgroups that the dispatcher places on one XCD (id mod 8) take one contiguous range of the list of tiles, so that
+// they share that XCD's L2.
+__device__ inline uint32_t xcd_range(uint32_t bid, uint32_t total) {
+  if (total < 32) return bid;
+  const uint32_t q = total / 8, r = total % 8, xcd = bid % 8, loc = bid / 8;
+  return xcd * q + (xcd < r ? xcd : r) + loc;
+}
+// Column groups of up to 8 tile rows within one group's tiles: compact patches.
+__device__ inline void raster(uint32_t in, uint32_t tiles_m, uint32_t tiles_n, uint32_t &tm, uint32_t &tn) {
+  const uint32_t per = 8 * tiles_n, first = in / per * 8, rows = tiles_m - first < 8 ? tiles_m - first : 8;
+  const uint32_t rest = in % per;
+  tm = first + rest % rows;
+  tn = rest / rows;
+}
+
+// Ragged columns: the tile of workgroup `bid` in the list of all groups' tiles (every wave works it out for itself:
+// 64 groups at a time, one a lane).  False: there are fewer tiles.
+__device__ inline bool place_tile(const GroupedArgs &args, uint32_t bid, uint32_t tiles_m, uint32_t bn, TilePlace &t) {
+  if (args.offsets == nullptr) {
+    const uint32_t tiles_n = (args.n + bn - 1) / bn, total = tiles_m * tiles_n;
+    if (bid >= total) return false;
+    t.group = 0;
+    t.lo = 0;
+    t.hi = args.n;
+    raster(xcd_range(bid, total), tiles_m, tiles_n, t.tm, t.tn);
+    return true;
+  }
+  const int lane = threadIdx.x & 63;
+  uint32_t all = 0;
+  for (uint32_t g0 = 0; g0 < args.groups; g0 += 64) {
+    uint32_t lo = 0, hi = 0;
+    if (g0 + lane < args.groups) group_span(args.offsets, g0 + lane, args.n, lo, hi);
+    const uint32_t sum = wave_inclusive_sum((hi - lo + bn - 1) / bn, lane);
+    all += __builtin_amdgcn_readlane(sum, 63);
+  }
+  const uint32_t total = all * tiles_m;
+  if (bid >= total) return false;
+  const uint32_t id = xcd_range(bid, total), column = id / tiles_m;
+  uint32_t before = 0;
+  for (uint32_t g0 = 0; g0 < args.groups; g0 += 64) {
+    uint32_t lo = 0, hi = 0;
+    if (g0 + lane < args.groups) group_span(args.offsets, g0 + lane, args.n, lo, hi);
+    const uint32_t mine = (hi - lo + bn - 1) / bn, sum = before + wave_inclusive_sum(mine, lane);
+    const uint64_t beyond = __ballot(column < sum);
+    if (beyond != 0) {
+      const int at = __builtin_ctzll(beyond);
+      t.group = g0 + at;
+      t.lo = __builtin_amdgcn_readlane(lo, at);
+      t.hi = __builtin_amdgcn_readlane(hi, at);
+      const uint32_t tiles_n = __builtin_amdgcn_readlane(mine, at);
+      const uint32_t first = __builtin_amdgcn_readlane(sum, at) - tiles_n;
+      raster(id - first * tiles_m, tiles_m, tiles_n, t.tm, t.tn);
+      return true;
+    }
+    before = __builtin_amdgcn_readlane(sum, 63);
+  }
+  return false;
+}
+
+template <Elem E_, bool A_KC_, bool B_KC_, int BM_, int BN_, int WM_, int WN_, int NSTAGE_, bool DIRECT_, bool RAGGED_K_,
+          int OCC_>
+struct GroupedCfg {
+  using T = elem_traits<E_>;
+  static constexpr Elem E = E_;
+  static constexpr bool A_KC = A_KC_, B_KC = B_KC_, DIRECT = DIRECT_, RAGGED_K = RAGGED_K_;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NSTAGE = NSTAGE_, OCC = OCC_;
+  static constexpr int WAVES = (BM / WM) * (BN / WN), NT = WAVES * 64;
+  static constexpr int TM = WM / 16, TN = WN / 16;
+  static constexpr int A_PLANE = BM * T::ROW_BYTES, B_PLANE = BN * T::ROW_BYTES;
+  static constexpr int A_STAGE = A_PLANE * T::NP, B_STAGE = B_PLANE * T::NP, STAGE = A_STAGE + B_STAGE;
+  static constexpr int LDS_BYTES = NSTAGE * STAGE;
+  static_assert(!DIRECT || !T::F32, "FP32 operands are split in registers");
+  static_assert(!T::I8 || (A_KC && B_KC), "8-bit integers: K-contiguous operands");
+  static_assert(A_KC || T::F32 || BM >= 128, "a line's pieces are exchanged among eight");
+  static_assert(B_KC || T::F32 || BN >= 128, "a line's pieces are exchanged among eight");
+  static_assert(LDS_BYTES <= 160 * 1024, "LDS");
+  // (the waits of the direct form count a step's loads, the same number for every wave)
+  static_assert(!DIRECT || (BM * T::ROW_BYTES / 16 % NT == 0 && BN * T::ROW_BYTES / 16 % NT == 0), "whole rounds of loads");
+};
+
+// Staging of one operand's K-step by NT threads.  A unit is one 16-byte chunk of LDS (FP32: one in each plane).
+template <Elem E, bool KC, int ROWS, int NT> struct grouped_loader {
+  using T = elem_traits<E>;
+  // row-contiguous images exist for 16-bit values only; FP32 ends in K-contiguous planes either way
+  static constexpr bool LINES = !KC && !T::F32;
+  static constexpr int UNITS = ROWS * T::ROW_BYTES / 16;
+  static constexpr int U = (UNITS + NT - 1) / NT;
+  static constexpr bool PARTIAL = UNITS < NT;
+  static_assert(UNITS % NT == 0 || (PARTIAL && UNITS % 64 == 0), "whole waves");
+  static constexpr int LINE_CHUNKS = ROWS / 8;            // 16-byte chunks of a line
+  static constexpr int ROW_CHUNKS = T::ROW_BYTES / 16;
+
+  __device__ static inline bool active(int tid) { return !PARTIAL || tid < UNITS; }
+
+  // Position `id` of the image (in 16-byte chunks, as memory -> LDS loads fill it): row (LINES: first of 8 rows) and
+  // first K-value (LINES: the line) of what lies there.
+  __device__ static inline void at(int id, int &row, int &k) {
+    if constexpr (LINES) {
+      k = id / LINE_CHUNKS;
+      const int c = id % LINE_CHUNKS;
+      row = ((((c >> 1) ^ line_swizzle(k)) << 1) | (c & 1)) * 8;
+    } else if constexpr (T::F32) {
+      // (not an image position: FP32 chunks are written one by one, in whatever order reads memory best)
+      if constexpr (KC) {
+        row = id / ROW_CHUNKS;
+        k = id % ROW_CHUNKS * T::CHUNK;
+      } else {
+        row = id % ROWS;
+        k = id / ROWS * T::CHUNK;
+      }
+    } else {
+      row = id / ROW_CHUNKS;
+      k = ((id % ROW_CHUNKS) ^ ((row >> 1) & 7)) * T::CHUNK;
+    }
+  }
+
+  // Byte offset from the tile's origin (row 0, K-value 0 of the step) of the unit that fills position id.
+  // `rows`: those that exist; one beyond them reads the last again (its products are not stored).
+  __device__ static inline uint64_t offset(int id, uint64_t ld, int rows) {
+    int row, k;
+    at(id, row, k);
+    const int last = LINES ? rows - 8 : rows - 1;
+    row = row < last ? row : last;
+    return (KC ? (uint64_t)row * ld + k : (uint64_t)k * ld + row) * T::BYTES;
+  }
+
+  // memory -> LDS, 16 bytes a lane.  `left`: K-values from the step's first to the end; TAIL: fewer than a step has.
+  template <bool TAIL>
+  __device__ static inline void direct(const char *base, const uint32_t (&off)[U], char *lds_op, int tid, int wave, int left) {
+    typedef const void __attribute__((address_space(1))) *gptr_t;
+    typedef void __attribute__((address_space(3))) *lptr_t;
+    if (!active(tid)) return;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const char *p = base + off[u];
+      if constexpr (TAIL) {
+        int row, k;
+        at(tid + u * NT, row, k);
+        if (k >= left) p = reinterpret_cast<const char *>(&g_grouped_zeros);
+      }
+      __builtin_amdgcn_global_load_lds((gptr_t)p, (lptr_t)(lds_op + (wave * 64 + u * NT) * 16), 16, 0, 0);
+    }
+  }
+
+  struct Regs {
+    typename std::conditional<T::F32, f8_t, u4_t>::type v[U];
+  };
+
+  // memory -> registers, any alignment and size; nothing beyond `rows` x `left` is read, zeros come in its place
+  // (rows: except where a last row is read again instead)
+  template <bool TAIL>
+  __device__ static inline void fetch(Regs &r, const char *base, uint64_t ld, int rows, int left, int tid) {
+    if (!active(tid)) return;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      int row, k;
+      at(tid + u * NT, row, k);
+      if constexpr (T::F32) {
+        row = row < rows ? row : rows - 1;
+        const float *p = reinterpret_cast<const float *>(base);
+        if constexpr (KC) {
+          p += (uint64_t)row * ld + k;
+          if (!TAIL || k + 8 <= left) {
+            typedef float f4u_t __attribute__((ext_vector_type(4), aligned(4)));
+            const f4u_t x = reinterpret_cast<const f4u_t *>(p)[0], y = reinterpret_cast<const f4u_t *>(p)[1];
+            r.v[u] = f8_t{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) r.v[u][j] = k + j < left ? p[j] : 0.0f;
+          }
+        } else {
+          p += (uint64_t)k * ld + row;
+#pragma unroll
+          for (int j = 0; j < 8; j++) r.v[u][j] = (!TAIL || k + j < left) ? p[(uint64_t)j * ld] : 0.0f;
+        }
+      } else if constexpr (T::I8) {
+        row = row < rows ? row : rows - 1;
+        const char *p = base + (uint64_t)row * ld + k;
+        typedef uint32_t u4u_t __attribute__((ext_vector_type(4), aligned(1)));
+        if (!TAIL || k + 16 <= left) {
+          const u4u_t x = *reinterpret_cast<const u4u_t *>(p);
+          r.v[u] = u4_t{x.x, x.y, x.z, x.w};
+        } else {
+          u4_t x = {0, 0, 0, 0};
+#pragma unroll
+          for (int j = 0; j < 16; j++)
+            if (k + j < left) x[j / 4] |= (uint32_t)(uint8_t)p[j] << (j % 4 * 8);
+          r.v[u] = x;
+        }
+      } else {
+        // 16-bit: eight along K, or (LINES) eight rows of one line
+        if constexpr (!LINES) row = row < rows ? row : rows - 1;
+        const uint16_t *p = reinterpret_cast<const uint16_t *>(base) +
+                            (KC ? (uint64_t)row * ld + k : (uint64_t)k * ld + row);
+        const int have = LINES ? (TAIL && k >= left ? 0 : rows - row) : TAIL ? left - k : 8;
+        typedef uint32_t u4u_t __attribute__((ext_vector_type(4), aligned(2)));
+        if (have >= 8) {
+          const u4u_t x = *reinterpret_cast<const u4u_t *>(p);
+          r.v[u] = u4_t{x.x, x.y, x.z, x.w};
+        } else {
+          u4_t x = {0, 0, 0, 0};
+#pragma unroll
+          for (int j = 0; j < 8; j++)
+            if (j < have) x[j / 2] |= (uint32_t)p[j] << (j % 2 * 16);
+          r.v[u] = x;
+        }
+      }
+    }
+  }
+
+  // registers -> LDS
+  __device__ static inline void put(const Regs &r, char *lds_op, int tid) {
+    if (!active(tid)) return;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int id = tid + u * NT;
+      if constexpr (T::F32) {
+        int row, k;
+        at(id, row, k);
+        u4_t out[T::NP];
+        splitter<T::P>::run(r.v[u], out);
+#pragma unroll
+        for (int p = 0; p < T::NP; p++)
+          *reinterpret_cast<u4_t *>(lds_op + p * ROWS * T::ROW_BYTES + chunk_offset<T::ROW_BYTES>(row, k / T::CHUNK)) = out[p];
+      } else {
+        *reinterpret_cast<u4_t *>(lds_op + id * 16) = r.v[u];
+      }
+    }
+  }
+};
+
+template <Elem E>
+__device__ inline typename elem_traits<E>::acc_t grouped_mfma(const u4_t a, const u4_t b, const typename elem_traits<E>::acc_t c) {
+  if constexpr (E == Elem::I8)
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i4_t, a), __builtin_bit_cast(i4_t, b), c, 0, 0, 0);
+  else
+    return mfma_block<elem_traits<E>::IS_BF16>(a, b, c);
+}
+
+// Results of a column, one or four of them, in the type that C has.
+template <uint32_t OUT> struct out_type;
+template <> struct out_type<OUT_F32> { typedef float type; };
+template <> struct out_type<OUT_F16> { typedef _Float16 type; };
+template <> struct out_type<OUT_BF16> { typedef __bf16 type; };
+
+// x[0 .. 3]: rows row .. row + 3 of one column; `c`: where row `row` lies.  Not stored: rows from m on.
+template <uint32_t OUT>
+__device__ inline void store_four(char *c, const f4v_t x, float beta, uint32_t row, uint32_t m, bool vec) {
+  typedef typename out_type<OUT>::type O;
+  typedef O o4_t __attribute__((ext_vector_type(4)));
+  O *p = reinterpret_cast<O *>(c);
+  if (vec) { // (m is a multiple of 4)
+    if (row >= m) return;
+    f4v_t y = x;
+    if (beta != 0.0f) {
+      const o4_t old = *reinterpret_cast<const o4_t *>(p);
+#pragma unroll
+      for (int v = 0; v < 4; v++) y[v] += beta * (float)old[v];
+    }
+    *reinterpret_cast<o4_t *>(p) = __builtin_convertvector(y, o4_t);
+  } else {
+#pragma unroll
+    for (int v = 0; v < 4; v++)
+      if (row + v < m) p[v] = (O)(beta != 0.0f ? x[v] + beta * (float)p[v] : x[v]);
+  }
+}
+
+template <class Cfg>
+__global__ __launch_bounds__(Cfg::NT) __attribute__((amdgpu_waves_per_eu(Cfg::OCC, Cfg::OCC)))
+void grouped_kernel(const GroupedArgs args) {
+  using T = typename Cfg::T;
+  constexpr int BM = Cfg::BM, BN = Cfg::BN, TM = Cfg::TM, TN = Cfg::TN, NT = Cfg::NT, BK = T::BK;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave % (BM / Cfg::WM), wn = wave / (BM / Cfg::WM);
+
+  // ---- which tile ----
+  const uint32_t tiles_m = (args.m + BM - 1) / BM;
+  TilePlace t;
+  uint32_t n0, n_end, klen;
+  const char *a = args.a, *b = args.b;
+  char *c = args.c;
+  const uint64_t out_bytes = args.out == OUT_F32 ? 4 : 2;
+  if constexpr (Cfg::RAGGED_K) {
+    const uint32_t tiles_n = (args.n + BN - 1) / BN, per = tiles_m * tiles_n;
+    const uint32_t id = xcd_range(blockIdx.x, per * args.groups);
+    t.group = id / per;
+    raster(id % per, tiles_m, tiles_n, t.tm, t.tn);
+    group_span(args.offsets, t.group, args.k, t.lo, t.hi);
+    t.lo = __builtin_amdgcn_readfirstlane(t.lo);
+    t.hi = __builtin_amdgcn_readfirstlane(t.hi);
+    n0 = t.tn * BN;
+    n_end = args.n;
+    klen = t.hi - t.lo;
+    a += (uint64_t)t.lo * args.lda * T::BYTES;
+    b += (uint64_t)t.lo * args.ldb * T::BYTES;
+    c += (uint64_t)t.group * args.stride_c * out_bytes;
+  } else {
+    if (!place_tile(args, blockIdx.x, tiles_m, BN, t)) return;
+    n0 = t.lo + t.tn * BN;
+    n_end = t.hi;
+    klen = args.k;
+    a += (uint64_t)t.group * args.stride_a * T::BYTES;
+  }
+  const uint32_t m0 = t.tm * BM;
+  const int rows_a = (int)(args.m - m0 < (uint32_t)BM ? args.m - m0 : BM);
+  const int rows_b = (int)(n_end - n0 < (uint32_t)BN ? n_end - n0 : BN);
+
+  using LA = grouped_loader<Cfg::E, Cfg::A_KC, BM, NT>;
+  using LB = grouped_loader<Cfg::E, Cfg::B_KC, BN, NT>;
+  a += (Cfg::A_KC ? (uint64_t)m0 * args.lda : (uint64_t)m0) * T::BYTES;
+  b += (Cfg::B_KC ? (uint64_t)n0 * args.ldb : (uint64_t)n0) * T::BYTES;
+  const uint64_t a_step = (Cfg::A_KC ? (uint64_t)BK : (uint64_t)BK * args.lda) * T::BYTES;
+  const uint64_t b_step = (Cfg::B_KC ? (uint64_t)BK : (uint64_t)BK * args.ldb) * T::BYTES;
+
+  typename T::acc_t acc[T::NACC][TN][TM];
+#pragma unroll
+  for (int s = 0; s < T::NACC; s++)
+#pragma unroll
+    for (int j = 0; j < TN; j++)
+#pragma unroll
+      for (int i = 0; i < TM; i++)
+#pragma unroll
+        for (int v = 0; v < 4; v++) acc[s][j][i][v] = 0;
+
+  // ---- fragments ----
+  // Lane l of a 16-row MFMA supplies row l % 16 and the 16 bytes number l / 16 of the slice's 64.
+  const int frow = lane & 15, fg = lane >> 4;
+  auto frag = [&](const char *op, const int row0, const int p, const int slice, auto kc_tag, auto rows_tag) -> u4_t {
+    constexpr bool KC = decltype(kc_tag)::value;
+    constexpr int ROWS = decltype(rows_tag)::value;
+    if constexpr (KC || T::F32) {
+      return *reinterpret_cast<const u4_t *>(op + p * ROWS * T::ROW_BYTES +
+                                             chunk_offset<T::ROW_BYTES>(row0 + frow, slice * 4 + fg));
+    } else {
+      typedef short s4_t __attribute__((ext_vector_type(4)));
+      typedef __attribute__((address_space(3))) s4_t *tr_t;
+      typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
+      // lane l % 16 of a quarter names line (l % 16) / 4 and a quarter of the 32-byte piece; the quarter's K-values are
+      // 8 fg .. 8 fg + 3, then + 4 (line_swizzle is the same for both)
+      const int k = slice * 32 + fg * 8 + (frow >> 2);
+      const int off = k * (ROWS * 2) + (((row0 >> 4) ^ line_swizzle(k)) << 5) + (frow & 3) * 8;
+      const u2_t x = __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_t)(op + off)));
+      const u2_t y = __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_t)(op + off + 4 * ROWS * 2)));
+      return u4_t{x[0], x[1], y[0], y[1]};
+    }
+  };
+  auto multiply = [&](const char *stage) {
+    const char *sa = stage, *sb = stage + Cfg::A_STAGE;
+#pragma unroll
+    for (int s = 0; s < T::SLICES; s++) {
+      u4_t fa[T::NP][TM], fb[T::NP][TN];
+#pragma unroll
+      for (int p = 0; p < T::NP; p++) {
+#pragma unroll
+        for (int j = 0; j < TN; j++)
+          fb[p][j] = frag(sb, wn * Cfg::WN + j * 16, p, s, std::integral_constant<bool, Cfg::B_KC>{}, std::integral_constant<int, BN>{});
+#pragma unroll
+        for (int i = 0; i < TM; i++)
+          fa[p][i] = frag(sa, wm * Cfg::WM + i * 16, p, s, std::integral_constant<bool, Cfg::A_KC>{}, std::integral_constant<int, BM>{});
+      }
+#pragma unroll
+      for (int q = 0; q < T::NPROD; q++) {
+        constexpr int ZERO = 0;
+        const int pa = T::F32 ? prec_traits<T::P>::PA[q] : ZERO, pb = T::F32 ? prec_traits<T::P>::PB[q] : ZERO;
+        const int ac = T::F32 ? prec_traits<T::P>::ACC[q] : ZERO;
+#pragma unroll
+        for (int i = 0; i < TM; i++)
+#pragma unroll
+          for (int j = 0; j < TN; j++) acc[ac][j][i] = grouped_mfma<Cfg::E>(fa[pa][i], fb[pb][j], acc[ac][j][i]);
+      }
+    }
+  };
+
+  // ---- K loop ----
+  const int steps = (int)((klen + BK - 1) / BK), whole = (int)(klen / BK);
+  if constexpr (Cfg::DIRECT) {
+    // NSTAGE - 1 steps ahead; a buffer is filled again once all waves have read it, i.e. behind the barrier of the
+    // step after
+    constexpr int AHEAD = Cfg::NSTAGE - 1;
+    constexpr int LOADS = LA::U + LB::U;
+    uint32_t offa[LA::U], offb[LB::U];
+#pragma unroll
+    for (int u = 0; u < LA::U; u++) offa[u] = (uint32_t)LA::offset(tid + u * NT, args.lda, rows_a);
+#pragma unroll
+    for (int u = 0; u < LB::U; u++) offb[u] = (uint32_t)LB::offset(tid + u * NT, args.ldb, rows_b);
+    auto issue = [&](int step) {
+      char *sa = lds + (step % Cfg::NSTAGE) * Cfg::STAGE, *sb = sa + Cfg::A_STAGE;
+      const char *pa = a + (uint64_t)step * a_step, *pb = b + (uint64_t)step * b_step;
+      if (step < whole) {
+        LA::template direct<false>(pa, offa, sa, tid, wave, BK);
+        LB::template direct<false>(pb, offb, sb, tid, wave, BK);
+      } else {
+        const int left = (int)klen - step * BK;
+        LA::template direct<true>(pa, offa, sa, tid, wave, left);
+        LB::template direct<true>(pb, offb, sb, tid, wave, left);
+      }
+    };
+    for (int s = 0; s < AHEAD && s < steps; s++) issue(s);
+    for (int s = 0; s < steps; s++) {
+      // everything but the loads of the AHEAD - 1 steps after this one has landed
+      if (AHEAD > 1 && s + AHEAD <= steps) __builtin_amdgcn_s_waitcnt(waitcnt_vm(LOADS * (AHEAD - 1)));
+      else __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+      block_sync_lds();
+      if (s + AHEAD < steps) issue(s + AHEAD);
+      multiply(lds + (s % Cfg::NSTAGE) * Cfg::STAGE);
+    }
+  } else {
+    static_assert(Cfg::DIRECT || Cfg::NSTAGE == 2, "two buffers");
+    typename LA::Regs ra;
+    typename LB::Regs rb;
+    auto fetch = [&](int step) {
+      const char *pa = a + (uint64_t)step * a_step, *pb = b + (uint64_t)step * b_step;
+      if (step < whole) {
+        LA::template fetch<false>(ra, pa, args.lda, rows_a, BK, tid);
+        LB::template fetch<false>(rb, pb, args.ldb, rows_b, BK, tid);
+      } else {
+        const int left = (int)klen - step * BK;
+        LA::template fetch<true>(ra, pa, args.lda, rows_a, left, tid);
+        LB::template fetch<true>(rb, pb, args.ldb, rows_b, left, tid);
+      }
+    };
+    auto put = [&](int step) {
+      char *sa = lds + (step & 1) * Cfg::STAGE;
+      LA::put(ra, sa, tid);
+      LB::put(rb, sa + Cfg::A_STAGE, tid);
+    };
+    if (steps > 0) {
+      fetch(0);
+      put(0);
+      block_sync_lds();
+    }
+    for (int s = 0; s < steps; s++) {
+      if (s + 1 < steps) fetch(s + 1);
+      multiply(lds + (s & 1) * Cfg::STAGE);
+      if (s + 1 < steps) put(s + 1);
+      block_sync_lds();
+    }
+  }
+
+  // ---- results ----
+  // Register v of lane l: MFMA row 4 (l / 16) + v (of C), column l % 16 (token).
+  auto write = [&](auto out_tag) {
+    constexpr uint32_t OUT = decltype(out_tag)::value;
+    constexpr uint64_t OB = sizeof(typename out_type<OUT>::type);
+#pragma unroll
+    for (int j = 0; j < TN; j++) {
+      const uint32_t col = n0 + wn * Cfg::WN + j * 16 + frow;
+      if (col >= n_end) continue;
+      float sb = 1.0f;
+      if constexpr (T::I8) sb = args.scale_b[col];
+#pragma unroll
+      for (int i = 0; i < TM; i++) {
+        const uint32_t row = m0 + wm * Cfg::WM + i * 16 + fg * 4;
+        f4v_t x;
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+          if constexpr (T::I8) {
+            const uint32_t r = row + v < args.m ? row + v : args.m - 1;
+            x[v] = (float)acc[0][j][i][v] * args.scale_a[(uint64_t)t.group * args.m + r] * sb;
+          } else {
+            x[v] = acc[0][j][i][v];
+            if constexpr (T::NACC == 2) x[v] += acc[1][j][i][v] * prec_traits<T::P>::CORR_SCALE;
+            x[v] *= args.alpha;
+          }
+        }
+        store_four<OUT>(c + ((uint64_t)col * args.ldc + row) * OB, x, args.beta, row, args.m, args.vec_c != 0);
+      }
+    }
+  };
+  if constexpr (T::F32) {
+    write(std::integral_constant<uint32_t, OUT_F32>{});
+  } else {
+    if (args.out == OUT_F32) write(std::integral_constant<uint32_t, OUT_F32>{});
+    else if (Cfg::E == Elem::F16 || (T::I8 && args.out == OUT_F16)) write(std::integral_constant<uint32_t, OUT_F16>{});
+    else write(std::integral_constant<uint32_t, OUT_BF16>{});
+  }
+}
+
+template <class Cfg> void launch_grouped(const GroupedArgs &args, uint32_t workgroups, hipStream_t stream) {
+  static device_flags_t done = {};
+  allow_dynamic_lds(reinterpret_cast<const void *>(&grouped_kernel<Cfg>), Cfg::LDS_BYTES, done);
+  hipLaunchKernelGGL(grouped_kernel<Cfg>, dim3(workgroups), dim3(Cfg::NT), Cfg::LDS_BYTES, stream, args);
+}
+template <class Cfg> constexpr GroupedKernel grouped_entry() { return {&launch_grouped<Cfg>, Cfg::BM, Cfg::BN}; }
+
+} // namespace cumpsgemm_amd

@@ -149,6 +149,64 @@ hipblasStatus_t cuMpSGEMM_cgemm_2xNx2(cuMpSGEMM_handle_t handle, hipblasOperatio
                                       const hipComplex *beta, hipComplex *c, uint64_t ldc,
                                       uint64_t stridec, uint64_t batch_count);
 
+/* ---- products of experts' layers (no counterpart in the reference) ---------
+ * `offsets`: group_count + 1 ints in DEVICE memory, ascending; group g has the
+ * tokens offsets[g] .. offsets[g + 1] - 1.  A group may have none.  The kernels
+ * read them, the host does not: no call waits for the device, allocates or
+ * keeps anything, and all can be captured into a graph, whose replays take the
+ * offsets of the time.  Values outside 0 .. token count are brought into it,
+ * and an offset below the one before it gives an empty group; what tokens
+ * overlap then and which results are written is undefined, but nothing outside
+ * the operands is touched.  Results repeat bit for bit.
+ * type_ab = HIP_R_32F: compute_mode FP16TCEC, TF32TCEC, FP16TC or TF32TC, as in
+ *   cuMpSGEMM_sgemm; type_c = HIP_R_32F.  (An infinity is not split: what it
+ *   multiplies becomes NaN, as there.)
+ * type_ab = HIP_R_16F or HIP_R_16BF: products are exact, sums FP32; type_c the
+ *   same type or HIP_R_32F, rounded once; compute_mode is not looked at.
+ * Errors as cuMpSGEMM_sgemm: HIPBLAS_STATUS_INVALID_VALUE and nothing launched.
+ *
+ * Tokens times their group's matrix, forward or for the tokens' gradient:
+ *   C[:, j] = alpha * op(A_g) * B[:, j] + beta * C[:, j],  j a token of group g.
+ * op(A_g) is m x k, A_g at a + g * stridea (elements); B is k x n, C is m x n, a
+ * token a column.  Columns of no group are not written.  With beta = 0, C is
+ * not read.  C must not overlap A or B. */
+hipblasStatus_t cuMpSGEMM_gemm_grouped(cuMpSGEMM_handle_t handle, hipblasOperation_t op_A, uint64_t m,
+                                       uint64_t n, uint64_t k, const float *alpha, const void *a,
+                                       uint64_t lda, uint64_t stridea, const void *b, uint64_t ldb,
+                                       const float *beta, void *c, uint64_t ldc, const int *offsets,
+                                       uint64_t group_count, cuMpSGEMM_compute_mode_t compute_mode,
+                                       hipDataType type_ab, hipDataType type_c);
+/* A product over each group's tokens, the gradient of the matrices:
+ *   C_g = alpha * A[:, tokens of g] * B[:, tokens of g]^T + beta * C_g
+ * A is m x k, B is n x k, a token a column; C_g is m x n at c + g * stridec.  A
+ * group without tokens gets beta * C_g (zeros with beta = 0).  beta = 1
+ * accumulates. */
+hipblasStatus_t cuMpSGEMM_gemm_grouped_k(cuMpSGEMM_handle_t handle, uint64_t m, uint64_t n, uint64_t k,
+                                         const float *alpha, const void *a, uint64_t lda, const void *b,
+                                         uint64_t ldb, const float *beta, void *c, uint64_t ldc,
+                                         uint64_t stridec, const int *offsets, uint64_t group_count,
+                                         cuMpSGEMM_compute_mode_t compute_mode, hipDataType type_ab,
+                                         hipDataType type_c);
+/* 8-bit integers with a scale for each channel and each token:
+ *   C[i, j] = scale_a[g * m + i] * scale_b[j] * sum_l A_g[l, i] * B[l, j]
+ * A_g is k x m at a + g * stridea (a channel's k weights contiguous), B is
+ * k x n (a token's k values contiguous), C is m x n of type_c = HIP_R_32F, _16F
+ * or _16BF.  The sums are exact 32-bit integers: k <= 131071.  offsets = NULL
+ * with group_count = 1: one matrix for all n tokens. */
+hipblasStatus_t cuMpSGEMM_gemm_i8(cuMpSGEMM_handle_t handle, uint64_t m, uint64_t n, uint64_t k,
+                                  const int8_t *a, uint64_t lda, uint64_t stridea, const float *scale_a,
+                                  const int8_t *b, uint64_t ldb, const float *scale_b, void *c,
+                                  uint64_t ldc, hipDataType type_c, const int *offsets,
+                                  uint64_t group_count);
+/* The n columns (tokens) of x, k values each of type_x = HIP_R_32F, _16F or
+ * _16BF, as 8-bit integers: scale[j] = max |x[:, j]| / 127, q[i, j] = 127 x[i, j] /
+ * max |x[:, j]| rounded to nearest, ties to even (x / scale, for a maximum below
+ * 2^-119).  A column of zeros has scale 0; one with an infinity or a NaN has
+ * scale NaN and zeros. */
+hipblasStatus_t cuMpSGEMM_quantize_i8(cuMpSGEMM_handle_t handle, uint64_t k, uint64_t n, const void *x,
+                                      uint64_t ldx, hipDataType type_x, int8_t *q, uint64_t ldq,
+                                      float *scale);
+
 /* cumpsgemm::exp_stats_ext<T> / exp_max_ext<T> (reference cumpsgemm.hpp:37-46) */
 unsigned cuMpSGEMM_exp_stats_ext_s(cuMpSGEMM_handle_t h, unsigned m, unsigned n, const float *ptr,
                                    unsigned ld, unsigned batch, unsigned stride);
