@@ -39,11 +39,12 @@ bool out_of(hipDataType type, uint32_t &out) {
   return true;
 }
 uint32_t bytes_of(Elem e) { return (int)e <= 3 ? 4 : e == Elem::I8 ? 1 : 2; }
-bool is_f32(Elem e) { return (int)e <= 3; }
 
 // Whether an operand can go straight from memory to LDS: its contiguous extent is whole 16-byte chunks, they are
 // aligned, and the offsets of a tile and step fit 32 bits (`lines`: rows or K-lines that a step spans).
+// FP32: the offsets alone.
 bool chunks_ok(const void *p, uint64_t extent, uint64_t ld, uint64_t stride, uint32_t bytes, uint64_t lines) {
+  if (bytes == 4) return lines * ld * bytes < 0x7fffffffull;
   return (uintptr_t)p % 16 == 0 && extent * bytes % 16 == 0 && ld * bytes % 16 == 0 && stride * bytes % 16 == 0 &&
          lines * ld * bytes < 0x7fffffffull;
 }
@@ -57,16 +58,21 @@ hipblasStatus_t launched() {
   return hipGetLastError() == hipSuccess ? HIPBLAS_STATUS_SUCCESS : HIPBLAS_STATUS_EXECUTION_FAILED;
 }
 
+// CUMPSGEMM_FORCE_TILE_CLASS (0 - 2) goes before the rules; where there is no such kernel, the 128 x 128 one serves.
+const GroupedKernel *choose(Elem e, bool a_kc, bool ragged_k, bool direct, int cls) {
+  const int forced = tuning().force_cls;
+  const GroupedKernel *k = lookup_grouped(e, a_kc, ragged_k, direct, forced >= 0 && forced < kGroupedClasses ? forced : cls);
+  return k != nullptr ? k : lookup_grouped(e, a_kc, ragged_k, direct, TILE_128);
+}
+
 // Ragged columns: B and C have args.n columns in args.groups groups.
 hipblasStatus_t run_columns(cuMpSGEMM_handle *h, Elem e, bool a_kc, GroupedArgs &args, const char *label) {
   const uint32_t bytes = bytes_of(e);
-  const bool direct = !is_f32(e) &&
-                      chunks_ok(args.a, a_kc ? args.k : args.m, args.lda, args.stride_a, bytes, a_kc ? 256 : 64) &&
+  const bool direct = chunks_ok(args.a, a_kc ? args.k : args.m, args.lda, args.stride_a, bytes, a_kc ? 256 : 64) &&
                       chunks_ok(args.b, args.k, args.ldb, 0, bytes, 256);
   const uint64_t each = args.n / args.groups; // tokens of a group, on average
   int cls = each >= 192 ? TILE_256 : each >= 48 ? TILE_128 : TILE_NARROW;
-  if (!direct && !is_f32(e)) cls = TILE_128;
-  const GroupedKernel *k = lookup_grouped(e, a_kc, false, direct, cls);
+  const GroupedKernel *k = choose(e, a_kc, false, direct, cls);
   if (k == nullptr) return HIPBLAS_STATUS_INTERNAL_ERROR;
   // no more tiles of columns than this: every group has one that is not full
   const uint64_t columns = args.offsets == nullptr ? (args.n + k->bn - 1) / k->bn
@@ -151,10 +157,10 @@ hipblasStatus_t cuMpSGEMM_gemm_grouped_k(cuMpSGEMM_handle_t h, uint64_t m, uint6
   args.out = out;
   args.vec_c = four_at_once(c, m, ldc, stridec, out);
   const uint32_t bytes = bytes_of(e);
-  const bool direct = !is_f32(e) && chunks_ok(a, m, lda, 0, bytes, 64) && chunks_ok(b, n, ldb, 0, bytes, 64);
+  const bool direct = chunks_ok(a, m, lda, 0, bytes, 64) && chunks_ok(b, n, ldb, 0, bytes, 64);
   const uint64_t tiles = ((m + 255) / 256) * ((n + 255) / 256) * group_count;
-  const int cls = (direct || is_f32(e)) && tiles >= h->num_cus ? TILE_256 : TILE_128;
-  const GroupedKernel *kern = lookup_grouped(e, false, true, direct, cls);
+  const int cls = direct && tiles >= h->num_cus ? TILE_256 : TILE_128;
+  const GroupedKernel *kern = choose(e, false, true, direct, cls);
   if (kern == nullptr) return HIPBLAS_STATUS_INTERNAL_ERROR;
   const uint64_t per = ((m + kern->bm - 1) / kern->bm) * ((n + kern->bn - 1) / kern->bn);
   if (per > kMost || per * group_count > kMost) return HIPBLAS_STATUS_INVALID_VALUE;

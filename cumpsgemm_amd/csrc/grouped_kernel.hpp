@@ -48,6 +48,16 @@ template <int ROW_BYTES> __device__ inline int chunk_offset(int row, int chunk) 
   if constexpr (ROW_BYTES == 64) return lds_offset(row, chunk);
   else return row * 128 + ((chunk ^ ((row >> 1) & 7)) << 4);
 }
+// what M0 holds for a load to LDS (wave-uniform)
+__device__ inline uint32_t lds_address(const char *p) {
+  return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char *)p);
+}
+// an address that is the same for all lanes, whatever the compiler can see of that
+__device__ inline const char *uniform_address(const char *p) {
+  const uint64_t x = (uint64_t)p;
+  const uint32_t high = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32)), low = __builtin_amdgcn_readfirstlane((uint32_t)x);
+  return (const char *)((uint64_t)high << 32 | low); // (low is unsigned here: the builtin's own int would carry its sign up)
+}
 // which 32-byte piece of line k holds piece p of a row-contiguous image
 __device__ inline int line_swizzle(int k) { return (k & 3) | (((k >> 3) & 1) << 2); }
 
@@ -133,6 +143,8 @@ __device__ inline bool place_tile(const GroupedArgs &args, uint32_t bid, uint32_
   return false;
 }
 
+// DIRECT: 16-bit and 8-bit operands go straight from memory to LDS, 16 aligned bytes a lane; FP32 operands, which are
+// split in registers, are read with 32-bit offsets from uniform bases.  Otherwise: any alignment, any size.
 template <Elem E_, bool A_KC_, bool B_KC_, int BM_, int BN_, int WM_, int WN_, int NSTAGE_, bool DIRECT_, bool RAGGED_K_,
           int OCC_>
 struct GroupedCfg {
@@ -145,15 +157,18 @@ struct GroupedCfg {
   static constexpr int A_PLANE = BM * T::ROW_BYTES, B_PLANE = BN * T::ROW_BYTES;
   static constexpr int A_STAGE = A_PLANE * T::NP, B_STAGE = B_PLANE * T::NP, STAGE = A_STAGE + B_STAGE;
   static constexpr int LDS_BYTES = NSTAGE * STAGE;
-  static_assert(!DIRECT || !T::F32, "FP32 operands are split in registers");
   static_assert(!T::I8 || (A_KC && B_KC), "8-bit integers: K-contiguous operands");
   static_assert(A_KC || T::F32 || BM >= 128, "a line's pieces are exchanged among eight");
   static_assert(B_KC || T::F32 || BN >= 128, "a line's pieces are exchanged among eight");
   static_assert(LDS_BYTES <= 160 * 1024, "LDS");
   // (the waits of the direct form count a step's loads, the same number for every wave)
-  static_assert(!DIRECT || (BM * T::ROW_BYTES / 16 % NT == 0 && BN * T::ROW_BYTES / 16 % NT == 0), "whole rounds of loads");
+  static_assert(!DIRECT || T::F32 || (BM * T::ROW_BYTES / 16 % NT == 0 && BN * T::ROW_BYTES / 16 % NT == 0), "whole rounds of loads");
 };
 
+// (M0 is among the registers that the loads below say they change; nothing of the compiler's lives in it longer than
+// from one instruction to the next, which is what it warns of)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 // Staging of one operand's K-step by NT threads.  A unit is one 16-byte chunk of LDS (FP32: one in each plane).
 template <Elem E, bool KC, int ROWS, int NT> struct grouped_loader {
   using T = elem_traits<E>;
@@ -200,110 +215,122 @@ template <Elem E, bool KC, int ROWS, int NT> struct grouped_loader {
     return (KC ? (uint64_t)row * ld + k : (uint64_t)k * ld + row) * T::BYTES;
   }
 
-  // memory -> LDS, 16 bytes a lane.  `left`: K-values from the step's first to the end; TAIL: fewer than a step has.
-  template <bool TAIL>
-  __device__ static inline void direct(const char *base, const uint32_t (&off)[U], char *lds_op, int tid, int wave, int left) {
-    typedef const void __attribute__((address_space(1))) *gptr_t;
-    typedef void __attribute__((address_space(3))) *lptr_t;
-    if (!active(tid)) return;
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-      const char *p = base + off[u];
-      if constexpr (TAIL) {
-        int row, k;
-        at(tid + u * NT, row, k);
-        if (k >= left) p = reinterpret_cast<const char *>(&g_grouped_zeros);
-      }
-      __builtin_amdgcn_global_load_lds((gptr_t)p, (lptr_t)(lds_op + (wave * 64 + u * NT) * 16), 16, 0, 0);
-    }
+  // memory -> LDS, 16 bytes a lane: load number u of a whole step, from the uniform base + off.
+  // (Assembly: of such a load the compiler knows no more than that it writes LDS, and makes every read of LDS beside
+  // one wait for all reads before it, and a transposing read for the loads themselves: 8 experts, 16384 x 4096 x 2048
+  // over K in BF16, 898 us that way.  The kernel waits for them itself, before the barrier in front of their first
+  // read; they write no register.  M0 must be written one instruction ahead, and an address that a vector instruction put
+  // into scalar registers five, which the compiler does not see to here.)
+  __device__ static inline void direct(int u, const char *base, uint32_t off, uint32_t lds_op, int wave) {
+    const uint32_t to = lds_op + (uint32_t)((wave * 64 + u * NT) * 16);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory", "m0");
+  }
+  // ... of a step that has only `left` K-values: zeros from there on
+  __device__ static inline void direct_tail(int u, const char *base, uint32_t off, uint32_t lds_op, int tid, int wave, int left) {
+    int row, k;
+    at(tid + u * NT, row, k);
+    const char *p = k < left ? base + off : reinterpret_cast<const char *>(&g_grouped_zeros);
+    const uint32_t to = lds_op + (uint32_t)((wave * 64 + u * NT) * 16);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(p) : "memory", "m0");
   }
 
   struct Regs {
     typename std::conditional<T::F32, f8_t, u4_t>::type v[U];
   };
 
-  // memory -> registers, any alignment and size; nothing beyond `rows` x `left` is read, zeros come in its place
-  // (rows: except where a last row is read again instead)
-  template <bool TAIL>
-  __device__ static inline void fetch(Regs &r, const char *base, uint64_t ld, int rows, int left, int tid) {
+  // memory -> registers, unit u of a whole step (FAST: with the 32-bit offset `off` from the uniform base)
+  template <bool FAST>
+  __device__ static inline void fetch(Regs &r, int u, const char *base, uint64_t ld, uint32_t off, int rows, int tid) {
     if (!active(tid)) return;
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-      int row, k;
-      at(tid + u * NT, row, k);
-      if constexpr (T::F32) {
-        row = row < rows ? row : rows - 1;
-        const float *p = reinterpret_cast<const float *>(base);
-        if constexpr (KC) {
-          p += (uint64_t)row * ld + k;
-          if (!TAIL || k + 8 <= left) {
-            typedef float f4u_t __attribute__((ext_vector_type(4), aligned(4)));
-            const f4u_t x = reinterpret_cast<const f4u_t *>(p)[0], y = reinterpret_cast<const f4u_t *>(p)[1];
-            r.v[u] = f8_t{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-          } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++) r.v[u][j] = k + j < left ? p[j] : 0.0f;
-          }
-        } else {
-          p += (uint64_t)k * ld + row;
-#pragma unroll
-          for (int j = 0; j < 8; j++) r.v[u][j] = (!TAIL || k + j < left) ? p[(uint64_t)j * ld] : 0.0f;
-        }
-      } else if constexpr (T::I8) {
-        row = row < rows ? row : rows - 1;
-        const char *p = base + (uint64_t)row * ld + k;
-        typedef uint32_t u4u_t __attribute__((ext_vector_type(4), aligned(1)));
-        if (!TAIL || k + 16 <= left) {
-          const u4u_t x = *reinterpret_cast<const u4u_t *>(p);
-          r.v[u] = u4_t{x.x, x.y, x.z, x.w};
-        } else {
-          u4_t x = {0, 0, 0, 0};
-#pragma unroll
-          for (int j = 0; j < 16; j++)
-            if (k + j < left) x[j / 4] |= (uint32_t)(uint8_t)p[j] << (j % 4 * 8);
-          r.v[u] = x;
-        }
+    if constexpr (T::F32 && FAST) {
+      if constexpr (KC) {
+        typedef float f4u_t __attribute__((ext_vector_type(4), aligned(4)));
+        const f4u_t *p = reinterpret_cast<const f4u_t *>(base + off);
+        const f4u_t x = p[0], y = p[1];
+        r.v[u] = f8_t{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
       } else {
-        // 16-bit: eight along K, or (LINES) eight rows of one line
-        if constexpr (!LINES) row = row < rows ? row : rows - 1;
-        const uint16_t *p = reinterpret_cast<const uint16_t *>(base) +
-                            (KC ? (uint64_t)row * ld + k : (uint64_t)k * ld + row);
-        const int have = LINES ? (TAIL && k >= left ? 0 : rows - row) : TAIL ? left - k : 8;
-        typedef uint32_t u4u_t __attribute__((ext_vector_type(4), aligned(2)));
-        if (have >= 8) {
-          const u4u_t x = *reinterpret_cast<const u4u_t *>(p);
-          r.v[u] = u4_t{x.x, x.y, x.z, x.w};
-        } else {
-          u4_t x = {0, 0, 0, 0};
+        // the descriptor holds the uniform base, the scalar offset picks the K-line: no vector arithmetic
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, 0xffffffff, 0x00020000);
+        const uint32_t line = __builtin_amdgcn_readfirstlane((uint32_t)ld * 4u);
 #pragma unroll
-          for (int j = 0; j < 8; j++)
-            if (j < have) x[j / 2] |= (uint32_t)p[j] << (j % 2 * 16);
-          r.v[u] = x;
-        }
+        for (int j = 0; j < 8; j++)
+          r.v[u][j] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rsrc, off, j * line, 0));
+      }
+    } else {
+      fetch_tail(r, u, base, ld, rows, 1 << 30, tid);
+    }
+  }
+
+  // ... any step: `left` K-values from its first to the end, any alignment.  Nothing beyond `rows` x `left` is read:
+  // zeros come in the place of K-values, the last row again in that of rows.
+  __device__ static inline void fetch_tail(Regs &r, int u, const char *base, uint64_t ld, int rows, int left, int tid) {
+    if (!active(tid)) return;
+    int row, k;
+    at(tid + u * NT, row, k);
+    if constexpr (T::F32) {
+      row = row < rows ? row : rows - 1;
+      const float *p = reinterpret_cast<const float *>(base) + (KC ? (uint64_t)row * ld + k : (uint64_t)k * ld + row);
+      const uint64_t step = KC ? 1 : ld;
+      // (no branches: a value past the end is read from the step's first K-value and replaced)
+      const int64_t first = -(int64_t)k * (int64_t)step;
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const bool in = k + j < left;
+        const float x = p[in ? (int64_t)(j * step) : first];
+        r.v[u][j] = in ? x : 0.0f;
+      }
+    } else if constexpr (T::I8) {
+      row = row < rows ? row : rows - 1;
+      const char *p = base + (uint64_t)row * ld + k;
+      typedef uint32_t u4u_t __attribute__((ext_vector_type(4), aligned(1)));
+      if (k + 16 <= left) {
+        const u4u_t x = *reinterpret_cast<const u4u_t *>(p);
+        r.v[u] = u4_t{x.x, x.y, x.z, x.w};
+      } else {
+        u4_t x = {0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < 16; j++)
+          if (k + j < left) x[j / 4] |= (uint32_t)(uint8_t)p[j] << (j % 4 * 8);
+        r.v[u] = x;
+      }
+    } else {
+      // 16-bit: eight along K, or (LINES) eight rows of one line
+      if constexpr (!LINES) row = row < rows ? row : rows - 1;
+      const uint16_t *p = reinterpret_cast<const uint16_t *>(base) + (KC ? (uint64_t)row * ld + k : (uint64_t)k * ld + row);
+      const int have = LINES ? (k >= left ? 0 : rows - row) : left - k;
+      typedef uint32_t u4u_t __attribute__((ext_vector_type(4), aligned(2)));
+      if (have >= 8) {
+        const u4u_t x = *reinterpret_cast<const u4u_t *>(p);
+        r.v[u] = u4_t{x.x, x.y, x.z, x.w};
+      } else {
+        u4_t x = {0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+          if (j < have) x[j / 2] |= (uint32_t)p[j] << (j % 2 * 16);
+        r.v[u] = x;
       }
     }
   }
 
   // registers -> LDS
-  __device__ static inline void put(const Regs &r, char *lds_op, int tid) {
+  __device__ static inline void put(const Regs &r, int u, char *lds_op, int tid) {
     if (!active(tid)) return;
+    const int id = tid + u * NT;
+    if constexpr (T::F32) {
+      int row, k;
+      at(id, row, k);
+      u4_t out[T::NP];
+      splitter<T::P>::run(r.v[u], out);
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      const int id = tid + u * NT;
-      if constexpr (T::F32) {
-        int row, k;
-        at(id, row, k);
-        u4_t out[T::NP];
-        splitter<T::P>::run(r.v[u], out);
-#pragma unroll
-        for (int p = 0; p < T::NP; p++)
-          *reinterpret_cast<u4_t *>(lds_op + p * ROWS * T::ROW_BYTES + chunk_offset<T::ROW_BYTES>(row, k / T::CHUNK)) = out[p];
-      } else {
-        *reinterpret_cast<u4_t *>(lds_op + id * 16) = r.v[u];
-      }
+      for (int p = 0; p < T::NP; p++)
+        *reinterpret_cast<u4_t *>(lds_op + p * ROWS * T::ROW_BYTES + chunk_offset<T::ROW_BYTES>(row, k / T::CHUNK)) = out[p];
+    } else {
+      *reinterpret_cast<u4_t *>(lds_op + id * 16) = r.v[u];
     }
   }
 };
+
+#pragma clang diagnostic pop
 
 template <Elem E>
 __device__ inline typename elem_traits<E>::acc_t grouped_mfma(const u4_t a, const u4_t b, const typename elem_traits<E>::acc_t c) {
@@ -387,6 +414,8 @@ void grouped_kernel(const GroupedArgs args) {
   using LB = grouped_loader<Cfg::E, Cfg::B_KC, BN, NT>;
   a += (Cfg::A_KC ? (uint64_t)m0 * args.lda : (uint64_t)m0) * T::BYTES;
   b += (Cfg::B_KC ? (uint64_t)n0 * args.ldb : (uint64_t)n0) * T::BYTES;
+  a = uniform_address(a);
+  b = uniform_address(b);
   const uint64_t a_step = (Cfg::A_KC ? (uint64_t)BK : (uint64_t)BK * args.lda) * T::BYTES;
   const uint64_t b_step = (Cfg::B_KC ? (uint64_t)BK : (uint64_t)BK * args.ldb) * T::BYTES;
 
@@ -422,97 +451,154 @@ void grouped_kernel(const GroupedArgs args) {
       return u4_t{x[0], x[1], y[0], y[1]};
     }
   };
-  auto multiply = [&](const char *stage) {
+  // A step's MFMAs, row block after row block of every slice; the fragments of the next row blocks (AHEAD_A of them) and of the
+  // next slice's columns are on their way meanwhile.  `beside(g)`:
+  // what else is done beside row block g.
+  constexpr int BLOCKS = T::SLICES * TM;
+  auto multiply = [&](const char *stage, auto beside) {
     const char *sa = stage, *sb = stage + Cfg::A_STAGE;
+    constexpr int AHEAD_A = T::F32 ? 1 : 2; // (FP32: a block is three or six times as many MFMAs)
+    u4_t fa[AHEAD_A + 1][T::NP], fb[T::SLICES][T::NP][TN];
+    auto read_a = [&](const int g) {
 #pragma unroll
-    for (int s = 0; s < T::SLICES; s++) {
-      u4_t fa[T::NP][TM], fb[T::NP][TN];
+      for (int p = 0; p < T::NP; p++)
+        fa[g % (AHEAD_A + 1)][p] = frag(sa, wm * Cfg::WM + (g % TM) * 16, p, g / TM, std::integral_constant<bool, Cfg::A_KC>{},
+                                        std::integral_constant<int, BM>{});
+    };
+    auto read_b = [&](const int s) {
 #pragma unroll
-      for (int p = 0; p < T::NP; p++) {
+      for (int p = 0; p < T::NP; p++)
 #pragma unroll
         for (int j = 0; j < TN; j++)
-          fb[p][j] = frag(sb, wn * Cfg::WN + j * 16, p, s, std::integral_constant<bool, Cfg::B_KC>{}, std::integral_constant<int, BN>{});
+          fb[s][p][j] = frag(sb, wn * Cfg::WN + j * 16, p, s, std::integral_constant<bool, Cfg::B_KC>{},
+                             std::integral_constant<int, BN>{});
+    };
+    read_a(0);
+    read_b(0);
+    if (AHEAD_A > 1 && BLOCKS > 1) read_a(1);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < TM; i++)
-          fa[p][i] = frag(sa, wm * Cfg::WM + i * 16, p, s, std::integral_constant<bool, Cfg::A_KC>{}, std::integral_constant<int, BM>{});
-      }
+    for (int g = 0; g < BLOCKS; g++) {
+      const int s = g / TM, i = g % TM;
+      if (g + AHEAD_A < BLOCKS) read_a(g + AHEAD_A);
+      if (i == (TM > 1 ? TM - 2 : 0) && s + 1 < T::SLICES) read_b(s + 1);
+      beside(g);
 #pragma unroll
       for (int q = 0; q < T::NPROD; q++) {
-        constexpr int ZERO = 0;
-        const int pa = T::F32 ? prec_traits<T::P>::PA[q] : ZERO, pb = T::F32 ? prec_traits<T::P>::PB[q] : ZERO;
-        const int ac = T::F32 ? prec_traits<T::P>::ACC[q] : ZERO;
+        const int pa = T::F32 ? prec_traits<T::P>::PA[q] : 0, pb = T::F32 ? prec_traits<T::P>::PB[q] : 0;
+        const int ac = T::F32 ? prec_traits<T::P>::ACC[q] : 0;
 #pragma unroll
-        for (int i = 0; i < TM; i++)
-#pragma unroll
-          for (int j = 0; j < TN; j++) acc[ac][j][i] = grouped_mfma<Cfg::E>(fa[pa][i], fb[pb][j], acc[ac][j][i]);
+        for (int j = 0; j < TN; j++)
+          acc[ac][j][i] = grouped_mfma<Cfg::E>(fa[g % (AHEAD_A + 1)][pa], fb[s][pb][j], acc[ac][j][i]);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
+  auto nothing = [](int) {};
 
   // ---- K loop ----
-  const int steps = (int)((klen + BK - 1) / BK), whole = (int)(klen / BK);
-  if constexpr (Cfg::DIRECT) {
+  // A K that ends inside a step has that step multiplied first, so that the loop has whole steps only: step s begins
+  // at K-value (s - partial) BK, the partial one behind them all.
+  const int whole = (int)(klen / BK), left = (int)(klen % BK), partial = left != 0, steps = whole + partial;
+  auto a_at = [&](int s) { return a + (uint64_t)(partial && s == 0 ? whole : s - partial) * a_step; };
+  auto b_at = [&](int s) { return b + (uint64_t)(partial && s == 0 ? whole : s - partial) * b_step; };
+  uint32_t offa[LA::U], offb[LB::U];
+#pragma unroll
+  for (int u = 0; u < LA::U; u++) offa[u] = (uint32_t)LA::offset(tid + u * NT, args.lda, rows_a);
+#pragma unroll
+  for (int u = 0; u < LB::U; u++) offb[u] = (uint32_t)LB::offset(tid + u * NT, args.ldb, rows_b);
+  constexpr int LOADS = LA::U + LB::U;
+  // which of a step's loads (A's, then B's) are issued beside row block g
+  auto share = [](int g, auto f) {
+#pragma unroll
+    for (int l = 0; l < LOADS; l++)
+      if (l * BLOCKS / LOADS == g) f(l);
+  };
+  if constexpr (Cfg::DIRECT && !T::F32) {
     // NSTAGE - 1 steps ahead; a buffer is filled again once all waves have read it, i.e. behind the barrier of the
     // step after
     constexpr int AHEAD = Cfg::NSTAGE - 1;
-    constexpr int LOADS = LA::U + LB::U;
-    uint32_t offa[LA::U], offb[LB::U];
-#pragma unroll
-    for (int u = 0; u < LA::U; u++) offa[u] = (uint32_t)LA::offset(tid + u * NT, args.lda, rows_a);
-#pragma unroll
-    for (int u = 0; u < LB::U; u++) offb[u] = (uint32_t)LB::offset(tid + u * NT, args.ldb, rows_b);
-    auto issue = [&](int step) {
-      char *sa = lds + (step % Cfg::NSTAGE) * Cfg::STAGE, *sb = sa + Cfg::A_STAGE;
-      const char *pa = a + (uint64_t)step * a_step, *pb = b + (uint64_t)step * b_step;
-      if (step < whole) {
-        LA::template direct<false>(pa, offa, sa, tid, wave, BK);
-        LB::template direct<false>(pb, offb, sb, tid, wave, BK);
-      } else {
-        const int left = (int)klen - step * BK;
-        LA::template direct<true>(pa, offa, sa, tid, wave, left);
-        LB::template direct<true>(pb, offb, sb, tid, wave, left);
-      }
+    const uint32_t lds0 = lds_address(lds);
+    auto issue = [&](int l, const char *pa, const char *pb, uint32_t stage) {
+      if (l < LA::U) LA::direct(l, pa, offa[l], stage, wave);
+      else LB::direct(l - LA::U, pb, offb[l - LA::U], stage + Cfg::A_STAGE, wave);
     };
-    for (int s = 0; s < AHEAD && s < steps; s++) issue(s);
-    for (int s = 0; s < steps; s++) {
+    for (int s = 0; s < AHEAD && s < steps; s++) {
+      const uint32_t stage = lds0 + s * Cfg::STAGE;
+      const char *pa = a_at(s), *pb = b_at(s);
+      if (partial && s == 0) {
+#pragma unroll
+        for (int u = 0; u < LA::U; u++) LA::direct_tail(u, pa, offa[u], stage, tid, wave, left);
+#pragma unroll
+        for (int u = 0; u < LB::U; u++) LB::direct_tail(u, pb, offb[u], stage + Cfg::A_STAGE, tid, wave, left);
+      } else {
+#pragma unroll
+        for (int l = 0; l < LOADS; l++) issue(l, pa, pb, stage);
+      }
+    }
+    int at = 0; // buffer of step s
+    for (int s = 0; s < steps - AHEAD; s++) {
       // everything but the loads of the AHEAD - 1 steps after this one has landed
-      if (AHEAD > 1 && s + AHEAD <= steps) __builtin_amdgcn_s_waitcnt(waitcnt_vm(LOADS * (AHEAD - 1)));
-      else __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+      __builtin_amdgcn_s_waitcnt(waitcnt_vm(LOADS * (AHEAD - 1)));
       block_sync_lds();
-      if (s + AHEAD < steps) issue(s + AHEAD);
-      multiply(lds + (s % Cfg::NSTAGE) * Cfg::STAGE);
+      const int next = at == 0 ? Cfg::NSTAGE - 1 : at - 1; // of step s + AHEAD
+      const char *pa = a_at(s + AHEAD), *pb = b_at(s + AHEAD);
+      const uint32_t stage = lds0 + next * Cfg::STAGE;
+      multiply(lds + at * Cfg::STAGE, [&](int g) { share(g, [&](int l) { issue(l, pa, pb, stage); }); });
+      at = at + 1 == Cfg::NSTAGE ? 0 : at + 1;
+    }
+    for (int s = steps > AHEAD ? steps - AHEAD : 0; s < steps; s++) {
+      __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+      block_sync_lds();
+      multiply(lds + at * Cfg::STAGE, nothing);
+      at = at + 1 == Cfg::NSTAGE ? 0 : at + 1;
     }
   } else {
-    static_assert(Cfg::DIRECT || Cfg::NSTAGE == 2, "two buffers");
+    // through registers: step s + 1 is written to LDS and step s + 2 asked for beside the MFMAs of step s
+    static_assert(Cfg::NSTAGE == 2 || (Cfg::DIRECT && !T::F32), "two buffers");
     typename LA::Regs ra;
     typename LB::Regs rb;
-    auto fetch = [&](int step) {
-      const char *pa = a + (uint64_t)step * a_step, *pb = b + (uint64_t)step * b_step;
-      if (step < whole) {
-        LA::template fetch<false>(ra, pa, args.lda, rows_a, BK, tid);
-        LB::template fetch<false>(rb, pb, args.ldb, rows_b, BK, tid);
-      } else {
-        const int left = (int)klen - step * BK;
-        LA::template fetch<true>(ra, pa, args.lda, rows_a, left, tid);
-        LB::template fetch<true>(rb, pb, args.ldb, rows_b, left, tid);
-      }
+    auto put = [&](int l, char *stage) {
+      if (l < LA::U) LA::put(ra, l, stage, tid);
+      else LB::put(rb, l - LA::U, stage + Cfg::A_STAGE, tid);
     };
-    auto put = [&](int step) {
-      char *sa = lds + (step & 1) * Cfg::STAGE;
-      LA::put(ra, sa, tid);
-      LB::put(rb, sa + Cfg::A_STAGE, tid);
+    auto fetch = [&](int l, const char *pa, const char *pb) {
+      if (l < LA::U) LA::template fetch<Cfg::DIRECT>(ra, l, pa, args.lda, offa[l], rows_a, tid);
+      else LB::template fetch<Cfg::DIRECT>(rb, l - LA::U, pb, args.ldb, offb[l - LA::U], rows_b, tid);
     };
     if (steps > 0) {
-      fetch(0);
-      put(0);
+      const char *pa = a_at(0), *pb = b_at(0);
+      if (partial) {
+#pragma unroll
+        for (int u = 0; u < LA::U; u++) LA::fetch_tail(ra, u, pa, args.lda, rows_a, left, tid);
+#pragma unroll
+        for (int u = 0; u < LB::U; u++) LB::fetch_tail(rb, u, pb, args.ldb, rows_b, left, tid);
+      } else {
+#pragma unroll
+        for (int l = 0; l < LOADS; l++) fetch(l, pa, pb);
+      }
+#pragma unroll
+      for (int l = 0; l < LOADS; l++) put(l, lds);
+      if (steps > 1) {
+        pa = a_at(1), pb = b_at(1);
+#pragma unroll
+        for (int l = 0; l < LOADS; l++) fetch(l, pa, pb);
+      }
       block_sync_lds();
     }
-    for (int s = 0; s < steps; s++) {
-      if (s + 1 < steps) fetch(s + 1);
-      multiply(lds + (s & 1) * Cfg::STAGE);
-      if (s + 1 < steps) put(s + 1);
+    for (int s = 0; s < steps - 1; s++) {
+      const int ask = s + 2 < steps ? s + 2 : s + 1; // (the last time: the same step again, unused)
+      const char *pa = a_at(ask), *pb = b_at(ask);
+      char *stage = lds + ((s + 1) & 1) * Cfg::STAGE;
+      multiply(lds + (s & 1) * Cfg::STAGE, [&](int g) {
+        share(g, [&](int l) {
+          put(l, stage);
+          fetch(l, pa, pb);
+        });
+      });
       block_sync_lds();
     }
+    if (steps > 0) multiply(lds + ((steps - 1) & 1) * Cfg::STAGE, nothing);
   }
 
   // ---- results ----

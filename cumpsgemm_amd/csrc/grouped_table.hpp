@@ -15,17 +15,19 @@ constexpr GroupedKernel grouped_of() {
   return grouped_entry<GroupedCfg<E, A_KC, B_KC, BM, BN, WM, WN, NSTAGE, DIRECT, RAGGED_K, 2>>();
 }
 
-// FP32: through registers always
 template <Elem E> constexpr GroupedTable grouped_table_f32() {
   GroupedTable t{};
-  t.columns[0][0][TILE_256] = grouped_of<E, false, true, 256, 128, 64, 64, 2, false, false>();
   t.columns[0][0][TILE_128] = grouped_of<E, false, true, 128, 128, 64, 32, 2, false, false>();
-  t.columns[0][0][TILE_NARROW] = grouped_of<E, false, true, 128, 32, 32, 32, 2, false, false>();
-  t.columns[1][0][TILE_256] = grouped_of<E, true, true, 256, 128, 64, 64, 2, false, false>();
   t.columns[1][0][TILE_128] = grouped_of<E, true, true, 128, 128, 64, 32, 2, false, false>();
-  t.columns[1][0][TILE_NARROW] = grouped_of<E, true, true, 128, 32, 32, 32, 2, false, false>();
-  t.over_k[0][TILE_256] = grouped_of<E, false, false, 256, 128, 64, 64, 2, false, true>();
+  t.columns[0][1][TILE_256] = grouped_of<E, false, true, 256, 128, 64, 64, 2, true, false>();
+  t.columns[0][1][TILE_128] = grouped_of<E, false, true, 128, 128, 64, 32, 2, true, false>();
+  t.columns[0][1][TILE_NARROW] = grouped_of<E, false, true, 128, 32, 32, 32, 2, true, false>();
+  t.columns[1][1][TILE_256] = grouped_of<E, true, true, 256, 128, 64, 64, 2, true, false>();
+  t.columns[1][1][TILE_128] = grouped_of<E, true, true, 128, 128, 64, 32, 2, true, false>();
+  t.columns[1][1][TILE_NARROW] = grouped_of<E, true, true, 128, 32, 32, 32, 2, true, false>();
   t.over_k[0][TILE_128] = grouped_of<E, false, false, 128, 128, 64, 32, 2, false, true>();
+  t.over_k[1][TILE_256] = grouped_of<E, false, false, 256, 128, 64, 64, 2, true, true>();
+  t.over_k[1][TILE_128] = grouped_of<E, false, false, 128, 128, 64, 32, 2, true, true>();
   return t;
 }
 
