@@ -5,7 +5,7 @@
 // columns are tokens (n), so that a lane holds four results next to each other in memory.
 //
 // LDS images of an operand's K-step (ROWS rows of C or tokens):
-//   K-contiguous: ROWS rows of ROW_BYTES bytes.  128 bytes of 16-bit or 8-bit values; 64 bytes (32 values) in each
+//   K-contiguous: ROWS rows of ROW_BYTES bytes (128 or 64) of 16-bit or 8-bit values; 64 bytes (32 values) in each
 //     plane of a split FP32 operand.  The 16-byte chunks of a row are exchanged (chunk ^ f(row)) so that the sixteen
 //     rows that one part of a ds_read_b128 touches fall on sixteen different bank groups.
 //   row-contiguous (16-bit operands whose rows, not K, are contiguous: op N weights, and both operands of the
@@ -34,9 +34,6 @@ template <Elem E> struct elem_traits {
   static constexpr int NPROD = F32 ? prec_traits<P>::NPROD : 1;
   static constexpr int NACC = F32 ? prec_traits<P>::NACC : 1;
   static constexpr int CHUNK = I8 ? 16 : 8;         // K-values of a 16-byte chunk in LDS
-  static constexpr int ROW_BYTES = F32 ? 64 : 128;  // of a K-contiguous row in LDS
-  static constexpr int BK = ROW_BYTES / 16 * CHUNK; // K-values of a step
-  static constexpr int SLICES = ROW_BYTES / 64;     // MFMAs deep
   typedef typename std::conditional<I8, i4_t, f4v_t>::type acc_t;
 };
 
@@ -44,19 +41,23 @@ template <Elem E> struct elem_traits {
 static __device__ const u4_t g_grouped_zeros = {0, 0, 0, 0};
 
 // offset of a 16-byte chunk in a K-contiguous image
+template <int ROW_BYTES> __device__ inline int row_swizzle(int row) {
+  return ROW_BYTES == 64 ? lds_swizzle(row) : (row >> 1) & 7;
+}
 template <int ROW_BYTES> __device__ inline int chunk_offset(int row, int chunk) {
-  if constexpr (ROW_BYTES == 64) return lds_offset(row, chunk);
-  else return row * 128 + ((chunk ^ ((row >> 1) & 7)) << 4);
+  return row * ROW_BYTES + ((chunk ^ row_swizzle<ROW_BYTES>(row)) << 4);
 }
 // what M0 holds for a load to LDS (wave-uniform)
 __device__ inline uint32_t lds_address(const char *p) {
   return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char *)p);
 }
 // an address that is the same for all lanes, whatever the compiler can see of that
+// (and one of global memory: a pointer made of a number would be read with flat loads, which wait for LDS as well)
 __device__ inline const char *uniform_address(const char *p) {
   const uint64_t x = (uint64_t)p;
   const uint32_t high = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32)), low = __builtin_amdgcn_readfirstlane((uint32_t)x);
-  return (const char *)((uint64_t)high << 32 | low); // (low is unsigned here: the builtin's own int would carry its sign up)
+  typedef const char __attribute__((address_space(1))) *gptr_t;
+  return (const char *)(gptr_t)((uint64_t)high << 32 | low); // (low is unsigned here: the builtin's own int would carry its sign up)
 }
 // which 32-byte piece of line k holds piece p of a row-contiguous image
 __device__ inline int line_swizzle(int k) { return (k & 3) | (((k >> 3) & 1) << 2); }
@@ -99,43 +100,47 @@ __device__ inline void raster(uint32_t in, uint32_t tiles_m, uint32_t tiles_n, u
   tn = rest / rows;
 }
 
-// Ragged columns: the tile of workgroup `bid` in the list of all groups' tiles (every wave works it out for itself:
-// 64 groups at a time, one a lane).  False: there are fewer tiles.
+// Ragged columns: the tile of workgroup `bid` in the list of all groups' tiles: whole columns of tiles first, then the
+// groups' last columns, which have fewer than bn tokens and take less time, so that what keeps some CUs longest is short.
+// (Every wave works it out for itself, 64 groups at a time, one a lane.)  False: there are fewer tiles.
 __device__ inline bool place_tile(const GroupedArgs &args, uint32_t bid, uint32_t tiles_m, uint32_t bn, TilePlace &t) {
-  if (args.offsets == nullptr) {
-    const uint32_t tiles_n = (args.n + bn - 1) / bn, total = tiles_m * tiles_n;
-    if (bid >= total) return false;
-    t.group = 0;
-    t.lo = 0;
-    t.hi = args.n;
-    raster(xcd_range(bid, total), tiles_m, tiles_n, t.tm, t.tn);
-    return true;
-  }
   const int lane = threadIdx.x & 63;
-  uint32_t all = 0;
+  auto span_of = [&](uint32_t g, uint32_t &lo, uint32_t &hi) {
+    lo = hi = 0;
+    if (g >= args.groups) return;
+    if (args.offsets != nullptr) group_span(args.offsets, g, args.n, lo, hi);
+    else hi = args.n;
+  };
+  uint32_t whole = 0, last = 0; // columns of tiles, of all groups
   for (uint32_t g0 = 0; g0 < args.groups; g0 += 64) {
-    uint32_t lo = 0, hi = 0;
-    if (g0 + lane < args.groups) group_span(args.offsets, g0 + lane, args.n, lo, hi);
-    const uint32_t sum = wave_inclusive_sum((hi - lo + bn - 1) / bn, lane);
-    all += __builtin_amdgcn_readlane(sum, 63);
+    uint32_t lo, hi;
+    span_of(g0 + lane, lo, hi);
+    whole += __builtin_amdgcn_readlane(wave_inclusive_sum((hi - lo) / bn, lane), 63);
+    last += __builtin_popcountll(__ballot((hi - lo) % bn != 0));
   }
-  const uint32_t total = all * tiles_m;
-  if (bid >= total) return false;
-  const uint32_t id = xcd_range(bid, total), column = id / tiles_m;
+  const bool in_whole = bid < whole * tiles_m;
+  if (!in_whole && bid - whole * tiles_m >= last * tiles_m) return false;
+  const uint32_t id = in_whole ? xcd_range(bid, whole * tiles_m) : xcd_range(bid - whole * tiles_m, last * tiles_m);
+  const uint32_t column = id / tiles_m;
   uint32_t before = 0;
   for (uint32_t g0 = 0; g0 < args.groups; g0 += 64) {
-    uint32_t lo = 0, hi = 0;
-    if (g0 + lane < args.groups) group_span(args.offsets, g0 + lane, args.n, lo, hi);
-    const uint32_t mine = (hi - lo + bn - 1) / bn, sum = before + wave_inclusive_sum(mine, lane);
+    uint32_t lo, hi;
+    span_of(g0 + lane, lo, hi);
+    const uint32_t full = (hi - lo) / bn, mine = in_whole ? full : (hi - lo) % bn != 0;
+    const uint32_t sum = before + wave_inclusive_sum(mine, lane);
     const uint64_t beyond = __ballot(column < sum);
     if (beyond != 0) {
       const int at = __builtin_ctzll(beyond);
       t.group = g0 + at;
       t.lo = __builtin_amdgcn_readlane(lo, at);
       t.hi = __builtin_amdgcn_readlane(hi, at);
-      const uint32_t tiles_n = __builtin_amdgcn_readlane(mine, at);
-      const uint32_t first = __builtin_amdgcn_readlane(sum, at) - tiles_n;
-      raster(id - first * tiles_m, tiles_m, tiles_n, t.tm, t.tn);
+      if (in_whole) {
+        const uint32_t tiles_n = __builtin_amdgcn_readlane(full, at);
+        raster(id - (__builtin_amdgcn_readlane(sum, at) - tiles_n) * tiles_m, tiles_m, tiles_n, t.tm, t.tn);
+      } else {
+        t.tm = id % tiles_m;
+        t.tn = __builtin_amdgcn_readlane(full, at);
+      }
       return true;
     }
     before = __builtin_amdgcn_readlane(sum, 63);
@@ -145,24 +150,31 @@ __device__ inline bool place_tile(const GroupedArgs &args, uint32_t bid, uint32_
 
 // DIRECT: 16-bit and 8-bit operands go straight from memory to LDS, 16 aligned bytes a lane; FP32 operands, which are
 // split in registers, are read with 32-bit offsets from uniform bases.  Otherwise: any alignment, any size.
-template <Elem E_, bool A_KC_, bool B_KC_, int BM_, int BN_, int WM_, int WN_, int NSTAGE_, bool DIRECT_, bool RAGGED_K_,
-          int OCC_>
+template <Elem E_, bool A_KC_, bool B_KC_, int BM_, int BN_, int WM_, int WN_, int ROW_BYTES_, int NSTAGE_, bool DIRECT_,
+          bool RAGGED_K_, int OCC_>
 struct GroupedCfg {
   using T = elem_traits<E_>;
   static constexpr Elem E = E_;
   static constexpr bool A_KC = A_KC_, B_KC = B_KC_, DIRECT = DIRECT_, RAGGED_K = RAGGED_K_;
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NSTAGE = NSTAGE_, OCC = OCC_;
-  static constexpr int WAVES = (BM / WM) * (BN / WN), NT = WAVES * 64;
+  static constexpr int WAVES_M = BM / WM, WAVES_N = BN / WN, NT = WAVES_M * WAVES_N * 64;
   static constexpr int TM = WM / 16, TN = WN / 16;
-  static constexpr int A_PLANE = BM * T::ROW_BYTES, B_PLANE = BN * T::ROW_BYTES;
+  static constexpr int ROW_BYTES = ROW_BYTES_;
+  static constexpr int BK = ROW_BYTES / 16 * T::CHUNK; // K-values of a step
+  static constexpr int SLICES = ROW_BYTES / 64;        // MFMAs deep
+  static_assert(ROW_BYTES == 64 || (ROW_BYTES == 128 && !T::F32), "rows in LDS");
+  static constexpr int A_PLANE = BM * ROW_BYTES, B_PLANE = BN * ROW_BYTES;
   static constexpr int A_STAGE = A_PLANE * T::NP, B_STAGE = B_PLANE * T::NP, STAGE = A_STAGE + B_STAGE;
-  static constexpr int LDS_BYTES = NSTAGE * STAGE;
+  // (the results pass through LDS: sixteen columns of each wave at a time, four floats further
+  // apart than they are long, so that sixteen columns' pieces fall on different banks)
+  static constexpr int PITCH = WM + 4, OUT_BYTES = WAVES_M * WAVES_N * 16 * PITCH * 4;
+  static constexpr int LDS_BYTES = NSTAGE * STAGE > OUT_BYTES ? NSTAGE * STAGE : OUT_BYTES;
   static_assert(!T::I8 || (A_KC && B_KC), "8-bit integers: K-contiguous operands");
   static_assert(A_KC || T::F32 || BM >= 128, "a line's pieces are exchanged among eight");
   static_assert(B_KC || T::F32 || BN >= 128, "a line's pieces are exchanged among eight");
   static_assert(LDS_BYTES <= 160 * 1024, "LDS");
   // (the waits of the direct form count a step's loads, the same number for every wave)
-  static_assert(!DIRECT || T::F32 || (BM * T::ROW_BYTES / 16 % NT == 0 && BN * T::ROW_BYTES / 16 % NT == 0), "whole rounds of loads");
+  static_assert(!DIRECT || T::F32 || (BM * ROW_BYTES / 16 % NT == 0 && BN * ROW_BYTES / 16 % NT == 0), "whole rounds of loads");
 };
 
 // (M0 is among the registers that the loads below say they change; nothing of the compiler's lives in it longer than
@@ -170,16 +182,16 @@ struct GroupedCfg {
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 // Staging of one operand's K-step by NT threads.  A unit is one 16-byte chunk of LDS (FP32: one in each plane).
-template <Elem E, bool KC, int ROWS, int NT> struct grouped_loader {
+template <Elem E, bool KC, int ROWS, int ROW_BYTES, int NT> struct grouped_loader {
   using T = elem_traits<E>;
   // row-contiguous images exist for 16-bit values only; FP32 ends in K-contiguous planes either way
   static constexpr bool LINES = !KC && !T::F32;
-  static constexpr int UNITS = ROWS * T::ROW_BYTES / 16;
+  static constexpr int UNITS = ROWS * ROW_BYTES / 16;
   static constexpr int U = (UNITS + NT - 1) / NT;
   static constexpr bool PARTIAL = UNITS < NT;
   static_assert(UNITS % NT == 0 || (PARTIAL && UNITS % 64 == 0), "whole waves");
   static constexpr int LINE_CHUNKS = ROWS / 8;            // 16-byte chunks of a line
-  static constexpr int ROW_CHUNKS = T::ROW_BYTES / 16;
+  static constexpr int ROW_CHUNKS = ROW_BYTES / 16;
 
   __device__ static inline bool active(int tid) { return !PARTIAL || tid < UNITS; }
 
@@ -201,16 +213,16 @@ template <Elem E, bool KC, int ROWS, int NT> struct grouped_loader {
       }
     } else {
       row = id / ROW_CHUNKS;
-      k = ((id % ROW_CHUNKS) ^ ((row >> 1) & 7)) * T::CHUNK;
+      k = ((id % ROW_CHUNKS) ^ row_swizzle<ROW_BYTES>(row)) * T::CHUNK;
     }
   }
 
   // Byte offset from the tile's origin (row 0, K-value 0 of the step) of the unit that fills position id.
-  // `rows`: those that exist; one beyond them reads the last again (its products are not stored).
+  // `rows`: those that exist; one (LINES: eight) beyond them reads the last again (its products are not stored).
   __device__ static inline uint64_t offset(int id, uint64_t ld, int rows) {
     int row, k;
     at(id, row, k);
-    const int last = LINES ? rows - 8 : rows - 1;
+    const int last = LINES ? (rows - 1) & ~7 : rows - 1;
     row = row < last ? row : last;
     return (KC ? (uint64_t)row * ld + k : (uint64_t)k * ld + row) * T::BYTES;
   }
@@ -238,77 +250,86 @@ template <Elem E, bool KC, int ROWS, int NT> struct grouped_loader {
     typename std::conditional<T::F32, f8_t, u4_t>::type v[U];
   };
 
-  // memory -> registers, unit u of a whole step (FAST: with the 32-bit offset `off` from the uniform base)
-  template <bool FAST>
-  __device__ static inline void fetch(Regs &r, int u, const char *base, uint64_t ld, uint32_t off, int rows, int tid) {
+  // memory -> registers, unit u of a whole step.  off: the unit's offset() from the uniform base, in 32 bits if FAST.
+  // (rows, safe: see fetch_tail)
+  template <bool FAST, class OFF>
+  __device__ static inline void fetch(Regs &r, int u, const char *base, uint64_t ld, OFF off, int rows, int64_t safe, int tid) {
     if (!active(tid)) return;
-    if constexpr (T::F32 && FAST) {
-      if constexpr (KC) {
-        typedef float f4u_t __attribute__((ext_vector_type(4), aligned(4)));
-        const f4u_t *p = reinterpret_cast<const f4u_t *>(base + off);
-        const f4u_t x = p[0], y = p[1];
-        r.v[u] = f8_t{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-      } else {
-        // the descriptor holds the uniform base, the scalar offset picks the K-line: no vector arithmetic
-        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, 0xffffffff, 0x00020000);
-        const uint32_t line = __builtin_amdgcn_readfirstlane((uint32_t)ld * 4u);
+    if constexpr (T::F32 && KC) {
+      typedef float f4u_t __attribute__((ext_vector_type(4), aligned(4)));
+      const f4u_t *p = reinterpret_cast<const f4u_t *>(base + off);
+      const f4u_t x = p[0], y = p[1];
+      r.v[u] = f8_t{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+    } else if constexpr (T::F32 && FAST) {
+      // the descriptor holds the uniform base, the scalar offset picks the K-line: no vector arithmetic
+      const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, 0xffffffff, 0x00020000);
+      const uint32_t line = __builtin_amdgcn_readfirstlane((uint32_t)ld * 4u);
 #pragma unroll
-        for (int j = 0; j < 8; j++)
-          r.v[u][j] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rsrc, off, j * line, 0));
-      }
+      for (int j = 0; j < 8; j++)
+        r.v[u][j] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rsrc, off, j * line, 0));
+    } else if constexpr (T::F32) {
+      const float *p = reinterpret_cast<const float *>(base + off);
+#pragma unroll
+      for (int j = 0; j < 8; j++) r.v[u][j] = p[(uint64_t)j * ld];
     } else {
-      fetch_tail(r, u, base, ld, rows, 1 << 30, tid);
+      // (rows of 16-bit values may begin anywhere: the type promises no more and leaves the instruction to the compiler)
+      typedef uint32_t u4u2_t __attribute__((ext_vector_type(4), aligned(2)));
+      typedef uint32_t u4u1_t __attribute__((ext_vector_type(4), aligned(1)));
+      typedef typename std::conditional<T::I8, u4u1_t, u4u2_t>::type u4u_t;
+      if (!LINES || rows >= ROWS) { // (uniform)
+        const u4u_t x = *reinterpret_cast<const u4u_t *>(base + off);
+        r.v[u] = u4_t{x.x, x.y, x.z, x.w};
+      } else {
+        fetch_tail(r, u, base, ld, rows, 1 << 30, safe, tid);
+      }
     }
   }
 
-  // ... any step: `left` K-values from its first to the end, any alignment.  Nothing beyond `rows` x `left` is read:
-  // zeros come in the place of K-values, the last row again in that of rows.
-  __device__ static inline void fetch_tail(Regs &r, int u, const char *base, uint64_t ld, int rows, int left, int tid) {
+  // ... any step: `left` K-values (one at least) from its first to the end.  Zeros come in the place of K-values beyond
+  // it, the last row again in that of rows.  A 16-byte chunk that sticks out beyond the last row (LINES) or K-value is
+  // read whole all the same, where what follows it is the next line or row of the matrix: for the first `safe` lines
+  // (rows, K-contiguous) counted from the base.  The others are read value by value.
+  __device__ static inline void fetch_tail(Regs &r, int u, const char *base, uint64_t ld, int rows, int left, int64_t safe, int tid) {
     if (!active(tid)) return;
     int row, k;
     at(tid + u * NT, row, k);
     if constexpr (T::F32) {
       row = row < rows ? row : rows - 1;
-      const float *p = reinterpret_cast<const float *>(base) + (KC ? (uint64_t)row * ld + k : (uint64_t)k * ld + row);
       const uint64_t step = KC ? 1 : ld;
-      // (no branches: a value past the end is read from the step's first K-value and replaced)
-      const int64_t first = -(int64_t)k * (int64_t)step;
+      const float *p = reinterpret_cast<const float *>(base) + (KC ? (uint64_t)row * ld : (uint64_t)row);
+      // (without branches: a value past the end is read from the step's first K-value and replaced)
 #pragma unroll
       for (int j = 0; j < 8; j++) {
         const bool in = k + j < left;
-        const float x = p[in ? (int64_t)(j * step) : first];
+        const float x = p[in ? (uint64_t)(k + j) * step : 0];
         r.v[u][j] = in ? x : 0.0f;
       }
-    } else if constexpr (T::I8) {
-      row = row < rows ? row : rows - 1;
-      const char *p = base + (uint64_t)row * ld + k;
-      typedef uint32_t u4u_t __attribute__((ext_vector_type(4), aligned(1)));
-      if (k + 16 <= left) {
-        const u4u_t x = *reinterpret_cast<const u4u_t *>(p);
-        r.v[u] = u4_t{x.x, x.y, x.z, x.w};
-      } else {
-        u4_t x = {0, 0, 0, 0};
-#pragma unroll
-        for (int j = 0; j < 16; j++)
-          if (k + j < left) x[j / 4] |= (uint32_t)(uint8_t)p[j] << (j % 4 * 8);
-        r.v[u] = x;
-      }
     } else {
-      // 16-bit: eight along K, or (LINES) eight rows of one line
-      if constexpr (!LINES) row = row < rows ? row : rows - 1;
-      const uint16_t *p = reinterpret_cast<const uint16_t *>(base) + (KC ? (uint64_t)row * ld + k : (uint64_t)k * ld + row);
-      const int have = LINES ? (k >= left ? 0 : rows - row) : left - k;
-      typedef uint32_t u4u_t __attribute__((ext_vector_type(4), aligned(2)));
-      if (have >= 8) {
-        const u4u_t x = *reinterpret_cast<const u4u_t *>(p);
-        r.v[u] = u4_t{x.x, x.y, x.z, x.w};
+      typedef typename std::conditional<T::I8, uint8_t, uint16_t>::type V;
+      typedef uint32_t u4u2_t __attribute__((ext_vector_type(4), aligned(2)));
+      typedef uint32_t u4u1_t __attribute__((ext_vector_type(4), aligned(1)));
+      typedef typename std::conditional<T::I8, u4u1_t, u4u2_t>::type u4u_t;
+      constexpr int BITS = T::BYTES * 8, PER = 32 / BITS;
+      const int last = LINES ? (rows - 1) & ~7 : rows - 1;
+      row = row < last ? row : last;
+      const int begins = k < left ? k : 0;               // (a chunk with nothing in it reads the step's first)
+      const int keep = LINES ? (k < left ? 8 : 0) : left - k; // values of the chunk that count
+      const int have = LINES ? rows - row : left - begins;    // ... that exist
+      const V *p = reinterpret_cast<const V *>(base) + (KC ? (uint64_t)row * ld + begins : (uint64_t)begins * ld + row);
+      u4_t x = {0, 0, 0, 0};
+      if (have >= T::CHUNK || (LINES ? begins : row) < safe) {
+        const u4u_t y = *reinterpret_cast<const u4u_t *>(p);
+        x = u4_t{y.x, y.y, y.z, y.w};
       } else {
-        u4_t x = {0, 0, 0, 0};
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-          if (j < have) x[j / 2] |= (uint32_t)p[j] << (j % 2 * 16);
-        r.v[u] = x;
+        for (int j = 0; j < T::CHUNK; j++)
+          if (j < have) x[j / PER] |= (uint32_t)p[j] << (j % PER * BITS);
       }
+#pragma unroll
+      for (int d = 0; d < 4; d++) {
+        const int n = keep - d * PER; // values of this word that count
+        x[d] = n >= PER ? x[d] : n > 0 ? x[d] & ((1u << (n * BITS & 31)) - 1) : 0;
+      }
+      r.v[u] = x;
     }
   }
 
@@ -323,7 +344,7 @@ template <Elem E, bool KC, int ROWS, int NT> struct grouped_loader {
       splitter<T::P>::run(r.v[u], out);
 #pragma unroll
       for (int p = 0; p < T::NP; p++)
-        *reinterpret_cast<u4_t *>(lds_op + p * ROWS * T::ROW_BYTES + chunk_offset<T::ROW_BYTES>(row, k / T::CHUNK)) = out[p];
+        *reinterpret_cast<u4_t *>(lds_op + p * ROWS * ROW_BYTES + chunk_offset<ROW_BYTES>(row, k / T::CHUNK)) = out[p];
     } else {
       *reinterpret_cast<u4_t *>(lds_op + id * 16) = r.v[u];
     }
@@ -368,54 +389,30 @@ __device__ inline void store_four(char *c, const f4v_t x, float beta, uint32_t r
   }
 }
 
-template <class Cfg>
-__global__ __launch_bounds__(Cfg::NT) __attribute__((amdgpu_waves_per_eu(Cfg::OCC, Cfg::OCC)))
-void grouped_kernel(const GroupedArgs args) {
+// A tile's place in memory: what its loops need to know.
+struct TileWork {
+  const char *a, *b;       // row m0, token n0 (ragged K: column n0), K-value 0
+  char *c;                 // of its group
+  uint32_t group, m0, n0, n_end, klen;
+  int rows_a, rows_b;      // rows and columns that exist
+  // lines (rows, K-contiguous operand) from a and b to the matrix's last but one; 0 where one is shorter than a chunk
+  int64_t safe_a, safe_b;
+};
+
+// One tile, TN column blocks of 16 for each wave: all that a wave has room for, or (a group's last tile) as many as the
+// tile's columns need.  The waves take column blocks in turn, so that a part of a tile is a part of every wave's work.
+template <class Cfg, int TN>
+__device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w, char *lds) {
   using T = typename Cfg::T;
-  constexpr int BM = Cfg::BM, BN = Cfg::BN, TM = Cfg::TM, TN = Cfg::TN, NT = Cfg::NT, BK = T::BK;
-  extern __shared__ __attribute__((aligned(16))) char lds[];
+  constexpr int BM = Cfg::BM, BN = Cfg::BN, TM = Cfg::TM, NT = Cfg::NT, BK = Cfg::BK, RB = Cfg::ROW_BYTES, SLICES = Cfg::SLICES;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave % (BM / Cfg::WM), wn = wave / (BM / Cfg::WM);
-
-  // ---- which tile ----
-  const uint32_t tiles_m = (args.m + BM - 1) / BM;
-  TilePlace t;
-  uint32_t n0, n_end, klen;
-  const char *a = args.a, *b = args.b;
-  char *c = args.c;
-  const uint64_t out_bytes = args.out == OUT_F32 ? 4 : 2;
-  if constexpr (Cfg::RAGGED_K) {
-    const uint32_t tiles_n = (args.n + BN - 1) / BN, per = tiles_m * tiles_n;
-    const uint32_t id = xcd_range(blockIdx.x, per * args.groups);
-    t.group = id / per;
-    raster(id % per, tiles_m, tiles_n, t.tm, t.tn);
-    group_span(args.offsets, t.group, args.k, t.lo, t.hi);
-    t.lo = __builtin_amdgcn_readfirstlane(t.lo);
-    t.hi = __builtin_amdgcn_readfirstlane(t.hi);
-    n0 = t.tn * BN;
-    n_end = args.n;
-    klen = t.hi - t.lo;
-    a += (uint64_t)t.lo * args.lda * T::BYTES;
-    b += (uint64_t)t.lo * args.ldb * T::BYTES;
-    c += (uint64_t)t.group * args.stride_c * out_bytes;
-  } else {
-    if (!place_tile(args, blockIdx.x, tiles_m, BN, t)) return;
-    n0 = t.lo + t.tn * BN;
-    n_end = t.hi;
-    klen = args.k;
-    a += (uint64_t)t.group * args.stride_a * T::BYTES;
-  }
-  const uint32_t m0 = t.tm * BM;
-  const int rows_a = (int)(args.m - m0 < (uint32_t)BM ? args.m - m0 : BM);
-  const int rows_b = (int)(n_end - n0 < (uint32_t)BN ? n_end - n0 : BN);
-
-  using LA = grouped_loader<Cfg::E, Cfg::A_KC, BM, NT>;
-  using LB = grouped_loader<Cfg::E, Cfg::B_KC, BN, NT>;
-  a += (Cfg::A_KC ? (uint64_t)m0 * args.lda : (uint64_t)m0) * T::BYTES;
-  b += (Cfg::B_KC ? (uint64_t)n0 * args.ldb : (uint64_t)n0) * T::BYTES;
-  a = uniform_address(a);
-  b = uniform_address(b);
+  const int wm = wave % Cfg::WAVES_M, wn = wave / Cfg::WAVES_M;
+  using LA = grouped_loader<Cfg::E, Cfg::A_KC, BM, RB, NT>;
+  using LB = grouped_loader<Cfg::E, Cfg::B_KC, BN, RB, NT>;
+  // rounds of loads that B's columns need
+  constexpr int UB = LB::LINES ? LB::U : (TN * 16 * Cfg::WAVES_N * RB / 16 + NT - 1) / NT;
+  const char *a = w.a, *b = w.b;
   const uint64_t a_step = (Cfg::A_KC ? (uint64_t)BK : (uint64_t)BK * args.lda) * T::BYTES;
   const uint64_t b_step = (Cfg::B_KC ? (uint64_t)BK : (uint64_t)BK * args.ldb) * T::BYTES;
 
@@ -436,8 +433,7 @@ void grouped_kernel(const GroupedArgs args) {
     constexpr bool KC = decltype(kc_tag)::value;
     constexpr int ROWS = decltype(rows_tag)::value;
     if constexpr (KC || T::F32) {
-      return *reinterpret_cast<const u4_t *>(op + p * ROWS * T::ROW_BYTES +
-                                             chunk_offset<T::ROW_BYTES>(row0 + frow, slice * 4 + fg));
+      return *reinterpret_cast<const u4_t *>(op + p * ROWS * RB + chunk_offset<RB>(row0 + frow, slice * 4 + fg));
     } else {
       typedef short s4_t __attribute__((ext_vector_type(4)));
       typedef __attribute__((address_space(3))) s4_t *tr_t;
@@ -451,37 +447,43 @@ void grouped_kernel(const GroupedArgs args) {
       return u4_t{x[0], x[1], y[0], y[1]};
     }
   };
-  // A step's MFMAs, row block after row block of every slice; the fragments of the next row blocks (AHEAD_A of them) and of the
-  // next slice's columns are on their way meanwhile.  `beside(g)`:
-  // what else is done beside row block g.
-  constexpr int BLOCKS = T::SLICES * TM;
-  auto multiply = [&](const char *stage, auto beside) {
-    const char *sa = stage, *sb = stage + Cfg::A_STAGE;
-    constexpr int AHEAD_A = T::F32 ? 1 : 2; // (FP32: a block is three or six times as many MFMAs)
-    u4_t fa[AHEAD_A + 1][T::NP], fb[T::SLICES][T::NP][TN];
-    auto read_a = [&](const int g) {
+  // A step's MFMAs go row block after row block of every slice.  The fragments of the row blocks to come and of the
+  // next slice's columns are on their way meanwhile: AHEAD_A row blocks (FP32, whose blocks are three or six times as
+  // many MFMAs: one) in a ring of four, columns in two sets.
+  constexpr int BLOCKS = SLICES * TM, AHEAD_A = T::F32 ? 1 : 2, RING = T::F32 ? 2 : 4;
+  static_assert(BLOCKS % RING == 0, "a step begins where the ring does");
+  u4_t fa[RING][T::NP], fb[2][T::NP][TN];
+  auto read_a = [&](const char *stage, const int g) {
 #pragma unroll
-      for (int p = 0; p < T::NP; p++)
-        fa[g % (AHEAD_A + 1)][p] = frag(sa, wm * Cfg::WM + (g % TM) * 16, p, g / TM, std::integral_constant<bool, Cfg::A_KC>{},
-                                        std::integral_constant<int, BM>{});
-    };
-    auto read_b = [&](const int s) {
+    for (int p = 0; p < T::NP; p++)
+      fa[g % RING][p] = frag(stage, wm * Cfg::WM + (g % TM) * 16, p, g / TM, std::integral_constant<bool, Cfg::A_KC>{},
+                             std::integral_constant<int, BM>{});
+  };
+  auto read_b = [&](const char *stage, const int s, const int set) { // (set: of fragments)
 #pragma unroll
-      for (int p = 0; p < T::NP; p++)
+    for (int p = 0; p < T::NP; p++)
 #pragma unroll
-        for (int j = 0; j < TN; j++)
-          fb[s][p][j] = frag(sb, wn * Cfg::WN + j * 16, p, s, std::integral_constant<bool, Cfg::B_KC>{},
+      for (int j = 0; j < TN; j++)
+        fb[set][p][j] = frag(stage + Cfg::A_STAGE, (j * Cfg::WAVES_N + wn) * 16, p, s, std::integral_constant<bool, Cfg::B_KC>{},
                              std::integral_constant<int, BN>{});
-    };
-    read_a(0);
-    read_b(0);
-    if (AHEAD_A > 1 && BLOCKS > 1) read_a(1);
+  };
+  // the fragments that a step's first MFMAs need
+  auto begin = [&](const char *stage) {
+    read_a(stage, 0);
+    read_b(stage, 0, 0);
+    if (AHEAD_A > 1) read_a(stage, 1);
+  };
+  // Row blocks `from` .. `to` - 1 of a step; `beside(g)`: what else is done beside block g.  next: the next step's
+  // buffer, if its first fragments are to be read beside the last blocks (it is complete by then).
+  auto multiply = [&](const char *stage, const char *next, auto from, auto to, auto beside) {
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int g = 0; g < BLOCKS; g++) {
+    for (int g = from.value; g < to.value; g++) {
       const int s = g / TM, i = g % TM;
-      if (g + AHEAD_A < BLOCKS) read_a(g + AHEAD_A);
-      if (i == (TM > 1 ? TM - 2 : 0) && s + 1 < T::SLICES) read_b(s + 1);
+      if (g + AHEAD_A < BLOCKS) read_a(stage, g + AHEAD_A);
+      else if (next != nullptr) read_a(next, g + AHEAD_A - BLOCKS);
+      if (i == (TM > 4 ? TM - 3 : TM > 1 ? TM - 2 : 0) && s + 1 < SLICES) read_b(stage, s + 1, (s + 1) % 2);
+      if (g == BLOCKS - AHEAD_A && next != nullptr) read_b(next, 0, 0);
       beside(g);
 #pragma unroll
       for (int q = 0; q < T::NPROD; q++) {
@@ -489,154 +491,243 @@ void grouped_kernel(const GroupedArgs args) {
         const int ac = T::F32 ? prec_traits<T::P>::ACC[q] : 0;
 #pragma unroll
         for (int j = 0; j < TN; j++)
-          acc[ac][j][i] = grouped_mfma<Cfg::E>(fa[g % (AHEAD_A + 1)][pa], fb[s][pb][j], acc[ac][j][i]);
+          acc[ac][j][i] = grouped_mfma<Cfg::E>(fa[g % RING][pa], fb[s % 2][pb][j], acc[ac][j][i]);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
   };
   auto nothing = [](int) {};
+  constexpr std::integral_constant<int, 0> first;
+  constexpr std::integral_constant<int, BLOCKS> end;
 
   // ---- K loop ----
   // A K that ends inside a step has that step multiplied first, so that the loop has whole steps only: step s begins
   // at K-value (s - partial) BK, the partial one behind them all.
-  const int whole = (int)(klen / BK), left = (int)(klen % BK), partial = left != 0, steps = whole + partial;
-  auto a_at = [&](int s) { return a + (uint64_t)(partial && s == 0 ? whole : s - partial) * a_step; };
-  auto b_at = [&](int s) { return b + (uint64_t)(partial && s == 0 ? whole : s - partial) * b_step; };
-  uint32_t offa[LA::U], offb[LB::U];
+  const int whole = (int)(w.klen / BK), left = (int)(w.klen % BK), partial = left != 0, steps = whole + partial;
+  auto a_at = [&](int s) { return a + (uint64_t)(s < partial ? whole : s - partial) * a_step; };
+  auto b_at = [&](int s) { return b + (uint64_t)(s < partial ? whole : s - partial) * b_step; };
+  typedef typename std::conditional<Cfg::DIRECT, uint32_t, uint64_t>::type off_t;
+  off_t offa[LA::U], offb[UB];
 #pragma unroll
-  for (int u = 0; u < LA::U; u++) offa[u] = (uint32_t)LA::offset(tid + u * NT, args.lda, rows_a);
+  for (int u = 0; u < LA::U; u++) offa[u] = (off_t)LA::offset(tid + u * NT, args.lda, w.rows_a);
 #pragma unroll
-  for (int u = 0; u < LB::U; u++) offb[u] = (uint32_t)LB::offset(tid + u * NT, args.ldb, rows_b);
-  constexpr int LOADS = LA::U + LB::U;
-  // which of a step's loads (A's, then B's) are issued beside row block g
-  auto share = [](int g, auto f) {
-#pragma unroll
-    for (int l = 0; l < LOADS; l++)
-      if (l * BLOCKS / LOADS == g) f(l);
-  };
+  for (int u = 0; u < UB; u++) offb[u] = (off_t)LB::offset(tid + u * NT, args.ldb, w.rows_b);
+  constexpr int LOADS = LA::U + UB;
   if constexpr (Cfg::DIRECT && !T::F32) {
-    // NSTAGE - 1 steps ahead; a buffer is filled again once all waves have read it, i.e. behind the barrier of the
-    // step after
-    constexpr int AHEAD = Cfg::NSTAGE - 1;
+    // One barrier a step, in front of its last AHEAD_A row blocks, whose fragments every wave has in registers by then.
+    // Behind it the step's buffer is free, and the loads of step s + NSTAGE go there; and the next step's buffer is
+    // complete, so that its first fragments are read beside the last MFMAs of this one.
+    static_assert(SLICES == 2, "the two sets of column fragments");
+    constexpr std::integral_constant<int, BLOCKS - AHEAD_A> last;
     const uint32_t lds0 = lds_address(lds);
     auto issue = [&](int l, const char *pa, const char *pb, uint32_t stage) {
       if (l < LA::U) LA::direct(l, pa, offa[l], stage, wave);
       else LB::direct(l - LA::U, pb, offb[l - LA::U], stage + Cfg::A_STAGE, wave);
     };
-    for (int s = 0; s < AHEAD && s < steps; s++) {
+    for (int s = 0; s < Cfg::NSTAGE && s < steps; s++) {
       const uint32_t stage = lds0 + s * Cfg::STAGE;
       const char *pa = a_at(s), *pb = b_at(s);
-      if (partial && s == 0) {
+      if (s < partial) {
 #pragma unroll
         for (int u = 0; u < LA::U; u++) LA::direct_tail(u, pa, offa[u], stage, tid, wave, left);
 #pragma unroll
-        for (int u = 0; u < LB::U; u++) LB::direct_tail(u, pb, offb[u], stage + Cfg::A_STAGE, tid, wave, left);
+        for (int u = 0; u < UB; u++) LB::direct_tail(u, pb, offb[u], stage + Cfg::A_STAGE, tid, wave, left);
       } else {
 #pragma unroll
         for (int l = 0; l < LOADS; l++) issue(l, pa, pb, stage);
       }
     }
-    int at = 0; // buffer of step s
-    for (int s = 0; s < steps - AHEAD; s++) {
-      // everything but the loads of the AHEAD - 1 steps after this one has landed
-      __builtin_amdgcn_s_waitcnt(waitcnt_vm(LOADS * (AHEAD - 1)));
+    if (steps > 0) {
+      if (steps >= Cfg::NSTAGE) __builtin_amdgcn_s_waitcnt(waitcnt_vm(LOADS * (Cfg::NSTAGE - 1)));
+      else __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
       block_sync_lds();
-      const int next = at == 0 ? Cfg::NSTAGE - 1 : at - 1; // of step s + AHEAD
-      const char *pa = a_at(s + AHEAD), *pb = b_at(s + AHEAD);
-      const uint32_t stage = lds0 + next * Cfg::STAGE;
-      multiply(lds + at * Cfg::STAGE, [&](int g) { share(g, [&](int l) { issue(l, pa, pb, stage); }); });
-      at = at + 1 == Cfg::NSTAGE ? 0 : at + 1;
+      begin(lds);
     }
-    for (int s = steps > AHEAD ? steps - AHEAD : 0; s < steps; s++) {
-      __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+    int at = 0; // buffer of step s
+    for (int s = 0; s < steps; s++) {
+      const int next = at + 1 == Cfg::NSTAGE ? 0 : at + 1;
+      const char *here = lds + at * Cfg::STAGE;
+      multiply(here, nullptr, first, last, nothing);
+      // everything but the loads of the steps behind the next one has landed (at the end none are left out of the wait)
+      if (s + Cfg::NSTAGE <= steps) __builtin_amdgcn_s_waitcnt(waitcnt_vm(LOADS * (Cfg::NSTAGE - 2)));
+      else __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
       block_sync_lds();
-      multiply(lds + at * Cfg::STAGE, nothing);
-      at = at + 1 == Cfg::NSTAGE ? 0 : at + 1;
+      const char *pa = a_at(s + Cfg::NSTAGE), *pb = b_at(s + Cfg::NSTAGE);
+      const uint32_t stage = lds0 + at * Cfg::STAGE;
+      const bool more = s + Cfg::NSTAGE < steps;
+      // (behind the last step, unused values are read)
+      multiply(here, lds + next * Cfg::STAGE, last, end, [&](int g) {
+        if (more) {
+#pragma unroll
+          for (int l = 0; l < LOADS; l++)
+            if (l * AHEAD_A / LOADS == g - last.value) issue(l, pa, pb, stage);
+        }
+      });
+      at = next;
     }
   } else {
     // through registers: step s + 1 is written to LDS and step s + 2 asked for beside the MFMAs of step s
     static_assert(Cfg::NSTAGE == 2 || (Cfg::DIRECT && !T::F32), "two buffers");
+    // which of a step's units (A's, then B's) come beside row block g
+    auto share = [](int g, auto f) {
+#pragma unroll
+      for (int l = 0; l < LOADS; l++)
+        if (l * BLOCKS / LOADS == g) f(l);
+    };
     typename LA::Regs ra;
     typename LB::Regs rb;
     auto put = [&](int l, char *stage) {
       if (l < LA::U) LA::put(ra, l, stage, tid);
       else LB::put(rb, l - LA::U, stage + Cfg::A_STAGE, tid);
     };
-    auto fetch = [&](int l, const char *pa, const char *pb) {
-      if (l < LA::U) LA::template fetch<Cfg::DIRECT>(ra, l, pa, args.lda, offa[l], rows_a, tid);
-      else LB::template fetch<Cfg::DIRECT>(rb, l - LA::U, pb, args.ldb, offb[l - LA::U], rows_b, tid);
+    auto fetch = [&](int l, const char *pa, const char *pb, int64_t k0) { // (k0: the step's first K-value)
+      if (l < LA::U) LA::template fetch<Cfg::DIRECT>(ra, l, pa, args.lda, offa[l], w.rows_a, Cfg::A_KC ? w.safe_a : w.safe_a - k0, tid);
+      else LB::template fetch<Cfg::DIRECT>(rb, l - LA::U, pb, args.ldb, offb[l - LA::U], w.rows_b, Cfg::B_KC ? w.safe_b : w.safe_b - k0, tid);
     };
     if (steps > 0) {
       const char *pa = a_at(0), *pb = b_at(0);
       if (partial) {
 #pragma unroll
-        for (int u = 0; u < LA::U; u++) LA::fetch_tail(ra, u, pa, args.lda, rows_a, left, tid);
+        for (int u = 0; u < LA::U; u++) LA::fetch_tail(ra, u, pa, args.lda, w.rows_a, left, Cfg::A_KC ? w.safe_a : w.safe_a - whole * BK, tid);
 #pragma unroll
-        for (int u = 0; u < LB::U; u++) LB::fetch_tail(rb, u, pb, args.ldb, rows_b, left, tid);
+        for (int u = 0; u < UB; u++) LB::fetch_tail(rb, u, pb, args.ldb, w.rows_b, left, Cfg::B_KC ? w.safe_b : w.safe_b - whole * BK, tid);
       } else {
 #pragma unroll
-        for (int l = 0; l < LOADS; l++) fetch(l, pa, pb);
+        for (int l = 0; l < LOADS; l++) fetch(l, pa, pb, 0);
       }
 #pragma unroll
       for (int l = 0; l < LOADS; l++) put(l, lds);
       if (steps > 1) {
         pa = a_at(1), pb = b_at(1);
 #pragma unroll
-        for (int l = 0; l < LOADS; l++) fetch(l, pa, pb);
+        for (int l = 0; l < LOADS; l++) fetch(l, pa, pb, (int64_t)(1 - partial) * BK);
       }
       block_sync_lds();
     }
     for (int s = 0; s < steps - 1; s++) {
       const int ask = s + 2 < steps ? s + 2 : s + 1; // (the last time: the same step again, unused)
       const char *pa = a_at(ask), *pb = b_at(ask);
+      const char *here = lds + (s & 1) * Cfg::STAGE;
       char *stage = lds + ((s + 1) & 1) * Cfg::STAGE;
-      multiply(lds + (s & 1) * Cfg::STAGE, [&](int g) {
+      begin(here);
+      multiply(here, nullptr, first, end, [&](int g) {
         share(g, [&](int l) {
           put(l, stage);
-          fetch(l, pa, pb);
+          fetch(l, pa, pb, (int64_t)(ask - partial) * BK);
         });
       });
       block_sync_lds();
     }
-    if (steps > 0) multiply(lds + ((steps - 1) & 1) * Cfg::STAGE, nothing);
+    if (steps > 0) {
+      const char *here = lds + ((steps - 1) & 1) * Cfg::STAGE;
+      begin(here);
+      multiply(here, nullptr, first, end, nothing);
+    }
   }
 
   // ---- results ----
-  // Register v of lane l: MFMA row 4 (l / 16) + v (of C), column l % 16 (token).
-  auto write = [&](auto out_tag) {
-    constexpr uint32_t OUT = decltype(out_tag)::value;
-    constexpr uint64_t OB = sizeof(typename out_type<OUT>::type);
+  // Register v of lane l: MFMA row 4 (l / 16) + v (of C), column l % 16 (token).  One column block after the other passes
+  // through LDS, each wave's through a part of its own, so that a wave's store covers the columns' whole WM rows.
+  block_sync_lds(); // (every wave has read its last fragments)
+  constexpr int PITCH = Cfg::PITCH;
+  float *mine = reinterpret_cast<float *>(lds) + wave * (16 * PITCH);
+  const uint32_t row0 = w.m0 + wm * Cfg::WM;
 #pragma unroll
-    for (int j = 0; j < TN; j++) {
-      const uint32_t col = n0 + wn * Cfg::WN + j * 16 + frow;
-      if (col >= n_end) continue;
-      float sb = 1.0f;
-      if constexpr (T::I8) sb = args.scale_b[col];
+  for (int j = 0; j < TN; j++) {
 #pragma unroll
-      for (int i = 0; i < TM; i++) {
-        const uint32_t row = m0 + wm * Cfg::WM + i * 16 + fg * 4;
-        f4v_t x;
+    for (int i = 0; i < TM; i++) {
+      f4v_t x;
 #pragma unroll
-        for (int v = 0; v < 4; v++) {
-          if constexpr (T::I8) {
-            const uint32_t r = row + v < args.m ? row + v : args.m - 1;
-            x[v] = (float)acc[0][j][i][v] * args.scale_a[(uint64_t)t.group * args.m + r] * sb;
-          } else {
-            x[v] = acc[0][j][i][v];
-            if constexpr (T::NACC == 2) x[v] += acc[1][j][i][v] * prec_traits<T::P>::CORR_SCALE;
-            x[v] *= args.alpha;
-          }
-        }
-        store_four<OUT>(c + ((uint64_t)col * args.ldc + row) * OB, x, args.beta, row, args.m, args.vec_c != 0);
+      for (int v = 0; v < 4; v++) {
+        x[v] = (float)acc[0][j][i][v];
+        if constexpr (T::NACC == 2) x[v] += acc[1][j][i][v] * prec_traits<T::P>::CORR_SCALE;
       }
+      *reinterpret_cast<f4v_t *>(mine + frow * PITCH + i * 16 + fg * 4) = x;
     }
-  };
-  if constexpr (T::F32) {
-    write(std::integral_constant<uint32_t, OUT_F32>{});
+    // (a wave's own writes and reads of LDS are carried out in order)
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    constexpr int LANES = Cfg::WM / 4, COLS = 64 / LANES; // lanes of a column, columns of a round
+    const uint32_t row = row0 + (lane % LANES) * 4, col0 = w.n0 + (j * Cfg::WAVES_N + wn) * 16;
+    f4v_t sa = {args.alpha, args.alpha, args.alpha, args.alpha};
+    if constexpr (T::I8) {
+#pragma unroll
+      for (int v = 0; v < 4; v++)
+        sa[v] = args.scale_a[(uint64_t)w.group * args.m + (row + v < args.m ? row + v : args.m - 1)];
+    }
+#pragma unroll 1
+    for (int r = 0; r < 16; r += COLS) {
+      const uint32_t col = col0 + r + lane / LANES;
+      if (col >= w.n_end) continue;
+      f4v_t x = *reinterpret_cast<const f4v_t *>(mine + (r + lane / LANES) * PITCH + (lane % LANES) * 4);
+      const float sb = T::I8 ? args.scale_b[col] : 1.0f;
+#pragma unroll
+      for (int v = 0; v < 4; v++) x[v] = T::I8 ? x[v] * sa[v] * sb : x[v] * sa[v];
+      const uint64_t at = (uint64_t)col * args.ldc + row;
+      if (T::F32 || args.out == OUT_F32) store_four<OUT_F32>(w.c + at * 4, x, args.beta, row, args.m, args.vec_c != 0);
+      else if (Cfg::E == Elem::F16 || (T::I8 && args.out == OUT_F16))
+        store_four<OUT_F16>(w.c + at * 2, x, args.beta, row, args.m, args.vec_c != 0);
+      else store_four<OUT_BF16>(w.c + at * 2, x, args.beta, row, args.m, args.vec_c != 0);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+  }
+}
+
+template <class Cfg>
+__global__ __launch_bounds__(Cfg::NT) __attribute__((amdgpu_waves_per_eu(Cfg::OCC, Cfg::OCC)))
+void grouped_kernel(const GroupedArgs args) {
+  using T = typename Cfg::T;
+  constexpr int BM = Cfg::BM, BN = Cfg::BN, TN = Cfg::TN;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const uint32_t tiles_m = (args.m + BM - 1) / BM;
+  TilePlace t;
+  TileWork w;
+  const char *a = args.a, *b = args.b;
+  w.c = args.c;
+  if constexpr (Cfg::RAGGED_K) {
+    const uint32_t tiles_n = (args.n + BN - 1) / BN, per = tiles_m * tiles_n;
+    const uint32_t id = xcd_range(blockIdx.x, per * args.groups);
+    t.group = id / per;
+    raster(id % per, tiles_m, tiles_n, t.tm, t.tn);
+    group_span(args.offsets, t.group, args.k, t.lo, t.hi);
+    t.lo = __builtin_amdgcn_readfirstlane(t.lo);
+    t.hi = __builtin_amdgcn_readfirstlane(t.hi);
+    w.n0 = t.tn * BN;
+    w.n_end = args.n;
+    w.klen = t.hi - t.lo;
+    a += (uint64_t)t.lo * args.lda * T::BYTES;
+    b += (uint64_t)t.lo * args.ldb * T::BYTES;
+    w.c += (uint64_t)t.group * args.stride_c * (args.out == OUT_F32 ? 4 : 2);
   } else {
-    if (args.out == OUT_F32) write(std::integral_constant<uint32_t, OUT_F32>{});
-    else if (Cfg::E == Elem::F16 || (T::I8 && args.out == OUT_F16)) write(std::integral_constant<uint32_t, OUT_F16>{});
-    else write(std::integral_constant<uint32_t, OUT_BF16>{});
+    if (!place_tile(args, blockIdx.x, tiles_m, BN, t)) return;
+    w.n0 = t.lo + t.tn * BN;
+    w.n_end = t.hi;
+    w.klen = args.k;
+    a += (uint64_t)t.group * args.stride_a * T::BYTES;
+  }
+  w.group = t.group;
+  w.m0 = t.tm * BM;
+  w.rows_a = (int)(args.m - w.m0 < (uint32_t)BM ? args.m - w.m0 : BM);
+  w.rows_b = (int)(w.n_end - w.n0 < (uint32_t)BN ? w.n_end - w.n0 : BN);
+  w.a = uniform_address(a + (Cfg::A_KC ? (uint64_t)w.m0 * args.lda : (uint64_t)w.m0) * T::BYTES);
+  w.b = uniform_address(b + (Cfg::B_KC ? (uint64_t)w.n0 * args.ldb : (uint64_t)w.n0) * T::BYTES);
+  // (what a chunk of 8 or 16 values can stick out by is less than a line that long)
+  auto safe = [&](bool kc, uint64_t ld, uint64_t extent, int64_t rows, int64_t lines) -> int64_t {
+    return extent < (uint64_t)T::CHUNK || ld < (uint64_t)T::CHUNK ? 0 : kc ? rows - 1 : lines - 1;
+  };
+  const int64_t lines = Cfg::RAGGED_K ? (int64_t)args.k - t.lo : (int64_t)args.k;
+  w.safe_a = safe(Cfg::A_KC, args.lda, Cfg::A_KC ? args.k : args.m, (int64_t)args.m - w.m0, lines);
+  w.safe_b = safe(Cfg::B_KC, args.ldb, Cfg::B_KC ? args.k : args.n, (int64_t)args.n - w.n0, lines);
+  if constexpr (Cfg::RAGGED_K) {
+    multiply_tile<Cfg, TN>(args, w, lds);
+  } else {
+    static_assert(TN == 2 || TN == 4, "column blocks of a wave");
+    const int blocks = (w.rows_b + 16 * Cfg::WAVES_N - 1) / (16 * Cfg::WAVES_N);
+    if (blocks >= TN) multiply_tile<Cfg, TN>(args, w, lds);
+    else if (blocks == 1) multiply_tile<Cfg, 1>(args, w, lds);
+    else if constexpr (TN == 4) {
+      if (blocks == 2) multiply_tile<Cfg, 2>(args, w, lds);
+      else multiply_tile<Cfg, 3>(args, w, lds);
+    }
   }
 }
 

@@ -10,49 +10,49 @@ struct GroupedTable {
   GroupedKernel over_k[2][kGroupedClasses]; // ragged K, both row-contiguous
 };
 
-template <Elem E, bool A_KC, bool B_KC, int BM, int BN, int WM, int WN, int NSTAGE, bool DIRECT, bool RAGGED_K>
+template <Elem E, bool A_KC, bool B_KC, int BM, int BN, int WM, int WN, int ROW_BYTES, int NSTAGE, bool DIRECT, bool RAGGED_K>
 constexpr GroupedKernel grouped_of() {
-  return grouped_entry<GroupedCfg<E, A_KC, B_KC, BM, BN, WM, WN, NSTAGE, DIRECT, RAGGED_K, 2>>();
+  return grouped_entry<GroupedCfg<E, A_KC, B_KC, BM, BN, WM, WN, ROW_BYTES, NSTAGE, DIRECT, RAGGED_K, 2>>();
 }
 
 template <Elem E> constexpr GroupedTable grouped_table_f32() {
   GroupedTable t{};
-  t.columns[0][0][TILE_128] = grouped_of<E, false, true, 128, 128, 64, 32, 2, false, false>();
-  t.columns[1][0][TILE_128] = grouped_of<E, true, true, 128, 128, 64, 32, 2, false, false>();
-  t.columns[0][1][TILE_256] = grouped_of<E, false, true, 256, 128, 64, 64, 2, true, false>();
-  t.columns[0][1][TILE_128] = grouped_of<E, false, true, 128, 128, 64, 32, 2, true, false>();
-  t.columns[0][1][TILE_NARROW] = grouped_of<E, false, true, 128, 32, 32, 32, 2, true, false>();
-  t.columns[1][1][TILE_256] = grouped_of<E, true, true, 256, 128, 64, 64, 2, true, false>();
-  t.columns[1][1][TILE_128] = grouped_of<E, true, true, 128, 128, 64, 32, 2, true, false>();
-  t.columns[1][1][TILE_NARROW] = grouped_of<E, true, true, 128, 32, 32, 32, 2, true, false>();
-  t.over_k[0][TILE_128] = grouped_of<E, false, false, 128, 128, 64, 32, 2, false, true>();
-  t.over_k[1][TILE_256] = grouped_of<E, false, false, 256, 128, 64, 64, 2, true, true>();
-  t.over_k[1][TILE_128] = grouped_of<E, false, false, 128, 128, 64, 32, 2, true, true>();
+  t.columns[0][0][TILE_128] = grouped_of<E, false, true, 128, 128, 64, 32, 64, 2, false, false>();
+  t.columns[1][0][TILE_128] = grouped_of<E, true, true, 128, 128, 64, 32, 64, 2, false, false>();
+  t.columns[0][1][TILE_256] = grouped_of<E, false, true, 256, 128, 64, 64, 64, 2, true, false>();
+  t.columns[0][1][TILE_128] = grouped_of<E, false, true, 128, 128, 64, 32, 64, 2, true, false>();
+  t.columns[0][1][TILE_NARROW] = grouped_of<E, false, true, 128, 32, 32, 32, 64, 2, true, false>();
+  t.columns[1][1][TILE_256] = grouped_of<E, true, true, 256, 128, 64, 64, 64, 2, true, false>();
+  t.columns[1][1][TILE_128] = grouped_of<E, true, true, 128, 128, 64, 32, 64, 2, true, false>();
+  t.columns[1][1][TILE_NARROW] = grouped_of<E, true, true, 128, 32, 32, 32, 64, 2, true, false>();
+  t.over_k[0][TILE_128] = grouped_of<E, false, false, 128, 128, 64, 32, 64, 2, false, true>();
+  t.over_k[1][TILE_256] = grouped_of<E, false, false, 256, 128, 64, 64, 64, 2, true, true>();
+  t.over_k[1][TILE_128] = grouped_of<E, false, false, 128, 128, 64, 32, 64, 2, true, true>();
   return t;
 }
 
 template <Elem E> constexpr GroupedTable grouped_table_16() {
   GroupedTable t{};
-  t.columns[0][0][TILE_128] = grouped_of<E, false, true, 128, 128, 64, 64, 2, false, false>();
-  t.columns[1][0][TILE_128] = grouped_of<E, true, true, 128, 128, 64, 64, 2, false, false>();
-  t.columns[0][1][TILE_256] = grouped_of<E, false, true, 256, 256, 128, 64, 2, true, false>();
-  t.columns[0][1][TILE_128] = grouped_of<E, false, true, 128, 128, 64, 64, 2, true, false>();
-  t.columns[0][1][TILE_NARROW] = grouped_of<E, false, true, 128, 32, 32, 32, 4, true, false>();
-  t.columns[1][1][TILE_256] = grouped_of<E, true, true, 256, 256, 128, 64, 2, true, false>();
-  t.columns[1][1][TILE_128] = grouped_of<E, true, true, 128, 128, 64, 64, 2, true, false>();
-  t.columns[1][1][TILE_NARROW] = grouped_of<E, true, true, 128, 32, 32, 32, 4, true, false>();
-  t.over_k[0][TILE_128] = grouped_of<E, false, false, 128, 128, 64, 64, 2, false, true>();
-  t.over_k[1][TILE_256] = grouped_of<E, false, false, 256, 256, 128, 64, 2, true, true>();
-  t.over_k[1][TILE_128] = grouped_of<E, false, false, 128, 128, 64, 64, 2, true, true>();
+  t.columns[0][0][TILE_128] = grouped_of<E, false, true, 128, 128, 64, 64, 128, 2, false, false>();
+  t.columns[1][0][TILE_128] = grouped_of<E, true, true, 128, 128, 64, 64, 128, 2, false, false>();
+  t.columns[0][1][TILE_256] = grouped_of<E, false, true, 256, 256, 128, 64, 128, 2, true, false>();
+  t.columns[0][1][TILE_128] = grouped_of<E, false, true, 128, 128, 64, 64, 128, 2, true, false>();
+  t.columns[0][1][TILE_NARROW] = grouped_of<E, false, true, 128, 32, 32, 32, 128, 4, true, false>();
+  t.columns[1][1][TILE_256] = grouped_of<E, true, true, 256, 256, 128, 64, 128, 2, true, false>();
+  t.columns[1][1][TILE_128] = grouped_of<E, true, true, 128, 128, 64, 64, 128, 2, true, false>();
+  t.columns[1][1][TILE_NARROW] = grouped_of<E, true, true, 128, 32, 32, 32, 128, 4, true, false>();
+  t.over_k[0][TILE_128] = grouped_of<E, false, false, 128, 128, 64, 64, 128, 2, false, true>();
+  t.over_k[1][TILE_256] = grouped_of<E, false, false, 256, 256, 128, 64, 128, 2, true, true>();
+  t.over_k[1][TILE_128] = grouped_of<E, false, false, 128, 128, 64, 64, 128, 2, true, true>();
   return t;
 }
 
 template <Elem E> constexpr GroupedTable grouped_table_i8() {
   GroupedTable t{};
-  t.columns[1][0][TILE_128] = grouped_of<E, true, true, 128, 128, 64, 64, 2, false, false>();
-  t.columns[1][1][TILE_256] = grouped_of<E, true, true, 256, 256, 128, 64, 2, true, false>();
-  t.columns[1][1][TILE_128] = grouped_of<E, true, true, 128, 128, 64, 64, 2, true, false>();
-  t.columns[1][1][TILE_NARROW] = grouped_of<E, true, true, 128, 32, 32, 32, 4, true, false>();
+  t.columns[1][0][TILE_128] = grouped_of<E, true, true, 128, 128, 64, 64, 128, 2, false, false>();
+  t.columns[1][1][TILE_256] = grouped_of<E, true, true, 256, 256, 128, 64, 128, 2, true, false>();
+  t.columns[1][1][TILE_128] = grouped_of<E, true, true, 128, 128, 64, 64, 128, 2, true, false>();
+  t.columns[1][1][TILE_NARROW] = grouped_of<E, true, true, 128, 32, 32, 32, 128, 4, true, false>();
   return t;
 }
 
