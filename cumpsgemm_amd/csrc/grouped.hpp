@@ -39,14 +39,8 @@ struct GroupedKernel {
   int bm, bn;
 };
 
-// Tiles of the tiled kernels, from the largest.
-enum TileClass : int { TILE_256 = 0, TILE_128 = 1, TILE_NARROW = 2, kGroupedClasses = 3 };
-
-// Which of the two ways an operand comes into LDS (grouped_kernel.hpp): straight from memory (16-bit and 8-bit
-// elements in rows of whole, aligned 16-byte chunks), or through registers (anything).
-const GroupedKernel *lookup_grouped(Elem e, bool a_kc, bool ragged_k, bool direct, int cls);
-
-// The kernels of few tokens to a group (grouped_stream.hpp).
-const GroupedKernel *lookup_grouped_stream(Elem e, bool a_kc, bool aligned);
+// Kernels of ragged columns: three tiles of the tiled kernel, from the largest, and the kernel of few tokens to a group
+// (grouped_stream.hpp), with 16 or 64 rows to a workgroup (row-contiguous matrices: 64).
+enum KernelClass : int { TILE_256 = 0, TILE_128 = 1, TILE_NARROW = 2, kGroupedClasses = 3, STREAM_16 = 3, STREAM_64 = 4, kKernelClasses = 5 };
 
 } // namespace cumpsgemm_amd

@@ -8,12 +8,14 @@ namespace cumpsgemm_amd {
 extern GroupedTable g_grouped_f32_fp16tcec, g_grouped_f32_fp16tc, g_grouped_f32_bf16x3, g_grouped_f32_bf16x2,
     g_grouped_f16, g_grouped_bf16, g_grouped_i8;
 
+// direct: the operands can take the shorter way into LDS (grouped_kernel.hpp); the kernel of few tokens takes any
 const GroupedKernel *lookup_grouped(Elem e, bool a_kc, bool ragged_k, bool direct, int cls) {
   static const GroupedTable *const tables[kNumElems] = {&g_grouped_f32_fp16tcec, &g_grouped_f32_fp16tc, &g_grouped_f32_bf16x3,
                                                         &g_grouped_f32_bf16x2, &g_grouped_f16, &g_grouped_bf16, &g_grouped_i8};
   const GroupedTable &t = *tables[(int)e];
-  const GroupedKernel *k = ragged_k ? &t.over_k[direct][cls] : &t.columns[a_kc][direct][cls];
-  return k->launch != nullptr ? k : nullptr;
+  const GroupedKernel *k = ragged_k ? (cls >= STREAM_16 ? nullptr : &t.over_k[direct][cls])
+                           : cls >= STREAM_16 ? &t.stream[a_kc][cls - STREAM_16] : &t.columns[a_kc][direct][cls];
+  return k != nullptr && k->launch != nullptr ? k : nullptr;
 }
 
 namespace {
@@ -58,10 +60,10 @@ hipblasStatus_t launched() {
   return hipGetLastError() == hipSuccess ? HIPBLAS_STATUS_SUCCESS : HIPBLAS_STATUS_EXECUTION_FAILED;
 }
 
-// CUMPSGEMM_FORCE_TILE_CLASS (0 - 2) goes before the rules; where there is no such kernel, the 128 x 128 one serves.
+// CUMPSGEMM_FORCE_TILE_CLASS (0 - 4) goes before the rules; where there is no such kernel, the 128 x 128 one serves.
 const GroupedKernel *choose(Elem e, bool a_kc, bool ragged_k, bool direct, int cls) {
   const int forced = tuning().force_cls;
-  const GroupedKernel *k = lookup_grouped(e, a_kc, ragged_k, direct, forced >= 0 && forced < kGroupedClasses ? forced : cls);
+  const GroupedKernel *k = lookup_grouped(e, a_kc, ragged_k, direct, forced >= 0 && forced < kKernelClasses ? forced : cls);
   return k != nullptr ? k : lookup_grouped(e, a_kc, ragged_k, direct, TILE_128);
 }
 
@@ -71,7 +73,7 @@ hipblasStatus_t run_columns(cuMpSGEMM_handle *h, Elem e, bool a_kc, GroupedArgs 
   const bool direct = chunks_ok(args.a, a_kc ? args.k : args.m, args.lda, args.stride_a, bytes, a_kc ? 256 : 64) &&
                       chunks_ok(args.b, args.k, args.ldb, 0, bytes, 256);
   const uint64_t each = args.n / args.groups; // tokens of a group, on average
-  int cls = each >= 192 ? TILE_256 : each >= 48 ? TILE_128 : TILE_NARROW;
+  int cls = each >= 192 ? TILE_256 : each >= 48 ? TILE_128 : each > 8 ? TILE_NARROW : STREAM_16;
   const GroupedKernel *k = choose(e, a_kc, false, direct, cls);
   if (k == nullptr) return HIPBLAS_STATUS_INTERNAL_ERROR;
   // no more tiles of columns than this: every group has one that is not full

@@ -341,7 +341,13 @@ template <Elem E, bool KC, int ROWS, int ROW_BYTES, int NT> struct grouped_loade
       int row, k;
       at(id, row, k);
       u4_t out[T::NP];
-      splitter<T::P>::run(r.v[u], out);
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        uint32_t terms[T::NP];
+        split_pair<T::P, false>(r.v[u][2 * q], r.v[u][2 * q + 1], 1.0f, 2048.0f, terms);
+#pragma unroll
+        for (int p = 0; p < T::NP; p++) out[p][q] = terms[p];
+      }
 #pragma unroll
       for (int p = 0; p < T::NP; p++)
         *reinterpret_cast<u4_t *>(lds_op + p * ROWS * ROW_BYTES + chunk_offset<ROW_BYTES>(row, k / T::CHUNK)) = out[p];
@@ -452,6 +458,10 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
   // many MFMAs: one) in a ring of four, columns in two sets.
   constexpr int BLOCKS = SLICES * TM, AHEAD_A = T::F32 ? 1 : 2, RING = T::F32 ? 2 : 4;
   static_assert(BLOCKS % RING == 0, "a step begins where the ring does");
+#ifndef GROUPED_VALU
+#define GROUPED_VALU 3
+#endif
+  constexpr int SCHED_VALU = GROUPED_VALU;
   u4_t fa[RING][T::NP], fb[2][T::NP][TN];
   auto read_a = [&](const char *stage, const int g) {
 #pragma unroll
@@ -493,6 +503,17 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
         for (int j = 0; j < TN; j++)
           acc[ac][j][i] = grouped_mfma<Cfg::E>(fa[g % RING][pa], fb[s % 2][pb][j], acc[ac][j][i]);
       }
+      if constexpr (T::F32) {
+        // the splitting between the MFMAs, not in front of them: both waves of a SIMD pass the barrier together
+#pragma unroll
+        for (int x = 0; x < T::NPROD * TN; x++) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); // MFMA
+          __builtin_amdgcn_sched_group_barrier(0x002, SCHED_VALU, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0); // LDS reads
+          __builtin_amdgcn_sched_group_barrier(0x200, 1, 0); // LDS writes
+          __builtin_amdgcn_sched_group_barrier(0x020, 1, 0); // loads
+        }
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -515,8 +536,8 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
   constexpr int LOADS = LA::U + UB;
   if constexpr (Cfg::DIRECT && !T::F32) {
     // One barrier a step, in front of its last AHEAD_A row blocks, whose fragments every wave has in registers by then.
-    // Behind it the step's buffer is free, and the loads of step s + NSTAGE go there; and the next step's buffer is
-    // complete, so that its first fragments are read beside the last MFMAs of this one.
+    // Behind it the step's buffer is free, and the loads of step s + NSTAGE begin to go there; and the next step's buffer
+    // is complete, so that its first fragments are read beside the last MFMAs of this one.
     static_assert(SLICES == 2, "the two sets of column fragments");
     constexpr std::integral_constant<int, BLOCKS - AHEAD_A> last;
     const uint32_t lds0 = lds_address(lds);
@@ -543,16 +564,29 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
       block_sync_lds();
       begin(lds);
     }
-    int at = 0; // buffer of step s
+    // A CU takes 16 clocks for each of these loads, as long as an MFMA, and a wave that asks for more waits with its
+    // MFMAs: they are spread over half a step, and land in the other half.
+    constexpr int SPREAD = BLOCKS / 2 > AHEAD_A ? BLOCKS / 2 : AHEAD_A;
+    int at = 0, before = 0; // buffers of steps s and s - 1
+    const char *qa = uniform_address(a_at(Cfg::NSTAGE)), *qb = uniform_address(b_at(Cfg::NSTAGE)); // of step s + NSTAGE
     for (int s = 0; s < steps; s++) {
       const int next = at + 1 == Cfg::NSTAGE ? 0 : at + 1;
       const char *here = lds + at * Cfg::STAGE;
-      multiply(here, nullptr, first, last, nothing);
+      // the rest of what was begun beside the last row blocks of the step before
+      const bool rest = s > 0 && s - 1 + Cfg::NSTAGE < steps;
+      const char *pa = qa - a_step, *pb = qb - b_step;
+      const uint32_t old_stage = lds0 + before * Cfg::STAGE;
+      multiply(here, nullptr, first, last, [&](int g) {
+        if (rest) {
+#pragma unroll
+          for (int l = 0; l < LOADS; l++)
+            if (l * SPREAD / LOADS == g + AHEAD_A) issue(l, pa, pb, old_stage);
+        }
+      });
       // everything but the loads of the steps behind the next one has landed (at the end none are left out of the wait)
       if (s + Cfg::NSTAGE <= steps) __builtin_amdgcn_s_waitcnt(waitcnt_vm(LOADS * (Cfg::NSTAGE - 2)));
       else __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
       block_sync_lds();
-      const char *pa = a_at(s + Cfg::NSTAGE), *pb = b_at(s + Cfg::NSTAGE);
       const uint32_t stage = lds0 + at * Cfg::STAGE;
       const bool more = s + Cfg::NSTAGE < steps;
       // (behind the last step, unused values are read)
@@ -560,9 +594,12 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
         if (more) {
 #pragma unroll
           for (int l = 0; l < LOADS; l++)
-            if (l * AHEAD_A / LOADS == g - last.value) issue(l, pa, pb, stage);
+            if (l * SPREAD / LOADS == g - last.value) issue(l, qa, qb, stage);
         }
       });
+      qa += a_step;
+      qb += b_step;
+      before = at;
       at = next;
     }
   } else {

@@ -1,6 +1,7 @@
 // Instances of the experts' products, one translation unit for each kind of operand (grouped_inst_*.hip).
 #pragma once
 #include "grouped_kernel.hpp"
+#include "grouped_stream.hpp"
 
 namespace cumpsgemm_amd {
 
@@ -8,11 +9,13 @@ struct GroupedTable {
   // [A K-contiguous][through registers, direct][tile]; B K-contiguous
   GroupedKernel columns[2][2][kGroupedClasses];
   GroupedKernel over_k[2][kGroupedClasses]; // ragged K, both row-contiguous
+  GroupedKernel stream[2][2];               // few tokens; [A K-contiguous][16 rows, 64 rows]
 };
 
-template <Elem E, bool A_KC, bool B_KC, int BM, int BN, int WM, int WN, int ROW_BYTES, int NSTAGE, bool DIRECT, bool RAGGED_K>
+template <Elem E, bool A_KC, bool B_KC, int BM, int BN, int WM, int WN, int ROW_BYTES, int NSTAGE, bool DIRECT, bool RAGGED_K,
+          int OCC = 2>
 constexpr GroupedKernel grouped_of() {
-  return grouped_entry<GroupedCfg<E, A_KC, B_KC, BM, BN, WM, WN, ROW_BYTES, NSTAGE, DIRECT, RAGGED_K, 2>>();
+  return grouped_entry<GroupedCfg<E, A_KC, B_KC, BM, BN, WM, WN, ROW_BYTES, NSTAGE, DIRECT, RAGGED_K, OCC>>();
 }
 
 template <Elem E> constexpr GroupedTable grouped_table_f32() {
@@ -28,6 +31,8 @@ template <Elem E> constexpr GroupedTable grouped_table_f32() {
   t.over_k[0][TILE_128] = grouped_of<E, false, false, 128, 128, 64, 32, 64, 2, false, true>();
   t.over_k[1][TILE_256] = grouped_of<E, false, false, 256, 128, 64, 64, 64, 2, true, true>();
   t.over_k[1][TILE_128] = grouped_of<E, false, false, 128, 128, 64, 32, 64, 2, true, true>();
+  t.stream[0][0] = t.stream[0][1] = stream_entry<E, false, 4>();
+  t.stream[1][0] = stream_entry<E, true, 1>();
   return t;
 }
 
@@ -44,6 +49,8 @@ template <Elem E> constexpr GroupedTable grouped_table_16() {
   t.over_k[0][TILE_128] = grouped_of<E, false, false, 128, 128, 64, 64, 128, 2, false, true>();
   t.over_k[1][TILE_256] = grouped_of<E, false, false, 256, 256, 128, 64, 128, 2, true, true>();
   t.over_k[1][TILE_128] = grouped_of<E, false, false, 128, 128, 64, 64, 128, 2, true, true>();
+  t.stream[0][0] = t.stream[0][1] = stream_entry<E, false, 4>();
+  t.stream[1][0] = stream_entry<E, true, 1>();
   return t;
 }
 
@@ -53,6 +60,7 @@ template <Elem E> constexpr GroupedTable grouped_table_i8() {
   t.columns[1][1][TILE_256] = grouped_of<E, true, true, 256, 256, 128, 64, 128, 2, true, false>();
   t.columns[1][1][TILE_128] = grouped_of<E, true, true, 128, 128, 64, 64, 128, 2, true, false>();
   t.columns[1][1][TILE_NARROW] = grouped_of<E, true, true, 128, 32, 32, 32, 128, 4, true, false>();
+  t.stream[1][0] = stream_entry<E, true, 1>();
   return t;
 }
 
