@@ -52,6 +52,7 @@ _native = None
 _CALL_FUNCTIONS = ("cuMpSGEMM_sgemm", "cuMpSGEMM_cgemm", "cuMpSGEMM_sgemm_strided_batch", "cuMpSGEMM_cgemm_strided_batch",
                    "cuMpSGEMM_sgemm_pipeline", "cuMpSGEMM_cgemm_pipeline", "cuMpSGEMM_sgemm_Mx2x2",
                    "cuMpSGEMM_cgemm_Mx2x2", "cuMpSGEMM_sgemm_2xNx2", "cuMpSGEMM_cgemm_2xNx2")
+_GROUPED_FUNCTIONS = ("cuMpSGEMM_gemm_grouped", "cuMpSGEMM_gemm_grouped_k", "cuMpSGEMM_gemm_i8", "cuMpSGEMM_quantize_i8")
 
 
 def lib():
@@ -75,6 +76,7 @@ def lib():
         try:
             from . import _call
             _call.bind(*(ctypes.cast(getattr(L, name), _ptr).value for name in _CALL_FUNCTIONS))
+            _call.bind_grouped(*(ctypes.cast(getattr(L, name), _ptr).value for name in _GROUPED_FUNCTIONS))
             _native = _call
         except ImportError:
             _native = None  # not built: every call goes through ctypes
@@ -321,6 +323,11 @@ class Handle:
     def gemm_grouped(self, op_a, m, n, k, alpha, a, lda, stridea, b, ldb, beta, c, ldc, offsets, groups, mode,
                      type_ab=R_32F, type_c=R_32F):
         """Tokens (the columns of b, n of them) times their group's matrix; offsets: groups + 1 int32 on the device."""
+        if _native is not None:
+            st = _native.gemm_grouped(self._addr, op_a, m, n, k, alpha, a, lda, stridea, b, ldb, beta, c, ldc, offsets,
+                                      groups, mode, type_ab, type_c)
+            if st is not None:
+                return st
         return self._L.cuMpSGEMM_gemm_grouped(self._h, op_a, m, n, k, _scalar(alpha, False), _dptr(a), lda, stridea,
                                               _dptr(b), ldb, _scalar(beta, False), _dptr(c), ldc, _dptr(offsets),
                                               groups, int(mode), int(type_ab), int(type_c))
@@ -328,17 +335,31 @@ class Handle:
     def gemm_grouped_k(self, m, n, k, alpha, a, lda, b, ldb, beta, c, ldc, stridec, offsets, groups, mode,
                        type_ab=R_32F, type_c=R_32F):
         """For each group, the product over its tokens (k in all): the gradient of the groups' matrices."""
+        if _native is not None:
+            st = _native.gemm_grouped_k(self._addr, m, n, k, alpha, a, lda, b, ldb, beta, c, ldc, stridec, offsets,
+                                        groups, mode, type_ab, type_c)
+            if st is not None:
+                return st
         return self._L.cuMpSGEMM_gemm_grouped_k(self._h, m, n, k, _scalar(alpha, False), _dptr(a), lda, _dptr(b), ldb,
                                                 _scalar(beta, False), _dptr(c), ldc, stridec, _dptr(offsets), groups,
                                                 int(mode), int(type_ab), int(type_c))
 
     def gemm_i8(self, m, n, k, a, lda, stridea, scale_a, b, ldb, scale_b, c, ldc, type_c=R_32F, offsets=None, groups=1):
         """8-bit integers with a scale for each channel of a and each token (column of b); grouped with offsets."""
+        if _native is not None:
+            st = _native.gemm_i8(self._addr, m, n, k, a, lda, stridea, scale_a, b, ldb, scale_b, c, ldc, type_c, offsets,
+                                 groups)
+            if st is not None:
+                return st
         return self._L.cuMpSGEMM_gemm_i8(self._h, m, n, k, _dptr(a), lda, stridea, _dptr(scale_a), _dptr(b), ldb,
                                          _dptr(scale_b), _dptr(c), ldc, int(type_c), _dptr(offsets), groups)
 
     def quantize_i8(self, k, n, x, ldx, type_x, q, ldq, scale):
         """The n columns of x as 8-bit integers with a scale each."""
+        if _native is not None:
+            st = _native.quantize_i8(self._addr, k, n, x, ldx, type_x, q, ldq, scale)
+            if st is not None:
+                return st
         return self._L.cuMpSGEMM_quantize_i8(self._h, k, n, _dptr(x), ldx, int(type_x), _dptr(q), ldq, _dptr(scale))
 
     # ---- exponent statistics ----

@@ -28,6 +28,13 @@ struct Functions {
   decltype(&cuMpSGEMM_cgemm_2xNx2) cgemm_2xNx2;
 } f;
 constexpr Py_ssize_t kFunctions = sizeof(Functions) / sizeof(void *);
+struct GroupedFunctions { // products of experts' layers
+  decltype(&cuMpSGEMM_gemm_grouped) grouped;
+  decltype(&cuMpSGEMM_gemm_grouped_k) grouped_k;
+  decltype(&cuMpSGEMM_gemm_i8) i8;
+  decltype(&cuMpSGEMM_quantize_i8) quantize;
+} fg;
+constexpr Py_ssize_t kGroupedFunctions = sizeof(GroupedFunctions) / sizeof(void *);
 PyObject *data_ptr_name;
 
 // The arguments of a call, taken one after the other; `ok` goes false at the first
@@ -211,20 +218,104 @@ PyObject *twoxnx2(PyObject *, PyObject *const *args, Py_ssize_t n) {
   if (!count_is(n, 17) || !is_complex(args[0], cplx)) return nullptr;
   return cplx ? by2x2_of<hipComplex>(args + 1, f.cgemm_2xNx2) : by2x2_of<float>(args + 1, f.sgemm_2xNx2);
 }
-// the addresses of the functions, in the order of `Functions`
-PyObject *bind(PyObject *, PyObject *const *args, Py_ssize_t n) {
-  if (!count_is(n, kFunctions)) return nullptr;
-  void *p[kFunctions];
-  for (Py_ssize_t i = 0; i < kFunctions; i++) {
+// handle, op_a, m, n, k, alpha, a, lda, stride_a, b, ldb, beta, c, ldc, offsets, groups, mode, type_ab, type_c
+PyObject *gemm_grouped(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+  if (!count_is(n_args, 19)) return nullptr;
+  Args x{args};
+  auto *const h = x.ptr<cuMpSGEMM_handle>();
+  const auto op_a = x.op();
+  const uint64_t m = x.u64(), n = x.u64(), k = x.u64();
+  float alpha{}, beta{};
+  x.scalar(alpha);
+  void *const a = x.ptr<void>();
+  const uint64_t lda = x.u64(), stride_a = x.u64();
+  void *const b = x.ptr<void>();
+  const uint64_t ldb = x.u64();
+  x.scalar(beta);
+  void *const c = x.ptr<void>();
+  const uint64_t ldc = x.u64();
+  const int *const offsets = x.ptr<int>();
+  const uint64_t groups = x.u64();
+  const auto mode = (cuMpSGEMM_compute_mode_t)(int)x.u64();
+  const auto type_ab = (hipDataType)(int)x.u64(), type_c = (hipDataType)(int)x.u64();
+  return status(x, [&] {
+    return fg.grouped(h, op_a, m, n, k, &alpha, a, lda, stride_a, b, ldb, &beta, c, ldc, offsets, groups, mode, type_ab, type_c);
+  });
+}
+// handle, m, n, k, alpha, a, lda, b, ldb, beta, c, ldc, stride_c, offsets, groups, mode, type_ab, type_c
+PyObject *gemm_grouped_k(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+  if (!count_is(n_args, 18)) return nullptr;
+  Args x{args};
+  auto *const h = x.ptr<cuMpSGEMM_handle>();
+  const uint64_t m = x.u64(), n = x.u64(), k = x.u64();
+  float alpha{}, beta{};
+  x.scalar(alpha);
+  void *const a = x.ptr<void>();
+  const uint64_t lda = x.u64();
+  void *const b = x.ptr<void>();
+  const uint64_t ldb = x.u64();
+  x.scalar(beta);
+  void *const c = x.ptr<void>();
+  const uint64_t ldc = x.u64(), stride_c = x.u64();
+  const int *const offsets = x.ptr<int>();
+  const uint64_t groups = x.u64();
+  const auto mode = (cuMpSGEMM_compute_mode_t)(int)x.u64();
+  const auto type_ab = (hipDataType)(int)x.u64(), type_c = (hipDataType)(int)x.u64();
+  return status(x, [&] {
+    return fg.grouped_k(h, m, n, k, &alpha, a, lda, b, ldb, &beta, c, ldc, stride_c, offsets, groups, mode, type_ab, type_c);
+  });
+}
+// handle, m, n, k, a, lda, stride_a, scale_a, b, ldb, scale_b, c, ldc, type_c, offsets, groups
+PyObject *gemm_i8(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+  if (!count_is(n_args, 16)) return nullptr;
+  Args x{args};
+  auto *const h = x.ptr<cuMpSGEMM_handle>();
+  const uint64_t m = x.u64(), n = x.u64(), k = x.u64();
+  const int8_t *const a = x.ptr<int8_t>();
+  const uint64_t lda = x.u64(), stride_a = x.u64();
+  const float *const scale_a = x.ptr<float>();
+  const int8_t *const b = x.ptr<int8_t>();
+  const uint64_t ldb = x.u64();
+  const float *const scale_b = x.ptr<float>();
+  void *const c = x.ptr<void>();
+  const uint64_t ldc = x.u64();
+  const auto type_c = (hipDataType)(int)x.u64();
+  const int *const offsets = x.ptr<int>();
+  const uint64_t groups = x.u64();
+  return status(x, [&] {
+    return fg.i8(h, m, n, k, a, lda, stride_a, scale_a, b, ldb, scale_b, c, ldc, type_c, offsets, groups);
+  });
+}
+// handle, k, n, x, ldx, type_x, q, ldq, scale
+PyObject *quantize_i8(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+  if (!count_is(n_args, 9)) return nullptr;
+  Args x{args};
+  auto *const h = x.ptr<cuMpSGEMM_handle>();
+  const uint64_t k = x.u64(), n = x.u64();
+  void *const values = x.ptr<void>();
+  const uint64_t ldx = x.u64();
+  const auto type_x = (hipDataType)(int)x.u64();
+  int8_t *const q = x.ptr<int8_t>();
+  const uint64_t ldq = x.u64();
+  float *const scale = x.ptr<float>();
+  return status(x, [&] { return fg.quantize(h, k, n, values, ldx, type_x, q, ldq, scale); });
+}
+// the addresses of the functions, in the order of `Functions` (`GroupedFunctions`)
+PyObject *bind_to(void *to, PyObject *const *args, Py_ssize_t n, const Py_ssize_t want) {
+  if (!count_is(n, want)) return nullptr;
+  void *p[kFunctions > kGroupedFunctions ? kFunctions : kGroupedFunctions];
+  for (Py_ssize_t i = 0; i < want; i++) {
     p[i] = PyLong_AsVoidPtr(args[i]);
     if (p[i] == nullptr) {
       if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "no function");
       return nullptr;
     }
   }
-  memcpy(&f, p, sizeof f);
+  memcpy(to, p, want * sizeof(void *));
   Py_RETURN_NONE;
 }
+PyObject *bind(PyObject *, PyObject *const *args, Py_ssize_t n) { return bind_to(&f, args, n, kFunctions); }
+PyObject *bind_grouped(PyObject *, PyObject *const *args, Py_ssize_t n) { return bind_to(&fg, args, n, kGroupedFunctions); }
 
 PyMethodDef methods[] = {{"bind", (PyCFunction)(void (*)(void))bind, METH_FASTCALL, nullptr},
                          {"gemm", (PyCFunction)(void (*)(void))gemm, METH_FASTCALL, nullptr},
@@ -232,6 +323,11 @@ PyMethodDef methods[] = {{"bind", (PyCFunction)(void (*)(void))bind, METH_FASTCA
                          {"pipeline", (PyCFunction)(void (*)(void))pipeline, METH_FASTCALL, nullptr},
                          {"mx2x2", (PyCFunction)(void (*)(void))mx2x2, METH_FASTCALL, nullptr},
                          {"twoxnx2", (PyCFunction)(void (*)(void))twoxnx2, METH_FASTCALL, nullptr},
+                         {"bind_grouped", (PyCFunction)(void (*)(void))bind_grouped, METH_FASTCALL, nullptr},
+                         {"gemm_grouped", (PyCFunction)(void (*)(void))gemm_grouped, METH_FASTCALL, nullptr},
+                         {"gemm_grouped_k", (PyCFunction)(void (*)(void))gemm_grouped_k, METH_FASTCALL, nullptr},
+                         {"gemm_i8", (PyCFunction)(void (*)(void))gemm_i8, METH_FASTCALL, nullptr},
+                         {"quantize_i8", (PyCFunction)(void (*)(void))quantize_i8, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_call", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 } // namespace

@@ -522,6 +522,8 @@ PreSplitChoice choose_pre_split(const cuMpSGEMM_handle *h, bool a_kc, bool b_kc,
   return ch;
 }
 
+} // namespace
+
 // The handle's workspace only grows.  Returns the buffer, or nullptr: no memory
 // or over the cap (the caller falls back to the in-loop kernels) or, with
 // *failed set, the stream is broken.
@@ -563,6 +565,8 @@ void *ensure_pack_workspace(cuMpSGEMM_handle *h, uint64_t bytes, bool *failed) {
   h->pack_ws_bytes = bytes;
   return h->pack_ws;
 }
+
+namespace {
 
 // `args`: the call's arguments (scalars, C, conj flags, launch flag); `accept_*`:
 // the launch-flag masks of the two AUTO candidates.

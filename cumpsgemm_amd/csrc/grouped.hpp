@@ -32,6 +32,10 @@ struct GroupedArgs {
   uint32_t vec_c;           // four results of a column can be stored at once
   const float *scale_a;     // 8-bit integers: [groups][m] and [n]
   const float *scale_b;
+  // ragged K: each group's K in this many parts of whole steps, whose sums go to `partial` as whole tiles, [group]
+  // [tile column][tile row][part][column of the tile][row of the tile], and are added in that order by a second launch
+  uint32_t splits;          // 1: none
+  float *partial;
 };
 
 struct GroupedKernel {
@@ -40,7 +44,10 @@ struct GroupedKernel {
 };
 
 // Kernels of ragged columns: three tiles of the tiled kernel, from the largest, and the kernel of few tokens to a group
-// (grouped_stream.hpp), with 16 or 64 rows to a workgroup (row-contiguous matrices: 64).
-enum KernelClass : int { TILE_256 = 0, TILE_128 = 1, TILE_NARROW = 2, kGroupedClasses = 3, STREAM_16 = 3, STREAM_64 = 4, kKernelClasses = 5 };
+// (grouped_stream.hpp).  Ragged K: the first two.
+enum KernelClass : int { TILE_256 = 0, TILE_128 = 1, TILE_NARROW = 2, kGroupedClasses = 3, STREAM = 3 };
+
+// Adds the parts (bm x bn: the tile that they were computed with).
+void launch_grouped_join(const GroupedArgs &args, int bm, int bn, hipStream_t stream);
 
 } // namespace cumpsgemm_amd

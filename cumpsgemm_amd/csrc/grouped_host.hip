@@ -1,6 +1,7 @@
 // Experts' products: arguments, the choice of a kernel, launch.  See grouped.hpp.
 #include "grouped_table.hpp"
 #include "handle.hpp"
+#include <algorithm>
 #include <cumpsgemm/cumpsgemm_ext.h>
 
 namespace cumpsgemm_amd {
@@ -13,9 +14,38 @@ const GroupedKernel *lookup_grouped(Elem e, bool a_kc, bool ragged_k, bool direc
   static const GroupedTable *const tables[kNumElems] = {&g_grouped_f32_fp16tcec, &g_grouped_f32_fp16tc, &g_grouped_f32_bf16x3,
                                                         &g_grouped_f32_bf16x2, &g_grouped_f16, &g_grouped_bf16, &g_grouped_i8};
   const GroupedTable &t = *tables[(int)e];
-  const GroupedKernel *k = ragged_k ? (cls >= STREAM_16 ? nullptr : &t.over_k[direct][cls])
-                           : cls >= STREAM_16 ? &t.stream[a_kc][cls - STREAM_16] : &t.columns[a_kc][direct][cls];
+  const GroupedKernel *k = ragged_k ? (cls == STREAM ? nullptr : &t.over_k[direct][cls])
+                           : cls == STREAM ? &t.stream[a_kc] : &t.columns[a_kc][direct][cls];
   return k != nullptr && k->launch != nullptr ? k : nullptr;
+}
+
+// One thread: four rows of one column of a tile, the parts in their order.
+__global__ __launch_bounds__(256) void grouped_join_kernel(const GroupedArgs args, const uint32_t bm, const uint32_t bn) {
+  const uint32_t tiles_m = (args.m + bm - 1) / bm, tiles_n = (args.n + bn - 1) / bn, fours = bm * bn / 4;
+  const uint32_t at = blockIdx.x % (fours / 256) * 256 + threadIdx.x; // of the tile's fours
+  const uint64_t tile = blockIdx.x / (fours / 256);
+  const uint32_t row = tile % tiles_m * bm + at % (bm / 4) * 4, col = tile / tiles_m % tiles_n * bn + at / (bm / 4);
+  if (row >= args.m || col >= args.n) return;
+  const float *p = args.partial + tile * args.splits * (bm * bn) + (uint64_t)at * 4;
+  f4v_t x = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (uint32_t s = 0; s < args.splits; s++) {
+    const f4v_t y = *reinterpret_cast<const f4v_t *>(p + (uint64_t)s * (bm * bn));
+#pragma unroll
+    for (int v = 0; v < 4; v++) x[v] += y[v];
+  }
+#pragma unroll
+  for (int v = 0; v < 4; v++) x[v] *= args.alpha;
+  const uint64_t c = (tile / (tiles_m * tiles_n)) * args.stride_c + (uint64_t)col * args.ldc + row;
+  const bool vec = args.vec_c != 0;
+  if (args.out == OUT_F32) store_four<OUT_F32>(args.c + c * 4, x, args.beta, row, args.m, vec);
+  else if (args.out == OUT_F16) store_four<OUT_F16>(args.c + c * 2, x, args.beta, row, args.m, vec);
+  else store_four<OUT_BF16>(args.c + c * 2, x, args.beta, row, args.m, vec);
+}
+
+void launch_grouped_join(const GroupedArgs &args, int bm, int bn, hipStream_t stream) {
+  const uint64_t tiles = (uint64_t)((args.m + bm - 1) / bm) * ((args.n + bn - 1) / bn) * args.groups;
+  hipLaunchKernelGGL(grouped_join_kernel, dim3((uint32_t)(tiles * (bm * bn / 4 / 256))), dim3(256), 0, stream, args, (uint32_t)bm,
+                     (uint32_t)bn);
 }
 
 namespace {
@@ -60,11 +90,31 @@ hipblasStatus_t launched() {
   return hipGetLastError() == hipSuccess ? HIPBLAS_STATUS_SUCCESS : HIPBLAS_STATUS_EXECUTION_FAILED;
 }
 
-// CUMPSGEMM_FORCE_TILE_CLASS (0 - 4) goes before the rules; where there is no such kernel, the 128 x 128 one serves.
-const GroupedKernel *choose(Elem e, bool a_kc, bool ragged_k, bool direct, int cls) {
-  const int forced = tuning().force_cls;
-  const GroupedKernel *k = lookup_grouped(e, a_kc, ragged_k, direct, forced >= 0 && forced < kKernelClasses ? forced : cls);
-  return k != nullptr ? k : lookup_grouped(e, a_kc, ragged_k, direct, TILE_128);
+// What a kernel takes, in us: fixed + steps * max(alone, each * (workgroups / CUs + 0.2 of a round beyond the first)).
+// alone: a step where a CU has one workgroup; each: of a workgroup's step where they queue.  Fitted to 956 calls (m x k of
+// 512^2 to 4096 x 2048, 1 - 64 groups of 1 - 8192 tokens, uneven by e^(0.4 N(0,1)), op T) with every kernel in turn; what
+// the choice by it loses against the best kernel, as a geometric mean: BF16 4.2 %, 8-bit 5.1 %, FP32 3.6 % (FP16TCEC) and
+// 2.9 % (TF32TCEC).  By tokens to a group alone (192, 48, 8) it was 25, 28, 21 and 28 %.
+struct Cost {
+  float fixed, alone, each;
+  int slots, step; // workgroups to a CU; K-values of a step (the kernel of few tokens: of its eight waves)
+};
+const Cost &cost_of(Elem e, int cls) {
+  static const Cost sixteen[4] = {{7.5f, 0.69f, 1.69f, 1, 64}, {5.1f, 0.45f, 0.67f, 2, 64}, {5.4f, 0.24f, 0.37f, 2, 64}, {4.9f, 0.66f, 0.71f, 2, 512}};
+  static const Cost eight[4] = {{10.2f, 0.62f, 1.77f, 1, 128}, {6.7f, 0.33f, 0.74f, 2, 128}, {4.9f, 0.31f, 0.51f, 2, 128}, {4.0f, 0.85f, 0.86f, 2, 1024}};
+  static const Cost fp32[4] = {{8.7f, 0.76f, 1.59f, 1, 32}, {5.2f, 0.58f, 0.87f, 1, 32}, {5.2f, 0.48f, 0.52f, 3, 32}, {4.5f, 0.61f, 0.78f, 2, 256}};
+  static const Cost fp32x3[4] = {{11.3f, 1.24f, 2.24f, 1, 32}, {6.3f, 0.91f, 1.27f, 1, 32}, {6.4f, 0.66f, 0.64f, 2, 32}, {4.8f, 0.63f, 0.78f, 2, 256}};
+  return (e == Elem::I8 ? eight : e == Elem::F32_BF16X3 ? fp32x3 : (int)e <= 3 ? fp32 : sixteen)[cls];
+}
+double cost_us(const Cost &c, double workgroups, double steps, double cus) {
+  return c.fixed + steps * std::max<double>(c.alone, c.each * (workgroups / cus + (workgroups > cus * c.slots ? 0.2 * c.slots : 0.0)));
+}
+// CUMPSGEMM_FORCE_TILE_CLASS goes before the rule where there is such a kernel.
+bool forced(Elem e, bool a_kc, bool ragged_k, bool direct, int &cls) {
+  const int want = tuning().force_cls;
+  if (want < 0 || want > STREAM || lookup_grouped(e, a_kc, ragged_k, direct, want) == nullptr) return false;
+  cls = want;
+  return true;
 }
 
 // Ragged columns: B and C have args.n columns in args.groups groups.
@@ -72,9 +122,24 @@ hipblasStatus_t run_columns(cuMpSGEMM_handle *h, Elem e, bool a_kc, GroupedArgs 
   const uint32_t bytes = bytes_of(e);
   const bool direct = chunks_ok(args.a, a_kc ? args.k : args.m, args.lda, args.stride_a, bytes, a_kc ? 256 : 64) &&
                       chunks_ok(args.b, args.k, args.ldb, 0, bytes, 256);
-  const uint64_t each = args.n / args.groups; // tokens of a group, on average
-  int cls = each >= 192 ? TILE_256 : each >= 48 ? TILE_128 : each > 8 ? TILE_NARROW : STREAM_16;
-  const GroupedKernel *k = choose(e, a_kc, false, direct, cls);
+  int cls = TILE_128;
+  if (!forced(e, a_kc, false, direct, cls)) {
+    double best = 0.0;
+    for (int c = TILE_256; c <= STREAM; c++) {
+      const GroupedKernel *const kern = lookup_grouped(e, a_kc, false, direct, c);
+      if (kern == nullptr) continue;
+      // columns of tiles, the groups' sizes being unknown here: half of each group's last one, or one for each group
+      const double some = std::min(args.n, args.groups), each = (double)args.n / args.groups;
+      const double columns = args.groups == 1 ? (args.n + kern->bn - 1) / kern->bn
+                             : each < kern->bn / 2 ? some : (double)args.n / kern->bn + 0.5 * some;
+      const Cost &cost = cost_of(e, c);
+      // (the kernel of few tokens: in workgroups of 16 rows, as fitted; where rows are contiguous it has 64 in one)
+      const double rows = c == STREAM ? (args.m + 15) / 16 : (args.m + kern->bm - 1) / kern->bm;
+      const double us = cost_us(cost, columns * rows, (args.k + cost.step - 1) / cost.step, h->num_cus);
+      if (best == 0.0 || us < best) best = us, cls = c;
+    }
+  }
+  const GroupedKernel *k = lookup_grouped(e, a_kc, false, direct, cls);
   if (k == nullptr) return HIPBLAS_STATUS_INTERNAL_ERROR;
   // no more tiles of columns than this: every group has one that is not full
   const uint64_t columns = args.offsets == nullptr ? (args.n + k->bn - 1) / k->bn
@@ -160,14 +225,40 @@ hipblasStatus_t cuMpSGEMM_gemm_grouped_k(cuMpSGEMM_handle_t h, uint64_t m, uint6
   args.vec_c = four_at_once(c, m, ldc, stridec, out);
   const uint32_t bytes = bytes_of(e);
   const bool direct = chunks_ok(a, m, lda, 0, bytes, 64) && chunks_ok(b, n, ldb, 0, bytes, 64);
-  const uint64_t tiles = ((m + 255) / 256) * ((n + 255) / 256) * group_count;
-  const int cls = direct && tiles >= h->num_cus ? TILE_256 : TILE_128;
-  const GroupedKernel *kern = choose(e, false, true, direct, cls);
+  // The tile, and in how many parts K is taken where there are too few tiles for the CUs: at least four steps to a
+  // part, the sums written and read once more.
+  int cls = TILE_128;
+  args.splits = 1;
+  const bool fixed_cls = forced(e, false, true, direct, cls);
+  double best = 0.0;
+  for (int c = fixed_cls ? cls : TILE_256; c <= (fixed_cls ? cls : (int)TILE_128); c++) {
+    const GroupedKernel *const kern = lookup_grouped(e, false, true, direct, c);
+    if (kern == nullptr) continue;
+    const Cost &cost = cost_of(e, c);
+    const double tiles = (double)((m + kern->bm - 1) / kern->bm) * ((n + kern->bn - 1) / kern->bn) * group_count;
+    const double steps = (double)k / group_count / cost.step + 0.5;
+    for (uint32_t s = 1; s <= 16; s *= 2) {
+      if (s > 1 && (steps < 4.0 * s || tiles * s > 4.0 * h->num_cus)) break;
+      const double us = cost_us(cost, tiles * s, steps / s, h->num_cus) +
+                        (s == 1 ? 0.0 : 4.0 + tiles * s * kern->bm * kern->bn * 8.0 / 4.0e6);
+      if (best == 0.0 || us < best) best = us, cls = c, args.splits = s;
+    }
+  }
+  if (tuning().force_split > 0) args.splits = (uint32_t)std::min(tuning().force_split, 64);
+  const GroupedKernel *const kern = lookup_grouped(e, false, true, direct, cls);
   if (kern == nullptr) return HIPBLAS_STATUS_INTERNAL_ERROR;
   const uint64_t per = ((m + kern->bm - 1) / kern->bm) * ((n + kern->bn - 1) / kern->bn);
   if (per > kMost || per * group_count > kMost) return HIPBLAS_STATUS_INVALID_VALUE;
+  if (per * group_count > kMost / 64) args.splits = 1;
+  if (args.splits > 1) {
+    bool failed = false;
+    args.partial = (float *)ensure_pack_workspace(h, per * group_count * args.splits * kern->bm * kern->bn * 4, &failed);
+    if (failed) return HIPBLAS_STATUS_EXECUTION_FAILED;
+    if (args.partial == nullptr) args.splits = 1; // (no memory, or a graph is being captured)
+  }
   ProfileScope prof(h, "gemm_grouped_k");
-  kern->launch(args, (uint32_t)(per * group_count), h->stream);
+  kern->launch(args, (uint32_t)(per * group_count * args.splits), h->stream);
+  if (args.splits > 1) launch_grouped_join(args, kern->bm, kern->bn, h->stream);
   return launched();
 }
 

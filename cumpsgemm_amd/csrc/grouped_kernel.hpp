@@ -399,6 +399,7 @@ __device__ inline void store_four(char *c, const f4v_t x, float beta, uint32_t r
 struct TileWork {
   const char *a, *b;       // row m0, token n0 (ragged K: column n0), K-value 0
   char *c;                 // of its group
+  float *partial;          // where a part's sums go (ragged K in parts)
   uint32_t group, m0, n0, n_end, klen;
   int rows_a, rows_b;      // rows and columns that exist
   // lines (rows, K-contiguous operand) from a and b to the matrix's last but one; 0 where one is shorter than a chunk
@@ -696,6 +697,12 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
       const uint32_t col = col0 + r + lane / LANES;
       if (col >= w.n_end) continue;
       f4v_t x = *reinterpret_cast<const f4v_t *>(mine + (r + lane / LANES) * PITCH + (lane % LANES) * 4);
+      if constexpr (Cfg::RAGGED_K) {
+        if (args.splits > 1) {
+          *reinterpret_cast<f4v_t *>(w.partial + (uint64_t)(col - w.n0) * BM + (row - w.m0)) = x;
+          continue;
+        }
+      }
       const float sb = T::I8 ? args.scale_b[col] : 1.0f;
 #pragma unroll
       for (int v = 0; v < 4; v++) x[v] = T::I8 ? x[v] * sa[v] * sb : x[v] * sa[v];
@@ -722,12 +729,21 @@ void grouped_kernel(const GroupedArgs args) {
   w.c = args.c;
   if constexpr (Cfg::RAGGED_K) {
     const uint32_t tiles_n = (args.n + BN - 1) / BN, per = tiles_m * tiles_n;
-    const uint32_t id = xcd_range(blockIdx.x, per * args.groups);
+    const uint32_t all = per * args.groups, split_id = xcd_range(blockIdx.x, all * args.splits);
+    const uint32_t id = split_id % all, split = split_id / all;
     t.group = id / per;
     raster(id % per, tiles_m, tiles_n, t.tm, t.tn);
     group_span(args.offsets, t.group, args.k, t.lo, t.hi);
     t.lo = __builtin_amdgcn_readfirstlane(t.lo);
     t.hi = __builtin_amdgcn_readfirstlane(t.hi);
+    if (args.splits > 1) {
+      const uint32_t len = t.hi - t.lo, part = ((len + Cfg::BK - 1) / Cfg::BK + args.splits - 1) / args.splits * Cfg::BK;
+      const uint32_t from = split * part < len ? split * part : len;
+      t.hi = t.lo + (len - from < part ? len : from + part);
+      t.lo += from;
+      w.partial = args.partial + (((uint64_t)t.group * tiles_n + t.tn) * tiles_m + t.tm) * args.splits * (BM * BN) +
+                  (uint64_t)split * (BM * BN);
+    }
     w.n0 = t.tn * BN;
     w.n_end = args.n;
     w.klen = t.hi - t.lo;

@@ -13,15 +13,15 @@ namespace cumpsgemm_amd {
 
 constexpr int kStreamWaves = 8, kStreamTokens = 16;
 
-// BLOCKS: of 16 rows of the matrix, for a workgroup.
-template <Elem E, bool A_KC, int BLOCKS_> struct StreamCfg {
+template <Elem E, bool A_KC> struct StreamCfg {
   using T = elem_traits<E>;
-  static_assert(A_KC || BLOCKS_ == 4, "row-contiguous: four rows a lane");
-  static constexpr int BLOCKS = BLOCKS_, ROWS = BLOCKS * 16;
+  // 16 rows of the matrix each, for a workgroup (row-contiguous: four rows a lane).  K-contiguous with four, us, with one
+  // -> four: BF16 2048 x 1024, 2 tokens to 2 of 8 groups 4.8 -> 7.0, 64 to 64 27.4 -> 22.1, where the 128 x 32 tiles take 21.0.
+  static constexpr int BLOCKS = A_KC ? 1 : 4, ROWS = BLOCKS * 16;
   // K-values of a wave's step: 128 bytes of a row, one or two MFMAs deep (row-contiguous: one, 32 lines)
   static constexpr int SLICES = A_KC && !T::F32 ? 2 : 1;
   static constexpr int KS = SLICES * 4 * T::CHUNK;
-  static constexpr int UNROLL = A_KC && BLOCKS == 1 ? 4 : 2; // steps under way
+  static constexpr int UNROLL = A_KC ? 4 : 2; // steps under way
 };
 
 // eight or sixteen K-values of a 16-byte chunk (FP32: 32 bytes), as they lie in memory
@@ -100,10 +100,11 @@ template <Elem E> __device__ inline stream_line<E> stream_load_line_part(const c
   return r;
 }
 
-template <Elem E, bool A_KC, int BLOCKS>
+template <Elem E, bool A_KC>
 __global__ __launch_bounds__(kStreamWaves * 64) void grouped_stream_kernel(const GroupedArgs args) {
   using T = elem_traits<E>;
-  using C = StreamCfg<E, A_KC, BLOCKS>;
+  using C = StreamCfg<E, A_KC>;
+  constexpr int BLOCKS = C::BLOCKS;
   __shared__ __attribute__((aligned(16))) float sums[kStreamWaves][kStreamTokens][C::ROWS + 4];
   const int tid = threadIdx.x, lane = tid & 63, frow = lane & 15, fg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -304,11 +305,11 @@ __global__ __launch_bounds__(kStreamWaves * 64) void grouped_stream_kernel(const
   }
 }
 
-template <Elem E, bool A_KC, int BLOCKS> void launch_grouped_stream(const GroupedArgs &args, uint32_t workgroups, hipStream_t stream) {
-  hipLaunchKernelGGL((grouped_stream_kernel<E, A_KC, BLOCKS>), dim3(workgroups), dim3(kStreamWaves * 64), 0, stream, args);
+template <Elem E, bool A_KC> void launch_grouped_stream(const GroupedArgs &args, uint32_t workgroups, hipStream_t stream) {
+  hipLaunchKernelGGL((grouped_stream_kernel<E, A_KC>), dim3(workgroups), dim3(kStreamWaves * 64), 0, stream, args);
 }
-template <Elem E, bool A_KC, int BLOCKS> constexpr GroupedKernel stream_entry() {
-  return {&launch_grouped_stream<E, A_KC, BLOCKS>, BLOCKS * 16, kStreamTokens};
+template <Elem E, bool A_KC> constexpr GroupedKernel stream_entry() {
+  return {&launch_grouped_stream<E, A_KC>, StreamCfg<E, A_KC>::ROWS, kStreamTokens};
 }
 
 } // namespace cumpsgemm_amd

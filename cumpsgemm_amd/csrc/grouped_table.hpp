@@ -9,7 +9,7 @@ struct GroupedTable {
   // [A K-contiguous][through registers, direct][tile]; B K-contiguous
   GroupedKernel columns[2][2][kGroupedClasses];
   GroupedKernel over_k[2][kGroupedClasses]; // ragged K, both row-contiguous
-  GroupedKernel stream[2][2];               // few tokens; [A K-contiguous][16 rows, 64 rows]
+  GroupedKernel stream[2];                  // few tokens; [A K-contiguous]
 };
 
 template <Elem E, bool A_KC, bool B_KC, int BM, int BN, int WM, int WN, int ROW_BYTES, int NSTAGE, bool DIRECT, bool RAGGED_K,
@@ -31,8 +31,8 @@ template <Elem E> constexpr GroupedTable grouped_table_f32() {
   t.over_k[0][TILE_128] = grouped_of<E, false, false, 128, 128, 64, 32, 64, 2, false, true>();
   t.over_k[1][TILE_256] = grouped_of<E, false, false, 256, 128, 64, 64, 64, 2, true, true>();
   t.over_k[1][TILE_128] = grouped_of<E, false, false, 128, 128, 64, 32, 64, 2, true, true>();
-  t.stream[0][0] = t.stream[0][1] = stream_entry<E, false, 4>();
-  t.stream[1][0] = stream_entry<E, true, 1>();
+  t.stream[0] = stream_entry<E, false>();
+  t.stream[1] = stream_entry<E, true>();
   return t;
 }
 
@@ -49,8 +49,8 @@ template <Elem E> constexpr GroupedTable grouped_table_16() {
   t.over_k[0][TILE_128] = grouped_of<E, false, false, 128, 128, 64, 64, 128, 2, false, true>();
   t.over_k[1][TILE_256] = grouped_of<E, false, false, 256, 256, 128, 64, 128, 2, true, true>();
   t.over_k[1][TILE_128] = grouped_of<E, false, false, 128, 128, 64, 64, 128, 2, true, true>();
-  t.stream[0][0] = t.stream[0][1] = stream_entry<E, false, 4>();
-  t.stream[1][0] = stream_entry<E, true, 1>();
+  t.stream[0] = stream_entry<E, false>();
+  t.stream[1] = stream_entry<E, true>();
   return t;
 }
 
@@ -60,7 +60,7 @@ template <Elem E> constexpr GroupedTable grouped_table_i8() {
   t.columns[1][1][TILE_256] = grouped_of<E, true, true, 256, 256, 128, 64, 128, 2, true, false>();
   t.columns[1][1][TILE_128] = grouped_of<E, true, true, 128, 128, 64, 64, 128, 2, true, false>();
   t.columns[1][1][TILE_NARROW] = grouped_of<E, true, true, 128, 32, 32, 32, 128, 4, true, false>();
-  t.stream[1][0] = stream_entry<E, true, 1>();
+  t.stream[1] = stream_entry<E, true>();
   return t;
 }
 

@@ -160,6 +160,9 @@ struct ProfileScope {
 
 void check_hip(hipError_t err, const char *what);
 
+// The handle's workspace, grown to `bytes` (gemm_host.hip); null: not to be had now, *failed: the stream is broken.
+void *ensure_pack_workspace(cuMpSGEMM_handle *h, uint64_t bytes, bool *failed);
+
 // Statistics of the two operands of a GEMM with one launch per pass instead
 // of two; same results and slot numbering as exp_stats_ext / exp_max_ext
 // called for A, then for B.

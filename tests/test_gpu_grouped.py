@@ -219,6 +219,43 @@ def test_over_k_tiles_strides_alpha_beta(cg, handle, kind):
         check(got, want, size, kind, max(sizes), dtype_of(kind))
 
 
+@pytest.mark.parametrize("parts", [2, 3, 16])
+@pytest.mark.parametrize("kind", KINDS)
+def test_over_k_in_parts(cg, torch_gpu, kind, parts, monkeypatch):
+    """K of every group in parts that are added in order: groups shorter than their parts, and the same bits each time."""
+    monkeypatch.setenv("CUMPSGEMM_FORCE_KSPLIT", str(parts))
+    h = cg.Handle(stream=torch.cuda.current_stream())
+    for m, n, sizes, pads in ((264, 136, [300, 0, 65, 1], (0, 0, 0, 0)), (67, 33, [1000], (1, 3, 5, 7))):
+        runs = [run_over_k(cg, h, kind, m, n, sizes, alpha=0.75, beta=0.5, pads=pads) for _ in range(2)]
+        check(*runs[0], kind, max(sizes), dtype_of(kind))
+        assert torch.equal(runs[0][0], runs[1][0]) and h.workspace_size() > 0
+    h.close()
+
+
+def test_over_k_takes_parts_where_tiles_are_few(cg, torch_gpu):
+    h = cg.Handle(stream=torch.cuda.current_stream())
+    for kind in ("FP16TCEC", "bf16"):
+        got, want, size = run_over_k(cg, h, kind, 256, 256, [4000, 96])
+        check(got, want, size, kind, 4000, dtype_of(kind))
+    assert h.workspace_size() > 0
+    h.close()
+
+
+@pytest.mark.parametrize("cls", [0, 1, 2, 3])
+@pytest.mark.parametrize("kind", KINDS + ["i8"])
+def test_every_kernel_at_sizes_that_it_would_not_be_chosen_for(cg, handle, kind, cls, monkeypatch):
+    monkeypatch.setenv("CUMPSGEMM_FORCE_TILE_CLASS", str(cls))
+    for m, k, sizes in ((264, 200, [1, 0, 300, 33, 129, 257]), (520, 64, [17, 65, 191]), (72, 1000, [20])):
+        if kind == "i8":
+            run_i8(cg, handle, m, k // 16 * 16, sizes, torch.float32)
+            continue
+        for op in "TN":
+            got, want, size = run_columns(cg, handle, kind, op, m, k, sizes, alpha=1.5, beta=0.5)
+            check(got, want, size, kind, k, dtype_of(kind))
+        got, want, size = run_over_k(cg, handle, kind, m, 136, sizes)
+        check(got, want, size, kind, max(sizes), dtype_of(kind))
+
+
 @pytest.mark.parametrize("kind", ["f16", "bf16"])
 def test_over_k_accumulates_in_fp32(cg, handle, kind):
     got, want, size = run_over_k(cg, handle, kind, 136, 72, [100, 0, 31], beta=1.0, out=torch.float32)
