@@ -51,6 +51,7 @@ void launch_grouped_join(const GroupedArgs &args, int bm, int bn, hipStream_t st
 namespace {
 
 constexpr uint64_t kMost = 0x7fffffffull;
+constexpr uint64_t kMostWorkgroups = 0xffffffffull / 512; // (a launch has fewer than 2^32 threads)
 
 bool elem_of(hipDataType type, cuMpSGEMM_compute_mode_t mode, Elem &e) {
   if (type == HIP_R_16F) e = Elem::F16;
@@ -117,6 +118,13 @@ bool forced(Elem e, bool a_kc, bool ragged_k, bool direct, int &cls) {
   return true;
 }
 
+// Ragged columns: no more tiles than this, where every group has a column of them that is not full.
+uint64_t most_tiles(const GroupedArgs &args, const GroupedKernel &k) {
+  const uint64_t columns = args.offsets == nullptr ? (args.n + k.bn - 1) / k.bn
+                                                   : (uint64_t)args.n / k.bn + std::min(args.n, args.groups);
+  return columns * ((args.m + k.bm - 1) / k.bm);
+}
+
 // Ragged columns: B and C have args.n columns in args.groups groups.
 hipblasStatus_t run_columns(cuMpSGEMM_handle *h, Elem e, bool a_kc, GroupedArgs &args, const char *label) {
   const uint32_t bytes = bytes_of(e);
@@ -127,7 +135,7 @@ hipblasStatus_t run_columns(cuMpSGEMM_handle *h, Elem e, bool a_kc, GroupedArgs 
     double best = 0.0;
     for (int c = TILE_256; c <= STREAM; c++) {
       const GroupedKernel *const kern = lookup_grouped(e, a_kc, false, direct, c);
-      if (kern == nullptr) continue;
+      if (kern == nullptr || most_tiles(args, *kern) > kMostWorkgroups) continue;
       // columns of tiles, the groups' sizes being unknown here: half of each group's last one, or one for each group
       const double some = std::min(args.n, args.groups), each = (double)args.n / args.groups;
       const double columns = args.groups == 1 ? (args.n + kern->bn - 1) / kern->bn
@@ -141,11 +149,8 @@ hipblasStatus_t run_columns(cuMpSGEMM_handle *h, Elem e, bool a_kc, GroupedArgs 
   }
   const GroupedKernel *k = lookup_grouped(e, a_kc, false, direct, cls);
   if (k == nullptr) return HIPBLAS_STATUS_INTERNAL_ERROR;
-  // no more tiles of columns than this: every group has one that is not full
-  const uint64_t columns = args.offsets == nullptr ? (args.n + k->bn - 1) / k->bn
-                                                   : (uint64_t)args.n / k->bn + std::min(args.n, args.groups);
-  const uint64_t workgroups = columns * ((args.m + k->bm - 1) / k->bm);
-  if (workgroups > kMost) return HIPBLAS_STATUS_INVALID_VALUE;
+  const uint64_t workgroups = most_tiles(args, *k);
+  if (workgroups > kMostWorkgroups) return HIPBLAS_STATUS_INVALID_VALUE;
   ProfileScope prof(h, label);
   k->launch(args, (uint32_t)workgroups, h->stream);
   return launched();
@@ -248,8 +253,9 @@ hipblasStatus_t cuMpSGEMM_gemm_grouped_k(cuMpSGEMM_handle_t h, uint64_t m, uint6
   const GroupedKernel *const kern = lookup_grouped(e, false, true, direct, cls);
   if (kern == nullptr) return HIPBLAS_STATUS_INTERNAL_ERROR;
   const uint64_t per = ((m + kern->bm - 1) / kern->bm) * ((n + kern->bn - 1) / kern->bn);
-  if (per > kMost || per * group_count > kMost) return HIPBLAS_STATUS_INVALID_VALUE;
-  if (per * group_count > kMost / 64) args.splits = 1;
+  if (per > kMostWorkgroups || per * group_count > kMostWorkgroups) return HIPBLAS_STATUS_INVALID_VALUE;
+  // (the launch that joins the parts has up to 64 workgroups to a tile)
+  if (per * group_count > kMostWorkgroups / 64) args.splits = 1;
   if (args.splits > 1) {
     bool failed = false;
     args.partial = (float *)ensure_pack_workspace(h, per * group_count * args.splits * kern->bm * kern->bn * 4, &failed);

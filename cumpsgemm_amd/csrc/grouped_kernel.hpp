@@ -141,7 +141,8 @@ __device__ inline bool place_tile(const GroupedArgs &args, uint32_t bid, uint32_
         t.tm = id % tiles_m;
         t.tn = __builtin_amdgcn_readlane(full, at);
       }
-      return true;
+      // (offsets out of order can make these sums overflow: no tile outside its group)
+      return t.tm < tiles_m && (uint64_t)t.tn * bn < t.hi - t.lo;
     }
     before = __builtin_amdgcn_readlane(sum, 63);
   }

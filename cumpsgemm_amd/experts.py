@@ -1,0 +1,145 @@
+"""One layer of experts on the library's grouped products: each token is multiplied with the matrix of its expert.
+
+    python -m cumpsgemm_amd.experts [tokens [features_in [features_out [experts]]]]
+
+runs a training step in FP32 on split operands and in BF16 (forward, the gradients of tokens and matrices), then serves
+the trained matrices in 8-bit integers, and prints how far each result is from FP64.
+
+Tensors hold a token (an output channel) in a row, which the library's column-major calls read as a column."""
+import sys
+
+from . import _lib as lib
+
+
+def group_by_expert(experts, count):
+    """(order, offsets): the tokens' numbers sorted by expert (those of one expert in their order), and where each expert's
+    begin, `count` + 1 int32.  On the tensor's own device, without waiting for it."""
+    import torch
+    order = torch.argsort(experts, stable=True)
+    first = torch.arange(count + 1, device=experts.device, dtype=experts.dtype)
+    return order, torch.searchsorted(experts[order], first).to(torch.int32)
+
+
+def _type(t):
+    import torch
+    return {torch.float32: lib.R_32F, torch.float16: lib.R_16F, torch.bfloat16: lib.R_16BF}[t.dtype]
+
+
+def _check(status):
+    if status != lib.STATUS_SUCCESS:
+        raise RuntimeError(f"hipblasStatus {status}")
+
+
+class Experts:
+    """y[t] = weights[expert of t] @ x[t]; weights: [experts, features out, features in], FP32, FP16 or BF16, on the GPU.
+    mode: how FP32 operands are multiplied."""
+
+    def __init__(self, handle, weights, mode=lib.FP16TCEC):
+        self.handle, self.weights, self.mode = handle, weights.contiguous(), mode
+
+    def forward(self, x, experts):
+        """(y, what backward needs)"""
+        import torch
+        w = self.weights
+        count, out, inner = w.shape
+        order, offsets = group_by_expert(experts, count)
+        grouped = x[order]
+        y = torch.empty(len(x), out, device=x.device, dtype=x.dtype)
+        _check(self.handle.gemm_grouped(lib.OP_T, out, len(x), inner, 1.0, w, inner, out * inner, grouped, inner, 0.0, y, out,
+                                        offsets, count, self.mode, _type(x), _type(y)))
+        return torch.empty_like(y).index_copy_(0, order, y), (grouped, order, offsets)
+
+    def backward(self, saved, dy, dw=None):
+        """(gradient of x, gradient of the weights in FP32: added to dw if there is one)"""
+        import torch
+        grouped, order, offsets = saved
+        w = self.weights
+        count, out, inner = w.shape
+        dy = dy[order]
+        dx = torch.empty_like(grouped)
+        _check(self.handle.gemm_grouped(lib.OP_N, inner, len(dy), out, 1.0, w, inner, out * inner, dy, out, 0.0, dx, inner,
+                                        offsets, count, self.mode, _type(dy), _type(dx)))
+        beta = 0.0 if dw is None else 1.0
+        if dw is None:
+            dw = torch.empty(w.shape, device=w.device, dtype=torch.float32)
+        # (stored as the weights are, features in contiguous: rows of x times rows of dy)
+        _check(self.handle.gemm_grouped_k(inner, out, len(dy), 1.0, grouped, inner, dy, out, beta, dw, inner, out * inner,
+                                          offsets, count, self.mode, _type(dy), lib.R_32F))
+        return torch.empty_like(dx).index_copy_(0, order, dx), dw
+
+    def to_int8(self):
+        """The same layer for serving, in 8-bit integers with a scale for each output channel."""
+        import torch
+        count, out, inner = self.weights.shape
+        q = torch.empty(count, out, inner, device=self.weights.device, dtype=torch.int8)
+        scale = torch.empty(count, out, device=self.weights.device, dtype=torch.float32)
+        _check(self.handle.quantize_i8(inner, count * out, self.weights, inner, _type(self.weights), q, inner, scale))
+        return Int8Experts(self.handle, q, scale)
+
+
+class Int8Experts:
+    """weights: [experts, features out, features in] 8-bit integers, scale: [experts, features out]."""
+
+    def __init__(self, handle, weights, scale):
+        self.handle, self.weights, self.scale = handle, weights, scale
+
+    def forward(self, x, experts):
+        """x in FP32, FP16 or BF16, a scale taken for each token; y of the same type"""
+        import torch
+        count, out, inner = self.weights.shape
+        order, offsets = group_by_expert(experts, count)
+        grouped = x[order]
+        q = torch.empty(len(x), inner, device=x.device, dtype=torch.int8)
+        scale = torch.empty(len(x), device=x.device, dtype=torch.float32)
+        y = torch.empty(len(x), out, device=x.device, dtype=x.dtype)
+        _check(self.handle.quantize_i8(inner, len(x), grouped, inner, _type(x), q, inner, scale))
+        _check(self.handle.gemm_i8(out, len(x), inner, self.weights, inner, out * inner, self.scale, q, inner, scale, y, out,
+                                   _type(y), offsets, count))
+        return torch.empty_like(y).index_copy_(0, order, y)
+
+
+def reference(weights, x, experts, dy):
+    """y, dx and dw in FP64, expert by expert."""
+    import torch
+    w, x, dy = weights.double(), x.double(), dy.double()
+    y, dx, dw = torch.empty_like(dy), torch.empty_like(x), torch.zeros_like(w)
+    for e in range(len(w)):
+        rows = torch.nonzero(experts == e)[:, 0]
+        y[rows] = x[rows] @ w[e].t().contiguous()
+        dx[rows] = dy[rows] @ w[e]
+        dw[e] = dy[rows].t().contiguous() @ x[rows]
+    return y, dx, dw
+
+
+def main(argv=None):
+    """Prints one line for each result; returns {result: relative error against FP64}."""
+    import torch
+    args = [int(a) for a in (sys.argv[1:] if argv is None else argv)]
+    tokens, inner, out, count = args + [1000, 512, 768, 8][len(args):]
+    g = torch.Generator(device="cuda").manual_seed(1)
+    weights = torch.randn(count, out, inner, generator=g, device="cuda") * inner ** -0.5
+    x = torch.randn(tokens, inner, generator=g, device="cuda")
+    dy = torch.randn(tokens, out, generator=g, device="cuda")
+    experts = torch.randint(count, (tokens,), generator=g, device="cuda")
+    handle = lib.Handle(stream=torch.cuda.current_stream())
+    errors = {}
+
+    def report(name, got, want):
+        errors[name] = float((got.double() - want).norm() / want.norm())
+        print(f"{name:24s} relative error {errors[name]:.2e}")
+
+    for name, dtype in (("FP16TCEC", torch.float32), ("BF16", torch.bfloat16)):
+        layer = Experts(handle, weights.to(dtype))
+        xs, ds = x.to(dtype), dy.to(dtype)
+        y, saved = layer.forward(xs, experts)
+        dx, dw = layer.backward(saved, ds)
+        for part, got, want in zip(("y", "dx", "dw"), (y, dx, dw), reference(layer.weights, xs, experts, ds)):
+            report(f"{name} {part}", got, want)
+    report("8-bit integers y", Experts(handle, weights).to_int8().forward(x, experts), reference(weights, x, experts, dy)[0])
+    torch.cuda.synchronize()
+    handle.close()
+    return errors
+
+
+if __name__ == "__main__":
+    main()
