@@ -107,6 +107,15 @@ const Cost &cost_of(Elem e, int cls) {
   static const Cost fp32x3[4] = {{11.3f, 1.24f, 2.24f, 1, 32}, {6.3f, 0.91f, 1.27f, 1, 32}, {6.4f, 0.66f, 0.64f, 2, 32}, {4.8f, 0.63f, 0.78f, 2, 256}};
   return (e == Elem::I8 ? eight : e == Elem::F32_BF16X3 ? fp32x3 : (int)e <= 3 ? fp32 : sixteen)[cls];
 }
+// The same for products over K (342 calls, 1 - 64 groups of 16 - 16384 tokens, results of 256^2 - 4096 x 2048, K in 1 - 16
+// parts, both tiles): a group's K can be longer than the average one's, which counts where a CU has one workgroup, and parts
+// are written and read once more, 3.2 TB/s.  Loses 3.6 % (BF16), 2.0 % (FP16TCEC) and 2.1 % (TF32TCEC).
+const Cost &cost_over_k(Elem e, int cls) {
+  static const Cost sixteen[2] = {{11.4f, 1.23f, 2.32f, 1, 64}, {7.3f, 0.65f, 0.67f, 2, 64}};
+  static const Cost fp32[2] = {{11.6f, 1.27f, 1.89f, 1, 32}, {7.2f, 0.86f, 1.13f, 1, 32}};
+  static const Cost fp32x3[2] = {{14.7f, 2.10f, 3.00f, 1, 32}, {6.7f, 1.24f, 1.61f, 1, 32}};
+  return (e == Elem::F32_BF16X3 ? fp32x3 : (int)e <= 3 ? fp32 : sixteen)[cls];
+}
 double cost_us(const Cost &c, double workgroups, double steps, double cus) {
   return c.fixed + steps * std::max<double>(c.alone, c.each * (workgroups / cus + (workgroups > cus * c.slots ? 0.2 * c.slots : 0.0)));
 }
@@ -230,8 +239,7 @@ hipblasStatus_t cuMpSGEMM_gemm_grouped_k(cuMpSGEMM_handle_t h, uint64_t m, uint6
   args.vec_c = four_at_once(c, m, ldc, stridec, out);
   const uint32_t bytes = bytes_of(e);
   const bool direct = chunks_ok(a, m, lda, 0, bytes, 64) && chunks_ok(b, n, ldb, 0, bytes, 64);
-  // The tile, and in how many parts K is taken where there are too few tiles for the CUs: at least four steps to a
-  // part, the sums written and read once more.
+  // The tile, and in how many parts K is taken: at least two steps to a part.
   int cls = TILE_128;
   args.splits = 1;
   const bool fixed_cls = forced(e, false, true, direct, cls);
@@ -239,13 +247,14 @@ hipblasStatus_t cuMpSGEMM_gemm_grouped_k(cuMpSGEMM_handle_t h, uint64_t m, uint6
   for (int c = fixed_cls ? cls : TILE_256; c <= (fixed_cls ? cls : (int)TILE_128); c++) {
     const GroupedKernel *const kern = lookup_grouped(e, false, true, direct, c);
     if (kern == nullptr) continue;
-    const Cost &cost = cost_of(e, c);
+    Cost cost = cost_over_k(e, c);
+    if (group_count > 1) cost.alone *= 1.6f;
     const double tiles = (double)((m + kern->bm - 1) / kern->bm) * ((n + kern->bn - 1) / kern->bn) * group_count;
     const double steps = (double)k / group_count / cost.step + 0.5;
     for (uint32_t s = 1; s <= 16; s *= 2) {
-      if (s > 1 && (steps < 4.0 * s || tiles * s > 4.0 * h->num_cus)) break;
+      if (s > 1 && (steps < 2.0 * s || tiles * s > 8.0 * h->num_cus)) break;
       const double us = cost_us(cost, tiles * s, steps / s, h->num_cus) +
-                        (s == 1 ? 0.0 : 4.0 + tiles * s * kern->bm * kern->bn * 8.0 / 4.0e6);
+                        (s == 1 ? 0.0 : 0.7 + tiles * kern->bm * kern->bn * 4.0 * (s + 1) / 3.2e6);
       if (best == 0.0 || us < best) best = us, cls = c, args.splits = s;
     }
   }

@@ -152,9 +152,8 @@ hipblasStatus_t cuMpSGEMM_cgemm_2xNx2(cuMpSGEMM_handle_t handle, hipblasOperatio
 /* ---- products of experts' layers (no counterpart in the reference) ---------
  * `offsets`: group_count + 1 ints in DEVICE memory, ascending; group g has the
  * tokens offsets[g] .. offsets[g + 1] - 1.  A group may have none.  The kernels
- * read them, the host does not: no call waits for the device, allocates or
- * keeps anything, and all can be captured into a graph, whose replays take the
- * offsets of the time.  Values outside 0 .. token count are brought into it,
+ * read them, the host does not: no call waits for their values, and all can be
+ * captured into a graph, whose replays take the offsets of the time.  Values outside 0 .. token count are brought into it,
  * and an offset below the one before it gives an empty group; what tokens
  * overlap then and which results are written is undefined, but nothing outside
  * the operands is touched.  Results repeat bit for bit.
@@ -180,7 +179,11 @@ hipblasStatus_t cuMpSGEMM_gemm_grouped(cuMpSGEMM_handle_t handle, hipblasOperati
  *   C_g = alpha * A[:, tokens of g] * B[:, tokens of g]^T + beta * C_g
  * A is m x k, B is n x k, a token a column; C_g is m x n at c + g * stridec.  A
  * group without tokens gets beta * C_g (zeros with beta = 0).  beta = 1
- * accumulates. */
+ * accumulates.  A call with fewer tiles than CUs takes K in parts, whose sums
+ * pass through the handle's workspace and are added in a fixed order: its first
+ * use allocates, as cuMpSGEMM_sgemm's does (cuMpSGEMM_get_workspace_size), and
+ * under capture, when it would have to grow, K is taken whole instead (the same
+ * result up to the order of summation). */
 hipblasStatus_t cuMpSGEMM_gemm_grouped_k(cuMpSGEMM_handle_t handle, uint64_t m, uint64_t n, uint64_t k,
                                          const float *alpha, const void *a, uint64_t lda, const void *b,
                                          uint64_t ldb, const float *beta, void *c, uint64_t ldc,
