@@ -44,8 +44,8 @@ struct GroupedKernel {
 };
 
 // Kernels of ragged columns: three tiles of the tiled kernel, from the largest, and the kernel of few tokens to a group
-// (grouped_stream.hpp).  Ragged K: the first two.
-enum KernelClass : int { TILE_256 = 0, TILE_128 = 1, TILE_NARROW = 2, kGroupedClasses = 3, STREAM = 3 };
+// (grouped_stream.hpp).  Ragged K: the first two, and one for matrices of fewer than eight 16-bit rows or columns.
+enum KernelClass : int { TILE_256 = 0, TILE_128 = 1, TILE_NARROW = 2, SHORT_LINES = 2, kGroupedClasses = 3, STREAM = 3 };
 
 // Adds the parts (bm x bn: the tile that they were computed with).
 void launch_grouped_join(const GroupedArgs &args, int bm, int bn, hipStream_t stream);

@@ -122,7 +122,7 @@ double cost_us(const Cost &c, double workgroups, double steps, double cus) {
 // CUMPSGEMM_FORCE_TILE_CLASS goes before the rule where there is such a kernel.
 bool forced(Elem e, bool a_kc, bool ragged_k, bool direct, int &cls) {
   const int want = tuning().force_cls;
-  if (want < 0 || want > STREAM || lookup_grouped(e, a_kc, ragged_k, direct, want) == nullptr) return false;
+  if (want < 0 || want > STREAM || (ragged_k && want == SHORT_LINES) || lookup_grouped(e, a_kc, ragged_k, direct, want) == nullptr) return false;
   cls = want;
   return true;
 }
@@ -140,7 +140,9 @@ hipblasStatus_t run_columns(cuMpSGEMM_handle *h, Elem e, bool a_kc, GroupedArgs 
   const bool direct = chunks_ok(args.a, a_kc ? args.k : args.m, args.lda, args.stride_a, bytes, a_kc ? 256 : 64) &&
                       chunks_ok(args.b, args.k, args.ldb, 0, bytes, 256);
   int cls = TILE_128;
-  if (!forced(e, a_kc, false, direct, cls)) {
+  if (bytes == 2 && !direct && !a_kc && args.m < 8) {
+    cls = STREAM; // (a line is shorter than the chunks that the tiled kernels read)
+  } else if (!forced(e, a_kc, false, direct, cls)) {
     double best = 0.0;
     for (int c = TILE_256; c <= STREAM; c++) {
       const GroupedKernel *const kern = lookup_grouped(e, a_kc, false, direct, c);
@@ -242,12 +244,14 @@ hipblasStatus_t cuMpSGEMM_gemm_grouped_k(cuMpSGEMM_handle_t h, uint64_t m, uint6
   // The tile, and in how many parts K is taken: at least two steps to a part.
   int cls = TILE_128;
   args.splits = 1;
-  const bool fixed_cls = forced(e, false, true, direct, cls);
+  const bool short_lines = bytes == 2 && !direct && (m < 8 || n < 8);
+  if (short_lines) cls = SHORT_LINES;
+  const bool fixed_cls = short_lines || forced(e, false, true, direct, cls);
   double best = 0.0;
-  for (int c = fixed_cls ? cls : TILE_256; c <= (fixed_cls ? cls : (int)TILE_128); c++) {
+  for (int c = fixed_cls ? cls : (int)TILE_256; c <= (fixed_cls ? cls : (int)TILE_128); c++) {
     const GroupedKernel *const kern = lookup_grouped(e, false, true, direct, c);
     if (kern == nullptr) continue;
-    Cost cost = cost_over_k(e, c);
+    Cost cost = cost_over_k(e, c == SHORT_LINES ? (int)TILE_128 : c);
     if (group_count > 1) cost.alone *= 1.6f;
     const double tiles = (double)((m + kern->bm - 1) / kern->bm) * ((n + kern->bn - 1) / kern->bn) * group_count;
     const double steps = (double)k / group_count / cost.step + 0.5;

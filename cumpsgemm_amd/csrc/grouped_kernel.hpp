@@ -150,13 +150,14 @@ __device__ inline bool place_tile(const GroupedArgs &args, uint32_t bid, uint32_
 }
 
 // DIRECT: 16-bit and 8-bit operands go straight from memory to LDS, 16 aligned bytes a lane; FP32 operands, which are
-// split in registers, are read with 32-bit offsets from uniform bases.  Otherwise: any alignment, any size.
+// split in registers, are read with 32-bit offsets from uniform bases.  Otherwise: any alignment, any size; but lines of
+// 16-bit values that are shorter than a chunk are for the CAREFUL kernels.
 template <Elem E_, bool A_KC_, bool B_KC_, int BM_, int BN_, int WM_, int WN_, int ROW_BYTES_, int NSTAGE_, bool DIRECT_,
-          bool RAGGED_K_, int OCC_>
+          bool RAGGED_K_, int OCC_, bool CAREFUL_>
 struct GroupedCfg {
   using T = elem_traits<E_>;
   static constexpr Elem E = E_;
-  static constexpr bool A_KC = A_KC_, B_KC = B_KC_, DIRECT = DIRECT_, RAGGED_K = RAGGED_K_;
+  static constexpr bool A_KC = A_KC_, B_KC = B_KC_, DIRECT = DIRECT_, RAGGED_K = RAGGED_K_, CAREFUL = CAREFUL_;
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NSTAGE = NSTAGE_, OCC = OCC_;
   static constexpr int WAVES_M = BM / WM, WAVES_N = BN / WN, NT = WAVES_M * WAVES_N * 64;
   static constexpr int TM = WM / 16, TN = WN / 16;
@@ -252,8 +253,9 @@ template <Elem E, bool KC, int ROWS, int ROW_BYTES, int NT> struct grouped_loade
   };
 
   // memory -> registers, unit u of a whole step.  off: the unit's offset() from the uniform base, in 32 bits if FAST.
-  // (rows, safe: see fetch_tail)
-  template <bool FAST, class OFF>
+  // A chunk of a line (LINES) may stick out beyond the rows, into the next line: not for the matrix's last line, unless
+  // CAREFUL (rows, safe: see fetch_tail).
+  template <bool FAST, bool CAREFUL, class OFF>
   __device__ static inline void fetch(Regs &r, int u, const char *base, uint64_t ld, OFF off, int rows, int64_t safe, int tid) {
     if (!active(tid)) return;
     if constexpr (T::F32 && KC) {
@@ -277,7 +279,7 @@ template <Elem E, bool KC, int ROWS, int ROW_BYTES, int NT> struct grouped_loade
       typedef uint32_t u4u2_t __attribute__((ext_vector_type(4), aligned(2)));
       typedef uint32_t u4u1_t __attribute__((ext_vector_type(4), aligned(1)));
       typedef typename std::conditional<T::I8, u4u1_t, u4u2_t>::type u4u_t;
-      if (!LINES || rows >= ROWS) { // (uniform)
+      if (!LINES || !CAREFUL) {
         const u4u_t x = *reinterpret_cast<const u4u_t *>(base + off);
         r.v[u] = u4_t{x.x, x.y, x.z, x.w};
       } else {
@@ -526,7 +528,11 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
   // ---- K loop ----
   // A K that ends inside a step has that step multiplied first, so that the loop has whole steps only: step s begins
   // at K-value (s - partial) BK, the partial one behind them all.
-  const int whole = (int)(w.klen / BK), left = (int)(w.klen % BK), partial = left != 0, steps = whole + partial;
+  // (Lines of any alignment: the last step counts as partial even if it is whole, since a chunk of the matrix's last line
+  // must not be read beyond its end.)
+  constexpr bool LAST_ASIDE = !T::F32 && !Cfg::DIRECT && (!Cfg::A_KC || !Cfg::B_KC);
+  const int whole = LAST_ASIDE ? (int)((w.klen > 0 ? w.klen - 1 : 0) / BK) : (int)(w.klen / BK), left = (int)w.klen - whole * BK;
+  const int partial = left != 0, steps = whole + partial;
   auto a_at = [&](int s) { return a + (uint64_t)(s < partial ? whole : s - partial) * a_step; };
   auto b_at = [&](int s) { return b + (uint64_t)(s < partial ? whole : s - partial) * b_step; };
   typedef typename std::conditional<Cfg::DIRECT, uint32_t, uint64_t>::type off_t;
@@ -613,50 +619,66 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
       for (int l = 0; l < LOADS; l++)
         if (l * BLOCKS / LOADS == g) f(l);
     };
-    typename LA::Regs ra;
-    typename LB::Regs rb;
-    auto put = [&](int l, char *stage) {
-      if (l < LA::U) LA::put(ra, l, stage, tid);
-      else LB::put(rb, l - LA::U, stage + Cfg::A_STAGE, tid);
+    // SETS of registers: 16-bit and 8-bit operands, whose steps are shorter than a load's way, are asked for a step earlier
+    constexpr int SETS = T::F32 ? 1 : 2;
+    typename LA::Regs ra[SETS];
+    typename LB::Regs rb[SETS];
+    auto put = [&](int l, const int set, char *stage) {
+      if (l < LA::U) LA::put(ra[set], l, stage, tid);
+      else LB::put(rb[set], l - LA::U, stage + Cfg::A_STAGE, tid);
     };
-    auto fetch = [&](int l, const char *pa, const char *pb, int64_t k0) { // (k0: the step's first K-value)
-      if (l < LA::U) LA::template fetch<Cfg::DIRECT>(ra, l, pa, args.lda, offa[l], w.rows_a, Cfg::A_KC ? w.safe_a : w.safe_a - k0, tid);
-      else LB::template fetch<Cfg::DIRECT>(rb, l - LA::U, pb, args.ldb, offb[l - LA::U], w.rows_b, Cfg::B_KC ? w.safe_b : w.safe_b - k0, tid);
+    auto fetch = [&](int l, const int set, const char *pa, const char *pb, int64_t k0) { // (k0: the step's first K-value)
+      constexpr bool FAST = Cfg::DIRECT, CAREFUL = Cfg::CAREFUL;
+      if (l < LA::U)
+        LA::template fetch<FAST, CAREFUL>(ra[set], l, pa, args.lda, offa[l], w.rows_a, Cfg::A_KC ? w.safe_a : w.safe_a - k0, tid);
+      else
+        LB::template fetch<FAST, CAREFUL>(rb[set], l - LA::U, pb, args.ldb, offb[l - LA::U], w.rows_b, Cfg::B_KC ? w.safe_b : w.safe_b - k0, tid);
+    };
+    auto ask = [&](int s, const int set) {
+      const char *pa = a_at(s), *pb = b_at(s);
+#pragma unroll
+      for (int l = 0; l < LOADS; l++) fetch(l, set, pa, pb, (int64_t)(s - partial) * BK);
     };
     if (steps > 0) {
-      const char *pa = a_at(0), *pb = b_at(0);
       if (partial) {
+        const char *pa = a_at(0), *pb = b_at(0);
 #pragma unroll
-        for (int u = 0; u < LA::U; u++) LA::fetch_tail(ra, u, pa, args.lda, w.rows_a, left, Cfg::A_KC ? w.safe_a : w.safe_a - whole * BK, tid);
+        for (int u = 0; u < LA::U; u++)
+          LA::fetch_tail(ra[0], u, pa, args.lda, w.rows_a, left, Cfg::A_KC ? w.safe_a : w.safe_a - whole * BK, tid);
 #pragma unroll
-        for (int u = 0; u < UB; u++) LB::fetch_tail(rb, u, pb, args.ldb, w.rows_b, left, Cfg::B_KC ? w.safe_b : w.safe_b - whole * BK, tid);
+        for (int u = 0; u < UB; u++)
+          LB::fetch_tail(rb[0], u, pb, args.ldb, w.rows_b, left, Cfg::B_KC ? w.safe_b : w.safe_b - whole * BK, tid);
       } else {
-#pragma unroll
-        for (int l = 0; l < LOADS; l++) fetch(l, pa, pb, 0);
+        ask(0, 0);
       }
+      if (SETS > 1 && steps > 1) ask(1, SETS - 1);
 #pragma unroll
-      for (int l = 0; l < LOADS; l++) put(l, lds);
-      if (steps > 1) {
-        pa = a_at(1), pb = b_at(1);
-#pragma unroll
-        for (int l = 0; l < LOADS; l++) fetch(l, pa, pb, (int64_t)(1 - partial) * BK);
-      }
+      for (int l = 0; l < LOADS; l++) put(l, 0, lds);
+      if (steps > SETS) ask(SETS, 0);
       block_sync_lds();
     }
-    for (int s = 0; s < steps - 1; s++) {
-      const int ask = s + 2 < steps ? s + 2 : s + 1; // (the last time: the same step again, unused)
-      const char *pa = a_at(ask), *pb = b_at(ask);
+    // step s: s + 1 goes to LDS from its set (the steps' take turns), and s + 1 + SETS is asked for (the last ones again,
+    // unused)
+    auto run = [&](int s, const int set) {
+      const int far = s + 1 + SETS < steps ? s + 1 + SETS : steps - 1;
+      const char *pa = a_at(far), *pb = b_at(far);
       const char *here = lds + (s & 1) * Cfg::STAGE;
       char *stage = lds + ((s + 1) & 1) * Cfg::STAGE;
       begin(here);
       multiply(here, nullptr, first, end, [&](int g) {
         share(g, [&](int l) {
-          put(l, stage);
-          fetch(l, pa, pb, (int64_t)(ask - partial) * BK);
+          put(l, set, stage);
+          fetch(l, set, pa, pb, (int64_t)(far - partial) * BK);
         });
       });
       block_sync_lds();
+    };
+    int s = 0;
+    for (; s + SETS < steps; s += SETS) {
+      run(s, SETS - 1);
+      if constexpr (SETS > 1) run(s + 1, 0);
     }
+    if (SETS > 1 && s + 1 < steps) run(s++, SETS - 1);
     if (steps > 0) {
       const char *here = lds + ((steps - 1) & 1) * Cfg::STAGE;
       begin(here);

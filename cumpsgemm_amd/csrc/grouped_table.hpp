@@ -13,9 +13,9 @@ struct GroupedTable {
 };
 
 template <Elem E, bool A_KC, bool B_KC, int BM, int BN, int WM, int WN, int ROW_BYTES, int NSTAGE, bool DIRECT, bool RAGGED_K,
-          int OCC = 2>
+          bool CAREFUL = false>
 constexpr GroupedKernel grouped_of() {
-  return grouped_entry<GroupedCfg<E, A_KC, B_KC, BM, BN, WM, WN, ROW_BYTES, NSTAGE, DIRECT, RAGGED_K, OCC>>();
+  return grouped_entry<GroupedCfg<E, A_KC, B_KC, BM, BN, WM, WN, ROW_BYTES, NSTAGE, DIRECT, RAGGED_K, 2, CAREFUL>>();
 }
 
 template <Elem E> constexpr GroupedTable grouped_table_f32() {
@@ -47,6 +47,7 @@ template <Elem E> constexpr GroupedTable grouped_table_16() {
   t.columns[1][1][TILE_128] = grouped_of<E, true, true, 128, 128, 64, 64, 128, 2, true, false>();
   t.columns[1][1][TILE_NARROW] = grouped_of<E, true, true, 128, 32, 32, 32, 128, 4, true, false>();
   t.over_k[0][TILE_128] = grouped_of<E, false, false, 128, 128, 64, 64, 128, 2, false, true>();
+  t.over_k[0][SHORT_LINES] = grouped_of<E, false, false, 128, 128, 64, 64, 128, 2, false, true, true>();
   t.over_k[1][TILE_256] = grouped_of<E, false, false, 256, 256, 128, 64, 128, 2, true, true>();
   t.over_k[1][TILE_128] = grouped_of<E, false, false, 128, 128, 64, 64, 128, 2, true, true>();
   t.stream[0] = stream_entry<E, false>();
