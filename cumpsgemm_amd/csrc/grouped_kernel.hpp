@@ -111,11 +111,18 @@ __device__ inline bool place_tile(const GroupedArgs &args, uint32_t bid, uint32_
     if (args.offsets != nullptr) group_span(args.offsets, g, args.n, lo, hi);
     else hi = args.n;
   };
+  // a lane's group: its span, how many whole columns, how many of the 64 groups up to it have in all
+  uint32_t lo, hi, full, sum;
+  auto look = [&](uint32_t g0) {
+    span_of(g0 + lane, lo, hi);
+    full = (hi - lo) / bn;
+    // (few tokens to a group: no group has a whole column, and nothing is to be added)
+    sum = __ballot(full != 0) != 0 ? wave_inclusive_sum(full, lane) : 0;
+  };
   uint32_t whole = 0, last = 0; // columns of tiles, of all groups
   for (uint32_t g0 = 0; g0 < args.groups; g0 += 64) {
-    uint32_t lo, hi;
-    span_of(g0 + lane, lo, hi);
-    whole += __builtin_amdgcn_readlane(wave_inclusive_sum((hi - lo) / bn, lane), 63);
+    look(g0);
+    whole += __builtin_amdgcn_readlane(sum, 63);
     last += __builtin_popcountll(__ballot((hi - lo) % bn != 0));
   }
   const bool in_whole = bid < whole * tiles_m;
@@ -124,11 +131,11 @@ __device__ inline bool place_tile(const GroupedArgs &args, uint32_t bid, uint32_
   const uint32_t column = id / tiles_m;
   uint32_t before = 0;
   for (uint32_t g0 = 0; g0 < args.groups; g0 += 64) {
-    uint32_t lo, hi;
-    span_of(g0 + lane, lo, hi);
-    const uint32_t full = (hi - lo) / bn, mine = in_whole ? full : (hi - lo) % bn != 0;
-    const uint32_t sum = before + wave_inclusive_sum(mine, lane);
-    const uint64_t beyond = __ballot(column < sum);
+    if (args.groups > 64) look(g0); // (or they are still there)
+    const uint64_t rest = __ballot((hi - lo) % bn != 0);
+    // columns up to this group's last: whole ones, or last ones
+    const uint32_t upto = before + (in_whole ? sum : (uint32_t)__builtin_popcountll(rest & (~0ull >> (63 - lane))));
+    const uint64_t beyond = __ballot(column < upto);
     if (beyond != 0) {
       const int at = __builtin_ctzll(beyond);
       t.group = g0 + at;
@@ -136,7 +143,7 @@ __device__ inline bool place_tile(const GroupedArgs &args, uint32_t bid, uint32_
       t.hi = __builtin_amdgcn_readlane(hi, at);
       if (in_whole) {
         const uint32_t tiles_n = __builtin_amdgcn_readlane(full, at);
-        raster(id - (__builtin_amdgcn_readlane(sum, at) - tiles_n) * tiles_m, tiles_m, tiles_n, t.tm, t.tn);
+        raster(id - (__builtin_amdgcn_readlane(upto, at) - tiles_n) * tiles_m, tiles_m, tiles_n, t.tm, t.tn);
       } else {
         t.tm = id % tiles_m;
         t.tn = __builtin_amdgcn_readlane(full, at);
@@ -144,7 +151,7 @@ __device__ inline bool place_tile(const GroupedArgs &args, uint32_t bid, uint32_
       // (offsets out of order can make these sums overflow: no tile outside its group)
       return t.tm < tiles_m && (uint64_t)t.tn * bn < t.hi - t.lo;
     }
-    before = __builtin_amdgcn_readlane(sum, 63);
+    before = __builtin_amdgcn_readlane(upto, 63);
   }
   return false;
 }
@@ -489,15 +496,18 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
   };
   // Row blocks `from` .. `to` - 1 of a step; `beside(g)`: what else is done beside block g.  next: the next step's
   // buffer, if its first fragments are to be read beside the last blocks (it is complete by then).
-  auto multiply = [&](const char *stage, const char *next, auto from, auto to, auto beside) {
+  auto multiply = [&](const char *stage, auto next, auto from, auto to, auto beside) {
+    constexpr bool HAS_NEXT = !std::is_same<decltype(next), std::nullptr_t>::value;
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int g = from.value; g < to.value; g++) {
       const int s = g / TM, i = g % TM;
       if (g + AHEAD_A < BLOCKS) read_a(stage, g + AHEAD_A);
-      else if (next != nullptr) read_a(next, g + AHEAD_A - BLOCKS);
+      else if constexpr (HAS_NEXT) read_a(next, g + AHEAD_A - BLOCKS);
       if (i == (TM > 4 ? TM - 3 : TM > 1 ? TM - 2 : 0) && s + 1 < SLICES) read_b(stage, s + 1, (s + 1) % 2);
-      if (g == BLOCKS - AHEAD_A && next != nullptr) read_b(next, 0, 0);
+      if constexpr (HAS_NEXT) {
+        if (g == BLOCKS - AHEAD_A) read_b(next, 0, 0);
+      }
       beside(g);
 #pragma unroll
       for (int q = 0; q < T::NPROD; q++) {
@@ -553,6 +563,8 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
       if (l < LA::U) LA::direct(l, pa, offa[l], stage, wave);
       else LB::direct(l - LA::U, pb, offb[l - LA::U], stage + Cfg::A_STAGE, wave);
     };
+    // (what the compiler has loaded is waited for here: a wait of its own inside the loop would be one for all loads)
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
     for (int s = 0; s < Cfg::NSTAGE && s < steps; s++) {
       const uint32_t stage = lds0 + s * Cfg::STAGE;
       const char *pa = a_at(s), *pb = b_at(s);
@@ -598,7 +610,7 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
       const uint32_t stage = lds0 + at * Cfg::STAGE;
       const bool more = s + Cfg::NSTAGE < steps;
       // (behind the last step, unused values are read)
-      multiply(here, lds + next * Cfg::STAGE, last, end, [&](int g) {
+      multiply(here, (const char *)lds + next * Cfg::STAGE, last, end, [&](int g) {
         if (more) {
 #pragma unroll
           for (int l = 0; l < LOADS; l++)
