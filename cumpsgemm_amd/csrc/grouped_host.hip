@@ -91,33 +91,39 @@ hipblasStatus_t launched() {
   return hipGetLastError() == hipSuccess ? HIPBLAS_STATUS_SUCCESS : HIPBLAS_STATUS_EXECUTION_FAILED;
 }
 
-// What a kernel takes, in us: fixed + steps * max(alone, each * (workgroups / CUs + 0.2 of a round beyond the first)).
-// alone: a step where a CU has one workgroup; each: of a workgroup's step where they queue.  Fitted to 956 calls (m x k of
-// 512^2 to 4096 x 2048, 1 - 64 groups of 1 - 8192 tokens, uneven by e^(0.4 N(0,1)), op T) with every kernel in turn; what
-// the choice by it loses against the best kernel, as a geometric mean: BF16 4.2 %, 8-bit 5.1 %, FP32 3.6 % (FP16TCEC) and
-// 2.9 % (TF32TCEC).  By tokens to a group alone (192, 48, 8) it was 25, 28, 21 and 28 %.
+// What a kernel takes, in us: fixed + steps * part * max(alone, each * (workgroups / CUs + 0.2 of a round beyond the first)).
+// alone: a step where a CU has one workgroup; each: of a workgroup's step where they queue; part: of a step for tiles with
+// `filled` of their columns, least + (1 - least) * filled.  Fitted to 956 calls (m x k of 512^2 to 4096 x 2048, 1 - 64 groups
+// of 1 - 8192 tokens, uneven by e^(0.4 N(0,1)), op T) with every kernel in turn; what the choice by it loses against the
+// best kernel, as a geometric mean: BF16 2.9 %, 8-bit 2.7 %, FP32 2.5 % in two and in three terms.  By tokens to a group
+// alone (192, 48, 8) it was 25, 28, 21 and 28 %.
 struct Cost {
   float fixed, alone, each;
   int slots, step; // workgroups to a CU; K-values of a step (the kernel of few tokens: of its eight waves)
+  float least;
 };
 const Cost &cost_of(Elem e, int cls) {
-  static const Cost sixteen[4] = {{7.5f, 0.69f, 1.69f, 1, 64}, {5.1f, 0.45f, 0.67f, 2, 64}, {5.4f, 0.24f, 0.37f, 2, 64}, {4.9f, 0.66f, 0.71f, 2, 512}};
-  static const Cost eight[4] = {{10.2f, 0.62f, 1.77f, 1, 128}, {6.7f, 0.33f, 0.74f, 2, 128}, {4.9f, 0.31f, 0.51f, 2, 128}, {4.0f, 0.85f, 0.86f, 2, 1024}};
-  static const Cost fp32[4] = {{8.7f, 0.76f, 1.59f, 1, 32}, {5.2f, 0.58f, 0.87f, 1, 32}, {5.2f, 0.48f, 0.52f, 3, 32}, {4.5f, 0.61f, 0.78f, 2, 256}};
-  static const Cost fp32x3[4] = {{11.3f, 1.24f, 2.24f, 1, 32}, {6.3f, 0.91f, 1.27f, 1, 32}, {6.4f, 0.66f, 0.64f, 2, 32}, {4.8f, 0.63f, 0.78f, 2, 256}};
+  static const Cost sixteen[4] = {{4.4f, 1.38f, 2.33f, 1, 64, 0.46f}, {4.0f, 0.58f, 0.75f, 2, 64, 0.67f},
+                                  {4.4f, 0.24f, 0.39f, 2, 64, 1.00f}, {3.4f, 0.90f, 0.96f, 2, 512, 0.41f}};
+  static const Cost eight[4] = {{6.5f, 1.87f, 3.02f, 1, 128, 0.27f}, {5.4f, 0.72f, 0.94f, 2, 128, 0.41f},
+                                {4.7f, 0.24f, 0.42f, 2, 128, 0.87f}, {3.1f, 1.14f, 1.01f, 2, 1024, 0.46f}};
+  static const Cost fp32[4] = {{7.9f, 1.16f, 1.81f, 1, 32, 0.57f}, {5.3f, 0.74f, 1.00f, 1, 32, 0.64f},
+                               {4.6f, 0.55f, 0.51f, 3, 32, 0.99f}, {3.8f, 0.89f, 0.98f, 2, 256, 0.43f}};
+  static const Cost fp32x3[4] = {{11.7f, 2.08f, 2.77f, 1, 32, 0.40f}, {7.5f, 1.18f, 1.50f, 1, 32, 0.56f},
+                                 {6.1f, 0.75f, 0.63f, 2, 32, 0.88f}, {3.9f, 0.90f, 0.99f, 2, 256, 0.42f}};
   return (e == Elem::I8 ? eight : e == Elem::F32_BF16X3 ? fp32x3 : (int)e <= 3 ? fp32 : sixteen)[cls];
 }
 // The same for products over K (342 calls, 1 - 64 groups of 16 - 16384 tokens, results of 256^2 - 4096 x 2048, K in 1 - 16
 // parts, both tiles): a group's K can be longer than the average one's, which counts where a CU has one workgroup, and parts
 // are written and read once more, 3.2 TB/s.  Loses 3.6 % (BF16), 2.0 % (FP16TCEC) and 2.1 % (TF32TCEC).
 const Cost &cost_over_k(Elem e, int cls) {
-  static const Cost sixteen[2] = {{11.4f, 1.23f, 2.32f, 1, 64}, {7.3f, 0.65f, 0.67f, 2, 64}};
-  static const Cost fp32[2] = {{11.6f, 1.27f, 1.89f, 1, 32}, {7.2f, 0.86f, 1.13f, 1, 32}};
-  static const Cost fp32x3[2] = {{14.7f, 2.10f, 3.00f, 1, 32}, {6.7f, 1.24f, 1.61f, 1, 32}};
+  static const Cost sixteen[2] = {{11.4f, 1.23f, 2.32f, 1, 64, 1.0f}, {7.3f, 0.65f, 0.67f, 2, 64, 1.0f}};
+  static const Cost fp32[2] = {{11.6f, 1.27f, 1.89f, 1, 32, 1.0f}, {7.2f, 0.86f, 1.13f, 1, 32, 1.0f}};
+  static const Cost fp32x3[2] = {{14.7f, 2.10f, 3.00f, 1, 32, 1.0f}, {6.7f, 1.24f, 1.61f, 1, 32, 1.0f}};
   return (e == Elem::F32_BF16X3 ? fp32x3 : (int)e <= 3 ? fp32 : sixteen)[cls];
 }
-double cost_us(const Cost &c, double workgroups, double steps, double cus) {
-  return c.fixed + steps * std::max<double>(c.alone, c.each * (workgroups / cus + (workgroups > cus * c.slots ? 0.2 * c.slots : 0.0)));
+double cost_us(const Cost &c, double workgroups, double steps, double cus, double filled = 1.0) {
+  return c.fixed + steps * (c.least + (1.0 - c.least) * filled) * std::max<double>(c.alone, c.each * (workgroups / cus + (workgroups > cus * c.slots ? 0.2 * c.slots : 0.0)));
 }
 // CUMPSGEMM_FORCE_TILE_CLASS goes before the rule where there is such a kernel.
 bool forced(Elem e, bool a_kc, bool ragged_k, bool direct, int &cls) {
@@ -154,7 +160,8 @@ hipblasStatus_t run_columns(cuMpSGEMM_handle *h, Elem e, bool a_kc, GroupedArgs 
       const Cost &cost = cost_of(e, c);
       // (the kernel of few tokens: in workgroups of 16 rows, as fitted; where rows are contiguous it has 64 in one)
       const double rows = c == STREAM ? (args.m + 15) / 16 : (args.m + kern->bm - 1) / kern->bm;
-      const double us = cost_us(cost, columns * rows, (args.k + cost.step - 1) / cost.step, h->num_cus);
+      const double us = cost_us(cost, columns * rows, (args.k + cost.step - 1) / cost.step, h->num_cus,
+                                std::min(1.0, each / kern->bn));
       if (best == 0.0 || us < best) best = us, cls = c;
     }
   }
