@@ -226,6 +226,10 @@ template <Elem E, bool KC, int ROWS, int ROW_BYTES, int NT> struct grouped_loade
     }
   }
 
+  // FP32: the K-value of the step that stands at place j of the chunk of place k on.  Any order will do that both operands
+  // have.
+  __device__ static constexpr int value_of(int k, int j) { return k / 2 + (j & 3) + (j >> 2) * 16; }
+
   // Byte offset from the tile's origin (row 0, K-value 0 of the step) of the unit that fills position id.
   // `rows`: those that exist; one (LINES: eight) beyond them reads the last again (its products are not stored).
   __device__ static inline uint64_t offset(int id, uint64_t ld, int rows) {
@@ -233,6 +237,7 @@ template <Elem E, bool KC, int ROWS, int ROW_BYTES, int NT> struct grouped_loade
     at(id, row, k);
     const int last = LINES ? (rows - 1) & ~7 : rows - 1;
     row = row < last ? row : last;
+    if constexpr (T::F32) k = value_of(k, 0);
     return (KC ? (uint64_t)row * ld + k : (uint64_t)k * ld + row) * T::BYTES;
   }
 
@@ -268,7 +273,7 @@ template <Elem E, bool KC, int ROWS, int ROW_BYTES, int NT> struct grouped_loade
     if constexpr (T::F32 && KC) {
       typedef float f4u_t __attribute__((ext_vector_type(4), aligned(4)));
       const f4u_t *p = reinterpret_cast<const f4u_t *>(base + off);
-      const f4u_t x = p[0], y = p[1];
+      const f4u_t x = p[0], y = p[4];
       r.v[u] = f8_t{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
     } else if constexpr (T::F32 && FAST) {
       // the descriptor holds the uniform base, the scalar offset picks the K-line: no vector arithmetic
@@ -276,11 +281,11 @@ template <Elem E, bool KC, int ROWS, int ROW_BYTES, int NT> struct grouped_loade
       const uint32_t line = __builtin_amdgcn_readfirstlane((uint32_t)ld * 4u);
 #pragma unroll
       for (int j = 0; j < 8; j++)
-        r.v[u][j] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rsrc, off, j * line, 0));
+        r.v[u][j] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rsrc, off, value_of(0, j) * line, 0));
     } else if constexpr (T::F32) {
       const float *p = reinterpret_cast<const float *>(base + off);
 #pragma unroll
-      for (int j = 0; j < 8; j++) r.v[u][j] = p[(uint64_t)j * ld];
+      for (int j = 0; j < 8; j++) r.v[u][j] = p[(uint64_t)value_of(0, j) * ld];
     } else {
       // (rows of 16-bit values may begin anywhere: the type promises no more and leaves the instruction to the compiler)
       typedef uint32_t u4u2_t __attribute__((ext_vector_type(4), aligned(2)));
@@ -310,8 +315,9 @@ template <Elem E, bool KC, int ROWS, int ROW_BYTES, int NT> struct grouped_loade
       // (without branches: a value past the end is read from the step's first K-value and replaced)
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        const bool in = k + j < left;
-        const float x = p[in ? (uint64_t)(k + j) * step : 0];
+        const int at = value_of(k, j);
+        const bool in = at < left;
+        const float x = p[in ? (uint64_t)at * step : 0];
         r.v[u][j] = in ? x : 0.0f;
       }
     } else {
@@ -496,7 +502,8 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
   };
   // Row blocks `from` .. `to` - 1 of a step; `beside(g)`: what else is done beside block g.  next: the next step's
   // buffer, if its first fragments are to be read beside the last blocks (it is complete by then).
-  auto multiply = [&](const char *stage, auto next, auto from, auto to, auto beside) {
+  // par: which set the step's first columns are in.
+  auto multiply = [&](const char *stage, auto next, auto from, auto to, const int par, auto beside) {
     constexpr bool HAS_NEXT = !std::is_same<decltype(next), std::nullptr_t>::value;
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -504,9 +511,9 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
       const int s = g / TM, i = g % TM;
       if (g + AHEAD_A < BLOCKS) read_a(stage, g + AHEAD_A);
       else if constexpr (HAS_NEXT) read_a(next, g + AHEAD_A - BLOCKS);
-      if (i == (TM > 4 ? TM - 3 : TM > 1 ? TM - 2 : 0) && s + 1 < SLICES) read_b(stage, s + 1, (s + 1) % 2);
+      if (i == (TM > 4 ? TM - 3 : TM > 1 ? TM - 2 : 0) && s + 1 < SLICES) read_b(stage, s + 1, (s + 1 + par) % 2);
       if constexpr (HAS_NEXT) {
-        if (g == BLOCKS - AHEAD_A) read_b(next, 0, 0);
+        if (g == BLOCKS - AHEAD_A) read_b(next, 0, (SLICES + par) % 2);
       }
       beside(g);
 #pragma unroll
@@ -515,7 +522,7 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
         const int ac = T::F32 ? prec_traits<T::P>::ACC[q] : 0;
 #pragma unroll
         for (int j = 0; j < TN; j++)
-          acc[ac][j][i] = grouped_mfma<Cfg::E>(fa[g % RING][pa], fb[s % 2][pb][j], acc[ac][j][i]);
+          acc[ac][j][i] = grouped_mfma<Cfg::E>(fa[g % RING][pa], fb[(s + par) % 2][pb][j], acc[ac][j][i]);
       }
       if constexpr (T::F32) {
         // the splitting between the MFMAs, not in front of them: both waves of a SIMD pass the barrier together
@@ -596,7 +603,7 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
       const bool rest = s > 0 && s - 1 + Cfg::NSTAGE < steps;
       const char *pa = qa - a_step, *pb = qb - b_step;
       const uint32_t old_stage = lds0 + before * Cfg::STAGE;
-      multiply(here, nullptr, first, last, [&](int g) {
+      multiply(here, nullptr, first, last, 0, [&](int g) {
         if (rest) {
 #pragma unroll
           for (int l = 0; l < LOADS; l++)
@@ -610,7 +617,7 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
       const uint32_t stage = lds0 + at * Cfg::STAGE;
       const bool more = s + Cfg::NSTAGE < steps;
       // (behind the last step, unused values are read)
-      multiply(here, (const char *)lds + next * Cfg::STAGE, last, end, [&](int g) {
+      multiply(here, (const char *)lds + next * Cfg::STAGE, last, end, 0, [&](int g) {
         if (more) {
 #pragma unroll
           for (int l = 0; l < LOADS; l++)
@@ -626,13 +633,16 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
     // through registers: step s + 1 is written to LDS and step s + 2 asked for beside the MFMAs of step s
     static_assert(Cfg::NSTAGE == 2 || (Cfg::DIRECT && !T::F32), "two buffers");
     // which of a step's units (A's, then B's) come beside row block g
-    auto share = [](int g, auto f) {
+    auto share = [](int g, int blocks, auto f) {
 #pragma unroll
       for (int l = 0; l < LOADS; l++)
-        if (l * BLOCKS / LOADS == g) f(l);
+        if (l * blocks / LOADS == g) f(l);
     };
     // SETS of registers: 16-bit and 8-bit operands, whose steps are shorter than a load's way, are asked for a step earlier
-    constexpr int SETS = T::F32 ? 1 : 2;
+    constexpr int SETS = T::F32 && T::NACC * Cfg::TM * Cfg::TN * 4 >= 128 ? 1 : 2;
+    // EARLY: the barrier comes before a step's last row block, beside which the next step's first fragments are read
+    constexpr bool EARLY = T::F32 && SETS > 1;
+    constexpr std::integral_constant<int, BLOCKS - AHEAD_A> last;
     typename LA::Regs ra[SETS];
     typename LB::Regs rb[SETS];
     auto put = [&](int l, const int set, char *stage) {
@@ -668,33 +678,46 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
       for (int l = 0; l < LOADS; l++) put(l, 0, lds);
       if (steps > SETS) ask(SETS, 0);
       block_sync_lds();
+      if (EARLY) begin(lds);
     }
     // step s: s + 1 goes to LDS from its set (the steps' take turns), and s + 1 + SETS is asked for (the last ones again,
     // unused)
-    auto run = [&](int s, const int set) {
+    auto run = [&](int s, const int set, const int par) {
       const int far = s + 1 + SETS < steps ? s + 1 + SETS : steps - 1;
       const char *pa = a_at(far), *pb = b_at(far);
       const char *here = lds + (s & 1) * Cfg::STAGE;
       char *stage = lds + ((s + 1) & 1) * Cfg::STAGE;
-      begin(here);
-      multiply(here, nullptr, first, end, [&](int g) {
-        share(g, [&](int l) {
+      auto beside = [&](int g) {
+        share(g, EARLY ? last.value : BLOCKS, [&](int l) {
           put(l, set, stage);
           fetch(l, set, pa, pb, (int64_t)(far - partial) * BK);
         });
-      });
-      block_sync_lds();
+      };
+      if constexpr (EARLY) {
+        multiply(here, nullptr, first, last, par, beside);
+        block_sync_lds();
+        multiply(here, (const char *)stage, last, end, par, nothing);
+      } else {
+        begin(here);
+        multiply(here, nullptr, first, end, 0, beside);
+        block_sync_lds();
+      }
     };
     int s = 0;
     for (; s + SETS < steps; s += SETS) {
-      run(s, SETS - 1);
-      if constexpr (SETS > 1) run(s + 1, 0);
+      run(s, SETS - 1, 0);
+      if constexpr (SETS > 1) run(s + 1, 0, 1);
     }
-    if (SETS > 1 && s + 1 < steps) run(s++, SETS - 1);
-    if (steps > 0) {
+    auto finish = [&](const int par) {
       const char *here = lds + ((steps - 1) & 1) * Cfg::STAGE;
-      begin(here);
-      multiply(here, nullptr, first, end, nothing);
+      if (!EARLY) begin(here);
+      multiply(here, nullptr, first, end, EARLY ? par : 0, nothing);
+    };
+    if (SETS > 1 && s + 1 < steps) {
+      run(s, SETS - 1, 0);
+      finish(1);
+    } else if (steps > 0) {
+      finish(0);
     }
   }
 
