@@ -475,10 +475,9 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
   // many MFMAs: one) in a ring of four, columns in two sets.
   constexpr int BLOCKS = SLICES * TM, AHEAD_A = T::F32 ? 1 : 2, RING = T::F32 ? 2 : 4;
   static_assert(BLOCKS % RING == 0, "a step begins where the ring does");
-#ifndef GROUPED_VALU
-#define GROUPED_VALU 3
-#endif
-  constexpr int SCHED_VALU = GROUPED_VALU;
+  constexpr int SCHED_VALU = 3; // vector instructions beside an MFMA of FP32 operands (two waves of a SIMD take turns)
+  // IN_PLACE: no registers are left for a second set of columns
+  constexpr bool IN_PLACE = T::F32 && T::NACC * Cfg::TM * Cfg::TN * 4 >= 128;
   u4_t fa[RING][T::NP], fb[2][T::NP][TN];
   auto read_a = [&](const char *stage, const int g) {
 #pragma unroll
@@ -486,13 +485,15 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
       fa[g % RING][p] = frag(stage, wm * Cfg::WM + (g % TM) * 16, p, g / TM, std::integral_constant<bool, Cfg::A_KC>{},
                              std::integral_constant<int, BM>{});
   };
+  auto frag_b = [&](const char *stage, const int p, const int j, const int s) {
+    return frag(stage + Cfg::A_STAGE, (j * Cfg::WAVES_N + wn) * 16, p, s, std::integral_constant<bool, Cfg::B_KC>{},
+                std::integral_constant<int, BN>{});
+  };
   auto read_b = [&](const char *stage, const int s, const int set) { // (set: of fragments)
 #pragma unroll
     for (int p = 0; p < T::NP; p++)
 #pragma unroll
-      for (int j = 0; j < TN; j++)
-        fb[set][p][j] = frag(stage + Cfg::A_STAGE, (j * Cfg::WAVES_N + wn) * 16, p, s, std::integral_constant<bool, Cfg::B_KC>{},
-                             std::integral_constant<int, BN>{});
+      for (int j = 0; j < TN; j++) fb[set][p][j] = frag_b(stage, p, j, s);
   };
   // the fragments that a step's first MFMAs need
   auto begin = [&](const char *stage) {
@@ -513,7 +514,7 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
       else if constexpr (HAS_NEXT) read_a(next, g + AHEAD_A - BLOCKS);
       if (i == (TM > 4 ? TM - 3 : TM > 1 ? TM - 2 : 0) && s + 1 < SLICES) read_b(stage, s + 1, (s + 1 + par) % 2);
       if constexpr (HAS_NEXT) {
-        if (g == BLOCKS - AHEAD_A) read_b(next, 0, (SLICES + par) % 2);
+        if (!IN_PLACE && g == BLOCKS - AHEAD_A) read_b(next, 0, (SLICES + par) % 2);
       }
       beside(g);
 #pragma unroll
@@ -523,6 +524,17 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
 #pragma unroll
         for (int j = 0; j < TN; j++)
           acc[ac][j][i] = grouped_mfma<Cfg::E>(fa[g % RING][pa], fb[(s + par) % 2][pb][j], acc[ac][j][i]);
+        if constexpr (HAS_NEXT && IN_PLACE) {
+          // a term's columns are read again behind the last product that has the old ones
+          __builtin_amdgcn_sched_barrier(0);
+          bool later = false;
+#pragma unroll
+          for (int q2 = q + 1; q2 < T::NPROD; q2++) later |= prec_traits<T::P>::PB[q2] == pb;
+          if (!later) {
+#pragma unroll
+            for (int j = 0; j < TN; j++) fb[par][pb][j] = frag_b(next, pb, j, 0);
+          }
+        }
       }
       if constexpr (T::F32) {
         // the splitting between the MFMAs, not in front of them: both waves of a SIMD pass the barrier together
@@ -639,9 +651,9 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
         if (l * blocks / LOADS == g) f(l);
     };
     // SETS of registers: 16-bit and 8-bit operands, whose steps are shorter than a load's way, are asked for a step earlier
-    constexpr int SETS = T::F32 && T::NACC * Cfg::TM * Cfg::TN * 4 >= 128 ? 1 : 2;
+    constexpr int SETS = IN_PLACE ? 1 : 2;
     // EARLY: the barrier comes before a step's last row block, beside which the next step's first fragments are read
-    constexpr bool EARLY = T::F32 && SETS > 1;
+    constexpr bool EARLY = T::F32;
     constexpr std::integral_constant<int, BLOCKS - AHEAD_A> last;
     typename LA::Regs ra[SETS];
     typename LB::Regs rb[SETS];
@@ -715,7 +727,7 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
     };
     if (SETS > 1 && s + 1 < steps) {
       run(s, SETS - 1, 0);
-      finish(1);
+      finish(SETS - 1);
     } else if (steps > 0) {
       finish(0);
     }
