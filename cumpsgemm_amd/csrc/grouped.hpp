@@ -47,6 +47,24 @@ struct GroupedKernel {
 // (grouped_stream.hpp).  Ragged K: the first two, and one for matrices of fewer than eight 16-bit rows or columns.
 enum KernelClass : int { TILE_256 = 0, TILE_128 = 1, TILE_NARROW = 2, SHORT_LINES = 2, kGroupedClasses = 3, STREAM = 3 };
 
+// Ragged K: how the lists of tiles, one for each group and part of its K, are dealt to the eight XCDs.  Each list is cut
+// into 2^log2_shares shares of at most `most` tiles; one after the other goes to the XCDs in turns of eight.
+struct DealOverK {
+  uint32_t log2_shares, most;
+};
+__host__ __device__ inline DealOverK deal_over_k(uint32_t tiles, uint64_t lists, uint32_t groups) {
+  // Groups differ in length, and four shares or more to an XCD even that out; a share is as large as that allows, since
+  // its tiles read the same operands.
+  const uint32_t all = groups == 1 ? 8 : 32;
+  uint32_t log2_shares = 0;
+  while (log2_shares < 3 && (lists << log2_shares) < all) log2_shares++;
+  return {log2_shares, (tiles + (1u << log2_shares) - 1) >> log2_shares};
+}
+inline uint64_t workgroups_over_k(uint32_t tiles, uint64_t lists, uint32_t groups) {
+  const DealOverK d = deal_over_k(tiles, lists, groups);
+  return ((lists << d.log2_shares) + 7) / 8 * 8 * d.most;
+}
+
 // Adds the parts (bm x bn: the tile that they were computed with).
 void launch_grouped_join(const GroupedArgs &args, int bm, int bn, hipStream_t stream);
 

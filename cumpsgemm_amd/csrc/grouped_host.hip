@@ -282,8 +282,10 @@ hipblasStatus_t cuMpSGEMM_gemm_grouped_k(cuMpSGEMM_handle_t h, uint64_t m, uint6
     if (failed) return HIPBLAS_STATUS_EXECUTION_FAILED;
     if (args.partial == nullptr) args.splits = 1; // (no memory, or a graph is being captured)
   }
+  const uint64_t workgroups = workgroups_over_k((uint32_t)per, group_count * args.splits, args.groups);
+  if (workgroups > kMostWorkgroups) return HIPBLAS_STATUS_INVALID_VALUE;
   ProfileScope prof(h, "gemm_grouped_k");
-  kern->launch(args, (uint32_t)(per * group_count * args.splits), h->stream);
+  kern->launch(args, (uint32_t)workgroups, h->stream);
   if (args.splits > 1) launch_grouped_join(args, kern->bm, kern->bn, h->stream);
   return launched();
 }

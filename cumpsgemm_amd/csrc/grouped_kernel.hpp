@@ -156,6 +156,46 @@ __device__ inline bool place_tile(const GroupedArgs &args, uint32_t bid, uint32_
   return false;
 }
 
+// Over K: the tile of workgroup `bid` and its part of K.  False: there is none.  The groups' results are equally many
+// tiles, but take as long as the groups are.  Each XCD (id mod 8) gets shares of several groups' tiles (deal_over_k), and
+// the longest groups come first, so that short ones are left for the CUs that are done early: 8 uneven experts, 16384
+// tokens, 4096 x 2048 in BF16: 307 us; the groups' tiles in contiguous ranges, as for ragged columns, 416 us (even ones:
+// 266 and 293 us).
+__device__ inline bool place_over_k(const GroupedArgs &args, uint32_t bid, uint32_t tiles_m, uint32_t tiles_n, TilePlace &t,
+                                    uint32_t &split) {
+  const uint32_t lists = args.groups * args.splits, per = tiles_m * tiles_n;
+  const DealOverK d = deal_over_k(per, lists, args.groups);
+  const uint32_t turn = bid / 8 / d.most, in = bid / 8 - turn * d.most, xcd = bid % 8;
+  // (every other turn goes the other way round)
+  const uint32_t share = turn * 8 + (turn % 2 ? 7 - xcd : xcd);
+  const uint32_t list = share >> d.log2_shares, part = share & ((1u << d.log2_shares) - 1);
+  if (list >= lists) return false;
+  const uint32_t tile = ((part * per) >> d.log2_shares) + in;
+  if (tile >= ((part + 1) * per) >> d.log2_shares) return false;
+  raster(tile, tiles_m, tiles_n, t.tm, t.tn);
+  t.group = args.splits == 1 ? list : list / args.splits;
+  split = args.splits == 1 ? 0 : list % args.splits;
+  // In place of a group's number its rank, by length in quarters of the mean.  (Not if all tiles are begun at once.  More
+  // groups: their lengths even out; short ones: looking takes as long as they do.)
+  if (args.groups > 1 && args.groups <= 64 && args.k / 128 >= args.groups && (uint64_t)per * lists > 256) {
+    const uint32_t lane = threadIdx.x & 63, quarter = args.k / args.groups / 4;
+    uint32_t lo = 0, hi = 0;
+    if (lane < args.groups) group_span(args.offsets, lane, args.k, lo, hi);
+    uint64_t longer = 0, as_long;
+    for (uint32_t least = 8 * quarter;; least -= quarter) {
+      if (least < quarter) least = 0;
+      as_long = __ballot(lane < args.groups && hi - lo >= least);
+      if (least == 0 || (uint32_t)__builtin_popcountll(as_long) > t.group) break;
+      longer = as_long;
+    }
+    const uint32_t rank = t.group - (uint32_t)__builtin_popcountll(longer);
+    as_long &= ~longer;
+    const uint32_t before = __builtin_amdgcn_mbcnt_hi((uint32_t)(as_long >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)as_long, 0));
+    t.group = __builtin_ctzll(__ballot((as_long >> lane & 1) != 0 && before == rank));
+  }
+  return true;
+}
+
 // DIRECT: 16-bit and 8-bit operands go straight from memory to LDS, 16 aligned bytes a lane; FP32 operands, which are
 // split in registers, are read with 32-bit offsets from uniform bases.  Otherwise: any alignment, any size; but lines of
 // 16-bit values that are shorter than a chunk are for the CAREFUL kernels.
@@ -798,11 +838,9 @@ void grouped_kernel(const GroupedArgs args) {
   const char *a = args.a, *b = args.b;
   w.c = args.c;
   if constexpr (Cfg::RAGGED_K) {
-    const uint32_t tiles_n = (args.n + BN - 1) / BN, per = tiles_m * tiles_n;
-    const uint32_t all = per * args.groups, split_id = xcd_range(blockIdx.x, all * args.splits);
-    const uint32_t id = split_id % all, split = split_id / all;
-    t.group = id / per;
-    raster(id % per, tiles_m, tiles_n, t.tm, t.tn);
+    const uint32_t tiles_n = (args.n + BN - 1) / BN;
+    uint32_t split;
+    if (!place_over_k(args, blockIdx.x, tiles_m, tiles_n, t, split)) return;
     group_span(args.offsets, t.group, args.k, t.lo, t.hi);
     t.lo = __builtin_amdgcn_readfirstlane(t.lo);
     t.hi = __builtin_amdgcn_readfirstlane(t.hi);
