@@ -95,7 +95,7 @@ hipblasStatus_t launched() {
 // alone: a step where a CU has one workgroup; each: of a workgroup's step where they queue; part: of a step for tiles with
 // `filled` of their columns, least + (1 - least) * filled.  Fitted to 956 calls (m x k of 512^2 to 4096 x 2048, 1 - 64 groups
 // of 1 - 8192 tokens, uneven by e^(0.4 N(0,1)), op T) with every kernel in turn; what the choice by it loses against the
-// best kernel, as a geometric mean: BF16 2.9 %, 8-bit 2.7 %, FP32 2.5 % in two and in three terms.  By tokens to a group
+// best kernel, as a geometric mean: BF16 2.9 %, 8-bit 2.7 %, FP32 2.7 % in two and 2.5 % in three terms.  By tokens to a group
 // alone (192, 48, 8) it was 25, 28, 21 and 28 %.
 struct Cost {
   float fixed, alone, each;
@@ -107,19 +107,19 @@ const Cost &cost_of(Elem e, int cls) {
                                   {4.4f, 0.24f, 0.39f, 2, 64, 1.00f}, {3.4f, 0.90f, 0.96f, 2, 512, 0.41f}};
   static const Cost eight[4] = {{6.5f, 1.87f, 3.02f, 1, 128, 0.27f}, {5.4f, 0.72f, 0.94f, 2, 128, 0.41f},
                                 {4.7f, 0.24f, 0.42f, 2, 128, 0.87f}, {3.1f, 1.14f, 1.01f, 2, 1024, 0.46f}};
-  static const Cost fp32[4] = {{7.9f, 1.16f, 1.81f, 1, 32, 0.57f}, {5.3f, 0.74f, 1.00f, 1, 32, 0.64f},
-                               {4.6f, 0.55f, 0.51f, 3, 32, 0.99f}, {3.8f, 0.89f, 0.98f, 2, 256, 0.43f}};
-  static const Cost fp32x3[4] = {{11.7f, 2.08f, 2.77f, 1, 32, 0.40f}, {7.5f, 1.18f, 1.50f, 1, 32, 0.56f},
-                                 {6.1f, 0.75f, 0.63f, 2, 32, 0.88f}, {3.9f, 0.90f, 0.99f, 2, 256, 0.42f}};
+  static const Cost fp32[4] = {{8.1f, 1.03f, 1.71f, 1, 32, 0.61f}, {5.9f, 0.62f, 0.91f, 1, 32, 0.62f},
+                               {6.1f, 0.45f, 0.49f, 3, 32, 1.00f}, {4.0f, 0.90f, 0.99f, 2, 256, 0.42f}};
+  static const Cost fp32x3[4] = {{11.1f, 1.93f, 2.64f, 1, 32, 0.42f}, {7.2f, 1.06f, 1.40f, 1, 32, 0.57f},
+                                 {5.8f, 0.78f, 0.61f, 2, 32, 0.88f}, {4.1f, 0.89f, 0.98f, 2, 256, 0.43f}};
   return (e == Elem::I8 ? eight : e == Elem::F32_BF16X3 ? fp32x3 : (int)e <= 3 ? fp32 : sixteen)[cls];
 }
 // The same for products over K (342 calls, 1 - 64 groups of 16 - 16384 tokens, results of 256^2 - 4096 x 2048, K in 1 - 16
 // parts, both tiles): a group's K can be longer than the average one's, which counts where a CU has one workgroup, and parts
-// are written and read once more, 3.2 TB/s.  Loses 3.6 % (BF16), 2.0 % (FP16TCEC) and 2.1 % (TF32TCEC).
+// are written and read once more, 2.8 TB/s.  Loses 3.6 % (BF16), 2.4 % (FP16TCEC) and 0.8 % (TF32TCEC).
 const Cost &cost_over_k(Elem e, int cls) {
-  static const Cost sixteen[2] = {{11.4f, 1.23f, 2.32f, 1, 64, 1.0f}, {7.3f, 0.65f, 0.67f, 2, 64, 1.0f}};
-  static const Cost fp32[2] = {{11.6f, 1.27f, 1.89f, 1, 32, 1.0f}, {7.2f, 0.86f, 1.13f, 1, 32, 1.0f}};
-  static const Cost fp32x3[2] = {{14.7f, 2.10f, 3.00f, 1, 32, 1.0f}, {6.7f, 1.24f, 1.61f, 1, 32, 1.0f}};
+  static const Cost sixteen[2] = {{11.5f, 1.25f, 2.17f, 1, 64, 1.0f}, {7.5f, 0.66f, 0.60f, 2, 64, 1.0f}};
+  static const Cost fp32[2] = {{12.1f, 1.15f, 1.69f, 1, 32, 1.0f}, {8.4f, 0.74f, 0.96f, 1, 32, 1.0f}};
+  static const Cost fp32x3[2] = {{14.8f, 1.90f, 2.65f, 1, 32, 1.0f}, {8.0f, 1.12f, 1.38f, 1, 32, 1.0f}};
   return (e == Elem::F32_BF16X3 ? fp32x3 : (int)e <= 3 ? fp32 : sixteen)[cls];
 }
 double cost_us(const Cost &c, double workgroups, double steps, double cus, double filled = 1.0) {
@@ -265,7 +265,7 @@ hipblasStatus_t cuMpSGEMM_gemm_grouped_k(cuMpSGEMM_handle_t h, uint64_t m, uint6
     for (uint32_t s = 1; s <= 16; s *= 2) {
       if (s > 1 && (steps < 2.0 * s || tiles * s > 8.0 * h->num_cus)) break;
       const double us = cost_us(cost, tiles * s, steps / s, h->num_cus) +
-                        (s == 1 ? 0.0 : 0.7 + tiles * kern->bm * kern->bn * 4.0 * (s + 1) / 3.2e6);
+                        (s == 1 ? 0.0 : 0.3 + tiles * kern->bm * kern->bn * 4.0 * (s + 1) / 2.8e6);
       if (best == 0.0 || us < best) best = us, cls = c, args.splits = s;
     }
   }
