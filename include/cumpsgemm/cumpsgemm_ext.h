@@ -69,7 +69,7 @@ int cuMpSGEMM_describe_tile_config(int compute_mode, int is_complex, int op_A, i
                                    int tile_class, char *buf, size_t buf_len);
 
 /* Bytes of device memory the handle currently holds as workspace for
- * pre-split operands (0 until a call takes that path; grows on demand; freed
+ * pre-split operands and for the parts of cuMpSGEMM_gemm_grouped_k (0 until a call takes that path; grows on demand; freed
  * by cuMpSGEMM_destroy).  No counterpart in the reference, whose kernels need
  * no workspace beyond the fixed scratch of its handle. */
 size_t cuMpSGEMM_get_workspace_size(cuMpSGEMM_handle_t handle);
@@ -87,7 +87,9 @@ const void *cuMpSGEMM_get_workspace_pointer(cuMpSGEMM_handle_t handle);
  * takes the small-product kernel, 1 - 5: this form of it wherever it can),
  * _NO_EDGE16_TWIN, _NO_FUSED_SCALING,
  * _PERSISTENT_MAX_STEPS, _MAX_WORKSPACE_BYTES) are read from the environment
- * once per process; this reads them again and publishes the new set as one
+ * once per process (the products of experts' layers below look at
+ * _FORCE_TILE_CLASS, 0 - 3: tiles of 256 and 128 rows, of 32 tokens, the kernel
+ * of few tokens, and over K at _FORCE_KSPLIT); this reads them again and publishes the new set as one
  * immutable snapshot.  Safe to call while other threads run GEMMs: a call in
  * flight goes on with the values it has already looked up and may take later
  * ones from the new set.  For tests and experiments.  The reference has no
@@ -179,7 +181,7 @@ hipblasStatus_t cuMpSGEMM_gemm_grouped(cuMpSGEMM_handle_t handle, hipblasOperati
  *   C_g = alpha * A[:, tokens of g] * B[:, tokens of g]^T + beta * C_g
  * A is m x k, B is n x k, a token a column; C_g is m x n at c + g * stridec.  A
  * group without tokens gets beta * C_g (zeros with beta = 0).  beta = 1
- * accumulates.  A call with fewer tiles than CUs takes K in parts, whose sums
+ * accumulates.  A call with few tiles may take K in parts, whose sums
  * pass through the handle's workspace and are added in a fixed order: its first
  * use allocates, as cuMpSGEMM_sgemm's does (cuMpSGEMM_get_workspace_size), and
  * under capture, when it would have to grow, K is taken whole instead (the same
