@@ -113,17 +113,28 @@ const Cost &cost_of(Elem e, int cls) {
                                  {5.8f, 0.78f, 0.61f, 2, 32, 0.88f}, {4.1f, 0.89f, 0.98f, 2, 256, 0.43f}};
   return (e == Elem::I8 ? eight : e == Elem::F32_BF16X3 ? fp32x3 : (int)e <= 3 ? fp32 : sixteen)[cls];
 }
-// The same for products over K (342 calls, 1 - 64 groups of 16 - 16384 tokens, results of 256^2 - 4096 x 2048, K in 1 - 16
-// parts, both tiles): a group's K can be longer than the average one's, which counts where a CU has one workgroup, and parts
-// are written and read once more, 2.8 TB/s.  Loses 3.6 % (BF16), 2.4 % (FP16TCEC) and 0.8 % (TF32TCEC).
-const Cost &cost_over_k(Elem e, int cls) {
-  static const Cost sixteen[2] = {{11.5f, 1.25f, 2.17f, 1, 64, 1.0f}, {7.5f, 0.66f, 0.60f, 2, 64, 1.0f}};
-  static const Cost fp32[2] = {{12.1f, 1.15f, 1.69f, 1, 32, 1.0f}, {8.4f, 0.74f, 0.96f, 1, 32, 1.0f}};
-  static const Cost fp32x3[2] = {{14.8f, 1.90f, 2.65f, 1, 32, 1.0f}, {8.0f, 1.12f, 1.38f, 1, 32, 1.0f}};
-  return (e == Elem::F32_BF16X3 ? fp32x3 : (int)e <= 3 ? fp32 : sixteen)[cls];
-}
 double cost_us(const Cost &c, double workgroups, double steps, double cus, double filled = 1.0) {
   return c.fixed + steps * (c.least + (1.0 - c.least) * filled) * std::max<double>(c.alone, c.each * (workgroups / cus + (workgroups > cus * c.slots ? 0.2 * c.slots : 0.0)));
+}
+// For products over K (342 calls, 1 - 64 groups of 16 - 16384 tokens, results of 256^2 - 4096 x 2048, K in 1 - 16 parts, both
+// tiles), whose groups often have a few steps only: every round of tiles also costs `round`, their first loads and the
+// write-out; a group's K can be longer than the average one's, which counts where a CU has one workgroup; and parts are
+// written and read once more, at 5.3 TB/s.  Loses 1.4 % (BF16), 2.0 % (FP16TCEC) and 0.4 % (TF32TCEC); without `round`
+// 3.6, 2.4 and 0.8 %.
+struct CostOverK {
+  float fixed, alone, each, round;
+  int slots, step;
+};
+double cost_over_k_us(Elem e, int cls, double tiles, double tile_bytes, double k, bool groups, uint32_t splits, double cus) {
+  static const CostOverK sixteen[2] = {{12.3f, 1.29f, 1.57f, 15.8f, 1, 64}, {6.0f, 0.70f, 0.47f, 3.8f, 2, 64}};
+  static const CostOverK fp32[2] = {{10.8f, 1.18f, 1.43f, 10.9f, 1, 32}, {6.7f, 0.76f, 0.83f, 5.3f, 1, 32}};
+  static const CostOverK fp32x3[2] = {{13.9f, 1.94f, 2.29f, 14.9f, 1, 32}, {6.5f, 1.13f, 1.25f, 5.1f, 1, 32}};
+  const CostOverK &c = (e == Elem::F32_BF16X3 ? fp32x3 : (int)e <= 3 ? fp32 : sixteen)[cls];
+  const double steps = k / c.step + 0.5, workgroups = tiles * splits, rounds = workgroups / cus;
+  if (splits > 1 && steps < 2.0 * splits) return 1e30; // (two steps to a part, at least)
+  return c.fixed + c.round * std::max(0.0, rounds - 1.0) +
+         steps / splits * std::max<double>(c.alone * (groups ? 1.6 : 1.0), c.each * (rounds + (rounds > c.slots ? 0.1 * c.slots : 0.0))) +
+         (splits == 1 ? 0.0 : 3.0 + tiles * tile_bytes * (splits + 1) / 5.3e6);
 }
 // CUMPSGEMM_FORCE_TILE_CLASS goes before the rule where there is such a kernel.
 bool forced(Elem e, bool a_kc, bool ragged_k, bool direct, int &cls) {
@@ -258,14 +269,11 @@ hipblasStatus_t cuMpSGEMM_gemm_grouped_k(cuMpSGEMM_handle_t h, uint64_t m, uint6
   for (int c = fixed_cls ? cls : (int)TILE_256; c <= (fixed_cls ? cls : (int)TILE_128); c++) {
     const GroupedKernel *const kern = lookup_grouped(e, false, true, direct, c);
     if (kern == nullptr) continue;
-    Cost cost = cost_over_k(e, c == SHORT_LINES ? (int)TILE_128 : c);
-    if (group_count > 1) cost.alone *= 1.6f;
     const double tiles = (double)((m + kern->bm - 1) / kern->bm) * ((n + kern->bn - 1) / kern->bn) * group_count;
-    const double steps = (double)k / group_count / cost.step + 0.5;
     for (uint32_t s = 1; s <= 16; s *= 2) {
-      if (s > 1 && (steps < 2.0 * s || tiles * s > 8.0 * h->num_cus)) break;
-      const double us = cost_us(cost, tiles * s, steps / s, h->num_cus) +
-                        (s == 1 ? 0.0 : 0.3 + tiles * kern->bm * kern->bn * 4.0 * (s + 1) / 2.8e6);
+      if (s > 1 && tiles * s > 8.0 * h->num_cus) break;
+      const double us = cost_over_k_us(e, c == SHORT_LINES ? (int)TILE_128 : c, tiles, kern->bm * kern->bn * 4.0,
+                                       (double)k / group_count, group_count > 1, s, h->num_cus);
       if (best == 0.0 || us < best) best = us, cls = c, args.splits = s;
     }
   }
