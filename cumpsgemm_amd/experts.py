@@ -22,7 +22,16 @@ def group_by_expert(experts, count):
 
 def _type(t):
     import torch
-    return {torch.float32: lib.R_32F, torch.float16: lib.R_16F, torch.bfloat16: lib.R_16BF}[t.dtype]
+    types = {torch.float32: lib.R_32F, torch.float16: lib.R_16F, torch.bfloat16: lib.R_16BF}
+    if t.dtype not in types:
+        raise ValueError(f"{t.dtype}: not FP32, FP16 or BF16")
+    return types[t.dtype]
+
+
+def _expect(name, t, dtype):
+    """The library is given addresses and one type for all operands: ValueError for a tensor that is of another."""
+    if t.dtype != dtype:
+        raise ValueError(f"{name} is of {t.dtype}, not of {dtype}")
 
 
 def _check(status):
@@ -35,12 +44,14 @@ class Experts:
     mode: how FP32 operands are multiplied."""
 
     def __init__(self, handle, weights, mode=lib.FP16TCEC):
+        _type(weights)
         self.handle, self.weights, self.mode = handle, weights.contiguous(), mode
 
     def forward(self, x, experts):
-        """(y, what backward needs)"""
+        """(y, what backward needs); x and y are of the weights' type"""
         import torch
         w = self.weights
+        _expect("x", x, w.dtype)
         count, out, inner = w.shape
         order, offsets = group_by_expert(experts, count)
         grouped = x[order]
@@ -54,6 +65,8 @@ class Experts:
         import torch
         grouped, order, offsets = saved
         w = self.weights
+        _expect("what forward saved", grouped, w.dtype)
+        _expect("dy", dy, w.dtype)
         count, out, inner = w.shape
         dy = dy[order]
         dx = torch.empty_like(grouped)
@@ -81,11 +94,15 @@ class Int8Experts:
     """weights: [experts, features out, features in] 8-bit integers, scale: [experts, features out]."""
 
     def __init__(self, handle, weights, scale):
+        import torch
+        _expect("weights", weights, torch.int8)
+        _expect("scale", scale, torch.float32)
         self.handle, self.weights, self.scale = handle, weights, scale
 
     def forward(self, x, experts):
         """x in FP32, FP16 or BF16, a scale taken for each token; y of the same type"""
         import torch
+        _type(x)
         count, out, inner = self.weights.shape
         order, offsets = group_by_expert(experts, count)
         grouped = x[order]

@@ -1,0 +1,146 @@
+"""What the layers of cumpsgemm_amd/experts.py refuse, and what they make of tokens, types and streams, on the CPU: in the
+handle's place stands one that computes the products from the addresses, types and sizes that it is given, as the library does."""
+import itertools
+
+import pytest
+import torch
+
+import cumpsgemm_amd as cg
+from cumpsgemm_amd import experts
+
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+class CpuHandle:
+    """The library's calls on tensors in host memory.  Reading or writing past the end of one raises (as_strided does)."""
+    TYPES = {cg.R_32F: torch.float32, cg.R_16F: torch.float16, cg.R_16BF: torch.bfloat16}
+
+    def __init__(self):
+        self.calls, self.modes, self.streams = 0, [], []
+
+    def set_stream(self, stream):
+        self.streams.append(stream)
+        return 0
+
+    @staticmethod
+    def memory(t, dtype, shape, strides):
+        """What lies at t's address, as `dtype`."""
+        flat = torch.as_strided(t, (t.untyped_storage().nbytes() // t.element_size() - t.storage_offset(),), (1,)).view(dtype)
+        return torch.as_strided(flat, shape, strides)
+
+    @staticmethod
+    def spans(offsets, groups, count):
+        for g in range(groups):
+            lo = min(max(int(offsets[g]), 0), count)
+            yield g, lo, max(lo, min(int(offsets[g + 1]), count))
+
+    def gemm_grouped(self, op, m, n, k, alpha, a, lda, stridea, b, ldb, beta, c, ldc, offsets, groups, mode, type_ab, type_c):
+        self.calls += 1
+        self.modes.append(("columns", mode))
+        rows, cols = (k, m) if op == cg.OP_N else (m, k)
+        a = self.memory(a, self.TYPES[type_ab], (groups, rows, cols), (stridea, lda, 1))
+        b = self.memory(b, self.TYPES[type_ab], (n, k), (ldb, 1))
+        c = self.memory(c, self.TYPES[type_c], (n, m), (ldc, 1))
+        for g, lo, hi in self.spans(offsets, groups, n):
+            y = alpha * (b[lo:hi].double() @ (a[g] if op == cg.OP_N else a[g].t()).double())
+            c[lo:hi] = (y if beta == 0 else y + beta * c[lo:hi].double()).to(c.dtype)
+        return 0
+
+    def gemm_grouped_k(self, m, n, k, alpha, a, lda, b, ldb, beta, c, ldc, stridec, offsets, groups, mode, type_ab, type_c):
+        self.calls += 1
+        self.modes.append(("over k", mode))
+        a = self.memory(a, self.TYPES[type_ab], (k, m), (lda, 1))
+        b = self.memory(b, self.TYPES[type_ab], (k, n), (ldb, 1))
+        c = self.memory(c, self.TYPES[type_c], (groups, n, m), (stridec, ldc, 1))
+        for g, lo, hi in self.spans(offsets, groups, k):
+            y = alpha * (b[lo:hi].t().double() @ a[lo:hi].double())
+            c[g] = (y if beta == 0 else y + beta * c[g].double()).to(c.dtype)
+        return 0
+
+    def quantize_i8(self, k, n, x, ldx, type_x, q, ldq, scale):
+        self.calls += 1
+        x = self.memory(x, self.TYPES[type_x], (n, k), (ldx, 1)).double()
+        q, scale = self.memory(q, torch.int8, (n, k), (ldq, 1)), self.memory(scale, torch.float32, (n,), (1,))
+        scale.copy_(x.abs().amax(1) / 127 if k else 0)
+        q.copy_(torch.round(torch.nan_to_num(x / scale[:, None])).clamp(-127, 127))
+        return 0
+
+    def gemm_i8(self, m, n, k, a, lda, stridea, scale_a, b, ldb, scale_b, c, ldc, type_c, offsets, groups):
+        self.calls += 1
+        a = self.memory(a, torch.int8, (groups, m, k), (stridea, lda, 1))
+        b = self.memory(b, torch.int8, (n, k), (ldb, 1))
+        scale_a = self.memory(scale_a, torch.float32, (groups, m), (m, 1))
+        scale_b = self.memory(scale_b, torch.float32, (n,), (1,))
+        c = self.memory(c, self.TYPES[type_c], (n, m), (ldc, 1))
+        for g, lo, hi in self.spans(offsets, groups, n):
+            y = b[lo:hi].double() @ a[g].t().double()
+            c[lo:hi] = (y * scale_a[g].double() * scale_b[lo:hi, None].double()).to(c.dtype)
+        return 0
+
+
+@pytest.fixture
+def handle(monkeypatch):
+    # (host memory takes the place of the GPU's)
+    monkeypatch.setattr(experts, "_stream_of", lambda t: "current", raising=False)
+    return CpuHandle()
+
+
+def layer_of(handle, dtype=torch.float32, shape=(3, 5, 7), tokens=11, **how):
+    """(layer, x, experts, dy)"""
+    g = torch.Generator().manual_seed(1)
+    count, out, inner = shape
+    return (experts.Experts(handle, torch.randn(*shape, generator=g).to(dtype), **how), torch.randn(tokens, inner, generator=g).to(dtype),
+            torch.randint(count, (tokens,), generator=g), torch.randn(tokens, out, generator=g).to(dtype))
+
+
+def int8_layer(handle, shape=(3, 5, 7)):
+    g = torch.Generator().manual_seed(2)
+    return experts.Int8Experts(handle, torch.randint(-127, 128, shape, generator=g).to(torch.int8), torch.rand(shape[:2], generator=g))
+
+
+def close(got, want, dtype):
+    # (one rounding of the result: the products here are computed in 64 bits)
+    bound = {torch.float32: 2.0 ** -23, torch.float16: 2.0 ** -10, torch.bfloat16: 2.0 ** -7}[dtype]
+    return got.shape == want.shape and bool(((got.double() - want).abs() <= bound * want.abs().clamp(min=2.0 ** -14)).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_a_step_as_the_handle_sees_it(handle, dtype):
+    layer, x, e, dy = layer_of(handle, dtype)
+    y, saved = layer.forward(x, e)
+    dx, dw = layer.backward(saved, dy)
+    want = experts.reference(layer.weights, x, e, dy)
+    assert y.dtype == dx.dtype == dtype and dw.dtype == torch.float32
+    assert close(y, want[0], dtype) and close(dx, want[1], dtype) and close(dw, want[2], torch.float32)
+
+
+def refused(handle, call, *args, **kwargs):
+    """ValueError, and nothing was launched."""
+    before = handle.calls
+    with pytest.raises(ValueError):
+        call(*args, **kwargs)
+    return handle.calls == before
+
+
+@pytest.mark.parametrize("weights,tokens", [p for p in itertools.product(TYPES + [torch.float64], repeat=2) if p[0] != p[1]], ids=str)
+def test_types_that_differ(handle, weights, tokens):
+    """One type goes to the library for all operands: FP32 tokens would have 16-bit weights read past their end."""
+    if weights == torch.float64:
+        with pytest.raises(ValueError):
+            layer_of(handle, weights)
+        return
+    layer, x, e, dy = layer_of(handle, weights)
+    _, saved = layer.forward(x, e)
+    assert refused(handle, layer.forward, x.to(tokens), e)
+    assert refused(handle, layer.backward, saved, dy.to(tokens))
+    assert refused(handle, layer.backward, (saved[0].to(tokens), *saved[1:]), dy)
+
+
+def test_types_of_the_layer_in_8_bits(handle):
+    layer, x, e, _ = layer_of(handle)
+    q = int8_layer(handle)
+    for weights, scale in ((q.weights.to(torch.uint8), q.scale), (q.weights.float(), q.scale), (q.weights, q.scale.double()), (q.weights, q.scale.half())):
+        with pytest.raises(ValueError):
+            experts.Int8Experts(handle, weights, scale)
+    for dtype in (torch.float64, torch.int8, torch.int32):
+        assert refused(handle, q.forward, x.to(dtype), e)
