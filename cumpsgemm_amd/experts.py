@@ -28,10 +28,19 @@ def _type(t):
     return types[t.dtype]
 
 
-def _expect(name, t, dtype):
-    """The library is given addresses and one type for all operands: ValueError for a tensor that is of another."""
-    if t.dtype != dtype:
+def _expect(name, t, shape, dtype=None):
+    """The library is given addresses, sizes and one type for all operands: ValueError for a tensor that is not as those say."""
+    if dtype is not None and t.dtype != dtype:
         raise ValueError(f"{name} is of {t.dtype}, not of {dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} is {list(t.shape)}, not {list(shape)}")
+
+
+def _sizes(name, weights):
+    """experts, features out, features in"""
+    if weights.dim() != 3:
+        raise ValueError(f"{name} are {list(weights.shape)}, not [experts, features out, features in]")
+    return weights.shape
 
 
 def _check(status):
@@ -45,14 +54,16 @@ class Experts:
 
     def __init__(self, handle, weights, mode=lib.FP16TCEC):
         _type(weights)
+        _sizes("weights", weights)
         self.handle, self.weights, self.mode = handle, weights.contiguous(), mode
 
     def forward(self, x, experts):
         """(y, what backward needs); x and y are of the weights' type"""
         import torch
         w = self.weights
-        _expect("x", x, w.dtype)
         count, out, inner = w.shape
+        _expect("x", x, (len(x), inner), w.dtype)
+        _expect("experts", experts, (len(x),))
         order, offsets = group_by_expert(experts, count)
         grouped = x[order]
         y = torch.empty(len(x), out, device=x.device, dtype=x.dtype)
@@ -65,9 +76,10 @@ class Experts:
         import torch
         grouped, order, offsets = saved
         w = self.weights
-        _expect("what forward saved", grouped, w.dtype)
-        _expect("dy", dy, w.dtype)
         count, out, inner = w.shape
+        _expect("x of what forward saved", grouped, (len(order), inner), w.dtype)
+        _expect("offsets of what forward saved", offsets, (count + 1,))
+        _expect("dy", dy, (len(order), out), w.dtype)
         dy = dy[order]
         dx = torch.empty_like(grouped)
         _check(self.handle.gemm_grouped(lib.OP_N, inner, len(dy), out, 1.0, w, inner, out * inner, dy, out, 0.0, dx, inner,
@@ -95,8 +107,9 @@ class Int8Experts:
 
     def __init__(self, handle, weights, scale):
         import torch
-        _expect("weights", weights, torch.int8)
-        _expect("scale", scale, torch.float32)
+        count, out, inner = _sizes("weights", weights)
+        _expect("weights", weights, (count, out, inner), torch.int8)
+        _expect("scale", scale, (count, out), torch.float32)
         self.handle, self.weights, self.scale = handle, weights, scale
 
     def forward(self, x, experts):
@@ -104,6 +117,8 @@ class Int8Experts:
         import torch
         _type(x)
         count, out, inner = self.weights.shape
+        _expect("x", x, (len(x), inner))
+        _expect("experts", experts, (len(x),))
         order, offsets = group_by_expert(experts, count)
         grouped = x[order]
         q = torch.empty(len(x), inner, device=x.device, dtype=torch.int8)

@@ -144,3 +144,47 @@ def test_types_of_the_layer_in_8_bits(handle):
             experts.Int8Experts(handle, weights, scale)
     for dtype in (torch.float64, torch.int8, torch.int32):
         assert refused(handle, q.forward, x.to(dtype), e)
+
+
+def shapes_beside(t):
+    """t with one feature, one row fewer and one more, transposed, in one dimension and in three."""
+    rows, cols = t.shape
+    return [t[:, :-1], torch.cat([t, t[:, :1]], 1), t[:-1], torch.cat([t, t[:1]]), t.t(), t[0], t.reshape(rows, cols, 1), t[:, :0]]
+
+
+def test_shapes_that_do_not_belong_together(handle):
+    """Tokens with fewer features than the weights would be read past their end, and so on."""
+    layer, x, e, dy = layer_of(handle)
+    _, saved = layer.forward(x, e)
+    for t in shapes_beside(x):
+        assert refused(handle, layer.forward, t, e)
+        assert refused(handle, int8_layer(handle).forward, t, e)
+        if t.dim() != 2 or t.shape[1] != x.shape[1]:
+            assert refused(handle, layer.backward, (t, *saved[1:]), dy)
+    for t in shapes_beside(dy):
+        assert refused(handle, layer.backward, saved, t)
+    for t in (e[:-1], torch.cat([e, e[:1]]), e[:, None], e[:0]):
+        assert refused(handle, layer.forward, x, t)
+        assert refused(handle, int8_layer(handle).forward, x, t)
+    # what another layer's forward saved
+    for shape in ((4, 5, 7), (2, 5, 7), (3, 5, 8)):
+        other, ox, oe, _ = layer_of(handle, shape=shape)
+        assert refused(handle, layer.backward, other.forward(ox, oe)[1], dy)
+
+
+def test_shapes_of_weights(handle):
+    q = int8_layer(handle)
+    for w in (torch.zeros(5, 7), torch.zeros(3, 5, 7, 1), torch.zeros(7)):
+        for make in (lambda: experts.Experts(handle, w), lambda: experts.Int8Experts(handle, w.to(torch.int8), q.scale)):
+            with pytest.raises(ValueError):
+                make()
+    for scale in (q.scale[:2], q.scale[:, :4], q.scale.t(), q.scale.reshape(-1), torch.rand(3, 5, 1)):
+        with pytest.raises(ValueError):
+            experts.Int8Experts(handle, q.weights, scale)
+
+
+def test_no_tokens(handle):
+    layer, x, e, dy = layer_of(handle, tokens=0)
+    y, saved = layer.forward(x, e)
+    dx, dw = layer.backward(saved, dy)
+    assert y.shape == dy.shape and dx.shape == x.shape and (dw == 0).all()
