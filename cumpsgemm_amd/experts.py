@@ -110,7 +110,7 @@ class Int8Experts:
         count, out, inner = _sizes("weights", weights)
         _expect("weights", weights, (count, out, inner), torch.int8)
         _expect("scale", scale, (count, out), torch.float32)
-        self.handle, self.weights, self.scale = handle, weights, scale
+        self.handle, self.weights, self.scale = handle, weights.contiguous(), scale.contiguous()
 
     def forward(self, x, experts):
         """x in FP32, FP16 or BF16, a scale taken for each token; y of the same type"""

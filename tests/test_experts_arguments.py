@@ -188,3 +188,28 @@ def test_no_tokens(handle):
     y, saved = layer.forward(x, e)
     dx, dw = layer.backward(saved, dy)
     assert y.shape == dy.shape and dx.shape == x.shape and (dw == 0).all()
+
+
+def test_layouts(handle):
+    """Views: transposed, every other row or column, broadcast."""
+    layer, x, e, dy = layer_of(handle)
+    q = int8_layer(handle)
+    y, saved = layer.forward(x, e)
+    dx, dw = layer.backward(saved, dy)
+    y8 = q.forward(x, e)
+
+    def views(t):
+        wide = torch.zeros(*t.shape[:-1], 2 * t.shape[-1], dtype=t.dtype)
+        wide[..., ::2] = t
+        yield wide[..., ::2]
+        yield t.transpose(-1, -2).contiguous().transpose(-1, -2)
+        yield torch.cat([torch.zeros_like(t), t])[len(t):]
+
+    for w, w8, s8, vx, ve, vdy in zip(views(layer.weights), views(q.weights), views(q.scale), views(x), [e.repeat_interleave(2)[::2]] * 3, views(dy)):
+        again = experts.Experts(handle, w)
+        vy, vsaved = again.forward(vx, ve)
+        assert torch.equal(vy, y) and all(torch.equal(a, b) for a, b in zip(again.backward(vsaved, vdy), (dx, dw)))
+        assert torch.equal(experts.Int8Experts(handle, w8, s8).forward(vx, ve), y8)
+    one = x[:1].expand(11, 7)
+    assert torch.equal(layer.forward(one, e)[0], layer.forward(one.clone(), e)[0])
+    assert torch.equal(layer.backward(saved, dy[:1].expand(11, 5))[0], layer.backward(saved, dy[:1].repeat(11, 1))[0])
