@@ -72,7 +72,7 @@ class Experts:
         return torch.empty_like(y).index_copy_(0, order, y), (grouped, order, offsets)
 
     def backward(self, saved, dy, dw=None):
-        """(gradient of x, gradient of the weights in FP32: added to dw if there is one)"""
+        """(gradient of x, gradient of the weights in FP32: added to dw, FP32 and contiguous, if there is one)"""
         import torch
         grouped, order, offsets = saved
         w = self.weights
@@ -80,6 +80,10 @@ class Experts:
         _expect("x of what forward saved", grouped, (len(order), inner), w.dtype)
         _expect("offsets of what forward saved", offsets, (count + 1,))
         _expect("dy", dy, (len(order), out), w.dtype)
+        if dw is not None:
+            _expect("dw", dw, w.shape, torch.float32)
+            if not dw.is_contiguous():
+                raise ValueError("dw is not contiguous")
         dy = dy[order]
         dx = torch.empty_like(grouped)
         _check(self.handle.gemm_grouped(lib.OP_N, inner, len(dy), out, 1.0, w, inner, out * inner, dy, out, 0.0, dx, inner,

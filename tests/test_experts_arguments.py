@@ -213,3 +213,19 @@ def test_layouts(handle):
     one = x[:1].expand(11, 7)
     assert torch.equal(layer.forward(one, e)[0], layer.forward(one.clone(), e)[0])
     assert torch.equal(layer.backward(saved, dy[:1].expand(11, 5))[0], layer.backward(saved, dy[:1].repeat(11, 1))[0])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_dw_is_fp32_contiguous_and_as_large_as_the_weights(handle, dtype):
+    """It is written as such: a 16-bit one, as the grad of 16-bit weights is, was written past its end."""
+    layer, x, e, dy = layer_of(handle, dtype)
+    _, saved = layer.forward(x, e)
+    _, once = layer.backward(saved, dy)
+    for dw in ([torch.zeros(3, 5, 7, dtype=t) for t in (torch.float16, torch.bfloat16, torch.float64)] +
+               [torch.zeros(3, 5, 6), torch.zeros(2, 5, 7), torch.zeros(3, 7, 5), torch.zeros(15, 7), torch.zeros(3, 5, 7, 1),
+                torch.zeros(3, 7, 5).transpose(1, 2), torch.zeros(3, 5, 14)[..., ::2], torch.zeros(1, 5, 7).expand(3, 5, 7)]):
+        assert refused(handle, layer.backward, saved, dy, dw)
+        assert (dw == 0).all()
+    dw = torch.ones(3, 5, 7)
+    assert layer.backward(saved, dy, dw)[1] is dw and close(dw, 1 + experts.reference(layer.weights, x, e, dy)[2], torch.float32)
+    layer.backward(saved, dy, torch.cat([dw, dw])[3:])  # (behind other tensors' gradients)
