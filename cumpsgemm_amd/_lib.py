@@ -213,7 +213,9 @@ class Handle:
     """cuMpSGEMM_handle_t bound to the current HIP device.
 
     Method names, argument order and meaning follow the C++ API of
-    include/cumpsgemm/cumpsgemm.hpp; ``cplx`` selects the hipComplex form."""
+    include/cumpsgemm/cumpsgemm.hpp; ``cplx`` selects the hipComplex form.
+    ``stream``: the address of the stream that set_stream was given last."""
+    stream = 0
 
     def __init__(self, stream=None):
         self._L = lib()
@@ -243,7 +245,8 @@ class Handle:
 
     def set_stream(self, stream):
         s = getattr(stream, "cuda_stream", stream)
-        return self._L.cuMpSGEMM_set_stream(self._h, _ptr(int(s) if s else 0))
+        self.stream = int(s) if s else 0
+        return self._L.cuMpSGEMM_set_stream(self._h, _ptr(self.stream))
 
     def workspace_size(self):
         """Bytes of device memory held for pre-split operands."""

@@ -5,7 +5,9 @@
 runs a training step in FP32 on split operands and in BF16 (forward, the gradients of tokens and matrices), then serves
 the trained matrices in 8-bit integers, and prints how far each result is from FP64.
 
-Tensors hold a token (an output channel) in a row, which the library's column-major calls read as a column."""
+Tensors hold a token (an output channel) in a row, which the library's column-major calls read as a column.  All work goes to
+torch's current stream, whichever the handle has; it is back on its own afterwards, behind that work."""
+import contextlib
 import sys
 
 from . import _lib as lib
@@ -48,6 +50,26 @@ def _check(status):
         raise RuntimeError(f"hipblasStatus {status}")
 
 
+def _stream_of(t):
+    """The address of torch's current stream on the GPU that t is on."""
+    import torch
+    if not t.is_cuda:
+        raise ValueError(f"weights on {t.device}, not on the GPU")
+    return torch.cuda.current_stream(t.device).cuda_stream
+
+
+@contextlib.contextmanager
+def _on_current_stream(handle, weights):
+    """The library's calls between torch's own, on one stream with them."""
+    before = handle.stream
+    handle.set_stream(_stream_of(weights))
+    try:
+        yield
+    finally:
+        if handle.stream != before:
+            handle.set_stream(before)
+
+
 class Experts:
     """y[t] = weights[expert of t] @ x[t]; weights: [experts, features out, features in], FP32, FP16 or BF16, on the GPU.
     mode: how FP32 operands are multiplied."""
@@ -67,8 +89,9 @@ class Experts:
         order, offsets = group_by_expert(experts, count)
         grouped = x[order]
         y = torch.empty(len(x), out, device=x.device, dtype=x.dtype)
-        _check(self.handle.gemm_grouped(lib.OP_T, out, len(x), inner, 1.0, w, inner, out * inner, grouped, inner, 0.0, y, out,
-                                        offsets, count, self.mode, _type(x), _type(y)))
+        with _on_current_stream(self.handle, w):
+            _check(self.handle.gemm_grouped(lib.OP_T, out, len(x), inner, 1.0, w, inner, out * inner, grouped, inner, 0.0, y, out,
+                                            offsets, count, self.mode, _type(x), _type(y)))
         return torch.empty_like(y).index_copy_(0, order, y), (grouped, order, offsets)
 
     def backward(self, saved, dy, dw=None):
@@ -86,14 +109,15 @@ class Experts:
                 raise ValueError("dw is not contiguous")
         dy = dy[order]
         dx = torch.empty_like(grouped)
-        _check(self.handle.gemm_grouped(lib.OP_N, inner, len(dy), out, 1.0, w, inner, out * inner, dy, out, 0.0, dx, inner,
-                                        offsets, count, self.mode, _type(dy), _type(dx)))
         beta = 0.0 if dw is None else 1.0
         if dw is None:
             dw = torch.empty(w.shape, device=w.device, dtype=torch.float32)
-        # (stored as the weights are, features in contiguous: rows of x times rows of dy)
-        _check(self.handle.gemm_grouped_k(inner, out, len(dy), 1.0, grouped, inner, dy, out, beta, dw, inner, out * inner,
-                                          offsets, count, self.mode, _type(dy), lib.R_32F))
+        with _on_current_stream(self.handle, w):
+            _check(self.handle.gemm_grouped(lib.OP_N, inner, len(dy), out, 1.0, w, inner, out * inner, dy, out, 0.0, dx, inner,
+                                            offsets, count, self.mode, _type(dy), _type(dx)))
+            # (stored as the weights are, features in contiguous: rows of x times rows of dy)
+            _check(self.handle.gemm_grouped_k(inner, out, len(dy), 1.0, grouped, inner, dy, out, beta, dw, inner, out * inner,
+                                              offsets, count, self.mode, _type(dy), lib.R_32F))
         return torch.empty_like(dx).index_copy_(0, order, dx), dw
 
     def to_int8(self):
@@ -102,7 +126,8 @@ class Experts:
         count, out, inner = self.weights.shape
         q = torch.empty(count, out, inner, device=self.weights.device, dtype=torch.int8)
         scale = torch.empty(count, out, device=self.weights.device, dtype=torch.float32)
-        _check(self.handle.quantize_i8(inner, count * out, self.weights, inner, _type(self.weights), q, inner, scale))
+        with _on_current_stream(self.handle, self.weights):
+            _check(self.handle.quantize_i8(inner, count * out, self.weights, inner, _type(self.weights), q, inner, scale))
         return Int8Experts(self.handle, q, scale)
 
 
@@ -128,9 +153,10 @@ class Int8Experts:
         q = torch.empty(len(x), inner, device=x.device, dtype=torch.int8)
         scale = torch.empty(len(x), device=x.device, dtype=torch.float32)
         y = torch.empty(len(x), out, device=x.device, dtype=x.dtype)
-        _check(self.handle.quantize_i8(inner, len(x), grouped, inner, _type(x), q, inner, scale))
-        _check(self.handle.gemm_i8(out, len(x), inner, self.weights, inner, out * inner, self.scale, q, inner, scale, y, out,
-                                   _type(y), offsets, count))
+        with _on_current_stream(self.handle, self.weights):
+            _check(self.handle.quantize_i8(inner, len(x), grouped, inner, _type(x), q, inner, scale))
+            _check(self.handle.gemm_i8(out, len(x), inner, self.weights, inner, out * inner, self.scale, q, inner, scale, y, out,
+                                       _type(y), offsets, count))
         return torch.empty_like(y).index_copy_(0, order, y)
 
 

@@ -16,10 +16,10 @@ class CpuHandle:
     TYPES = {cg.R_32F: torch.float32, cg.R_16F: torch.float16, cg.R_16BF: torch.bfloat16}
 
     def __init__(self):
-        self.calls, self.modes, self.streams = 0, [], []
+        self.calls, self.modes, self.stream, self.streams = 0, [], "its own", []
 
     def set_stream(self, stream):
-        self.streams.append(stream)
+        self.stream = stream
         return 0
 
     @staticmethod
@@ -36,6 +36,7 @@ class CpuHandle:
 
     def gemm_grouped(self, op, m, n, k, alpha, a, lda, stridea, b, ldb, beta, c, ldc, offsets, groups, mode, type_ab, type_c):
         self.calls += 1
+        self.streams.append(self.stream)
         self.modes.append(("columns", mode))
         rows, cols = (k, m) if op == cg.OP_N else (m, k)
         a = self.memory(a, self.TYPES[type_ab], (groups, rows, cols), (stridea, lda, 1))
@@ -48,6 +49,7 @@ class CpuHandle:
 
     def gemm_grouped_k(self, m, n, k, alpha, a, lda, b, ldb, beta, c, ldc, stridec, offsets, groups, mode, type_ab, type_c):
         self.calls += 1
+        self.streams.append(self.stream)
         self.modes.append(("over k", mode))
         a = self.memory(a, self.TYPES[type_ab], (k, m), (lda, 1))
         b = self.memory(b, self.TYPES[type_ab], (k, n), (ldb, 1))
@@ -59,6 +61,7 @@ class CpuHandle:
 
     def quantize_i8(self, k, n, x, ldx, type_x, q, ldq, scale):
         self.calls += 1
+        self.streams.append(self.stream)
         x = self.memory(x, self.TYPES[type_x], (n, k), (ldx, 1)).double()
         q, scale = self.memory(q, torch.int8, (n, k), (ldq, 1)), self.memory(scale, torch.float32, (n,), (1,))
         scale.copy_(x.abs().amax(1) / 127 if k else 0)
@@ -67,6 +70,7 @@ class CpuHandle:
 
     def gemm_i8(self, m, n, k, a, lda, stridea, scale_a, b, ldb, scale_b, c, ldc, type_c, offsets, groups):
         self.calls += 1
+        self.streams.append(self.stream)
         a = self.memory(a, torch.int8, (groups, m, k), (stridea, lda, 1))
         b = self.memory(b, torch.int8, (n, k), (ldb, 1))
         scale_a = self.memory(scale_a, torch.float32, (groups, m), (m, 1))
@@ -81,7 +85,7 @@ class CpuHandle:
 @pytest.fixture
 def handle(monkeypatch):
     # (host memory takes the place of the GPU's)
-    monkeypatch.setattr(experts, "_stream_of", lambda t: "current", raising=False)
+    monkeypatch.setattr(experts, "_stream_of", lambda t: "torch's", raising=False)
     return CpuHandle()
 
 
@@ -229,3 +233,37 @@ def test_dw_is_fp32_contiguous_and_as_large_as_the_weights(handle, dtype):
     dw = torch.ones(3, 5, 7)
     assert layer.backward(saved, dy, dw)[1] is dw and close(dw, 1 + experts.reference(layer.weights, x, e, dy)[2], torch.float32)
     layer.backward(saved, dy, torch.cat([dw, dw])[3:])  # (behind other tensors' gradients)
+
+
+def test_every_call_is_on_torchs_stream(handle):
+    """... and the handle on its own again, whatever happens in between."""
+    layer, x, e, dy = layer_of(handle)
+    _, saved = layer.forward(x, e)
+    layer.backward(saved, dy)
+    layer.to_int8().forward(x, e)
+    assert handle.streams == ["torch's"] * 6 and handle.stream == "its own"
+    handle.gemm_grouped = lambda *args: cg.STATUS_INVALID_VALUE
+    with pytest.raises(RuntimeError):
+        layer.forward(x, e)
+    assert handle.stream == "its own"
+
+
+def test_weights_on_the_host():
+    """(Without the fixture: the library would be given host memory's addresses.)"""
+    handle = CpuHandle()
+    layer, x, e, dy = layer_of(handle)
+    saved = (x, torch.arange(11), torch.tensor([0, 11, 11, 11], dtype=torch.int32))
+    for call in (lambda: layer.forward(x, e), lambda: layer.backward(saved, dy), layer.to_int8, lambda: int8_layer(handle).forward(x, e)):
+        assert refused(handle, call)
+
+
+def test_the_handle_knows_its_stream(cg):
+    class Stream:
+        cuda_stream = 4096
+    h = cg.Handle.__new__(cg.Handle)
+    h._h = None  # (no handle: the library refuses the call)
+    h._L = cg.lib()
+    assert h.stream == 0
+    for stream, want in ((Stream(), 4096), (8192, 8192), (None, 0), (0, 0)):
+        h.set_stream(stream)
+        assert h.stream == want

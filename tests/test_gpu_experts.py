@@ -1,0 +1,81 @@
+"""The layers of cumpsgemm_amd/experts.py on streams other than the handle's, and inside a graph."""
+import pytest
+import torch
+
+from cumpsgemm_amd import experts
+
+pytestmark = pytest.mark.gpu
+
+COUNT, OUT, INNER, TOKENS = 6, 136, 200, 300
+
+
+def data(seed, dtype):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(TOKENS, INNER, generator=g, device="cuda").to(dtype), torch.randint(COUNT, (TOKENS,), generator=g, device="cuda"),
+            torch.randn(TOKENS, OUT, generator=g, device="cuda").to(dtype))
+
+
+def step(layer, served, x, e, dy):
+    y, saved = layer.forward(x, e)
+    return (y, *layer.backward(saved, dy), served.forward(x, e))
+
+
+@pytest.fixture
+def layers(cg, torch_gpu):
+    h = cg.Handle(stream=torch.cuda.current_stream())
+
+    def make(dtype):
+        w = torch.randn(COUNT, OUT, INNER, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(dtype)
+        layer = experts.Experts(h, w)
+        return layer, layer.to_int8()
+    yield h, make
+    torch.cuda.synchronize()
+    h.close()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_on_another_stream_than_the_handles(layers, dtype):
+    """The tokens are written on that stream, behind other work; then the handle's own stream has the next step."""
+    h, make = layers
+    layer, served = make(dtype)
+    x, e, dy = data(2, dtype)
+    want = step(layer, served, x, e, dy)
+    torch.cuda.synchronize()
+    own, side, busy = h.stream, torch.cuda.Stream(), torch.randn(4096, 4096, device="cuda")
+    late = [torch.full_like(x, float("nan")), torch.zeros_like(e), torch.full_like(dy, float("nan"))]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(5):
+            busy = busy @ busy * 2.0 ** -6
+        for to, t in zip(late, (x, e, dy)):
+            to.copy_(t)
+        got = step(layer, served, *late)
+        assert h.stream == own
+    side.synchronize()
+    again = step(layer, served, x, e, dy)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, got, again))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_in_a_graph(layers, dtype):
+    """Captured on a stream that is not the handle's; replays take the tokens and experts of the time."""
+    h, make = layers
+    layer, served = make(dtype)
+    buffers = data(3, dtype)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        step(layer, served, *buffers)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        got = step(layer, served, *buffers)
+    for seed in (4, 5, 6, 4):
+        for to, t in zip(buffers, data(seed, dtype)):
+            to.copy_(t)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step(layer, served, *buffers)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
