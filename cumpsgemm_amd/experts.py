@@ -30,8 +30,10 @@ def _type(t):
     return types[t.dtype]
 
 
-def _expect(name, t, shape, dtype=None):
+def _expect(name, t, shape, device, dtype=None):
     """The library is given addresses, sizes and one type for all operands: ValueError for a tensor that is not as those say."""
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
     if dtype is not None and t.dtype != dtype:
         raise ValueError(f"{name} is of {t.dtype}, not of {dtype}")
     if tuple(t.shape) != tuple(shape):
@@ -84,8 +86,8 @@ class Experts:
         import torch
         w = self.weights
         count, out, inner = w.shape
-        _expect("x", x, (len(x), inner), w.dtype)
-        _expect("experts", experts, (len(x),))
+        _expect("x", x, (len(x), inner), w.device, w.dtype)
+        _expect("experts", experts, (len(x),), w.device)
         order, offsets = group_by_expert(experts, count)
         grouped = x[order]
         y = torch.empty(len(x), out, device=x.device, dtype=x.dtype)
@@ -100,11 +102,12 @@ class Experts:
         grouped, order, offsets = saved
         w = self.weights
         count, out, inner = w.shape
-        _expect("x of what forward saved", grouped, (len(order), inner), w.dtype)
-        _expect("offsets of what forward saved", offsets, (count + 1,))
-        _expect("dy", dy, (len(order), out), w.dtype)
+        _expect("x of what forward saved", grouped, (len(order), inner), w.device, w.dtype)
+        _expect("order of what forward saved", order, (len(order),), w.device, torch.int64)
+        _expect("offsets of what forward saved", offsets, (count + 1,), w.device, torch.int32)
+        _expect("dy", dy, (len(order), out), w.device, w.dtype)
         if dw is not None:
-            _expect("dw", dw, w.shape, torch.float32)
+            _expect("dw", dw, w.shape, w.device, torch.float32)
             if not dw.is_contiguous():
                 raise ValueError("dw is not contiguous")
         dy = dy[order]
@@ -137,8 +140,8 @@ class Int8Experts:
     def __init__(self, handle, weights, scale):
         import torch
         count, out, inner = _sizes("weights", weights)
-        _expect("weights", weights, (count, out, inner), torch.int8)
-        _expect("scale", scale, (count, out), torch.float32)
+        _expect("weights", weights, (count, out, inner), weights.device, torch.int8)
+        _expect("scale", scale, (count, out), weights.device, torch.float32)
         self.handle, self.weights, self.scale = handle, weights.contiguous(), scale.contiguous()
 
     def forward(self, x, experts):
@@ -146,8 +149,8 @@ class Int8Experts:
         import torch
         _type(x)
         count, out, inner = self.weights.shape
-        _expect("x", x, (len(x), inner))
-        _expect("experts", experts, (len(x),))
+        _expect("x", x, (len(x), inner), self.weights.device)
+        _expect("experts", experts, (len(x),), x.device)
         order, offsets = group_by_expert(experts, count)
         grouped = x[order]
         q = torch.empty(len(x), inner, device=x.device, dtype=torch.int8)

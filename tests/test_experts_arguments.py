@@ -267,3 +267,28 @@ def test_the_handle_knows_its_stream(cg):
     for stream, want in ((Stream(), 4096), (8192, 8192), (None, 0), (0, 0)):
         h.set_stream(stream)
         assert h.stream == want
+
+
+def test_tensors_on_two_devices(handle):
+    """(torch itself indexes one device's tensor by another's, and the offsets would be host memory.)"""
+    layer, x, e, dy = layer_of(handle)
+    q = int8_layer(handle)
+    _, saved = layer.forward(x, e)
+    for t in ((x.to("meta"), e), (x, e.to("meta")), (x.to("meta"), e.to("meta"))):
+        assert refused(handle, layer.forward, *t)
+        assert refused(handle, q.forward, *t)
+    assert refused(handle, layer.backward, saved, dy.to("meta"))
+    assert refused(handle, layer.backward, saved, dy, torch.zeros(3, 5, 7, device="meta"))
+    for i in range(3):
+        assert refused(handle, layer.backward, tuple(t.to("meta") if i == j else t for j, t in enumerate(saved)), dy)
+    with pytest.raises(ValueError):
+        experts.Int8Experts(handle, q.weights, q.scale.to("meta"))
+    with pytest.raises(ValueError):
+        experts.Int8Experts(handle, q.weights.to("meta"), q.scale)
+
+
+def test_what_forward_saved_holds_the_types_that_the_library_reads(handle):
+    layer, x, e, dy = layer_of(handle)
+    grouped, order, offsets = layer.forward(x, e)[1]
+    assert refused(handle, layer.backward, (grouped, order, offsets.long()), dy)
+    assert refused(handle, layer.backward, (grouped, order.bool(), offsets), dy)
