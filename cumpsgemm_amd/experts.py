@@ -15,7 +15,8 @@ from . import _lib as lib
 
 def group_by_expert(experts, count):
     """(order, offsets): the tokens' numbers sorted by expert (those of one expert in their order), and where each expert's
-    begin, `count` + 1 int32.  On the tensor's own device, without waiting for it."""
+    begin, `count` + 1 int32.  On the tensor's own device, without waiting for it.  Tokens of no expert (numbers below 0 or
+    from `count` on) come before the first one's and behind the last one's."""
     import torch
     order = torch.argsort(experts, stable=True)
     first = torch.arange(count + 1, device=experts.device, dtype=experts.dtype)
@@ -73,7 +74,8 @@ def _on_current_stream(handle, weights):
 
 
 class Experts:
-    """y[t] = weights[expert of t] @ x[t]; weights: [experts, features out, features in], FP32, FP16 or BF16, on the GPU.
+    """y[t] = weights[expert of t] @ x[t], zeros for a token of no expert (one that was dropped: a number below 0 or from
+    `experts` on), whose dy counts for nothing; weights: [experts, features out, features in], FP32, FP16 or BF16, on the GPU.
     mode: how FP32 operands are multiplied."""
 
     def __init__(self, handle, weights, mode=lib.FP16TCEC):
@@ -90,7 +92,7 @@ class Experts:
         _expect("experts", experts, (len(x),), w.device)
         order, offsets = group_by_expert(experts, count)
         grouped = x[order]
-        y = torch.empty(len(x), out, device=x.device, dtype=x.dtype)
+        y = torch.zeros(len(x), out, device=x.device, dtype=x.dtype)  # (the library writes the rows of experts' tokens only)
         with _on_current_stream(self.handle, w):
             _check(self.handle.gemm_grouped(lib.OP_T, out, len(x), inner, 1.0, w, inner, out * inner, grouped, inner, 0.0, y, out,
                                             offsets, count, self.mode, _type(x), _type(y)))
@@ -111,7 +113,7 @@ class Experts:
             if not dw.is_contiguous():
                 raise ValueError("dw is not contiguous")
         dy = dy[order]
-        dx = torch.empty_like(grouped)
+        dx = torch.zeros_like(grouped)
         beta = 0.0 if dw is None else 1.0
         if dw is None:
             dw = torch.empty(w.shape, device=w.device, dtype=torch.float32)
@@ -135,7 +137,8 @@ class Experts:
 
 
 class Int8Experts:
-    """weights: [experts, features out, features in] 8-bit integers, scale: [experts, features out]."""
+    """weights: [experts, features out, features in] 8-bit integers, scale: [experts, features out].  Tokens of no expert as in
+    Experts."""
 
     def __init__(self, handle, weights, scale):
         import torch
@@ -155,7 +158,7 @@ class Int8Experts:
         grouped = x[order]
         q = torch.empty(len(x), inner, device=x.device, dtype=torch.int8)
         scale = torch.empty(len(x), device=x.device, dtype=torch.float32)
-        y = torch.empty(len(x), out, device=x.device, dtype=x.dtype)
+        y = torch.zeros(len(x), out, device=x.device, dtype=x.dtype)  # (the library writes the rows of experts' tokens only)
         with _on_current_stream(self.handle, self.weights):
             _check(self.handle.quantize_i8(inner, len(x), grouped, inner, _type(x), q, inner, scale))
             _check(self.handle.gemm_i8(out, len(x), inner, self.weights, inner, out * inner, self.scale, q, inner, scale, y, out,

@@ -292,3 +292,32 @@ def test_what_forward_saved_holds_the_types_that_the_library_reads(handle):
     grouped, order, offsets = layer.forward(x, e)[1]
     assert refused(handle, layer.backward, (grouped, order, offsets.long()), dy)
     assert refused(handle, layer.backward, (grouped, order.bool(), offsets), dy)
+
+
+@pytest.fixture
+def memory_in_use():
+    """torch.empty gives NaN (and the largest integers) instead of whatever lies there."""
+    before = torch.utils.deterministic.fill_uninitialized_memory, torch.are_deterministic_algorithms_enabled()
+    torch.utils.deterministic.fill_uninitialized_memory = True
+    torch.use_deterministic_algorithms(True)
+    assert torch.isnan(torch.empty(3)).all()
+    yield
+    torch.utils.deterministic.fill_uninitialized_memory = before[0]
+    torch.use_deterministic_algorithms(before[1])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("numbers", [[-1, 0, 3, 1, -5, 2, 2, 7, 0, 1, -1], [-1] * 11, [3] * 11, [-1, 1 << 40, -(1 << 40), 0, 0, 0, 0, 0, 0, 0, 2]], ids=str)
+def test_tokens_of_no_expert(handle, memory_in_use, dtype, numbers):
+    """Zeros for them, whatever they hold, and nothing of them in the weights' gradient."""
+    layer, x, _, dy = layer_of(handle, dtype)
+    e = torch.tensor(numbers)
+    kept = (e >= 0) & (e < 3)
+    want = experts.reference(layer.weights, x[kept], e[kept], dy[kept])
+    x[~kept], dy[~kept] = float("nan"), float("inf")
+    y, saved = layer.forward(x, e)
+    dx, dw = layer.backward(saved, dy)
+    assert close(y[kept], want[0], dtype) and close(dx[kept], want[1], dtype) and close(dw, want[2], torch.float32)
+    assert (y[~kept] == 0).all() and (dx[~kept] == 0).all()
+    y8 = layer.to_int8().forward(x, e)
+    assert (y8[~kept] == 0).all() and torch.isfinite(y8).all()
