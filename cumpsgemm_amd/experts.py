@@ -18,6 +18,8 @@ def group_by_expert(experts, count):
     begin, `count` + 1 int32.  On the tensor's own device, without waiting for it.  Tokens of no expert (numbers below 0 or
     from `count` on) come before the first one's and behind the last one's."""
     import torch
+    if not experts.dtype.is_floating_point:  # (`count` itself need not fit the type that the numbers have)
+        experts = experts.to(torch.promote_types(experts.dtype, torch.int32))
     order = torch.argsort(experts, stable=True)
     first = torch.arange(count + 1, device=experts.device, dtype=experts.dtype)
     return order, torch.searchsorted(experts[order], first).to(torch.int32)

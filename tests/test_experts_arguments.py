@@ -321,3 +321,15 @@ def test_tokens_of_no_expert(handle, memory_in_use, dtype, numbers):
     assert (y[~kept] == 0).all() and (dx[~kept] == 0).all()
     y8 = layer.to_int8().forward(x, e)
     assert (y8[~kept] == 0).all() and torch.isfinite(y8).all()
+
+
+@pytest.mark.parametrize("count", [2, 127, 128, 129, 255, 256, 300, 40000])
+@pytest.mark.parametrize("dtype", [torch.bool, torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64], ids=str)
+def test_expert_numbers_of_any_integer_type(dtype, count):
+    """As many experts as the numbers' type holds, and more: `count` itself is beyond it then."""
+    most = min(count, 2 if dtype == torch.bool else torch.iinfo(dtype).max + 1)
+    e = torch.randint(most, (200,), generator=torch.Generator().manual_seed(count))
+    e[:2] = torch.tensor([0, most - 1])
+    order, offsets = experts.group_by_expert(e.to(dtype), count)
+    want = torch.cat([torch.zeros(1, dtype=torch.int64), torch.bincount(e, minlength=count).cumsum(0)])
+    assert torch.equal(order, torch.argsort(e, stable=True)) and torch.equal(offsets, want.to(torch.int32))
