@@ -78,12 +78,15 @@ def _on_current_stream(handle, weights):
 class Experts:
     """y[t] = weights[expert of t] @ x[t], zeros for a token of no expert (one that was dropped: a number below 0 or from
     `experts` on), whose dy counts for nothing; weights: [experts, features out, features in], FP32, FP16 or BF16, on the GPU.
-    mode: how FP32 operands are multiplied."""
+    mode, gradient_mode: how FP32 operands are multiplied, forward and for the gradients.  FP16TCEC splits into FP16 terms,
+    which hold nothing beyond 65504 and are off by up to 2^-36 however small the value is: 1.5e-4 of one of 1e-7, such as the
+    gradients of a mean over many tokens are (the terms of dy of 1e-6: 8.6e-6 of its norm; of 1e-9: 8.6e-3).  TF32TCEC's three
+    BF16 terms have FP32's range."""
 
-    def __init__(self, handle, weights, mode=lib.FP16TCEC):
+    def __init__(self, handle, weights, mode=lib.FP16TCEC, gradient_mode=lib.TF32TCEC):
         _type(weights)
         _sizes("weights", weights)
-        self.handle, self.weights, self.mode = handle, weights.contiguous(), mode
+        self.handle, self.weights, self.mode, self.gradient_mode = handle, weights.contiguous(), mode, gradient_mode
 
     def forward(self, x, experts):
         """(y, what backward needs); x and y are of the weights' type"""
@@ -121,10 +124,10 @@ class Experts:
             dw = torch.empty(w.shape, device=w.device, dtype=torch.float32)
         with _on_current_stream(self.handle, w):
             _check(self.handle.gemm_grouped(lib.OP_N, inner, len(dy), out, 1.0, w, inner, out * inner, dy, out, 0.0, dx, inner,
-                                            offsets, count, self.mode, _type(dy), _type(dx)))
+                                            offsets, count, self.gradient_mode, _type(dy), _type(dx)))
             # (stored as the weights are, features in contiguous: rows of x times rows of dy)
             _check(self.handle.gemm_grouped_k(inner, out, len(dy), 1.0, grouped, inner, dy, out, beta, dw, inner, out * inner,
-                                              offsets, count, self.mode, _type(dy), lib.R_32F))
+                                              offsets, count, self.gradient_mode, _type(dy), lib.R_32F))
         return torch.empty_like(dx).index_copy_(0, order, dx), dw
 
     def to_int8(self):
@@ -198,7 +201,7 @@ def main(argv=None):
         errors[name] = float((got.double() - want).norm() / want.norm())
         print(f"{name:24s} relative error {errors[name]:.2e}")
 
-    for name, dtype in (("FP16TCEC", torch.float32), ("BF16", torch.bfloat16)):
+    for name, dtype in (("FP32", torch.float32), ("BF16", torch.bfloat16)):
         layer = Experts(handle, weights.to(dtype))
         xs, ds = x.to(dtype), dy.to(dtype)
         y, saved = layer.forward(xs, experts)

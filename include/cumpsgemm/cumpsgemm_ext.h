@@ -161,7 +161,11 @@ hipblasStatus_t cuMpSGEMM_cgemm_2xNx2(cuMpSGEMM_handle_t handle, hipblasOperatio
  * the operands is touched.  Results repeat bit for bit.
  * type_ab = HIP_R_32F: compute_mode FP16TCEC, TF32TCEC, FP16TC or TF32TC, as in
  *   cuMpSGEMM_sgemm; type_c = HIP_R_32F.  (An infinity is not split: what it
- *   multiplies becomes NaN, as there.)
+ *   multiplies becomes NaN, as there.)  FP16TCEC and FP16TC have FP16's range:
+ *   beyond 65504 a value counts as an infinity, and FP16TCEC's two terms are off
+ *   by up to 2^-36 however small the value is (1.5e-4 of one of 1e-7).  Nothing
+ *   here scales operands or chooses a mode by their statistics: for gradients,
+ *   which are often that small, take TF32TCEC, whose terms have FP32's range.
  * type_ab = HIP_R_16F or HIP_R_16BF: products are exact, sums FP32; type_c the
  *   same type or HIP_R_32F, rounded once; compute_mode is not looked at.
  * Errors as cuMpSGEMM_sgemm: HIPBLAS_STATUS_INVALID_VALUE and nothing launched.

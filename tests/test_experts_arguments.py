@@ -333,3 +333,13 @@ def test_expert_numbers_of_any_integer_type(dtype, count):
     order, offsets = experts.group_by_expert(e.to(dtype), count)
     want = torch.cat([torch.zeros(1, dtype=torch.int64), torch.bincount(e, minlength=count).cumsum(0)])
     assert torch.equal(order, torch.argsort(e, stable=True)) and torch.equal(offsets, want.to(torch.int32))
+
+
+def test_modes(handle):
+    """The gradients' operands keep FP32's range unless another mode is asked for."""
+    layer, x, e, dy = layer_of(handle)
+    layer.backward(layer.forward(x, e)[1], dy)
+    assert handle.modes == [("columns", cg.FP16TCEC), ("columns", cg.TF32TCEC), ("over k", cg.TF32TCEC)]
+    layer, *_ = layer_of(handle, mode=cg.TF32TC, gradient_mode=cg.FP16TC)
+    layer.backward(layer.forward(x, e)[1], dy)
+    assert handle.modes[3:] == [("columns", cg.TF32TC), ("columns", cg.FP16TC), ("over k", cg.FP16TC)]

@@ -1,8 +1,9 @@
-"""The layers of cumpsgemm_amd/experts.py on streams other than the handle's, and inside a graph."""
+"""The layers of cumpsgemm_amd/experts.py on streams other than the handle's, inside a graph, and with small gradients."""
 import pytest
 import torch
 
 from cumpsgemm_amd import experts
+from test_gpu_grouped import check
 
 pytestmark = pytest.mark.gpu
 
@@ -79,3 +80,17 @@ def test_in_a_graph(layers, dtype):
         want = step(layer, served, *buffers)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("scale", [1.0, 1e-6, 1e-9, 1e-20, 1e6])
+def test_small_and_large_gradients_keep_their_digits(layers, scale):
+    """Expert by expert, under the bounds of test_gpu_grouped.py, which go by the sizes of the sums."""
+    layer, _ = layers[1](torch.float32)
+    x, e, dy = data(7, torch.float32)
+    dy = dy * scale
+    dx, dw = layer.backward(layer.forward(x, e)[1], dy)
+    for g in range(COUNT):
+        xs, ds, w = x[e == g].double(), dy[e == g].double(), layer.weights[g].double()
+        check(dx[e == g], ds @ w, ds.abs() @ w.abs(), "TF32TCEC", OUT, torch.float32)
+        dst = ds.t().contiguous()
+        check(dw[g], dst @ xs, dst.abs() @ xs.abs(), "TF32TCEC", len(xs), torch.float32)
