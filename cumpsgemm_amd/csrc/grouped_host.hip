@@ -94,9 +94,17 @@ hipblasStatus_t launched() {
 // What a kernel takes, in us: fixed + steps * part * max(alone, each * (workgroups / CUs + 0.2 of a round beyond the first)).
 // alone: a step where a CU has one workgroup; each: of a workgroup's step where they queue; part: of a step for tiles with
 // `filled` of their columns, least + (1 - least) * filled.  Fitted to 956 calls (m x k of 512^2 to 4096 x 2048, 1 - 64 groups
-// of 1 - 8192 tokens, uneven by e^(0.4 N(0,1)), op T) with every kernel in turn; what the choice by it loses against the
-// best kernel, as a geometric mean: BF16 2.9 %, 8-bit 2.7 %, FP32 2.7 % in two and 2.5 % in three terms.  By tokens to a group
-// alone (192, 48, 8) it was 25, 28, 21 and 28 %.
+// of 1 - 8192 tokens, uneven by e^(0.4 N(0,1))) with every kernel in turn: op T, aligned operands, in BF16, 8 bits, FP16TCEC and
+// TF32TCEC.  By tokens to a group alone (192, 48, 8) the choice lost 25, 28, 21 and 28 % against the best kernel there.  What it
+// loses now, as a geometric mean over 235 calls of those sizes, %:
+//                     BF16   8 bits   FP16TCEC   TF32TCEC   FP16TC   TF32TC
+//   op T               3.2     2.9       2.8        2.7       4.4      2.6
+//   op N               3.1                4.1        3.1       3.9      4.5
+//   op T, unaligned   14.7     6.3
+//   op N, unaligned    1.5
+// Not fitted to, and it shows: op T unaligned with 1 - 8 tokens to a group, where the kernel of few tokens takes two to four
+// times as long as the 128 x 128 tiles, at the aligned figures; and op N with 16 - 64 tokens in few groups, where it takes a
+// third to two thirds of the others' time, but is counted too high (run_columns).
 struct Cost {
   float fixed, alone, each;
   int slots, step; // workgroups to a CU; K-values of a step (the kernel of few tokens: of its eight waves)
@@ -117,9 +125,9 @@ double cost_us(const Cost &c, double workgroups, double steps, double cus, doubl
   return c.fixed + steps * (c.least + (1.0 - c.least) * filled) * std::max<double>(c.alone, c.each * (workgroups / cus + (workgroups > cus * c.slots ? 0.2 * c.slots : 0.0)));
 }
 // For products over K (342 calls, 1 - 64 groups of 16 - 16384 tokens, results of 256^2 - 4096 x 2048, K in 1 - 16 parts, both
-// tiles), whose groups often have a few steps only: every round of tiles also costs `round`, their first loads and the
-// write-out; a group's K can be longer than the average one's, which counts where a CU has one workgroup; and parts are
-// written and read once more, at 5.3 TB/s.  Loses 1.4 % (BF16), 2.0 % (FP16TCEC) and 0.4 % (TF32TCEC); without `round`
+// tiles; BF16, FP16TCEC and TF32TCEC, aligned), whose groups often have a few steps only: every round of tiles also costs
+// `round`, their first loads and the write-out; a group's K can be longer than the average one's, which counts where a CU
+// has one workgroup; and parts are written and read once more, at 5.3 TB/s.  Loses 1.4 % (BF16), 2.0 % (FP16TCEC) and 0.4 % (TF32TCEC); without `round`
 // 3.6, 2.4 and 0.8 %.
 struct CostOverK {
   float fixed, alone, each, round;
@@ -169,7 +177,8 @@ hipblasStatus_t run_columns(cuMpSGEMM_handle *h, Elem e, bool a_kc, GroupedArgs 
       const double columns = args.groups == 1 ? (args.n + kern->bn - 1) / kern->bn
                              : each < kern->bn / 2 ? some : (double)args.n / kern->bn + 0.5 * some;
       const Cost &cost = cost_of(e, c);
-      // (the kernel of few tokens: in workgroups of 16 rows, as fitted; where rows are contiguous it has 64 in one)
+      // (the kernel of few tokens: in workgroups of 16 rows, as fitted with op T; where rows are contiguous it has 64 in one,
+      // and this is too high)
       const double rows = c == STREAM ? (args.m + 15) / 16 : (args.m + kern->bm - 1) / kern->bm;
       const double us = cost_us(cost, columns * rows, (args.k + cost.step - 1) / cost.step, h->num_cus,
                                 std::min(1.0, each / kern->bn));

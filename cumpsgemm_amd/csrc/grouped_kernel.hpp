@@ -16,9 +16,12 @@
 // FP32 operands are split while they are staged, whatever their layout: a thread reads eight K-values of one row and
 // writes one chunk to each plane.
 //
-// What bounds it (us at 16384 tokens of 8 experts, 4096 x 2048, BF16; 4096 tokens, 2048 x 1024, FP16TCEC): 16 and 8 bits the
-// card's power limit beside the loads to LDS, 273 us = 1000 TFLOP/s (2159 TOP/s in 8 bits, 8192 x 4096 x 4096); FP32 the
-// LDS reads of a step, as long as its MFMAs, and power: 55.9 us = 922 TFLOP/s of MFMAs with even experts, 46.3 on zeros.
+// What it spends its time on, as far as measurements tell (us).  BF16, 16384 tokens of 8 experts, 4096 x 2048: 272 with uneven
+// experts, 230 with even ones, which are whole rounds of tiles, 190 on zeros, which leave the clock higher (random values:
+// 1.98 GHz, 44 % of it MFMAs); rows padded by 64 or 192 values are level.  8 bits, 8192 x 4096: 23.4 a thousand K-values
+// (2870 TOP/s) and 27 beside that, a tile's first loads, its write-out and the launch: at K = 4096 123, 2230 TOP/s.  FP16TCEC,
+// 4096 tokens of 8, 2048 x 1024: 78 with uneven experts in 128 x 128 tiles, 60 with even ones (256 x 128 tiles: 54, zeros 44);
+// 28 % MFMAs, and beside them as many clocks of LDS reads, which the schedule does not hide whole.
 #pragma once
 #include "gemm_kernel.hpp"
 #include "grouped.hpp"

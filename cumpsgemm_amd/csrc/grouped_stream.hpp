@@ -1,9 +1,11 @@
 // Experts' products for few tokens to a group (serving): the matrices are read once, straight into MFMA fragments.
 //
-// Bound by reading the weights: 64 tokens to 40 of 64 experts of 2048 x 1024 in BF16 32.3 us, 5.2 TB/s, the rate of a copy;
-// at one or two tokens of 1024 x 1024 by the launch and the way of a load, 5.5 us.  A workgroup of eight waves has 16 rows of one group's matrix (64 where the rows, not
-// K, are contiguous) and up to 16 of its tokens.  The waves share out K, 128 bytes of every row at a time, so that the
-// workgroup reads 1 KiB of each row side by side; each wave keeps several such loads under way, without LDS and
+// Bound by reading the weights: one token to each of 40 of 64 experts (and 24 more) of 2048 x 1024 in BF16 33.0 us, 5.1 TB/s, with
+// 24 sets of matrices in turn; 30.0 with the same set again and again, part of which the last-level cache holds.  (All 64
+// experts 48.4 us, 5.5 TB/s, where the 128 x 32 tiles, whose step is longer, read 6.0.)  At one or two tokens of 1024 x 1024
+// by the launch and the way of a load, 5.5 us.  A workgroup of eight waves has 16 rows of one group's matrix (64 where the
+// rows, not K, are contiguous) and up to 16 of its tokens.  The waves share out K, 128 bytes of every row at a time, so
+// that the workgroup reads 1 KiB of each row side by side; each wave keeps several such loads under way, without LDS and
 // without a barrier, and the eight partial sums are added through LDS in a fixed order at the end.
 // Splitting K over waves rather than giving each wave rows of its own keeps a CU's share of a small matrix small: 1024
 // rows are 64 workgroups, and a wave of the 128 KiB that 16 rows of 2048 FP32 values are reads 16.
@@ -17,7 +19,8 @@ constexpr int kStreamWaves = 8, kStreamTokens = 16;
 template <Elem E, bool A_KC> struct StreamCfg {
   using T = elem_traits<E>;
   // 16 rows of the matrix each, for a workgroup (row-contiguous: four rows a lane).  K-contiguous with four, us, with one
-  // -> four: BF16 2048 x 1024, 2 tokens to 2 of 8 groups 4.8 -> 7.0, 64 to 64 27.4 -> 22.1, where the 128 x 32 tiles take 21.0.
+  // -> four: BF16 2048 x 1024, 2 tokens to 2 of 8 groups 4.8 -> 7.0, 64 to 27 of 64 27.4 -> 22.1, where the 128 x 32 tiles take
+  // 21.0 (the same 113 MB of matrices again and again: they stay in the last-level cache).
   static constexpr int BLOCKS = A_KC ? 1 : 4, ROWS = BLOCKS * 16;
   // K-values of a wave's step: 128 bytes of a row, one or two MFMAs deep (row-contiguous: one, 32 lines)
   static constexpr int SLICES = A_KC && !T::F32 ? 2 : 1;
