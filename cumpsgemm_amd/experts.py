@@ -81,7 +81,7 @@ class Experts:
     mode, gradient_mode: how FP32 operands are multiplied, forward and for the gradients.  FP16TCEC splits into FP16 terms,
     which hold nothing beyond 65504 and are off by up to 2^-36 however small the value is: 1.5e-4 of one of 1e-7, such as the
     gradients of a mean over many tokens are (the terms of dy of 1e-6: 8.6e-6 of its norm; of 1e-9: 8.6e-3).  TF32TCEC's three
-    BF16 terms have FP32's range."""
+    BF16 terms have FP32's range.  The layer keeps the weights themselves, but a copy if they are not contiguous."""
 
     def __init__(self, handle, weights, mode=lib.FP16TCEC, gradient_mode=lib.TF32TCEC):
         _type(weights)
