@@ -94,3 +94,25 @@ def test_small_and_large_gradients_keep_their_digits(layers, scale):
         check(dx[e == g], ds @ w, ds.abs() @ w.abs(), "TF32TCEC", OUT, torch.float32)
         dst = ds.t().contiguous()
         check(dw[g], dst @ xs, dst.abs() @ xs.abs(), "TF32TCEC", len(xs), torch.float32)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=str)
+def test_dropped_tokens_are_zeros_and_count_for_nothing(layers, dtype):
+    """Numbers below 0 and beyond the last expert, their tokens NaN and infinities: as if those tokens were not there."""
+    layer, served = layers[1](dtype)
+    x, _, dy = data(8, dtype)
+    e = torch.randint(-2, COUNT + 3, (TOKENS,), generator=torch.Generator(device="cuda").manual_seed(9), device="cuda")
+    kept = (e >= 0) & (e < COUNT)
+    served_alone = served.forward(x[kept], e[kept])
+    x[~kept], dy[~kept] = float("nan"), float("inf")
+    torch.full((64 << 20,), float("nan"), device="cuda")  # (what the results' memory held before)
+    y, dx, dw, y8 = step(layer, served, x, e, dy)
+    assert (y[~kept] == 0).all() and (dx[~kept] == 0).all() and (y8[~kept] == 0).all()
+    assert torch.equal(y8[kept], served_alone)  # (sums of integers: any kernel's)
+    forward, gradients = ("FP16TCEC", "TF32TCEC") if dtype == torch.float32 else ("f16", "f16") if dtype == torch.float16 else ("bf16", "bf16")
+    for g in range(COUNT):
+        xs, ds, w = x[e == g].double(), dy[e == g].double(), layer.weights[g].double()
+        wt, dst = w.t().contiguous(), ds.t().contiguous()
+        check(y[e == g], xs @ wt, xs.abs() @ wt.abs(), forward, INNER, dtype)
+        check(dx[e == g], ds @ w, ds.abs() @ w.abs(), gradients, OUT, dtype)
+        check(dw[g], dst @ xs, dst.abs() @ xs.abs(), gradients, len(xs), torch.float32)
