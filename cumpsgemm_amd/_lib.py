@@ -19,7 +19,9 @@ MODE_NAMES = ["CUBLAS", "FP16TCEC", "TF32TCEC", "FP16TC", "TF32TC", "CUBLAS_SIMT
 STATUS_SUCCESS, STATUS_INVALID_VALUE = 0, 3
 
 # hipDataType
-R_32F, R_16F, R_8I, R_16BF = 0, 2, 3, 14
+R_32F, R_16F, R_8I, R_16BF, R_8F_E4M3, R_8F_E5M2 = 0, 2, 3, 14, 28, 29
+# cuMpSGEMM_activation_t
+SILU, GELU, GELU_TANH, RELU = range(4)
 
 _u64 = ctypes.c_uint64
 _u32 = ctypes.c_uint
@@ -53,6 +55,7 @@ _CALL_FUNCTIONS = ("cuMpSGEMM_sgemm", "cuMpSGEMM_cgemm", "cuMpSGEMM_sgemm_stride
                    "cuMpSGEMM_sgemm_pipeline", "cuMpSGEMM_cgemm_pipeline", "cuMpSGEMM_sgemm_Mx2x2",
                    "cuMpSGEMM_cgemm_Mx2x2", "cuMpSGEMM_sgemm_2xNx2", "cuMpSGEMM_cgemm_2xNx2")
 _GROUPED_FUNCTIONS = ("cuMpSGEMM_gemm_grouped", "cuMpSGEMM_gemm_grouped_k", "cuMpSGEMM_gemm_i8", "cuMpSGEMM_quantize_i8")
+_GATED_FUNCTIONS = ("cuMpSGEMM_gemm_gated", "cuMpSGEMM_gemm_gated_backward")
 
 
 def lib():
@@ -77,6 +80,7 @@ def lib():
             from . import _call
             _call.bind(*(ctypes.cast(getattr(L, name), _ptr).value for name in _CALL_FUNCTIONS))
             _call.bind_grouped(*(ctypes.cast(getattr(L, name), _ptr).value for name in _GROUPED_FUNCTIONS))
+            _call.bind_gated(*(ctypes.cast(getattr(L, name), _ptr).value for name in _GATED_FUNCTIONS))
             _native = _call
         except ImportError:
             _native = None  # not built: every call goes through ctypes
@@ -123,6 +127,10 @@ def _declare(L):
     L.cuMpSGEMM_gemm_i8.argtypes = [_ptr] + gemm_tail + [
         _ptr, _u64, _u64, _ptr, _ptr, _u64, _ptr, _ptr, _u64, _int, _ptr, _u64]
     L.cuMpSGEMM_quantize_i8.argtypes = [_ptr, _u64, _u64, _ptr, _u64, _int, _ptr, _u64, _ptr]
+    L.cuMpSGEMM_gemm_gated.argtypes = [_ptr, _int, _int] + gemm_tail + [
+        _ptr, _ptr, _u64, _u64, _ptr, _u64, _ptr, _u64, _ptr, _ptr, _u64, _ptr, _u64, _int, _int]
+    L.cuMpSGEMM_gemm_gated_backward.argtypes = [_ptr, _int, _int] + gemm_tail + [
+        _ptr, _u64, _u64, _ptr, _u64, _ptr, _ptr, _u64, _ptr, _ptr, _u64, _ptr, _u64, _ptr, _u64, _int, _int]
     L.cuMpSGEMM_get_workspace_size.argtypes = [_ptr]
     L.cuMpSGEMM_get_workspace_size.restype = ctypes.c_size_t
     L.cuMpSGEMM_get_workspace_pointer.argtypes = [_ptr]
@@ -364,6 +372,31 @@ class Handle:
             if st is not None:
                 return st
         return self._L.cuMpSGEMM_quantize_i8(self._h, k, n, _dptr(x), ldx, int(type_x), _dptr(q), ldq, _dptr(scale))
+
+    # ---- gated feed-forward blocks ----
+    def gemm_gated(self, op_a, activation, m, n, k, gate, up, lda, stridea, b, ldb, c, ldc, z_gate=None, z_up=None, ldz=0,
+                   offsets=None, groups=1, mode=FP16TCEC, type=R_32F):
+        """c = act(op(gate) b) * (op(up) b), token by token; z_gate and z_up get the two products, if given."""
+        if _native is not None:
+            st = _native.gemm_gated(self._addr, op_a, activation, m, n, k, gate, up, lda, stridea, b, ldb, c, ldc, z_gate, z_up,
+                                    ldz, offsets, groups, mode, type)
+            if st is not None:
+                return st
+        return self._L.cuMpSGEMM_gemm_gated(self._h, op_a, int(activation), m, n, k, _dptr(gate), _dptr(up), lda, stridea,
+                                            _dptr(b), ldb, _dptr(c), ldc, _dptr(z_gate), _dptr(z_up), ldz, _dptr(offsets),
+                                            groups, int(mode), int(type))
+
+    def gemm_gated_backward(self, op_a, activation, m, n, k, a, lda, stridea, b, ldb, z_gate, z_up, ldz, d_gate, d_up, ldd,
+                            c=None, ldc=0, offsets=None, groups=1, mode=FP16TCEC, type=R_32F):
+        """Gradients of gemm_gated's two products, where that of its result is op(a) b; c gets the result again, if given."""
+        if _native is not None:
+            st = _native.gemm_gated_backward(self._addr, op_a, activation, m, n, k, a, lda, stridea, b, ldb, z_gate, z_up, ldz,
+                                             d_gate, d_up, ldd, c, ldc, offsets, groups, mode, type)
+            if st is not None:
+                return st
+        return self._L.cuMpSGEMM_gemm_gated_backward(self._h, op_a, int(activation), m, n, k, _dptr(a), lda, stridea, _dptr(b),
+                                                     ldb, _dptr(z_gate), _dptr(z_up), ldz, _dptr(d_gate), _dptr(d_up), ldd,
+                                                     _dptr(c), ldc, _dptr(offsets), groups, int(mode), int(type))
 
     # ---- exponent statistics ----
     def exp_stats_ext(self, m, n, ptr, ld, batch=1, stride=0, cplx=False):

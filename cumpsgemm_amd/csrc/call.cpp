@@ -35,6 +35,11 @@ struct GroupedFunctions { // products of experts' layers
   decltype(&cuMpSGEMM_quantize_i8) quantize;
 } fg;
 constexpr Py_ssize_t kGroupedFunctions = sizeof(GroupedFunctions) / sizeof(void *);
+struct GatedFunctions { // gated feed-forward blocks
+  decltype(&cuMpSGEMM_gemm_gated) gated;
+  decltype(&cuMpSGEMM_gemm_gated_backward) backward;
+} fb;
+constexpr Py_ssize_t kGatedFunctions = sizeof(GatedFunctions) / sizeof(void *);
 PyObject *data_ptr_name;
 
 // The arguments of a call, taken one after the other; `ok` goes false at the first
@@ -300,7 +305,59 @@ PyObject *quantize_i8(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
   float *const scale = x.ptr<float>();
   return status(x, [&] { return fg.quantize(h, k, n, values, ldx, type_x, q, ldq, scale); });
 }
-// the addresses of the functions, in the order of `Functions` (`GroupedFunctions`)
+// handle, op_a, activation, m, n, k, gate, up, lda, stride_a, b, ldb, c, ldc, z_gate, z_up, ldz, offsets, groups, mode, type
+PyObject *gemm_gated(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+  if (!count_is(n_args, 21)) return nullptr;
+  Args x{args};
+  auto *const h = x.ptr<cuMpSGEMM_handle>();
+  const auto op_a = x.op();
+  const auto act = (cuMpSGEMM_activation_t)(int)x.u64();
+  const uint64_t m = x.u64(), n = x.u64(), k = x.u64();
+  void *const gate = x.ptr<void>(), *const up = x.ptr<void>();
+  const uint64_t lda = x.u64(), stride_a = x.u64();
+  void *const b = x.ptr<void>();
+  const uint64_t ldb = x.u64();
+  void *const c = x.ptr<void>();
+  const uint64_t ldc = x.u64();
+  void *const z_gate = x.ptr<void>(), *const z_up = x.ptr<void>();
+  const uint64_t ldz = x.u64();
+  const int *const offsets = x.ptr<int>();
+  const uint64_t groups = x.u64();
+  const auto mode = (cuMpSGEMM_compute_mode_t)(int)x.u64();
+  const auto type = (hipDataType)(int)x.u64();
+  return status(x, [&] {
+    return fb.gated(h, op_a, act, m, n, k, gate, up, lda, stride_a, b, ldb, c, ldc, z_gate, z_up, ldz, offsets, groups, mode, type);
+  });
+}
+// handle, op_a, activation, m, n, k, a, lda, stride_a, b, ldb, z_gate, z_up, ldz, d_gate, d_up, ldd, c, ldc, offsets, groups, mode,
+// type
+PyObject *gemm_gated_backward(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+  if (!count_is(n_args, 23)) return nullptr;
+  Args x{args};
+  auto *const h = x.ptr<cuMpSGEMM_handle>();
+  const auto op_a = x.op();
+  const auto act = (cuMpSGEMM_activation_t)(int)x.u64();
+  const uint64_t m = x.u64(), n = x.u64(), k = x.u64();
+  void *const a = x.ptr<void>();
+  const uint64_t lda = x.u64(), stride_a = x.u64();
+  void *const b = x.ptr<void>();
+  const uint64_t ldb = x.u64();
+  void *const z_gate = x.ptr<void>(), *const z_up = x.ptr<void>();
+  const uint64_t ldz = x.u64();
+  void *const d_gate = x.ptr<void>(), *const d_up = x.ptr<void>();
+  const uint64_t ldd = x.u64();
+  void *const c = x.ptr<void>();
+  const uint64_t ldc = x.u64();
+  const int *const offsets = x.ptr<int>();
+  const uint64_t groups = x.u64();
+  const auto mode = (cuMpSGEMM_compute_mode_t)(int)x.u64();
+  const auto type = (hipDataType)(int)x.u64();
+  return status(x, [&] {
+    return fb.backward(h, op_a, act, m, n, k, a, lda, stride_a, b, ldb, z_gate, z_up, ldz, d_gate, d_up, ldd, c, ldc, offsets, groups,
+                       mode, type);
+  });
+}
+// the addresses of the functions, in the order of `Functions` (`GroupedFunctions`, `GatedFunctions`)
 PyObject *bind_to(void *to, PyObject *const *args, Py_ssize_t n, const Py_ssize_t want) {
   if (!count_is(n, want)) return nullptr;
   void *p[kFunctions > kGroupedFunctions ? kFunctions : kGroupedFunctions];
@@ -317,6 +374,8 @@ PyObject *bind_to(void *to, PyObject *const *args, Py_ssize_t n, const Py_ssize_
 PyObject *bind(PyObject *, PyObject *const *args, Py_ssize_t n) { return bind_to(&f, args, n, kFunctions); }
 PyObject *bind_grouped(PyObject *, PyObject *const *args, Py_ssize_t n) { return bind_to(&fg, args, n, kGroupedFunctions); }
 
+PyObject *bind_gated(PyObject *, PyObject *const *args, Py_ssize_t n) { return bind_to(&fb, args, n, kGatedFunctions); }
+
 PyMethodDef methods[] = {{"bind", (PyCFunction)(void (*)(void))bind, METH_FASTCALL, nullptr},
                          {"gemm", (PyCFunction)(void (*)(void))gemm, METH_FASTCALL, nullptr},
                          {"strided_batch", (PyCFunction)(void (*)(void))strided_batch, METH_FASTCALL, nullptr},
@@ -328,6 +387,9 @@ PyMethodDef methods[] = {{"bind", (PyCFunction)(void (*)(void))bind, METH_FASTCA
                          {"gemm_grouped_k", (PyCFunction)(void (*)(void))gemm_grouped_k, METH_FASTCALL, nullptr},
                          {"gemm_i8", (PyCFunction)(void (*)(void))gemm_i8, METH_FASTCALL, nullptr},
                          {"quantize_i8", (PyCFunction)(void (*)(void))quantize_i8, METH_FASTCALL, nullptr},
+                         {"bind_gated", (PyCFunction)(void (*)(void))bind_gated, METH_FASTCALL, nullptr},
+                         {"gemm_gated", (PyCFunction)(void (*)(void))gemm_gated, METH_FASTCALL, nullptr},
+                         {"gemm_gated_backward", (PyCFunction)(void (*)(void))gemm_gated_backward, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_call", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 } // namespace

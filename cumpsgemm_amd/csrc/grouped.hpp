@@ -2,6 +2,9 @@
 //
 //   ragged columns (gemm_grouped, gemm_i8): C[:, j] = alpha op(A_g) B[:, j] + beta C[:, j]   for j in group g
 //   ragged K (gemm_grouped_k):              C_g     = alpha A[:, g] B[:, g]^T + beta C_g
+// and of gated feed-forward blocks, whose columns are ragged too, or all of one group:
+//   projections (gemm_gated):               C[:, j] = act(G[:, j]) * U[:, j],  G = op(gate_g) B, U = op(up_g) B
+//   their gradient (gemm_gated_backward):   dG = D * U * act'(G), dU = D * act(G),  D = op(A_g) B
 //
 // Column-major throughout.  Where a group begins and ends is read from device memory by the kernels themselves
 // (offsets[g], offsets[g + 1], brought into [0, count] and into order there, so that no value of them leads out of
@@ -12,9 +15,10 @@
 
 namespace cumpsgemm_amd {
 
-// What a kernel multiplies: FP32 in one of the four splits (gemm_kernel.hpp), FP16, BF16 or 8-bit integers.
-enum class Elem : int { F32_FP16TCEC = 0, F32_FP16TC = 1, F32_BF16X3 = 2, F32_BF16X2 = 3, F16 = 4, BF16 = 5, I8 = 6 };
-constexpr int kNumElems = 7;
+// What a kernel multiplies: FP32 in one of the four splits (gemm_kernel.hpp), FP16, BF16, 8-bit integers, or 8-bit floating
+// point (f8_kernel.hpp), A in E4M3 and B in E4M3 or E5M2.
+enum class Elem : int { F32_FP16TCEC = 0, F32_FP16TC = 1, F32_BF16X3 = 2, F32_BF16X2 = 3, F16 = 4, BF16 = 5, I8 = 6, E4M3 = 7, E5M2 = 8 };
+constexpr int kNumElems = 9;
 
 enum GroupedOut : uint32_t { OUT_F32 = 0, OUT_F16 = 1, OUT_BF16 = 2 };
 
@@ -32,6 +36,16 @@ struct GroupedArgs {
   uint32_t vec_c;           // four results of a column can be stored at once
   const float *scale_a;     // 8-bit integers: [groups][m] and [n]
   const float *scale_b;
+  // gated blocks.  Projections: `a` is the gate's matrix, `up` the other one, laid out like it; z[0], z[1]: where G and U go
+  // (null: nowhere).  Gradient: z is read, d[0] and d[1] get dG and dU, c act(G) * U (null: nowhere).
+  const char *up;
+  char *z[2];
+  char *d[2];
+  uint64_t ldz, ldd;
+  uint32_t act;             // cuMpSGEMM_activation_t
+  // 8-bit floating point: one scale for 128 x 128 of A, as it is stored, and for 128 values of a column of B
+  const float *scale_up;
+  uint64_t stride_scale;    // between the groups' scales of A
   // ragged K: each group's K in this many parts of whole steps, whose sums go to `partial` as whole tiles, [group]
   // [tile column][tile row][part][column of the tile][row of the tile], and are added in that order by a second launch
   uint32_t splits;          // 1: none
@@ -42,6 +56,9 @@ struct GroupedKernel {
   void (*launch)(const GroupedArgs &, uint32_t workgroups, hipStream_t);
   int bm, bn;
 };
+
+// What becomes of the sums: C as they are, a gated block's result, or its gradient.
+enum class Epilogue : int { STORE = 0, GATED = 1, GATED_BACKWARD = 2 };
 
 // Kernels of ragged columns: three tiles of the tiled kernel, from the largest, and the kernel of few tokens to a group
 // (grouped_stream.hpp).  Ragged K: the first two, and one for matrices of fewer than eight 16-bit rows or columns.

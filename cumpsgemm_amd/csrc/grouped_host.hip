@@ -8,12 +8,20 @@ namespace cumpsgemm_amd {
 
 extern GroupedTable g_grouped_f32_fp16tcec, g_grouped_f32_fp16tc, g_grouped_f32_bf16x3, g_grouped_f32_bf16x2,
     g_grouped_f16, g_grouped_bf16, g_grouped_i8;
+extern GroupedTable g_gated_f32_fp16tcec, g_gated_f32_fp16tc, g_gated_f32_bf16x3, g_gated_f32_bf16x2, g_gated_f16, g_gated_bf16;
+extern GroupedTable g_gated_backward_f32_fp16tcec, g_gated_backward_f32_fp16tc, g_gated_backward_f32_bf16x3,
+    g_gated_backward_f32_bf16x2, g_gated_backward_f16, g_gated_backward_bf16;
 
 // direct: the operands can take the shorter way into LDS (grouped_kernel.hpp); the kernel of few tokens takes any
-const GroupedKernel *lookup_grouped(Elem e, bool a_kc, bool ragged_k, bool direct, int cls) {
-  static const GroupedTable *const tables[kNumElems] = {&g_grouped_f32_fp16tcec, &g_grouped_f32_fp16tc, &g_grouped_f32_bf16x3,
-                                                        &g_grouped_f32_bf16x2, &g_grouped_f16, &g_grouped_bf16, &g_grouped_i8};
-  const GroupedTable &t = *tables[(int)e];
+const GroupedKernel *lookup_grouped(Elem e, bool a_kc, bool ragged_k, bool direct, int cls, Epilogue epi = Epilogue::STORE) {
+  static const GroupedTable *const tables[3][kNumElems] = {
+      {&g_grouped_f32_fp16tcec, &g_grouped_f32_fp16tc, &g_grouped_f32_bf16x3, &g_grouped_f32_bf16x2, &g_grouped_f16,
+       &g_grouped_bf16, &g_grouped_i8},
+      {&g_gated_f32_fp16tcec, &g_gated_f32_fp16tc, &g_gated_f32_bf16x3, &g_gated_f32_bf16x2, &g_gated_f16, &g_gated_bf16},
+      {&g_gated_backward_f32_fp16tcec, &g_gated_backward_f32_fp16tc, &g_gated_backward_f32_bf16x3, &g_gated_backward_f32_bf16x2,
+       &g_gated_backward_f16, &g_gated_backward_bf16}};
+  if (tables[(int)epi][(int)e] == nullptr) return nullptr;
+  const GroupedTable &t = *tables[(int)epi][(int)e];
   const GroupedKernel *k = ragged_k ? (cls == STREAM ? nullptr : &t.over_k[direct][cls])
                            : cls == STREAM ? &t.stream[a_kc] : &t.columns[a_kc][direct][cls];
   return k != nullptr && k->launch != nullptr ? k : nullptr;
@@ -145,9 +153,9 @@ double cost_over_k_us(Elem e, int cls, double tiles, double tile_bytes, double k
          (splits == 1 ? 0.0 : 3.0 + tiles * tile_bytes * (splits + 1) / 5.3e6);
 }
 // CUMPSGEMM_FORCE_TILE_CLASS goes before the rule where there is such a kernel.
-bool forced(Elem e, bool a_kc, bool ragged_k, bool direct, int &cls) {
+bool forced(Elem e, bool a_kc, bool ragged_k, bool direct, int &cls, Epilogue epi = Epilogue::STORE) {
   const int want = tuning().force_cls;
-  if (want < 0 || want > STREAM || (ragged_k && want == SHORT_LINES) || lookup_grouped(e, a_kc, ragged_k, direct, want) == nullptr) return false;
+  if (want < 0 || want > STREAM || (ragged_k && want == SHORT_LINES) || lookup_grouped(e, a_kc, ragged_k, direct, want, epi) == nullptr) return false;
   cls = want;
   return true;
 }
@@ -160,17 +168,19 @@ uint64_t most_tiles(const GroupedArgs &args, const GroupedKernel &k) {
 }
 
 // Ragged columns: B and C have args.n columns in args.groups groups.
-hipblasStatus_t run_columns(cuMpSGEMM_handle *h, Elem e, bool a_kc, GroupedArgs &args, const char *label) {
+hipblasStatus_t run_columns(cuMpSGEMM_handle *h, Elem e, bool a_kc, GroupedArgs &args, const char *label,
+                            Epilogue epi = Epilogue::STORE) {
   const uint32_t bytes = bytes_of(e);
   const bool direct = chunks_ok(args.a, a_kc ? args.k : args.m, args.lda, args.stride_a, bytes, a_kc ? 256 : 64) &&
-                      chunks_ok(args.b, args.k, args.ldb, 0, bytes, 256);
+                      chunks_ok(args.b, args.k, args.ldb, 0, bytes, 256) &&
+                      (epi != Epilogue::GATED || chunks_ok(args.up, 16, args.lda, args.stride_a, bytes, 0));
   int cls = TILE_128;
   if (bytes == 2 && !direct && !a_kc && args.m < 8) {
     cls = STREAM; // (a line is shorter than the chunks that the tiled kernels read)
-  } else if (!forced(e, a_kc, false, direct, cls)) {
+  } else if (!forced(e, a_kc, false, direct, cls, epi)) {
     double best = 0.0;
     for (int c = TILE_256; c <= STREAM; c++) {
-      const GroupedKernel *const kern = lookup_grouped(e, a_kc, false, direct, c);
+      const GroupedKernel *const kern = lookup_grouped(e, a_kc, false, direct, c, epi);
       if (kern == nullptr || most_tiles(args, *kern) > kMostWorkgroups) continue;
       // columns of tiles, the groups' sizes being unknown here: half of each group's last one, or one for each group
       const double some = std::min(args.n, args.groups), each = (double)args.n / args.groups;
@@ -185,13 +195,42 @@ hipblasStatus_t run_columns(cuMpSGEMM_handle *h, Elem e, bool a_kc, GroupedArgs 
       if (best == 0.0 || us < best) best = us, cls = c;
     }
   }
-  const GroupedKernel *k = lookup_grouped(e, a_kc, false, direct, cls);
+  const GroupedKernel *k = lookup_grouped(e, a_kc, false, direct, cls, epi);
   if (k == nullptr) return HIPBLAS_STATUS_INTERNAL_ERROR;
   const uint64_t workgroups = most_tiles(args, *k);
   if (workgroups > kMostWorkgroups) return HIPBLAS_STATUS_INVALID_VALUE;
   ProfileScope prof(h, label);
   k->launch(args, (uint32_t)workgroups, h->stream);
   return launched();
+}
+
+// What gated blocks and their gradients are given alike.  nothing: there is nothing to compute.
+hipblasStatus_t gated_arguments(cuMpSGEMM_handle *h, hipblasOperation_t op_A, cuMpSGEMM_activation_t activation, uint64_t m,
+                                uint64_t n, uint64_t k, const void *a, uint64_t lda, uint64_t stridea, const void *b, uint64_t ldb,
+                                const int *offsets, uint64_t group_count, cuMpSGEMM_compute_mode_t mode, hipDataType type, Elem &e,
+                                bool &nothing, GroupedArgs &args) {
+  nothing = false;
+  if (h == nullptr || (op_A != HIPBLAS_OP_N && op_A != HIPBLAS_OP_T && op_A != HIPBLAS_OP_C)) return HIPBLAS_STATUS_INVALID_VALUE;
+  if ((int)activation < CUMPSGEMM_SILU || (int)activation > CUMPSGEMM_RELU) return HIPBLAS_STATUS_INVALID_VALUE;
+  if (m > kMost || n > kMost || k > kMost || group_count > kMost) return HIPBLAS_STATUS_INVALID_VALUE;
+  if (!elem_of(type, mode, e) || !out_of(type, args.out)) return HIPBLAS_STATUS_INVALID_VALUE;
+  if (offsets == nullptr && group_count > 1) return HIPBLAS_STATUS_INVALID_VALUE;
+  nothing = m == 0 || n == 0 || group_count == 0;
+  if (nothing) return HIPBLAS_STATUS_SUCCESS;
+  if (k != 0 && (lda < (op_A != HIPBLAS_OP_N ? k : m) || ldb < k || a == nullptr || b == nullptr)) return HIPBLAS_STATUS_INVALID_VALUE;
+  args.m = (uint32_t)m;
+  args.n = (uint32_t)n;
+  args.k = (uint32_t)k;
+  args.groups = (uint32_t)group_count;
+  args.offsets = offsets;
+  args.a = (const char *)a;
+  args.b = (const char *)b;
+  args.lda = lda;
+  args.ldb = ldb;
+  args.stride_a = stridea;
+  args.alpha = 1.0f;
+  args.act = (uint32_t)activation;
+  return HIPBLAS_STATUS_SUCCESS;
 }
 } // namespace
 } // namespace cumpsgemm_amd
@@ -305,6 +344,57 @@ hipblasStatus_t cuMpSGEMM_gemm_grouped_k(cuMpSGEMM_handle_t h, uint64_t m, uint6
   kern->launch(args, (uint32_t)workgroups, h->stream);
   if (args.splits > 1) launch_grouped_join(args, kern->bm, kern->bn, h->stream);
   return launched();
+}
+
+hipblasStatus_t cuMpSGEMM_gemm_gated(cuMpSGEMM_handle_t h, hipblasOperation_t op_A, cuMpSGEMM_activation_t activation, uint64_t m,
+                                     uint64_t n, uint64_t k, const void *gate, const void *up, uint64_t lda, uint64_t stridea,
+                                     const void *b, uint64_t ldb, void *c, uint64_t ldc, void *z_gate, void *z_up, uint64_t ldz,
+                                     const int *offsets, uint64_t group_count, cuMpSGEMM_compute_mode_t mode, hipDataType type) {
+  GroupedArgs args{};
+  Elem e;
+  bool nothing;
+  const hipblasStatus_t st = gated_arguments(h, op_A, activation, m, n, k, gate, lda, stridea, b, ldb, offsets, group_count, mode, type, e, nothing, args);
+  if (st != HIPBLAS_STATUS_SUCCESS || nothing) return st;
+  if (ldc < m || c == nullptr || (k != 0 && up == nullptr)) return HIPBLAS_STATUS_INVALID_VALUE;
+  if ((z_gate == nullptr) != (z_up == nullptr) || (z_gate != nullptr && ldz < m)) return HIPBLAS_STATUS_INVALID_VALUE;
+  args.up = (const char *)up;
+  args.c = (char *)c;
+  args.ldc = ldc;
+  args.z[0] = (char *)z_gate;
+  args.z[1] = (char *)z_up;
+  args.ldz = ldz;
+  args.vec_c = four_at_once(c, m, ldc, 0, args.out) &&
+               (z_gate == nullptr || (four_at_once(z_gate, m, ldz, 0, args.out) && four_at_once(z_up, m, ldz, 0, args.out)));
+  return run_columns(h, e, op_A != HIPBLAS_OP_N, args, "gemm_gated", Epilogue::GATED);
+}
+
+hipblasStatus_t cuMpSGEMM_gemm_gated_backward(cuMpSGEMM_handle_t h, hipblasOperation_t op_A, cuMpSGEMM_activation_t activation,
+                                              uint64_t m, uint64_t n, uint64_t k, const void *a, uint64_t lda, uint64_t stridea,
+                                              const void *b, uint64_t ldb, const void *z_gate, const void *z_up, uint64_t ldz,
+                                              void *d_gate, void *d_up, uint64_t ldd, void *c, uint64_t ldc, const int *offsets,
+                                              uint64_t group_count, cuMpSGEMM_compute_mode_t mode, hipDataType type) {
+  GroupedArgs args{};
+  Elem e;
+  bool nothing;
+  const hipblasStatus_t st = gated_arguments(h, op_A, activation, m, n, k, a, lda, stridea, b, ldb, offsets, group_count, mode, type, e, nothing, args);
+  if (st != HIPBLAS_STATUS_SUCCESS || nothing) return st;
+  if (z_gate == nullptr || z_up == nullptr || ldz < m || d_gate == nullptr || d_up == nullptr || ldd < m || (c != nullptr && ldc < m))
+    return HIPBLAS_STATUS_INVALID_VALUE;
+  // (in place: with another leading dimension a column's gradients would be written over another's values)
+  if ((d_gate == z_gate || d_up == z_up || d_gate == z_up || d_up == z_gate) && (ldd != ldz || d_gate == z_up || d_up == z_gate))
+    return HIPBLAS_STATUS_INVALID_VALUE;
+  args.z[0] = (char *)z_gate;
+  args.z[1] = (char *)z_up;
+  args.ldz = ldz;
+  args.d[0] = (char *)d_gate;
+  args.d[1] = (char *)d_up;
+  args.ldd = ldd;
+  args.c = (char *)c;
+  args.ldc = ldc;
+  args.vec_c = four_at_once(z_gate, m, ldz, 0, args.out) && four_at_once(z_up, m, ldz, 0, args.out) &&
+               four_at_once(d_gate, m, ldd, 0, args.out) && four_at_once(d_up, m, ldd, 0, args.out) &&
+               (c == nullptr || four_at_once(c, m, ldc, 0, args.out));
+  return run_columns(h, e, op_A != HIPBLAS_OP_N, args, "gemm_gated_backward", Epilogue::GATED_BACKWARD);
 }
 
 hipblasStatus_t cuMpSGEMM_gemm_i8(cuMpSGEMM_handle_t h, uint64_t m, uint64_t n, uint64_t k, const int8_t *a, uint64_t lda,

@@ -23,6 +23,7 @@
 // 4096 tokens of 8, 2048 x 1024: 78 with uneven experts in 128 x 128 tiles, 60 with even ones (256 x 128 tiles: 54, zeros 44);
 // 28 % MFMAs, and beside them as many clocks of LDS reads, which the schedule does not hide whole.
 #pragma once
+#include "activation.hpp"
 #include "gemm_kernel.hpp"
 #include "grouped.hpp"
 #include "gemm_table.hpp"
@@ -33,14 +34,14 @@ typedef int i4_t __attribute__((ext_vector_type(4)));
 
 template <Elem E> struct elem_traits {
   static constexpr bool F32 = (int)E <= 3;
-  static constexpr bool I8 = E == Elem::I8;
+  static constexpr bool I8 = E == Elem::I8, F8 = E == Elem::E4M3 || E == Elem::E5M2;
   static constexpr Prec P = F32 ? (Prec)(int)E : Prec::FP16TC;
   static constexpr bool IS_BF16 = F32 ? prec_traits<P>::IS_BF16 : E == Elem::BF16;
-  static constexpr int BYTES = F32 ? 4 : I8 ? 1 : 2; // of an element in memory
+  static constexpr int BYTES = F32 ? 4 : I8 || F8 ? 1 : 2; // of an element in memory
   static constexpr int NP = F32 ? prec_traits<P>::NP : 1;
   static constexpr int NPROD = F32 ? prec_traits<P>::NPROD : 1;
   static constexpr int NACC = F32 ? prec_traits<P>::NACC : 1;
-  static constexpr int CHUNK = I8 ? 16 : 8;         // K-values of a 16-byte chunk in LDS
+  static constexpr int CHUNK = BYTES == 1 ? 16 : 8; // K-values of a 16-byte chunk in LDS
   typedef typename std::conditional<I8, i4_t, f4v_t>::type acc_t;
 };
 
@@ -68,6 +69,11 @@ __device__ inline const char *uniform_address(const char *p) {
 }
 // which 32-byte piece of line k holds piece p of a row-contiguous image
 __device__ inline int line_swizzle(int k) { return (k & 3) | (((k >> 3) & 1) << 2); }
+
+// the same for lines of 8-bit values: which 16-byte piece of line k holds piece p ^ this (f8_kernel.hpp)
+template <int ROWS> __device__ inline int byte_line_swizzle(int k) {
+  return ROWS >= 256 ? (k & 7) | (k >> 4 & 1) << 3 : (k >> 1 & 3) | (k >> 4 & 1) << 2;
+}
 
 // A tile's place: its group, and where that begins and ends.
 struct TilePlace {
@@ -207,12 +213,18 @@ __device__ inline bool place_over_k(const GroupedArgs &args, uint32_t bid, uint3
 // split in registers, are read with 32-bit offsets from uniform bases.  Otherwise: any alignment, any size; but lines of
 // 16-bit values that are shorter than a chunk are for the CAREFUL kernels.
 template <Elem E_, bool A_KC_, bool B_KC_, int BM_, int BN_, int WM_, int WN_, int ROW_BYTES_, int NSTAGE_, bool DIRECT_,
-          bool RAGGED_K_, int OCC_, bool CAREFUL_>
+          bool RAGGED_K_, int OCC_, bool CAREFUL_, Epilogue EPI_ = Epilogue::STORE>
 struct GroupedCfg {
   using T = elem_traits<E_>;
   static constexpr Elem E = E_;
   static constexpr bool A_KC = A_KC_, B_KC = B_KC_, DIRECT = DIRECT_, RAGGED_K = RAGGED_K_, CAREFUL = CAREFUL_;
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NSTAGE = NSTAGE_, OCC = OCC_;
+  static constexpr Epilogue EPI = EPI_;
+  // A gated block's tile has BM / 2 rows of the gate's matrix and as many of the other, sixteen of the one after sixteen of the
+  // other, so that a lane that holds a row's sum with the one holds that with the other, 16 x 16 blocks i and i + 1.
+  static constexpr bool GATED = EPI == Epilogue::GATED;
+  static constexpr int ROWS_OUT = GATED ? BM / 2 : BM, WAVE_ROWS_OUT = GATED ? WM / 2 : WM;
+  static_assert(!GATED || (WM_ % 32 == 0 && !RAGGED_K_), "pairs of blocks");
   static constexpr int WAVES_M = BM / WM, WAVES_N = BN / WN, NT = WAVES_M * WAVES_N * 64;
   static constexpr int TM = WM / 16, TN = WN / 16;
   static constexpr int ROW_BYTES = ROW_BYTES_;
@@ -238,7 +250,9 @@ struct GroupedCfg {
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 // Staging of one operand's K-step by NT threads.  A unit is one 16-byte chunk of LDS (FP32: one in each plane).
-template <Elem E, bool KC, int ROWS, int ROW_BYTES, int NT> struct grouped_loader {
+// GATED: the rows come from two matrices, sixteen at a time (GroupedCfg).  K-contiguous and FP32 operands: a wave's units
+// are all of one of them (side()).  LINES: a lane's; `apart` is what lies between the two matrices.
+template <Elem E, bool KC, int ROWS, int ROW_BYTES, int NT, bool GATED = false> struct grouped_loader {
   using T = elem_traits<E>;
   // row-contiguous images exist for 16-bit values only; FP32 ends in K-contiguous planes either way
   static constexpr bool LINES = !KC && !T::F32;
@@ -246,7 +260,7 @@ template <Elem E, bool KC, int ROWS, int ROW_BYTES, int NT> struct grouped_loade
   static constexpr int U = (UNITS + NT - 1) / NT;
   static constexpr bool PARTIAL = UNITS < NT;
   static_assert(UNITS % NT == 0 || (PARTIAL && UNITS % 64 == 0), "whole waves");
-  static constexpr int LINE_CHUNKS = ROWS / 8;            // 16-byte chunks of a line
+  static constexpr int LINE_CHUNKS = ROWS / T::CHUNK;     // 16-byte chunks of a line
   static constexpr int ROW_CHUNKS = ROW_BYTES / 16;
 
   __device__ static inline bool active(int tid) { return !PARTIAL || tid < UNITS; }
@@ -257,7 +271,8 @@ template <Elem E, bool KC, int ROWS, int ROW_BYTES, int NT> struct grouped_loade
     if constexpr (LINES) {
       k = id / LINE_CHUNKS;
       const int c = id % LINE_CHUNKS;
-      row = ((((c >> 1) ^ line_swizzle(k)) << 1) | (c & 1)) * 8;
+      if constexpr (T::BYTES == 1) row = (c ^ byte_line_swizzle<ROWS>(k)) * 16;
+      else row = ((((c >> 1) ^ line_swizzle(k)) << 1) | (c & 1)) * 8;
     } else if constexpr (T::F32) {
       // (not an image position: FP32 chunks are written one by one, in whatever order reads memory best)
       if constexpr (KC) {
@@ -265,6 +280,7 @@ template <Elem E, bool KC, int ROWS, int ROW_BYTES, int NT> struct grouped_loade
         k = id % ROW_CHUNKS * T::CHUNK;
       } else {
         row = id % ROWS;
+        if constexpr (GATED) row = (row % (ROWS / 2) / 16) * 32 + row / (ROWS / 2) * 16 + row % 16; // (half of them, then the others)
         k = id / ROWS * T::CHUNK;
       }
     } else {
@@ -278,15 +294,27 @@ template <Elem E, bool KC, int ROWS, int ROW_BYTES, int NT> struct grouped_loade
   // term, 4096 x 2048 x 1024 in 8 groups 43.6 us, so 39.2; in two or three terms 0 - 4 %.)
   __device__ static constexpr int value_of(int k, int j) { return k / 2 + (j & 3) + (j >> 2) * 16; }
 
+  // the row of its own matrix that row `row` of a tile is, and which of the two that is
+  __device__ static inline int own_row(int row) { return GATED ? (row >> 5) * 16 + (row & 15) : row; }
+  __device__ static inline int side_of(int row) { return GATED ? row >> 4 & 1 : 0; }
+  static_assert(!GATED || LINES || (NT * 16 / ROW_BYTES % 32 == 0 && UNITS >= NT), "every round of units begins on the same side");
+  __device__ static inline int side(int wave) {
+    int row, k;
+    at(wave * 64, row, k);
+    return side_of(row);
+  }
+
   // Byte offset from the tile's origin (row 0, K-value 0 of the step) of the unit that fills position id.
   // `rows`: those that exist; one (LINES: eight) beyond them reads the last again (its products are not stored).
-  __device__ static inline uint64_t offset(int id, uint64_t ld, int rows) {
+  __device__ static inline uint64_t offset(int id, uint64_t ld, int rows, uint64_t apart = 0) {
     int row, k;
     at(id, row, k);
-    const int last = LINES ? (rows - 1) & ~7 : rows - 1;
+    const uint64_t more = GATED && LINES && side_of(row) ? apart : 0;
+    row = own_row(row);
+    const int last = LINES ? (rows - 1) & -T::CHUNK : rows - 1;
     row = row < last ? row : last;
     if constexpr (T::F32) k = value_of(k, 0);
-    return (KC ? (uint64_t)row * ld + k : (uint64_t)k * ld + row) * T::BYTES;
+    return (KC ? (uint64_t)row * ld + k : (uint64_t)k * ld + row) * T::BYTES + more;
   }
 
   // memory -> LDS, 16 bytes a lane: load number u of a whole step, from the uniform base + off.
@@ -299,8 +327,13 @@ template <Elem E, bool KC, int ROWS, int ROW_BYTES, int NT> struct grouped_loade
     const uint32_t to = lds_op + (uint32_t)((wave * 64 + u * NT) * 16);
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory", "m0");
   }
+  // ... from a lane's own address
+  __device__ static inline void direct(int u, const char *base, uint64_t off, uint32_t lds_op, int wave) {
+    const uint32_t to = lds_op + (uint32_t)((wave * 64 + u * NT) * 16);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(base + off) : "memory", "m0");
+  }
   // ... of a step that has only `left` K-values: zeros from there on
-  __device__ static inline void direct_tail(int u, const char *base, uint32_t off, uint32_t lds_op, int tid, int wave, int left) {
+  __device__ static inline void direct_tail(int u, const char *base, uint64_t off, uint32_t lds_op, int tid, int wave, int left) {
     int row, k;
     at(tid + u * NT, row, k);
     const char *p = k < left ? base + off : reinterpret_cast<const char *>(&g_grouped_zeros);
@@ -316,7 +349,8 @@ template <Elem E, bool KC, int ROWS, int ROW_BYTES, int NT> struct grouped_loade
   // A chunk of a line (LINES) may stick out beyond the rows, into the next line: not for the matrix's last line, unless
   // CAREFUL (rows, safe: see fetch_tail).
   template <bool FAST, bool CAREFUL, class OFF>
-  __device__ static inline void fetch(Regs &r, int u, const char *base, uint64_t ld, OFF off, int rows, int64_t safe, int tid) {
+  __device__ static inline void fetch(Regs &r, int u, const char *base, uint64_t ld, OFF off, int rows, int64_t safe, int tid,
+                                      uint64_t apart = 0) {
     if (!active(tid)) return;
     if constexpr (T::F32 && KC) {
       typedef float f4u_t __attribute__((ext_vector_type(4), aligned(4)));
@@ -338,12 +372,12 @@ template <Elem E, bool KC, int ROWS, int ROW_BYTES, int NT> struct grouped_loade
       // (rows of 16-bit values may begin anywhere: the type promises no more and leaves the instruction to the compiler)
       typedef uint32_t u4u2_t __attribute__((ext_vector_type(4), aligned(2)));
       typedef uint32_t u4u1_t __attribute__((ext_vector_type(4), aligned(1)));
-      typedef typename std::conditional<T::I8, u4u1_t, u4u2_t>::type u4u_t;
+      typedef typename std::conditional<T::BYTES == 1, u4u1_t, u4u2_t>::type u4u_t;
       if (!LINES || !CAREFUL) {
         const u4u_t x = *reinterpret_cast<const u4u_t *>(base + off);
         r.v[u] = u4_t{x.x, x.y, x.z, x.w};
       } else {
-        fetch_tail(r, u, base, ld, rows, 1 << 30, safe, tid);
+        fetch_tail(r, u, base, ld, rows, 1 << 30, safe, tid, apart);
       }
     }
   }
@@ -352,10 +386,15 @@ template <Elem E, bool KC, int ROWS, int ROW_BYTES, int NT> struct grouped_loade
   // it, the last row again in that of rows.  A 16-byte chunk that sticks out beyond the last row (LINES) or K-value is
   // read whole all the same, where what follows it is the next line or row of the matrix: for the first `safe` lines
   // (rows, K-contiguous) counted from the base.  The others are read value by value.
-  __device__ static inline void fetch_tail(Regs &r, int u, const char *base, uint64_t ld, int rows, int left, int64_t safe, int tid) {
+  __device__ static inline void fetch_tail(Regs &r, int u, const char *base, uint64_t ld, int rows, int left, int64_t safe, int tid,
+                                           uint64_t apart = 0) {
     if (!active(tid)) return;
     int row, k;
     at(tid + u * NT, row, k);
+    if constexpr (GATED) {
+      if (LINES && side_of(row)) base += apart;
+      row = own_row(row);
+    }
     if constexpr (T::F32) {
       row = row < rows ? row : rows - 1;
       const uint64_t step = KC ? 1 : ld;
@@ -369,15 +408,15 @@ template <Elem E, bool KC, int ROWS, int ROW_BYTES, int NT> struct grouped_loade
         r.v[u][j] = in ? x : 0.0f;
       }
     } else {
-      typedef typename std::conditional<T::I8, uint8_t, uint16_t>::type V;
+      typedef typename std::conditional<T::BYTES == 1, uint8_t, uint16_t>::type V;
       typedef uint32_t u4u2_t __attribute__((ext_vector_type(4), aligned(2)));
       typedef uint32_t u4u1_t __attribute__((ext_vector_type(4), aligned(1)));
-      typedef typename std::conditional<T::I8, u4u1_t, u4u2_t>::type u4u_t;
+      typedef typename std::conditional<T::BYTES == 1, u4u1_t, u4u2_t>::type u4u_t;
       constexpr int BITS = T::BYTES * 8, PER = 32 / BITS;
-      const int last = LINES ? (rows - 1) & ~7 : rows - 1;
+      const int last = LINES ? (rows - 1) & -T::CHUNK : rows - 1;
       row = row < last ? row : last;
       const int begins = k < left ? k : 0;               // (a chunk with nothing in it reads the step's first)
-      const int keep = LINES ? (k < left ? 8 : 0) : left - k; // values of the chunk that count
+      const int keep = LINES ? (k < left ? T::CHUNK : 0) : left - k; // values of the chunk that count
       const int have = LINES ? rows - row : left - begins;    // ... that exist
       const V *p = reinterpret_cast<const V *>(base) + (KC ? (uint64_t)row * ld + begins : (uint64_t)begins * ld + row);
       u4_t x = {0, 0, 0, 0};
@@ -403,7 +442,7 @@ template <Elem E, bool KC, int ROWS, int ROW_BYTES, int NT> struct grouped_loade
     const int id = tid + u * NT;
     if constexpr (T::F32) {
       int row, k;
-      at(id, row, k);
+      at(id, row, k); // (the tile's row)
       u4_t out[T::NP];
 #pragma unroll
       for (int q = 0; q < 4; q++) {
@@ -459,9 +498,60 @@ __device__ inline void store_four(char *c, const f4v_t x, float beta, uint32_t r
   }
 }
 
+// Rows row .. row + 3 of column col of a gated block: the result, and the projections where they are wanted.
+template <uint32_t OUT, bool EXACT>
+__device__ inline void store_gated(const GroupedArgs &args, const f4v_t gate, const f4v_t up, uint32_t row, uint32_t col) {
+  constexpr int BYTES = sizeof(typename out_type<OUT>::type);
+  f4v_t x;
+  float slope;
+#pragma unroll
+  for (int v = 0; v < 4; v++) x[v] = activation<EXACT, false>(args.act, gate[v], slope) * up[v];
+  store_four<OUT>(args.c + ((uint64_t)col * args.ldc + row) * BYTES, x, 0.0f, row, args.m, args.vec_c != 0);
+  if (args.z[0] == nullptr) return;
+  const uint64_t at = ((uint64_t)col * args.ldz + row) * BYTES;
+  store_four<OUT>(args.z[0] + at, gate, 0.0f, row, args.m, args.vec_c != 0);
+  store_four<OUT>(args.z[1] + at, up, 0.0f, row, args.m, args.vec_c != 0);
+}
+// p[0 .. 3], zeros from row m on
+template <uint32_t OUT> __device__ inline f4v_t load_four(const char *c, uint32_t row, uint32_t m, bool vec) {
+  typedef typename out_type<OUT>::type O;
+  typedef O o4_t __attribute__((ext_vector_type(4)));
+  const O *p = reinterpret_cast<const O *>(c);
+  f4v_t x = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (vec) {
+    if (row < m) x = __builtin_convertvector(*reinterpret_cast<const o4_t *>(p), f4v_t);
+  } else {
+#pragma unroll
+    for (int v = 0; v < 4; v++)
+      if (row + v < m) x[v] = (float)p[v];
+  }
+  return x;
+}
+// ... of its gradient: x is that of act(G) * U.  (G and U are read before anything is written: dG and dU may take their place.)
+template <uint32_t OUT, bool EXACT>
+__device__ inline void store_gradients(const GroupedArgs &args, const f4v_t x, uint32_t row, uint32_t col) {
+  constexpr int BYTES = sizeof(typename out_type<OUT>::type);
+  const bool vec = args.vec_c != 0;
+  const uint64_t from = ((uint64_t)col * args.ldz + row) * BYTES, to = ((uint64_t)col * args.ldd + row) * BYTES;
+  const f4v_t gate = load_four<OUT>(args.z[0] + from, row, args.m, vec), up = load_four<OUT>(args.z[1] + from, row, args.m, vec);
+  f4v_t h, dg, du;
+#pragma unroll
+  for (int v = 0; v < 4; v++) {
+    float slope;
+    const float a = activation<EXACT, true>(args.act, gate[v], slope);
+    h[v] = a * up[v];
+    dg[v] = x[v] * up[v] * slope;
+    du[v] = x[v] * a;
+  }
+  store_four<OUT>(args.d[0] + to, dg, 0.0f, row, args.m, vec);
+  store_four<OUT>(args.d[1] + to, du, 0.0f, row, args.m, vec);
+  if (args.c != nullptr) store_four<OUT>(args.c + ((uint64_t)col * args.ldc + row) * BYTES, h, 0.0f, row, args.m, vec);
+}
+
 // A tile's place in memory: what its loops need to know.
 struct TileWork {
   const char *a, *b;       // row m0, token n0 (ragged K: column n0), K-value 0
+  const char *up;          // gated: row m0 of the other matrix
   char *c;                 // of its group
   float *partial;          // where a part's sums go (ragged K in parts)
   uint32_t group, m0, n0, n_end, klen;
@@ -469,6 +559,80 @@ struct TileWork {
   // lines (rows, K-contiguous operand) from a and b to the matrix's last but one; 0 where one is shorter than a chunk
   int64_t safe_a, safe_b;
 };
+
+// What a tile's sums become.  sum(j, i, v): register v of lane l, MFMA row 4 (l / 16) + v (of C), column l % 16 (token) of
+// column block j and row block i.  One column block after the other passes through LDS, each wave's through a part of its
+// own, so that a wave's store covers the columns' whole rows.
+template <class Cfg, int TN, class Sum>
+__device__ inline void write_tile(const GroupedArgs &args, const TileWork &w, char *lds, Sum sum) {
+  using T = typename Cfg::T;
+  constexpr int TM = Cfg::TM, BM = Cfg::BM, PITCH = Cfg::PITCH;
+  const int tid = threadIdx.x, lane = tid & 63, frow = lane & 15, fg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave % Cfg::WAVES_M, wn = wave / Cfg::WAVES_M;
+  block_sync_lds(); // (every wave has read its last fragments)
+  float *mine = reinterpret_cast<float *>(lds) + wave * (16 * PITCH);
+  const uint32_t row0 = w.m0 + wm * Cfg::WAVE_ROWS_OUT;
+  constexpr int LANES = Cfg::WAVE_ROWS_OUT / 4, COLS = 64 / LANES; // lanes of a column, columns of a round
+  const uint32_t row = row0 + (lane % LANES) * 4;
+  // calls f with the type that results have
+  auto typed = [&](auto f) {
+    if (T::F32 || args.out == OUT_F32) f(std::integral_constant<uint32_t, OUT_F32>{});
+    else if (Cfg::E == Elem::F16 || (T::BYTES == 1 && args.out == OUT_F16)) f(std::integral_constant<uint32_t, OUT_F16>{});
+    else f(std::integral_constant<uint32_t, OUT_BF16>{});
+  };
+#pragma unroll
+  for (int j = 0; j < TN; j++) {
+#pragma unroll
+    for (int i = 0; i < TM; i++) {
+      f4v_t x;
+#pragma unroll
+      for (int v = 0; v < 4; v++) x[v] = sum(j, i, v);
+      *reinterpret_cast<f4v_t *>(mine + frow * PITCH + i * 16 + fg * 4) = x;
+    }
+    // (a wave's own writes and reads of LDS are carried out in order)
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    const uint32_t col0 = w.n0 + (j * Cfg::WAVES_N + wn) * 16;
+    f4v_t sa = {args.alpha, args.alpha, args.alpha, args.alpha};
+    if constexpr (T::I8) {
+#pragma unroll
+      for (int v = 0; v < 4; v++)
+        sa[v] = args.scale_a[(uint64_t)w.group * args.m + (row + v < args.m ? row + v : args.m - 1)];
+    }
+#pragma unroll 1
+    for (int r = 0; r < 16; r += COLS) {
+      const uint32_t col = col0 + r + lane / LANES;
+      if (col >= w.n_end) continue;
+      if constexpr (Cfg::EPI == Epilogue::STORE) {
+        f4v_t x = *reinterpret_cast<const f4v_t *>(mine + (r + lane / LANES) * PITCH + (lane % LANES) * 4);
+        if constexpr (Cfg::RAGGED_K) {
+          if (args.splits > 1) {
+            *reinterpret_cast<f4v_t *>(w.partial + (uint64_t)(col - w.n0) * BM + (row - w.m0)) = x;
+            continue;
+          }
+        }
+        const float sb = T::I8 ? args.scale_b[col] : 1.0f;
+#pragma unroll
+        for (int v = 0; v < 4; v++) x[v] = T::I8 ? x[v] * sa[v] * sb : x[v] * sa[v];
+        const uint64_t at = (uint64_t)col * args.ldc + row;
+        typed([&](auto out) {
+          store_four<out.value>(w.c + at * sizeof(typename out_type<out.value>::type), x, args.beta, row, args.m, args.vec_c != 0);
+        });
+      } else {
+        const int own = lane % LANES * 4;
+        const float *p = mine + (r + lane / LANES) * PITCH + (Cfg::GATED ? (own >> 4) * 32 + (own & 15) : own);
+        const f4v_t x = *reinterpret_cast<const f4v_t *>(p);
+        if constexpr (Cfg::GATED) {
+          const f4v_t y = *reinterpret_cast<const f4v_t *>(p + 16);
+          typed([&](auto out) { store_gated<out.value, T::F32>(args, x, y, row, col); });
+        } else {
+          typed([&](auto out) { store_gradients<out.value, T::F32>(args, x, row, col); });
+        }
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+  }
+}
 
 // One tile, TN column blocks of 16 for each wave: all that a wave has room for, or (a group's last tile) as many as the
 // tile's columns need.  The waves take column blocks in turn, so that a part of a tile is a part of every wave's work.
@@ -479,11 +643,14 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave % Cfg::WAVES_M, wn = wave / Cfg::WAVES_M;
-  using LA = grouped_loader<Cfg::E, Cfg::A_KC, BM, RB, NT>;
+  using LA = grouped_loader<Cfg::E, Cfg::A_KC, BM, RB, NT, Cfg::GATED>;
   using LB = grouped_loader<Cfg::E, Cfg::B_KC, BN, RB, NT>;
   // rounds of loads that B's columns need
   constexpr int UB = LB::LINES ? LB::U : (TN * 16 * Cfg::WAVES_N * RB / 16 + NT - 1) / NT;
   const char *a = w.a, *b = w.b;
+  uint64_t apart = 0; // from a row of the gate's matrix to the other's
+  if constexpr (Cfg::GATED && LA::LINES) apart = (uint64_t)(w.up - w.a);
+  else if constexpr (Cfg::GATED) a = uniform_address(LA::side(wave) ? w.up : w.a);
   const uint64_t a_step = (Cfg::A_KC ? (uint64_t)BK : (uint64_t)BK * args.lda) * T::BYTES;
   const uint64_t b_step = (Cfg::B_KC ? (uint64_t)BK : (uint64_t)BK * args.ldb) * T::BYTES;
 
@@ -613,9 +780,11 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
   auto a_at = [&](int s) { return a + (uint64_t)(s < partial ? whole : s - partial) * a_step; };
   auto b_at = [&](int s) { return b + (uint64_t)(s < partial ? whole : s - partial) * b_step; };
   typedef typename std::conditional<Cfg::DIRECT, uint32_t, uint64_t>::type off_t;
-  off_t offa[LA::U], offb[UB];
+  typedef typename std::conditional<Cfg::GATED && LA::LINES, uint64_t, off_t>::type offa_t;
+  offa_t offa[LA::U];
+  off_t offb[UB];
 #pragma unroll
-  for (int u = 0; u < LA::U; u++) offa[u] = (off_t)LA::offset(tid + u * NT, args.lda, w.rows_a);
+  for (int u = 0; u < LA::U; u++) offa[u] = (offa_t)LA::offset(tid + u * NT, args.lda, w.rows_a, apart);
 #pragma unroll
   for (int u = 0; u < UB; u++) offb[u] = (off_t)LB::offset(tid + u * NT, args.ldb, w.rows_b);
   constexpr int LOADS = LA::U + UB;
@@ -715,7 +884,7 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
     auto fetch = [&](int l, const int set, const char *pa, const char *pb, int64_t k0) { // (k0: the step's first K-value)
       constexpr bool FAST = Cfg::DIRECT, CAREFUL = Cfg::CAREFUL;
       if (l < LA::U)
-        LA::template fetch<FAST, CAREFUL>(ra[set], l, pa, args.lda, offa[l], w.rows_a, Cfg::A_KC ? w.safe_a : w.safe_a - k0, tid);
+        LA::template fetch<FAST, CAREFUL>(ra[set], l, pa, args.lda, offa[l], w.rows_a, Cfg::A_KC ? w.safe_a : w.safe_a - k0, tid, apart);
       else
         LB::template fetch<FAST, CAREFUL>(rb[set], l - LA::U, pb, args.ldb, offb[l - LA::U], w.rows_b, Cfg::B_KC ? w.safe_b : w.safe_b - k0, tid);
     };
@@ -729,7 +898,7 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
         const char *pa = a_at(0), *pb = b_at(0);
 #pragma unroll
         for (int u = 0; u < LA::U; u++)
-          LA::fetch_tail(ra[0], u, pa, args.lda, w.rows_a, left, Cfg::A_KC ? w.safe_a : w.safe_a - whole * BK, tid);
+          LA::fetch_tail(ra[0], u, pa, args.lda, w.rows_a, left, Cfg::A_KC ? w.safe_a : w.safe_a - whole * BK, tid, apart);
 #pragma unroll
         for (int u = 0; u < UB; u++)
           LB::fetch_tail(rb[0], u, pb, args.ldb, w.rows_b, left, Cfg::B_KC ? w.safe_b : w.safe_b - whole * BK, tid);
@@ -785,56 +954,11 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
   }
 
   // ---- results ----
-  // Register v of lane l: MFMA row 4 (l / 16) + v (of C), column l % 16 (token).  One column block after the other passes
-  // through LDS, each wave's through a part of its own, so that a wave's store covers the columns' whole WM rows.
-  block_sync_lds(); // (every wave has read its last fragments)
-  constexpr int PITCH = Cfg::PITCH;
-  float *mine = reinterpret_cast<float *>(lds) + wave * (16 * PITCH);
-  const uint32_t row0 = w.m0 + wm * Cfg::WM;
-#pragma unroll
-  for (int j = 0; j < TN; j++) {
-#pragma unroll
-    for (int i = 0; i < TM; i++) {
-      f4v_t x;
-#pragma unroll
-      for (int v = 0; v < 4; v++) {
-        x[v] = (float)acc[0][j][i][v];
-        if constexpr (T::NACC == 2) x[v] += acc[1][j][i][v] * prec_traits<T::P>::CORR_SCALE;
-      }
-      *reinterpret_cast<f4v_t *>(mine + frow * PITCH + i * 16 + fg * 4) = x;
-    }
-    // (a wave's own writes and reads of LDS are carried out in order)
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
-    constexpr int LANES = Cfg::WM / 4, COLS = 64 / LANES; // lanes of a column, columns of a round
-    const uint32_t row = row0 + (lane % LANES) * 4, col0 = w.n0 + (j * Cfg::WAVES_N + wn) * 16;
-    f4v_t sa = {args.alpha, args.alpha, args.alpha, args.alpha};
-    if constexpr (T::I8) {
-#pragma unroll
-      for (int v = 0; v < 4; v++)
-        sa[v] = args.scale_a[(uint64_t)w.group * args.m + (row + v < args.m ? row + v : args.m - 1)];
-    }
-#pragma unroll 1
-    for (int r = 0; r < 16; r += COLS) {
-      const uint32_t col = col0 + r + lane / LANES;
-      if (col >= w.n_end) continue;
-      f4v_t x = *reinterpret_cast<const f4v_t *>(mine + (r + lane / LANES) * PITCH + (lane % LANES) * 4);
-      if constexpr (Cfg::RAGGED_K) {
-        if (args.splits > 1) {
-          *reinterpret_cast<f4v_t *>(w.partial + (uint64_t)(col - w.n0) * BM + (row - w.m0)) = x;
-          continue;
-        }
-      }
-      const float sb = T::I8 ? args.scale_b[col] : 1.0f;
-#pragma unroll
-      for (int v = 0; v < 4; v++) x[v] = T::I8 ? x[v] * sa[v] * sb : x[v] * sa[v];
-      const uint64_t at = (uint64_t)col * args.ldc + row;
-      if (T::F32 || args.out == OUT_F32) store_four<OUT_F32>(w.c + at * 4, x, args.beta, row, args.m, args.vec_c != 0);
-      else if (Cfg::E == Elem::F16 || (T::I8 && args.out == OUT_F16))
-        store_four<OUT_F16>(w.c + at * 2, x, args.beta, row, args.m, args.vec_c != 0);
-      else store_four<OUT_BF16>(w.c + at * 2, x, args.beta, row, args.m, args.vec_c != 0);
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
-  }
+  write_tile<Cfg, TN>(args, w, lds, [&](const int j, const int i, const int v) {
+    float x = (float)acc[0][j][i][v];
+    if constexpr (T::NACC == 2) x += acc[1][j][i][v] * prec_traits<T::P>::CORR_SCALE;
+    return x;
+  });
 }
 
 template <class Cfg>
@@ -843,7 +967,7 @@ void grouped_kernel(const GroupedArgs args) {
   using T = typename Cfg::T;
   constexpr int BM = Cfg::BM, BN = Cfg::BN, TN = Cfg::TN;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  const uint32_t tiles_m = (args.m + BM - 1) / BM;
+  const uint32_t tiles_m = (args.m + Cfg::ROWS_OUT - 1) / Cfg::ROWS_OUT;
   TilePlace t;
   TileWork w;
   const char *a = args.a, *b = args.b;
@@ -877,10 +1001,11 @@ void grouped_kernel(const GroupedArgs args) {
     a += (uint64_t)t.group * args.stride_a * T::BYTES;
   }
   w.group = t.group;
-  w.m0 = t.tm * BM;
-  w.rows_a = (int)(args.m - w.m0 < (uint32_t)BM ? args.m - w.m0 : BM);
+  w.m0 = t.tm * Cfg::ROWS_OUT;
+  w.rows_a = (int)(args.m - w.m0 < (uint32_t)Cfg::ROWS_OUT ? args.m - w.m0 : Cfg::ROWS_OUT);
   w.rows_b = (int)(w.n_end - w.n0 < (uint32_t)BN ? w.n_end - w.n0 : BN);
   w.a = uniform_address(a + (Cfg::A_KC ? (uint64_t)w.m0 * args.lda : (uint64_t)w.m0) * T::BYTES);
+  if constexpr (Cfg::GATED) w.up = uniform_address(w.a + (args.up - args.a));
   w.b = uniform_address(b + (Cfg::B_KC ? (uint64_t)w.n0 * args.ldb : (uint64_t)w.n0) * T::BYTES);
   // (what a chunk of 8 or 16 values can stick out by is less than a line that long)
   auto safe = [&](bool kc, uint64_t ld, uint64_t extent, int64_t rows, int64_t lines) -> int64_t {
@@ -908,6 +1033,6 @@ template <class Cfg> void launch_grouped(const GroupedArgs &args, uint32_t workg
   allow_dynamic_lds(reinterpret_cast<const void *>(&grouped_kernel<Cfg>), Cfg::LDS_BYTES, done);
   hipLaunchKernelGGL(grouped_kernel<Cfg>, dim3(workgroups), dim3(Cfg::NT), Cfg::LDS_BYTES, stream, args);
 }
-template <class Cfg> constexpr GroupedKernel grouped_entry() { return {&launch_grouped<Cfg>, Cfg::BM, Cfg::BN}; }
+template <class Cfg> constexpr GroupedKernel grouped_entry() { return {&launch_grouped<Cfg>, Cfg::ROWS_OUT, Cfg::BN}; }
 
 } // namespace cumpsgemm_amd

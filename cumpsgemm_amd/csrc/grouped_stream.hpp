@@ -16,8 +16,9 @@ namespace cumpsgemm_amd {
 
 constexpr int kStreamWaves = 8, kStreamTokens = 16;
 
-template <Elem E, bool A_KC> struct StreamCfg {
+template <Elem E, bool A_KC, Epilogue EPI = Epilogue::STORE> struct StreamCfg {
   using T = elem_traits<E>;
+  static constexpr int SIDES = EPI == Epilogue::GATED ? 2 : 1; // matrices: a gated block has the same rows of two
   // 16 rows of the matrix each, for a workgroup (row-contiguous: four rows a lane).  K-contiguous with four, us, with one
   // -> four: BF16 2048 x 1024, 2 tokens to 2 of 8 groups 4.8 -> 7.0, 64 to 27 of 64 27.4 -> 22.1, where the 128 x 32 tiles take
   // 21.0 (the same 113 MB of matrices again and again: they stay in the last-level cache).
@@ -25,7 +26,8 @@ template <Elem E, bool A_KC> struct StreamCfg {
   // K-values of a wave's step: 128 bytes of a row, one or two MFMAs deep (row-contiguous: one, 32 lines)
   static constexpr int SLICES = A_KC && !T::F32 ? 2 : 1;
   static constexpr int KS = SLICES * 4 * T::CHUNK;
-  static constexpr int UNROLL = A_KC ? 4 : 2; // steps under way
+  // (two matrices of FP32 lines: no registers are left for a second step)
+  static constexpr int UNROLL = A_KC ? 4 : SIDES > 1 && T::F32 ? 1 : 2; // steps under way
 };
 
 // eight or sixteen K-values of a 16-byte chunk (FP32: 32 bytes), as they lie in memory
@@ -104,11 +106,11 @@ template <Elem E> __device__ inline stream_line<E> stream_load_line_part(const c
   return r;
 }
 
-template <Elem E, bool A_KC>
+template <Elem E, bool A_KC, Epilogue EPI = Epilogue::STORE>
 __global__ __launch_bounds__(kStreamWaves * 64) void grouped_stream_kernel(const GroupedArgs args) {
   using T = elem_traits<E>;
-  using C = StreamCfg<E, A_KC>;
-  constexpr int BLOCKS = C::BLOCKS;
+  using C = StreamCfg<E, A_KC, EPI>;
+  constexpr int SIDES = C::SIDES, BLOCKS = C::BLOCKS * SIDES; // block i: rows of matrix i / C::BLOCKS
   __shared__ __attribute__((aligned(16))) float sums[kStreamWaves][kStreamTokens][C::ROWS + 4];
   const int tid = threadIdx.x, lane = tid & 63, frow = lane & 15, fg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -123,11 +125,12 @@ __global__ __launch_bounds__(kStreamWaves * 64) void grouped_stream_kernel(const
   // a token beyond the last reads the last again; its results are not stored
   const uint64_t b_row = (uint64_t)(n0 + ((uint32_t)frow < tokens ? frow : tokens - 1)) * args.ldb;
 
-  typename T::acc_t acc[T::NACC][C::BLOCKS];
+  const uint64_t apart = SIDES > 1 ? (uint64_t)(args.up - args.a) : 0;
+  typename T::acc_t acc[T::NACC][BLOCKS];
 #pragma unroll
   for (int s = 0; s < T::NACC; s++)
 #pragma unroll
-    for (int i = 0; i < C::BLOCKS; i++)
+    for (int i = 0; i < BLOCKS; i++)
 #pragma unroll
       for (int v = 0; v < 4; v++) acc[s][i][v] = 0;
   auto multiply = [&](const u4_t (&fa)[T::NP], const u4_t (&fb)[T::NP], const int i) {
@@ -145,8 +148,8 @@ __global__ __launch_bounds__(kStreamWaves * 64) void grouped_stream_kernel(const
     const char *pa[BLOCKS];
 #pragma unroll
     for (int i = 0; i < BLOCKS; i++) {
-      const uint32_t row = m0 + i * 16 + frow < args.m ? m0 + i * 16 + frow : args.m - 1;
-      pa[i] = a + ((uint64_t)row * args.lda + fg * T::CHUNK) * T::BYTES;
+      const uint32_t at = m0 + i % C::BLOCKS * 16 + frow, row = at < args.m ? at : args.m - 1;
+      pa[i] = a + i / C::BLOCKS * apart + ((uint64_t)row * args.lda + fg * T::CHUNK) * T::BYTES;
     }
     const char *pb = b + (b_row + fg * T::CHUNK) * T::BYTES;
     struct Step {
@@ -208,11 +211,13 @@ __global__ __launch_bounds__(kStreamWaves * 64) void grouped_stream_kernel(const
     const char *pb = b + (b_row + fg * 8) * T::BYTES;
     const uint64_t line = args.lda * T::BYTES;
     const bool inside = m0 + C::ROWS <= args.m; // (uniform)
-    auto take = [&](const stream_line<E> (&ra)[8], const stream_raw<E> &rb) {
+    auto take = [&](const stream_line<E> (&lines)[SIDES][8], const stream_raw<E> &rb) {
       u4_t fb[T::NP];
       stream_terms<E>(rb, fb);
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
+      for (int block = 0; block < BLOCKS; block++) {
+        const int i = block % 4;
+        const stream_line<E>(&ra)[8] = lines[block / 4];
         stream_raw<E> x;
         if constexpr (T::F32) {
 #pragma unroll
@@ -226,24 +231,27 @@ __global__ __launch_bounds__(kStreamWaves * 64) void grouped_stream_kernel(const
         }
         u4_t fa[T::NP];
         stream_terms<E>(x, fa);
-        multiply(fa, fb, i);
+        multiply(fa, fb, block);
       }
     };
-    auto load = [&](int s, stream_line<E> (&ra)[8], stream_raw<E> &rb) {
-      const char *p = pa + (uint64_t)s * C::KS * line;
-      if (inside) {
+    auto load = [&](int s, stream_line<E> (&ra)[SIDES][8], stream_raw<E> &rb) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) ra[j] = stream_load_line<E>(p + (uint64_t)j * line);
-      } else {
+      for (int side = 0; side < SIDES; side++) {
+        const char *p = pa + side * apart + (uint64_t)s * C::KS * line;
+        if (inside) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) ra[j] = stream_load_line_part<E>(p + (uint64_t)j * line, rows);
+          for (int j = 0; j < 8; j++) ra[side][j] = stream_load_line<E>(p + (uint64_t)j * line);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; j++) ra[side][j] = stream_load_line_part<E>(p + (uint64_t)j * line, rows);
+        }
       }
       rb = stream_load<E>(pb + (uint64_t)s * C::KS * T::BYTES);
     };
     constexpr int U = C::UNROLL;
     int s = wave;
     for (; s + (U - 1) * kStreamWaves < whole; s += U * kStreamWaves) {
-      stream_line<E> ra[U][8];
+      stream_line<E> ra[U][SIDES][8];
       stream_raw<E> rb[U];
 #pragma unroll
       for (int u = 0; u < U; u++) load(s + u * kStreamWaves, ra[u], rb[u]);
@@ -251,69 +259,113 @@ __global__ __launch_bounds__(kStreamWaves * 64) void grouped_stream_kernel(const
       for (int u = 0; u < U; u++) take(ra[u], rb[u]);
     }
     for (; s < whole; s += kStreamWaves) {
-      stream_line<E> ra[8];
+      stream_line<E> ra[SIDES][8];
       stream_raw<E> rb;
       load(s, ra, rb);
       take(ra, rb);
     }
     if (left != 0 && s == whole) {
-      stream_line<E> ra[8];
-      const char *p = pa + (uint64_t)whole * C::KS * line;
+      stream_line<E> ra[SIDES][8];
       const int have = left - fg * 8;
 #pragma unroll
-      for (int j = 0; j < 8; j++) ra[j] = stream_load_line_part<E>(p + (uint64_t)j * line, j < have ? rows : 0);
+      for (int side = 0; side < SIDES; side++) {
+        const char *p = pa + side * apart + (uint64_t)whole * C::KS * line;
+#pragma unroll
+        for (int j = 0; j < 8; j++) ra[side][j] = stream_load_line_part<E>(p + (uint64_t)j * line, j < have ? rows : 0);
+      }
       take(ra, stream_load_part<E>(pb + (uint64_t)whole * C::KS * T::BYTES, have));
     }
   }
 
   // ---- sums of the waves, in their order ----
   // Register v of lane l: MFMA row 4 (l / 16) + v, token l % 16.  Row-contiguous: row r of block i is row 4 r + i.
+  constexpr int PER = (C::ROWS * kStreamTokens + kStreamWaves * 64 - 1) / (kStreamWaves * 64); // results of a thread
+  float x[SIDES][PER];
 #pragma unroll
-  for (int i = 0; i < C::BLOCKS; i++)
+  for (int side = 0; side < SIDES; side++) {
+    if (side > 0) __syncthreads(); // (the sums of the side before have been read)
 #pragma unroll
-    for (int v = 0; v < 4; v++) {
-      const int r = 4 * fg + v;
-      float x;
-      if constexpr (T::I8) {
-        x = __int_as_float(acc[0][i][v]);
-      } else {
-        x = acc[0][i][v];
-        if constexpr (T::NACC == 2) x += acc[1][i][v] * prec_traits<T::P>::CORR_SCALE;
+    for (int i = 0; i < C::BLOCKS; i++)
+#pragma unroll
+      for (int v = 0; v < 4; v++) {
+        const int r = 4 * fg + v, block = side * C::BLOCKS + i;
+        float y;
+        if constexpr (T::I8) {
+          y = __int_as_float(acc[0][block][v]);
+        } else {
+          y = acc[0][block][v];
+          if constexpr (T::NACC == 2) y += acc[1][block][v] * prec_traits<T::P>::CORR_SCALE;
+        }
+        sums[wave][frow][A_KC ? i * 16 + r : 4 * r + i] = y;
       }
-      sums[wave][frow][A_KC ? i * 16 + r : 4 * r + i] = x;
+    __syncthreads();
+#pragma unroll
+    for (int at = 0; at < PER; at++) {
+      const int e = tid + at * kStreamWaves * 64, r = e % C::ROWS, j = e / C::ROWS;
+      if (j >= kStreamTokens) continue;
+      if constexpr (T::I8) {
+        int sum = 0;
+#pragma unroll
+        for (int w = 0; w < kStreamWaves; w++) sum += __float_as_int(sums[w][j][r]);
+        x[side][at] = (float)sum;
+      } else {
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kStreamWaves; w++) sum += sums[w][j][r];
+        x[side][at] = sum;
+      }
     }
-  __syncthreads();
-  for (int e = tid; e < C::ROWS * kStreamTokens; e += kStreamWaves * 64) {
+  }
+  auto typed = [&](auto f) {
+    if (T::F32 || args.out == OUT_F32) f((float)0);
+    else if (E == Elem::F16 || (T::BYTES == 1 && args.out == OUT_F16)) f((_Float16)0);
+    else f((__bf16)0);
+  };
+#pragma unroll
+  for (int at = 0; at < PER; at++) {
+    const int e = tid + at * kStreamWaves * 64;
     const uint32_t r = e % C::ROWS, j = e / C::ROWS, row = m0 + r, col = n0 + j;
     if (j >= tokens || row >= args.m) continue;
-    float x;
-    if constexpr (T::I8) {
-      int sum = 0;
-#pragma unroll
-      for (int w = 0; w < kStreamWaves; w++) sum += __float_as_int(sums[w][j][r]);
-      x = (float)sum * args.scale_a[(uint64_t)t.group * args.m + row] * args.scale_b[col];
+    const uint64_t c_at = (uint64_t)col * args.ldc + row, z_at = (uint64_t)col * args.ldz + row;
+    float y = x[0][at];
+    if constexpr (EPI == Epilogue::GATED) {
+      const float up = x[SIDES - 1][at];
+      float slope;
+      typed([&](auto o) {
+        typedef decltype(o) O;
+        reinterpret_cast<O *>(args.c)[c_at] = (O)(activation<T::F32, false>(args.act, y, slope) * up);
+        if (args.z[0] == nullptr) return;
+        reinterpret_cast<O *>(args.z[0])[z_at] = (O)y;
+        reinterpret_cast<O *>(args.z[1])[z_at] = (O)up;
+      });
+    } else if constexpr (EPI == Epilogue::GATED_BACKWARD) {
+      typed([&](auto o) {
+        typedef decltype(o) O;
+        const float gate = (float)reinterpret_cast<const O *>(args.z[0])[z_at], up = (float)reinterpret_cast<const O *>(args.z[1])[z_at];
+        const uint64_t d_at = (uint64_t)col * args.ldd + row;
+        float slope;
+        const float a = activation<T::F32, true>(args.act, gate, slope);
+        reinterpret_cast<O *>(args.d[0])[d_at] = (O)(y * up * slope);
+        reinterpret_cast<O *>(args.d[1])[d_at] = (O)(y * a);
+        if (args.c != nullptr) reinterpret_cast<O *>(args.c)[c_at] = (O)(a * up);
+      });
     } else {
-      x = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kStreamWaves; w++) x += sums[w][j][r];
-      x *= args.alpha;
+      if constexpr (T::I8) y = y * args.scale_a[(uint64_t)t.group * args.m + row] * args.scale_b[col];
+      else y *= args.alpha;
+      typed([&](auto o) {
+        typedef decltype(o) O;
+        O *c = reinterpret_cast<O *>(args.c);
+        c[c_at] = (O)(args.beta != 0.0f ? y + args.beta * (float)c[c_at] : y);
+      });
     }
-    const uint64_t at = (uint64_t)col * args.ldc + row;
-    auto put = [&](auto *c) {
-      typedef typename std::remove_pointer<decltype(c)>::type O;
-      c[at] = (O)(args.beta != 0.0f ? x + args.beta * (float)c[at] : x);
-    };
-    if (T::F32 || args.out == OUT_F32) put(reinterpret_cast<float *>(args.c));
-    else if (E == Elem::F16 || (T::I8 && args.out == OUT_F16)) put(reinterpret_cast<_Float16 *>(args.c));
-    else put(reinterpret_cast<__bf16 *>(args.c));
   }
 }
 
-template <Elem E, bool A_KC> void launch_grouped_stream(const GroupedArgs &args, uint32_t workgroups, hipStream_t stream) {
-  hipLaunchKernelGGL((grouped_stream_kernel<E, A_KC>), dim3(workgroups), dim3(kStreamWaves * 64), 0, stream, args);
+template <Elem E, bool A_KC, Epilogue EPI> void launch_grouped_stream(const GroupedArgs &args, uint32_t workgroups, hipStream_t stream) {
+  hipLaunchKernelGGL((grouped_stream_kernel<E, A_KC, EPI>), dim3(workgroups), dim3(kStreamWaves * 64), 0, stream, args);
 }
-template <Elem E, bool A_KC> constexpr GroupedKernel stream_entry() {
-  return {&launch_grouped_stream<E, A_KC>, StreamCfg<E, A_KC>::ROWS, kStreamTokens};
+template <Elem E, bool A_KC, Epilogue EPI = Epilogue::STORE> constexpr GroupedKernel stream_entry() {
+  return {&launch_grouped_stream<E, A_KC, EPI>, StreamCfg<E, A_KC>::ROWS, kStreamTokens};
 }
 
 } // namespace cumpsgemm_amd

@@ -13,9 +13,9 @@ struct GroupedTable {
 };
 
 template <Elem E, bool A_KC, bool B_KC, int BM, int BN, int WM, int WN, int ROW_BYTES, int NSTAGE, bool DIRECT, bool RAGGED_K,
-          bool CAREFUL = false>
+          bool CAREFUL = false, Epilogue EPI = Epilogue::STORE>
 constexpr GroupedKernel grouped_of() {
-  return grouped_entry<GroupedCfg<E, A_KC, B_KC, BM, BN, WM, WN, ROW_BYTES, NSTAGE, DIRECT, RAGGED_K, 2, CAREFUL>>();
+  return grouped_entry<GroupedCfg<E, A_KC, B_KC, BM, BN, WM, WN, ROW_BYTES, NSTAGE, DIRECT, RAGGED_K, 2, CAREFUL, EPI>>();
 }
 
 template <Elem E> constexpr GroupedTable grouped_table_f32() {
@@ -65,8 +65,33 @@ template <Elem E> constexpr GroupedTable grouped_table_i8() {
   return t;
 }
 
+// Gated blocks and their gradients: the same tiles.
+template <Elem E, Epilogue EPI, bool A_KC> constexpr void gated_entries(GroupedTable &t) {
+  if constexpr (elem_traits<E>::F32) {
+    t.columns[A_KC][0][TILE_128] = grouped_of<E, A_KC, true, 128, 128, 64, 32, 64, 2, false, false, false, EPI>();
+    t.columns[A_KC][1][TILE_256] = grouped_of<E, A_KC, true, 256, 128, 64, 64, 64, 2, true, false, false, EPI>();
+    t.columns[A_KC][1][TILE_128] = grouped_of<E, A_KC, true, 128, 128, 64, 32, 64, 2, true, false, false, EPI>();
+    t.columns[A_KC][1][TILE_NARROW] = grouped_of<E, A_KC, true, 128, 32, 32, 32, 64, 2, true, false, false, EPI>();
+  } else {
+    t.columns[A_KC][0][TILE_128] = grouped_of<E, A_KC, true, 128, 128, 64, 64, 128, 2, false, false, false, EPI>();
+    t.columns[A_KC][1][TILE_256] = grouped_of<E, A_KC, true, 256, 256, 128, 64, 128, 2, true, false, false, EPI>();
+    t.columns[A_KC][1][TILE_128] = grouped_of<E, A_KC, true, 128, 128, 64, 64, 128, 2, true, false, false, EPI>();
+    t.columns[A_KC][1][TILE_NARROW] = grouped_of<E, A_KC, true, 128, 32, 32, 32, 128, 4, true, false, false, EPI>();
+  }
+  t.stream[A_KC] = stream_entry<E, A_KC, EPI>();
+}
+template <Elem E, Epilogue EPI> constexpr GroupedTable gated_table() {
+  GroupedTable t{};
+  gated_entries<E, EPI, false>(t);
+  gated_entries<E, EPI, true>(t);
+  return t;
+}
+
 #define CUMPSGEMM_GROUPED_F32(sym, E) GroupedTable sym = grouped_table_f32<E>();
 #define CUMPSGEMM_GROUPED_16(sym, E) GroupedTable sym = grouped_table_16<E>();
 #define CUMPSGEMM_GROUPED_I8(sym, E) GroupedTable sym = grouped_table_i8<E>();
+#define CUMPSGEMM_GATED(kind, E)                                               \
+  GroupedTable g_gated_##kind = gated_table<E, Epilogue::GATED>();             \
+  GroupedTable g_gated_backward_##kind = gated_table<E, Epilogue::GATED_BACKWARD>();
 
 } // namespace cumpsgemm_amd

@@ -216,6 +216,49 @@ hipblasStatus_t cuMpSGEMM_quantize_i8(cuMpSGEMM_handle_t handle, uint64_t k, uin
                                       uint64_t ldx, hipDataType type_x, int8_t *q, uint64_t ldq,
                                       float *scale);
 
+/* ---- gated feed-forward blocks (no counterpart in the reference) -----------
+ * Both projections, the activation and the product in one kernel:
+ *   C[:, j] = act(G[:, j]) * U[:, j],   G = op(gate_g) B,  U = op(up_g) B
+ * for token j of group g, element by element; gate_g and up_g are m x k after
+ * op, at gate / up + g * stridea (elements), with the same lda (rows of one
+ * matrix may be interleaved with the other's, or follow them); B is k x n, C is
+ * m x n.  z_gate and z_up, both or neither NULL, get G and U (m x n, ldz), which
+ * the gradient needs.  All tensors are of one type: HIP_R_32F (compute_mode as
+ * in cuMpSGEMM_gemm_grouped), HIP_R_16F or HIP_R_16BF; G, U and C are each
+ * rounded once, from FP32 sums.  offsets and group_count as above, and offsets =
+ * NULL with group_count = 1: one block for all n tokens.  Columns of no group are
+ * not written.  C, z_gate and z_up must not overlap each other or the operands. */
+typedef enum {
+  CUMPSGEMM_SILU = 0,      /* x / (1 + e^-x) */
+  CUMPSGEMM_GELU = 1,      /* x times the distribution function of a normal variable */
+  CUMPSGEMM_GELU_TANH = 2, /* x (1 + tanh(sqrt(2 / pi) (x + 0.044715 x^3))) / 2 */
+  CUMPSGEMM_RELU = 3       /* max(x, 0) */
+} cuMpSGEMM_activation_t;
+hipblasStatus_t cuMpSGEMM_gemm_gated(cuMpSGEMM_handle_t handle, hipblasOperation_t op_A,
+                                     cuMpSGEMM_activation_t activation, uint64_t m, uint64_t n,
+                                     uint64_t k, const void *gate, const void *up, uint64_t lda,
+                                     uint64_t stridea, const void *b, uint64_t ldb, void *c,
+                                     uint64_t ldc, void *z_gate, void *z_up, uint64_t ldz,
+                                     const int *offsets, uint64_t group_count,
+                                     cuMpSGEMM_compute_mode_t compute_mode, hipDataType type);
+/* Its gradient, on top of the product that brings the gradient to it:
+ *   D[:, j] = op(A_g) B[:, j]             (the layer behind: A its matrix, B the gradients of its results)
+ *   d_gate = D * U * act'(G),  d_up = D * act(G),  C = act(G) * U
+ * G = z_gate and U = z_up as cuMpSGEMM_gemm_gated left them.  D is kept in FP32
+ * and not stored.  C, the block's result again, is what the gradient of A needs;
+ * NULL: not wanted.  d_gate and d_up (m x n, ldd) may be z_gate and z_up
+ * themselves, with ldd = ldz; apart from that nothing may overlap.  (At 0 the
+ * derivative of RELU is 0.) */
+hipblasStatus_t cuMpSGEMM_gemm_gated_backward(cuMpSGEMM_handle_t handle, hipblasOperation_t op_A,
+                                              cuMpSGEMM_activation_t activation, uint64_t m, uint64_t n,
+                                              uint64_t k, const void *a, uint64_t lda, uint64_t stridea,
+                                              const void *b, uint64_t ldb, const void *z_gate,
+                                              const void *z_up, uint64_t ldz, void *d_gate, void *d_up,
+                                              uint64_t ldd, void *c, uint64_t ldc, const int *offsets,
+                                              uint64_t group_count,
+                                              cuMpSGEMM_compute_mode_t compute_mode, hipDataType type);
+
+
 /* cumpsgemm::exp_stats_ext<T> / exp_max_ext<T> (reference cumpsgemm.hpp:37-46) */
 unsigned cuMpSGEMM_exp_stats_ext_s(cuMpSGEMM_handle_t h, unsigned m, unsigned n, const float *ptr,
                                    unsigned ld, unsigned batch, unsigned stride);
