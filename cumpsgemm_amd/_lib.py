@@ -55,7 +55,8 @@ _CALL_FUNCTIONS = ("cuMpSGEMM_sgemm", "cuMpSGEMM_cgemm", "cuMpSGEMM_sgemm_stride
                    "cuMpSGEMM_sgemm_pipeline", "cuMpSGEMM_cgemm_pipeline", "cuMpSGEMM_sgemm_Mx2x2",
                    "cuMpSGEMM_cgemm_Mx2x2", "cuMpSGEMM_sgemm_2xNx2", "cuMpSGEMM_cgemm_2xNx2")
 _GROUPED_FUNCTIONS = ("cuMpSGEMM_gemm_grouped", "cuMpSGEMM_gemm_grouped_k", "cuMpSGEMM_gemm_i8", "cuMpSGEMM_quantize_i8")
-_GATED_FUNCTIONS = ("cuMpSGEMM_gemm_gated", "cuMpSGEMM_gemm_gated_backward")
+_GATED_FUNCTIONS = ("cuMpSGEMM_gemm_gated", "cuMpSGEMM_gemm_gated_backward", "cuMpSGEMM_gemm_f8", "cuMpSGEMM_gemm_gated_f8",
+                    "cuMpSGEMM_quantize_f8")
 
 
 def lib():
@@ -131,6 +132,10 @@ def _declare(L):
         _ptr, _ptr, _u64, _u64, _ptr, _u64, _ptr, _u64, _ptr, _ptr, _u64, _ptr, _u64, _int, _int]
     L.cuMpSGEMM_gemm_gated_backward.argtypes = [_ptr, _int, _int] + gemm_tail + [
         _ptr, _u64, _u64, _ptr, _u64, _ptr, _ptr, _u64, _ptr, _ptr, _u64, _ptr, _u64, _ptr, _u64, _int, _int]
+    f8_tail = [_ptr, _u64, _int, _ptr, _ptr, _u64, _int, _ptr, _u64]
+    L.cuMpSGEMM_gemm_f8.argtypes = [_ptr, _int] + gemm_tail + [_ptr, _u64, _u64, _int, _ptr, _u64] + f8_tail
+    L.cuMpSGEMM_gemm_gated_f8.argtypes = [_ptr, _int] + gemm_tail + [_ptr, _ptr, _u64, _u64, _int, _ptr, _ptr, _u64] + f8_tail
+    L.cuMpSGEMM_quantize_f8.argtypes = [_ptr, _u64, _u64, _ptr, _u64, _u64, _int, _u64, _ptr, _u64, _u64, _int, _ptr, _u64]
     L.cuMpSGEMM_get_workspace_size.argtypes = [_ptr]
     L.cuMpSGEMM_get_workspace_size.restype = ctypes.c_size_t
     L.cuMpSGEMM_get_workspace_pointer.argtypes = [_ptr]
@@ -397,6 +402,40 @@ class Handle:
         return self._L.cuMpSGEMM_gemm_gated_backward(self._h, op_a, int(activation), m, n, k, _dptr(a), lda, stridea, _dptr(b),
                                                      ldb, _dptr(z_gate), _dptr(z_up), ldz, _dptr(d_gate), _dptr(d_up), ldd,
                                                      _dptr(c), ldc, _dptr(offsets), groups, int(mode), int(type))
+
+    # ---- 8-bit floating point ----
+    def gemm_f8(self, op_a, m, n, k, a, lda, stridea, type_a, scale_a, stridescale, b, ldb, type_b, scale_b, c, ldc,
+                type_c=R_32F, offsets=None, groups=1):
+        """FP8 with a scale for 128 x 128 of a and for 128 values of each token (column of b); grouped with offsets."""
+        if _native is not None:
+            st = _native.gemm_f8(self._addr, op_a, m, n, k, a, lda, stridea, type_a, scale_a, stridescale, b, ldb, type_b,
+                                 scale_b, c, ldc, type_c, offsets, groups)
+            if st is not None:
+                return st
+        return self._L.cuMpSGEMM_gemm_f8(self._h, op_a, m, n, k, _dptr(a), lda, stridea, int(type_a), _dptr(scale_a), stridescale,
+                                         _dptr(b), ldb, int(type_b), _dptr(scale_b), _dptr(c), ldc, int(type_c),
+                                         _dptr(offsets), groups)
+
+    def gemm_gated_f8(self, activation, m, n, k, gate, up, lda, stridea, type_a, scale_gate, scale_up, stridescale, b, ldb,
+                      type_b, scale_b, c, ldc, type_c=R_32F, offsets=None, groups=1):
+        """gemm_gated of such values."""
+        if _native is not None:
+            st = _native.gemm_gated_f8(self._addr, activation, m, n, k, gate, up, lda, stridea, type_a, scale_gate, scale_up,
+                                       stridescale, b, ldb, type_b, scale_b, c, ldc, type_c, offsets, groups)
+            if st is not None:
+                return st
+        return self._L.cuMpSGEMM_gemm_gated_f8(self._h, int(activation), m, n, k, _dptr(gate), _dptr(up), lda, stridea, int(type_a),
+                                               _dptr(scale_gate), _dptr(scale_up), stridescale, _dptr(b), ldb, int(type_b),
+                                               _dptr(scale_b), _dptr(c), ldc, int(type_c), _dptr(offsets), groups)
+
+    def quantize_f8(self, k, n, x, ldx, stridex, type_x, block_n, q, ldq, strideq, type_q, scale, batch=1):
+        """The n columns of x (of each of `batch` matrices) as FP8 with a scale for 128 values of block_n columns, 1 or 128."""
+        if _native is not None:
+            st = _native.quantize_f8(self._addr, k, n, x, ldx, stridex, type_x, block_n, q, ldq, strideq, type_q, scale, batch)
+            if st is not None:
+                return st
+        return self._L.cuMpSGEMM_quantize_f8(self._h, k, n, _dptr(x), ldx, stridex, int(type_x), block_n, _dptr(q), ldq, strideq,
+                                             int(type_q), _dptr(scale), batch)
 
     # ---- exponent statistics ----
     def exp_stats_ext(self, m, n, ptr, ld, batch=1, stride=0, cplx=False):

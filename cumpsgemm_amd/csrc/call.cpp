@@ -35,9 +35,12 @@ struct GroupedFunctions { // products of experts' layers
   decltype(&cuMpSGEMM_quantize_i8) quantize;
 } fg;
 constexpr Py_ssize_t kGroupedFunctions = sizeof(GroupedFunctions) / sizeof(void *);
-struct GatedFunctions { // gated feed-forward blocks
+struct GatedFunctions { // gated feed-forward blocks and 8-bit floating point
   decltype(&cuMpSGEMM_gemm_gated) gated;
   decltype(&cuMpSGEMM_gemm_gated_backward) backward;
+  decltype(&cuMpSGEMM_gemm_f8) f8;
+  decltype(&cuMpSGEMM_gemm_gated_f8) gated_f8;
+  decltype(&cuMpSGEMM_quantize_f8) quantize_f8;
 } fb;
 constexpr Py_ssize_t kGatedFunctions = sizeof(GatedFunctions) / sizeof(void *);
 PyObject *data_ptr_name;
@@ -357,6 +360,75 @@ PyObject *gemm_gated_backward(PyObject *, PyObject *const *args, Py_ssize_t n_ar
                        mode, type);
   });
 }
+// handle, op_a, m, n, k, a, lda, stride_a, type_a, scale_a, stride_scale, b, ldb, type_b, scale_b, c, ldc, type_c, offsets, groups
+PyObject *gemm_f8(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+  if (!count_is(n_args, 20)) return nullptr;
+  Args x{args};
+  auto *const h = x.ptr<cuMpSGEMM_handle>();
+  const auto op_a = x.op();
+  const uint64_t m = x.u64(), n = x.u64(), k = x.u64();
+  void *const a = x.ptr<void>();
+  const uint64_t lda = x.u64(), stride_a = x.u64();
+  const auto type_a = (hipDataType)(int)x.u64();
+  const float *const scale_a = x.ptr<float>();
+  const uint64_t stride_scale = x.u64();
+  void *const b = x.ptr<void>();
+  const uint64_t ldb = x.u64();
+  const auto type_b = (hipDataType)(int)x.u64();
+  const float *const scale_b = x.ptr<float>();
+  void *const c = x.ptr<void>();
+  const uint64_t ldc = x.u64();
+  const auto type_c = (hipDataType)(int)x.u64();
+  const int *const offsets = x.ptr<int>();
+  const uint64_t groups = x.u64();
+  return status(x, [&] {
+    return fb.f8(h, op_a, m, n, k, a, lda, stride_a, type_a, scale_a, stride_scale, b, ldb, type_b, scale_b, c, ldc, type_c, offsets, groups);
+  });
+}
+// handle, activation, m, n, k, gate, up, lda, stride_a, type_a, scale_gate, scale_up, stride_scale, b, ldb, type_b, scale_b, c, ldc,
+// type_c, offsets, groups
+PyObject *gemm_gated_f8(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+  if (!count_is(n_args, 22)) return nullptr;
+  Args x{args};
+  auto *const h = x.ptr<cuMpSGEMM_handle>();
+  const auto act = (cuMpSGEMM_activation_t)(int)x.u64();
+  const uint64_t m = x.u64(), n = x.u64(), k = x.u64();
+  void *const gate = x.ptr<void>(), *const up = x.ptr<void>();
+  const uint64_t lda = x.u64(), stride_a = x.u64();
+  const auto type_a = (hipDataType)(int)x.u64();
+  const float *const scale_gate = x.ptr<float>(), *const scale_up = x.ptr<float>();
+  const uint64_t stride_scale = x.u64();
+  void *const b = x.ptr<void>();
+  const uint64_t ldb = x.u64();
+  const auto type_b = (hipDataType)(int)x.u64();
+  const float *const scale_b = x.ptr<float>();
+  void *const c = x.ptr<void>();
+  const uint64_t ldc = x.u64();
+  const auto type_c = (hipDataType)(int)x.u64();
+  const int *const offsets = x.ptr<int>();
+  const uint64_t groups = x.u64();
+  return status(x, [&] {
+    return fb.gated_f8(h, act, m, n, k, gate, up, lda, stride_a, type_a, scale_gate, scale_up, stride_scale, b, ldb, type_b, scale_b, c, ldc,
+                       type_c, offsets, groups);
+  });
+}
+// handle, k, n, x, ldx, stride_x, type_x, block_n, q, ldq, stride_q, type_q, scale, batch
+PyObject *quantize_f8(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+  if (!count_is(n_args, 14)) return nullptr;
+  Args x{args};
+  auto *const h = x.ptr<cuMpSGEMM_handle>();
+  const uint64_t k = x.u64(), n = x.u64();
+  void *const values = x.ptr<void>();
+  const uint64_t ldx = x.u64(), stride_x = x.u64();
+  const auto type_x = (hipDataType)(int)x.u64();
+  const uint64_t block_n = x.u64();
+  void *const q = x.ptr<void>();
+  const uint64_t ldq = x.u64(), stride_q = x.u64();
+  const auto type_q = (hipDataType)(int)x.u64();
+  float *const scale = x.ptr<float>();
+  const uint64_t batch = x.u64();
+  return status(x, [&] { return fb.quantize_f8(h, k, n, values, ldx, stride_x, type_x, block_n, q, ldq, stride_q, type_q, scale, batch); });
+}
 // the addresses of the functions, in the order of `Functions` (`GroupedFunctions`, `GatedFunctions`)
 PyObject *bind_to(void *to, PyObject *const *args, Py_ssize_t n, const Py_ssize_t want) {
   if (!count_is(n, want)) return nullptr;
@@ -390,6 +462,9 @@ PyMethodDef methods[] = {{"bind", (PyCFunction)(void (*)(void))bind, METH_FASTCA
                          {"bind_gated", (PyCFunction)(void (*)(void))bind_gated, METH_FASTCALL, nullptr},
                          {"gemm_gated", (PyCFunction)(void (*)(void))gemm_gated, METH_FASTCALL, nullptr},
                          {"gemm_gated_backward", (PyCFunction)(void (*)(void))gemm_gated_backward, METH_FASTCALL, nullptr},
+                         {"gemm_f8", (PyCFunction)(void (*)(void))gemm_f8, METH_FASTCALL, nullptr},
+                         {"gemm_gated_f8", (PyCFunction)(void (*)(void))gemm_gated_f8, METH_FASTCALL, nullptr},
+                         {"quantize_f8", (PyCFunction)(void (*)(void))quantize_f8, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_call", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 } // namespace

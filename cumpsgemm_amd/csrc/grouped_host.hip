@@ -11,13 +11,15 @@ extern GroupedTable g_grouped_f32_fp16tcec, g_grouped_f32_fp16tc, g_grouped_f32_
 extern GroupedTable g_gated_f32_fp16tcec, g_gated_f32_fp16tc, g_gated_f32_bf16x3, g_gated_f32_bf16x2, g_gated_f16, g_gated_bf16;
 extern GroupedTable g_gated_backward_f32_fp16tcec, g_gated_backward_f32_fp16tc, g_gated_backward_f32_bf16x3,
     g_gated_backward_f32_bf16x2, g_gated_backward_f16, g_gated_backward_bf16;
+extern GroupedTable g_f8_e4m3, g_f8_e5m2, g_gated_f8_e4m3, g_gated_f8_e5m2;
 
 // direct: the operands can take the shorter way into LDS (grouped_kernel.hpp); the kernel of few tokens takes any
 const GroupedKernel *lookup_grouped(Elem e, bool a_kc, bool ragged_k, bool direct, int cls, Epilogue epi = Epilogue::STORE) {
   static const GroupedTable *const tables[3][kNumElems] = {
       {&g_grouped_f32_fp16tcec, &g_grouped_f32_fp16tc, &g_grouped_f32_bf16x3, &g_grouped_f32_bf16x2, &g_grouped_f16,
-       &g_grouped_bf16, &g_grouped_i8},
-      {&g_gated_f32_fp16tcec, &g_gated_f32_fp16tc, &g_gated_f32_bf16x3, &g_gated_f32_bf16x2, &g_gated_f16, &g_gated_bf16},
+       &g_grouped_bf16, &g_grouped_i8, &g_f8_e4m3, &g_f8_e5m2},
+      {&g_gated_f32_fp16tcec, &g_gated_f32_fp16tc, &g_gated_f32_bf16x3, &g_gated_f32_bf16x2, &g_gated_f16, &g_gated_bf16,
+       nullptr, &g_gated_f8_e4m3, &g_gated_f8_e5m2},
       {&g_gated_backward_f32_fp16tcec, &g_gated_backward_f32_fp16tc, &g_gated_backward_f32_bf16x3, &g_gated_backward_f32_bf16x2,
        &g_gated_backward_f16, &g_gated_backward_bf16}};
   if (tables[(int)epi][(int)e] == nullptr) return nullptr;
@@ -79,7 +81,7 @@ bool out_of(hipDataType type, uint32_t &out) {
   else return false;
   return true;
 }
-uint32_t bytes_of(Elem e) { return (int)e <= 3 ? 4 : e == Elem::I8 ? 1 : 2; }
+uint32_t bytes_of(Elem e) { return (int)e <= 3 ? 4 : (int)e >= (int)Elem::I8 ? 1 : 2; }
 
 // Whether an operand can go straight from memory to LDS: its contiguous extent is whole 16-byte chunks, they are
 // aligned, and the offsets of a tile and step fit 32 bits (`lines`: rows or K-lines that a step spans).
@@ -127,7 +129,7 @@ const Cost &cost_of(Elem e, int cls) {
                                {6.1f, 0.45f, 0.49f, 3, 32, 1.00f}, {4.0f, 0.90f, 0.99f, 2, 256, 0.42f}};
   static const Cost fp32x3[4] = {{11.1f, 1.93f, 2.64f, 1, 32, 0.42f}, {7.2f, 1.06f, 1.40f, 1, 32, 0.57f},
                                  {5.8f, 0.78f, 0.61f, 2, 32, 0.88f}, {4.1f, 0.89f, 0.98f, 2, 256, 0.43f}};
-  return (e == Elem::I8 ? eight : e == Elem::F32_BF16X3 ? fp32x3 : (int)e <= 3 ? fp32 : sixteen)[cls];
+  return ((int)e >= (int)Elem::I8 ? eight : e == Elem::F32_BF16X3 ? fp32x3 : (int)e <= 3 ? fp32 : sixteen)[cls];
 }
 double cost_us(const Cost &c, double workgroups, double steps, double cus, double filled = 1.0) {
   return c.fixed + steps * (c.least + (1.0 - c.least) * filled) * std::max<double>(c.alone, c.each * (workgroups / cus + (workgroups > cus * c.slots ? 0.2 * c.slots : 0.0)));
@@ -202,6 +204,41 @@ hipblasStatus_t run_columns(cuMpSGEMM_handle *h, Elem e, bool a_kc, GroupedArgs 
   ProfileScope prof(h, label);
   k->launch(args, (uint32_t)workgroups, h->stream);
   return launched();
+}
+
+// What products of 8-bit floating point and gated blocks of it are given alike.  nothing: there is nothing to compute.
+hipblasStatus_t f8_arguments(cuMpSGEMM_handle *h, uint64_t m, uint64_t n, uint64_t k, bool a_kc, const void *a, uint64_t lda,
+                             uint64_t stridea, hipDataType type_a, const float *scale_a, uint64_t stridescale, const void *b,
+                             uint64_t ldb, hipDataType type_b, const float *scale_b, void *c, uint64_t ldc, hipDataType type_c,
+                             const int *offsets, uint64_t group_count, Elem &e, bool &nothing, GroupedArgs &args) {
+  nothing = false;
+  if (h == nullptr || m > kMost || n > kMost || k > kMost || group_count > kMost) return HIPBLAS_STATUS_INVALID_VALUE;
+  if (type_a != HIP_R_8F_E4M3 || (type_b != HIP_R_8F_E4M3 && type_b != HIP_R_8F_E5M2)) return HIPBLAS_STATUS_INVALID_VALUE;
+  if (!out_of(type_c, args.out) || (offsets == nullptr && group_count > 1)) return HIPBLAS_STATUS_INVALID_VALUE;
+  nothing = m == 0 || n == 0 || group_count == 0;
+  if (nothing) return HIPBLAS_STATUS_SUCCESS;
+  if (ldc < m || c == nullptr) return HIPBLAS_STATUS_INVALID_VALUE;
+  if (k != 0 && (lda < (a_kc ? k : m) || ldb < k || a == nullptr || b == nullptr || scale_a == nullptr || scale_b == nullptr))
+    return HIPBLAS_STATUS_INVALID_VALUE;
+  e = type_b == HIP_R_8F_E4M3 ? Elem::E4M3 : Elem::E5M2;
+  args.m = (uint32_t)m;
+  args.n = (uint32_t)n;
+  args.k = (uint32_t)k;
+  args.groups = (uint32_t)group_count;
+  args.offsets = offsets;
+  args.a = (const char *)a;
+  args.b = (const char *)b;
+  args.c = (char *)c;
+  args.lda = lda;
+  args.ldb = ldb;
+  args.ldc = ldc;
+  args.stride_a = stridea;
+  args.alpha = 1.0f;
+  args.vec_c = four_at_once(c, m, ldc, 0, args.out);
+  args.scale_a = scale_a;
+  args.scale_b = scale_b;
+  args.stride_scale = stridescale;
+  return HIPBLAS_STATUS_SUCCESS;
 }
 
 // What gated blocks and their gradients are given alike.  nothing: there is nothing to compute.
@@ -395,6 +432,40 @@ hipblasStatus_t cuMpSGEMM_gemm_gated_backward(cuMpSGEMM_handle_t h, hipblasOpera
                four_at_once(d_gate, m, ldd, 0, args.out) && four_at_once(d_up, m, ldd, 0, args.out) &&
                (c == nullptr || four_at_once(c, m, ldc, 0, args.out));
   return run_columns(h, e, op_A != HIPBLAS_OP_N, args, "gemm_gated_backward", Epilogue::GATED_BACKWARD);
+}
+
+hipblasStatus_t cuMpSGEMM_gemm_f8(cuMpSGEMM_handle_t h, hipblasOperation_t op_A, uint64_t m, uint64_t n, uint64_t k, const void *a,
+                                  uint64_t lda, uint64_t stridea, hipDataType type_a, const float *scale_a, uint64_t stridescale,
+                                  const void *b, uint64_t ldb, hipDataType type_b, const float *scale_b, void *c, uint64_t ldc,
+                                  hipDataType type_c, const int *offsets, uint64_t group_count) {
+  if (op_A != HIPBLAS_OP_N && op_A != HIPBLAS_OP_T && op_A != HIPBLAS_OP_C) return HIPBLAS_STATUS_INVALID_VALUE;
+  const bool a_kc = op_A != HIPBLAS_OP_N;
+  GroupedArgs args{};
+  Elem e;
+  bool nothing;
+  const hipblasStatus_t st = f8_arguments(h, m, n, k, a_kc, a, lda, stridea, type_a, scale_a, stridescale, b, ldb, type_b, scale_b, c,
+                                          ldc, type_c, offsets, group_count, e, nothing, args);
+  if (st != HIPBLAS_STATUS_SUCCESS || nothing) return st;
+  return run_columns(h, e, a_kc, args, "gemm_f8");
+}
+
+hipblasStatus_t cuMpSGEMM_gemm_gated_f8(cuMpSGEMM_handle_t h, cuMpSGEMM_activation_t activation, uint64_t m, uint64_t n, uint64_t k,
+                                        const void *gate, const void *up, uint64_t lda, uint64_t stridea, hipDataType type_a,
+                                        const float *scale_gate, const float *scale_up, uint64_t stridescale, const void *b,
+                                        uint64_t ldb, hipDataType type_b, const float *scale_b, void *c, uint64_t ldc,
+                                        hipDataType type_c, const int *offsets, uint64_t group_count) {
+  if ((int)activation < CUMPSGEMM_SILU || (int)activation > CUMPSGEMM_RELU) return HIPBLAS_STATUS_INVALID_VALUE;
+  GroupedArgs args{};
+  Elem e;
+  bool nothing;
+  const hipblasStatus_t st = f8_arguments(h, m, n, k, true, gate, lda, stridea, type_a, scale_gate, stridescale, b, ldb, type_b, scale_b,
+                                          c, ldc, type_c, offsets, group_count, e, nothing, args);
+  if (st != HIPBLAS_STATUS_SUCCESS || nothing) return st;
+  if (k != 0 && (up == nullptr || scale_up == nullptr)) return HIPBLAS_STATUS_INVALID_VALUE;
+  args.up = (const char *)up;
+  args.scale_up = scale_up;
+  args.act = (uint32_t)activation;
+  return run_columns(h, e, true, args, "gemm_gated_f8", Epilogue::GATED);
 }
 
 hipblasStatus_t cuMpSGEMM_gemm_i8(cuMpSGEMM_handle_t h, uint64_t m, uint64_t n, uint64_t k, const int8_t *a, uint64_t lda,

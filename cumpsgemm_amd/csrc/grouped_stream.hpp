@@ -49,7 +49,7 @@ template <Elem E> __device__ inline stream_raw<E> stream_load(const char *p) {
   } else {
     typedef uint32_t u4u2_t __attribute__((ext_vector_type(4), aligned(2)));
     typedef uint32_t u4u1_t __attribute__((ext_vector_type(4), aligned(1)));
-    typedef typename std::conditional<T::I8, u4u1_t, u4u2_t>::type u4u_t;
+    typedef typename std::conditional<T::BYTES == 1, u4u1_t, u4u2_t>::type u4u_t;
     const u4u_t x = *reinterpret_cast<const u4u_t *>(p);
     r.v = u4_t{x.x, x.y, x.z, x.w};
   }
@@ -63,7 +63,7 @@ template <Elem E> __device__ inline stream_raw<E> stream_load_part(const char *p
 #pragma unroll
     for (int j = 0; j < 8; j++) r.v[j] = j < have ? reinterpret_cast<const float *>(p)[j] : 0.0f;
   } else {
-    typedef typename std::conditional<T::I8, uint8_t, uint16_t>::type V;
+    typedef typename std::conditional<T::BYTES == 1, uint8_t, uint16_t>::type V;
     constexpr int BITS = T::BYTES * 8, PER = 32 / BITS;
     u4_t x = {0, 0, 0, 0};
 #pragma unroll

@@ -259,6 +259,51 @@ hipblasStatus_t cuMpSGEMM_gemm_gated_backward(cuMpSGEMM_handle_t handle, hipblas
                                               cuMpSGEMM_compute_mode_t compute_mode, hipDataType type);
 
 
+/* ---- 8-bit floating point (OCP E4M3 and E5M2) with scales for blocks of 128 --
+ * type_a = HIP_R_8F_E4M3; type_b = HIP_R_8F_E4M3, or HIP_R_8F_E5M2 (gradients).
+ *   C[i, j] = sum_b scale_a(i, b) scale_b(b, j) sum_{l in block b} op(A_g)[i, l] B[l, j]
+ * for token j of group g; blocks of 128 K-values, the last one may be shorter.
+ * scale_b: ceil(k / 128) x n, a token's scales contiguous, block by block.
+ * scale_a: one for 128 x 128 of A_g as it is stored, blocks along its contiguous
+ * side first (what cuMpSGEMM_quantize_f8 with block_n = 128 gives): with op_A = T
+ * ceil(k / 128) x ceil(m / 128), with op_A = N, for the tokens' gradient with the
+ * same matrix, ceil(m / 128) x ceil(k / 128); the groups' at scale_a + g *
+ * stridescale.  Offsets, groups and strides as for the other products; offsets =
+ * NULL with group_count = 1: one matrix for all n tokens.  C is of type_c =
+ * HIP_R_32F, _16F or _16BF.  A block's products are summed by the matrix cores,
+ * which cut those of eight neighbours to multiples of 2^-13 of the largest one's
+ * power of two (2e-5 of the norm of a product of random values, whatever type_c
+ * is); the blocks' sums are scaled and added in FP32. */
+hipblasStatus_t cuMpSGEMM_gemm_f8(cuMpSGEMM_handle_t handle, hipblasOperation_t op_A, uint64_t m,
+                                  uint64_t n, uint64_t k, const void *a, uint64_t lda, uint64_t stridea,
+                                  hipDataType type_a, const float *scale_a, uint64_t stridescale,
+                                  const void *b, uint64_t ldb, hipDataType type_b, const float *scale_b,
+                                  void *c, uint64_t ldc, hipDataType type_c, const int *offsets,
+                                  uint64_t group_count);
+/* A gated block (cuMpSGEMM_gemm_gated, op_A = T) of such values: gate and up with
+ * a scale each for 128 x 128, laid out alike. */
+hipblasStatus_t cuMpSGEMM_gemm_gated_f8(cuMpSGEMM_handle_t handle, cuMpSGEMM_activation_t activation,
+                                        uint64_t m, uint64_t n, uint64_t k, const void *gate,
+                                        const void *up, uint64_t lda, uint64_t stridea,
+                                        hipDataType type_a, const float *scale_gate,
+                                        const float *scale_up, uint64_t stridescale, const void *b,
+                                        uint64_t ldb, hipDataType type_b, const float *scale_b, void *c,
+                                        uint64_t ldc, hipDataType type_c, const int *offsets,
+                                        uint64_t group_count);
+/* batch_count matrices of n columns, k values each, of type_x = HIP_R_32F, _16F or
+ * _16BF, x + i * stridex, as type_q = HIP_R_8F_E4M3 (M = 448) or HIP_R_8F_E5M2
+ * (M = 57344), q + i * strideq, with a scale for each block of 128 values of a column
+ * (block_n = 1: tokens) or of 128 columns (block_n = 128: matrices):
+ *   scale = max |x| / M,   q = M x / max |x| rounded to nearest, ties to even.
+ * scale: ceil(k / 128) x ceil(n / block_n) for each matrix, one behind the other.  (M x
+ * is exact in FP32 for 16-bit x, and rounded once for FP32 x.)  A block of zeros,
+ * or of numbers so small that the scale is 0, has scale 0 and zeros; one with an
+ * infinity or a NaN has scale NaN and zeros. */
+hipblasStatus_t cuMpSGEMM_quantize_f8(cuMpSGEMM_handle_t handle, uint64_t k, uint64_t n, const void *x,
+                                      uint64_t ldx, uint64_t stridex, hipDataType type_x,
+                                      uint64_t block_n, void *q, uint64_t ldq, uint64_t strideq,
+                                      hipDataType type_q, float *scale, uint64_t batch_count);
+
 /* cumpsgemm::exp_stats_ext<T> / exp_max_ext<T> (reference cumpsgemm.hpp:37-46) */
 unsigned cuMpSGEMM_exp_stats_ext_s(cuMpSGEMM_handle_t h, unsigned m, unsigned n, const float *ptr,
                                    unsigned ld, unsigned batch, unsigned stride);
