@@ -166,6 +166,8 @@ __device__ inline void multiply_f8_tile(const GroupedArgs &args, const TileWork 
 #pragma unroll
     for (int v = 0; v < 4; v++) acc[j][i][v] = fmaf(sums[q % RING][v], s[SIDES > 1 ? i & 1 : 0][j], acc[j][i][v]);
   };
+  // (else the compiler moves all of a step's additions behind its MFMAs, whose results then have no registers)
+  auto hold = [&](const int q) { asm volatile("" : "+v"(acc[q % TN][q / TN])); };
   auto enter = [&]() { // a step begins
 #pragma unroll
     for (int side = 0; side < SIDES; side++)
@@ -191,18 +193,23 @@ __device__ inline void multiply_f8_tile(const GroupedArgs &args, const TileWork 
         sums[q % RING] = f8_mfma<Cfg::E>(fa[g % 2], fb[j]);
         if (q >= DELAY) take(q - DELAY, now);
         else take(q - DELAY + MFMAS, old);
+        hold(q >= DELAY ? q - DELAY : q - DELAY + MFMAS);
         if constexpr (HAS_NEXT) {
+          // (the columns' next fragments take the place of the ones just used: there are no registers for both)
+          __builtin_amdgcn_sched_barrier(0);
           if (g + 1 == TM) read_b(next, j);
         }
       }
       if constexpr (HAS_NEXT) {
         if (g + 1 == TM) read_scales(next);
       }
+      if constexpr (!HAS_NEXT) {
 #pragma unroll
-      for (int j = 0; j < TN; j++) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); // MFMA
-        __builtin_amdgcn_sched_group_barrier(0x002, 5, 0); // vector
-        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0); // LDS reads
+        for (int j = 0; j < TN; j++) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); // MFMA
+          __builtin_amdgcn_sched_group_barrier(0x002, 5, 0); // vector
+          __builtin_amdgcn_sched_group_barrier(0x100, 2, 0); // LDS reads
+        }
       }
       __builtin_amdgcn_sched_barrier(0);
     }
