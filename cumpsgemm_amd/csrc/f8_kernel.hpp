@@ -11,6 +11,10 @@
 // multiples of 2^-13 of the largest one's power of two, then the sixteen such sums of a block are added in FP32, cut to 2^-23.
 // Products of random values come out 2e-5 of their norm from exact, a hundredth of what a result in BF16 is rounded by, a
 // tenth of FP16's.  (v_mfma_f32_16x16x32_fp8_fp8, at half the rate, gives the same bits.)
+// EXACT kernels take BF16 MFMAs instead, to which FP8 converts without rounding: products are exact, sums FP32, at half the
+// rate and with a conversion of every fragment.  That is for the kernels that wait for memory anyway, and for gated blocks whose
+// result is wider than BF16: it is FP8 again in the layer behind, where a value that was near half way between two of E4M3's
+// comes out a whole step away, and 2e-5 more before makes 4e-4 to 1e-3 of that layer's result (FP16's own rounding: 2e-4).
 //
 // LDS images: rows of 128 bytes as for 8-bit integers.  Operands whose rows, not K, are contiguous (A of op N): 128 lines of
 // BM bytes, read by ds_read_b64_tr_b8, which takes eight lines of sixteen rows and hands each lane one row's eight K-values.
@@ -29,6 +33,46 @@ template <Elem E> __device__ inline f4v_t f8_mfma(const i8v_t a, const i8v_t b) 
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, f4v_t{0.0f, 0.0f, 0.0f, 0.0f}, 0, E == Elem::E5M2 ? 1 : 0, 0, 0, 0, 0);
 }
 
+// eight values as BF16
+template <bool E5M2> __device__ inline u4_t f8_widen(const int lo, const int hi) {
+  typedef __bf16 b2_t __attribute__((ext_vector_type(2)));
+  u4_t x;
+  if constexpr (E5M2) {
+    x.x = __builtin_bit_cast(uint32_t, (b2_t)__builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(lo, 1.0f, false));
+    x.y = __builtin_bit_cast(uint32_t, (b2_t)__builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(lo, 1.0f, true));
+    x.z = __builtin_bit_cast(uint32_t, (b2_t)__builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(hi, 1.0f, false));
+    x.w = __builtin_bit_cast(uint32_t, (b2_t)__builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(hi, 1.0f, true));
+  } else {
+    x.x = __builtin_bit_cast(uint32_t, (b2_t)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false));
+    x.y = __builtin_bit_cast(uint32_t, (b2_t)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true));
+    x.z = __builtin_bit_cast(uint32_t, (b2_t)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false));
+    x.w = __builtin_bit_cast(uint32_t, (b2_t)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true));
+  }
+  return x;
+}
+// a fragment of 32 K-values, as the kernels multiply it: FP8 for one MFMA, or BF16 for four
+struct F8Wide {
+  u4_t v[4];
+};
+template <bool EXACT, bool E5M2> __device__ inline typename std::conditional<EXACT, F8Wide, i8v_t>::type f8_fragment(const i8v_t x) {
+  if constexpr (EXACT) {
+    F8Wide y;
+#pragma unroll
+    for (int c = 0; c < 4; c++) y.v[c] = f8_widen<E5M2>(x[2 * c], x[2 * c + 1]);
+    return y;
+  } else {
+    return x;
+  }
+}
+// (E: B's type, as above)
+template <Elem E> __device__ inline f4v_t f8_block(const i8v_t &a, const i8v_t &b) { return f8_mfma<E>(a, b); }
+template <Elem E> __device__ inline f4v_t f8_block(const F8Wide &a, const F8Wide &b) {
+  f4v_t x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int c = 0; c < 4; c++) x = mfma_block<true>(a.v[c], b.v[c], x);
+  return x;
+}
+
 // Where a step's scales lie: those of A belong to 128 x 128 of the matrix as it is stored, blocks along its contiguous side
 // first.
 struct F8Scales {
@@ -42,7 +86,7 @@ struct F8Scales {
   template <bool A_KC> __device__ inline uint64_t step_of_rows() const { return A_KC ? 4 : (uint64_t)mb * 4; }
 };
 
-template <Elem E, bool A_KC, int BM, int BN, int WM, int WN, int NSTAGE, bool DIRECT, Epilogue EPI>
+template <Elem E, bool A_KC, int BM, int BN, int WM, int WN, int NSTAGE, bool DIRECT, Epilogue EPI, bool EXACT_>
 struct F8Cfg : GroupedCfg<E, A_KC, true, BM, BN, WM, WN, 128, NSTAGE, DIRECT, false, 2, false, EPI> {
   using Base = GroupedCfg<E, A_KC, true, BM, BN, WM, WN, 128, NSTAGE, DIRECT, false, 2, false, EPI>;
   static_assert(Base::BK == 128, "a step is a block");
@@ -55,6 +99,7 @@ struct F8Cfg : GroupedCfg<E, A_KC, true, BM, BN, WM, WN, 128, NSTAGE, DIRECT, fa
   static constexpr int LDS_BYTES = NSTAGE * STAGE > Base::OUT_BYTES ? NSTAGE * STAGE : Base::OUT_BYTES;
   static_assert(LDS_BYTES <= 160 * 1024, "LDS");
   static constexpr int SIDES = Base::GATED ? 2 : 1;
+  static constexpr bool EXACT = EXACT_;
 };
 
 #pragma clang diagnostic push
@@ -125,13 +170,14 @@ __device__ inline void multiply_f8_tile(const GroupedArgs &args, const TileWork 
       return out;
     }
   };
-  i8v_t fa[2], fb[TN];
+  i8v_t fa[2];
+  typename std::conditional<Cfg::EXACT, F8Wide, i8v_t>::type fb[TN];
   float now[SIDES][TN], old[SIDES][TN], next_scales[SIDES][TN]; // of this step, the one before, the one behind
   auto read_a = [&](const char *stage, const int g) {
     fa[g % 2] = frag(stage, wm * Cfg::WM + g % TM * 16, std::integral_constant<bool, Cfg::A_KC>{});
   };
   auto read_b = [&](const char *stage, const int j) {
-    fb[j] = frag(stage + Cfg::A_STAGE, (j * Cfg::WAVES_N + wn) * 16, std::true_type{});
+    fb[j] = f8_fragment<Cfg::EXACT, Cfg::E == Elem::E5M2>(frag(stage + Cfg::A_STAGE, (j * Cfg::WAVES_N + wn) * 16, std::true_type{}));
   };
   auto read_scales = [&](const char *stage) {
     const float *s = reinterpret_cast<const float *>(stage + SCALES);
@@ -187,10 +233,11 @@ __device__ inline void multiply_f8_tile(const GroupedArgs &args, const TileWork 
       if (g + 1 < TM) read_a(stage, g + 1);
       else if constexpr (HAS_NEXT) read_a(next, 0);
       beside(g);
+      const auto a_now = f8_fragment<Cfg::EXACT, false>(fa[g % 2]);
 #pragma unroll
       for (int j = 0; j < TN; j++) {
         const int q = g * TN + j;
-        sums[q % RING] = f8_mfma<Cfg::E>(fa[g % 2], fb[j]);
+        sums[q % RING] = f8_block<Cfg::E>(a_now, fb[j]);
         if (q >= DELAY) take(q - DELAY, now);
         else take(q - DELAY + MFMAS, old);
         hold(q >= DELAY ? q - DELAY : q - DELAY + MFMAS);
@@ -383,9 +430,9 @@ template <class Cfg> void launch_f8(const GroupedArgs &args, uint32_t workgroups
   allow_dynamic_lds(reinterpret_cast<const void *>(&f8_kernel<Cfg>), Cfg::LDS_BYTES, done);
   hipLaunchKernelGGL(f8_kernel<Cfg>, dim3(workgroups), dim3(Cfg::NT), Cfg::LDS_BYTES, stream, args);
 }
-template <Elem E, bool A_KC, int BM, int BN, int WM, int WN, int NSTAGE, bool DIRECT, Epilogue EPI>
+template <Elem E, bool A_KC, int BM, int BN, int WM, int WN, int NSTAGE, bool DIRECT, Epilogue EPI, bool EXACT>
 constexpr GroupedKernel f8_entry() {
-  using Cfg = F8Cfg<E, A_KC, BM, BN, WM, WN, NSTAGE, DIRECT, EPI>;
+  using Cfg = F8Cfg<E, A_KC, BM, BN, WM, WN, NSTAGE, DIRECT, EPI, EXACT>;
   return {&launch_f8<Cfg>, Cfg::ROWS_OUT, Cfg::BN};
 }
 
@@ -436,10 +483,11 @@ __global__ __launch_bounds__(kStreamWaves * 64) void f8_stream_kernel(const Grou
   auto both = [](const stream_raw<E> &x, const stream_raw<E> &y) {
     return i8v_t{(int)x.v.x, (int)x.v.y, (int)x.v.z, (int)x.v.w, (int)y.v.x, (int)y.v.y, (int)y.v.z, (int)y.v.w};
   };
-  auto take = [&](const Step &x) {
+  auto take = [&](const Step &x) { // (exact: bound by memory)
+    const F8Wide fb = f8_fragment<true, E == Elem::E5M2>(both(x.b[0], x.b[1]));
 #pragma unroll
     for (int side = 0; side < SIDES; side++) {
-      const f4v_t y = f8_mfma<E>(both(x.a[side][0], x.a[side][1]), both(x.b[0], x.b[1]));
+      const f4v_t y = f8_block<E>(f8_fragment<true, false>(both(x.a[side][0], x.a[side][1])), fb);
       const float s = x.tokens * x.rows[side];
 #pragma unroll
       for (int v = 0; v < 4; v++) acc[side][v] = fmaf(y[v], s, acc[side][v]);
@@ -503,28 +551,29 @@ template <Elem E, Epilogue EPI> void launch_f8_stream(const GroupedArgs &args, u
 }
 
 // ---- tables ----
-template <Elem E, Epilogue EPI, bool A_KC> constexpr void f8_entries(GroupedTable &t) {
-  t.columns[A_KC][0][TILE_128] = f8_entry<E, A_KC, 128, 128, 64, 64, 2, false, EPI>();
-  t.columns[A_KC][1][TILE_256] = f8_entry<E, A_KC, 256, 256, 128, 64, 2, true, EPI>();
-  t.columns[A_KC][1][TILE_128] = f8_entry<E, A_KC, 128, 128, 64, 64, 2, true, EPI>();
-  t.columns[A_KC][1][TILE_NARROW] = f8_entry<E, A_KC, 128, 32, 32, 32, 3, true, EPI>();
+// Tiles of 32 tokens wait for memory, and are exact.
+template <Elem E, Epilogue EPI, bool A_KC, bool EXACT> constexpr void f8_entries(GroupedTable &t) {
+  t.columns[A_KC][0][TILE_128] = f8_entry<E, A_KC, 128, 128, 64, 64, 2, false, EPI, EXACT>();
+  if constexpr (!EXACT) t.columns[A_KC][1][TILE_256] = f8_entry<E, A_KC, 256, 256, 128, 64, 2, true, EPI, false>();
+  t.columns[A_KC][1][TILE_128] = f8_entry<E, A_KC, 128, 128, 64, 64, 2, true, EPI, EXACT>();
+  t.columns[A_KC][1][TILE_NARROW] = f8_entry<E, A_KC, 128, 32, 32, 32, 3, true, EPI, true>();
   if constexpr (A_KC) t.stream[A_KC] = {&launch_f8_stream<E, EPI>, 16, kStreamTokens};
 }
-
 template <Elem E> constexpr GroupedTable f8_table() {
   GroupedTable t{};
-  f8_entries<E, Epilogue::STORE, false>(t);
-  f8_entries<E, Epilogue::STORE, true>(t);
+  f8_entries<E, Epilogue::STORE, false, false>(t);
+  f8_entries<E, Epilogue::STORE, true, false>(t);
   return t;
 }
-template <Elem E> constexpr GroupedTable gated_f8_table() {
+template <Elem E, bool EXACT> constexpr GroupedTable gated_f8_table() {
   GroupedTable t{};
-  f8_entries<E, Epilogue::GATED, true>(t);
+  f8_entries<E, Epilogue::GATED, true, EXACT>(t);
   return t;
 }
 
-#define CUMPSGEMM_F8(kind, E)                  \
-  GroupedTable g_f8_##kind = f8_table<E>();    \
-  GroupedTable g_gated_f8_##kind = gated_f8_table<E>();
+#define CUMPSGEMM_F8(kind, E)                                        \
+  GroupedTable g_f8_##kind = f8_table<E>();                          \
+  GroupedTable g_gated_f8_##kind = gated_f8_table<E, false>();       \
+  GroupedTable g_gated_f8_exact_##kind = gated_f8_table<E, true>();
 
 } // namespace cumpsgemm_amd

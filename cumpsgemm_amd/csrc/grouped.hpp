@@ -57,8 +57,9 @@ struct GroupedKernel {
   int bm, bn;
 };
 
-// What becomes of the sums: C as they are, a gated block's result, or its gradient.
-enum class Epilogue : int { STORE = 0, GATED = 1, GATED_BACKWARD = 2 };
+// What becomes of the sums: C as they are, a gated block's result, or its gradient.  (GATED_EXACT: the kernels of GATED for 8-bit
+// floating point whose sums are exact, f8_kernel.hpp.)
+enum class Epilogue : int { STORE = 0, GATED = 1, GATED_BACKWARD = 2, GATED_EXACT = 3 };
 
 // Kernels of ragged columns: three tiles of the tiled kernel, from the largest, and the kernel of few tokens to a group
 // (grouped_stream.hpp).  Ragged K: the first two, and one for matrices of fewer than eight 16-bit rows or columns.

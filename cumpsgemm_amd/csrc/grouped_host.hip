@@ -11,17 +11,18 @@ extern GroupedTable g_grouped_f32_fp16tcec, g_grouped_f32_fp16tc, g_grouped_f32_
 extern GroupedTable g_gated_f32_fp16tcec, g_gated_f32_fp16tc, g_gated_f32_bf16x3, g_gated_f32_bf16x2, g_gated_f16, g_gated_bf16;
 extern GroupedTable g_gated_backward_f32_fp16tcec, g_gated_backward_f32_fp16tc, g_gated_backward_f32_bf16x3,
     g_gated_backward_f32_bf16x2, g_gated_backward_f16, g_gated_backward_bf16;
-extern GroupedTable g_f8_e4m3, g_f8_e5m2, g_gated_f8_e4m3, g_gated_f8_e5m2;
+extern GroupedTable g_f8_e4m3, g_f8_e5m2, g_gated_f8_e4m3, g_gated_f8_e5m2, g_gated_f8_exact_e4m3, g_gated_f8_exact_e5m2;
 
 // direct: the operands can take the shorter way into LDS (grouped_kernel.hpp); the kernel of few tokens takes any
 const GroupedKernel *lookup_grouped(Elem e, bool a_kc, bool ragged_k, bool direct, int cls, Epilogue epi = Epilogue::STORE) {
-  static const GroupedTable *const tables[3][kNumElems] = {
+  static const GroupedTable *const tables[4][kNumElems] = {
       {&g_grouped_f32_fp16tcec, &g_grouped_f32_fp16tc, &g_grouped_f32_bf16x3, &g_grouped_f32_bf16x2, &g_grouped_f16,
        &g_grouped_bf16, &g_grouped_i8, &g_f8_e4m3, &g_f8_e5m2},
       {&g_gated_f32_fp16tcec, &g_gated_f32_fp16tc, &g_gated_f32_bf16x3, &g_gated_f32_bf16x2, &g_gated_f16, &g_gated_bf16,
        nullptr, &g_gated_f8_e4m3, &g_gated_f8_e5m2},
       {&g_gated_backward_f32_fp16tcec, &g_gated_backward_f32_fp16tc, &g_gated_backward_f32_bf16x3, &g_gated_backward_f32_bf16x2,
-       &g_gated_backward_f16, &g_gated_backward_bf16}};
+       &g_gated_backward_f16, &g_gated_backward_bf16},
+      {nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, &g_gated_f8_exact_e4m3, &g_gated_f8_exact_e5m2}};
   if (tables[(int)epi][(int)e] == nullptr) return nullptr;
   const GroupedTable &t = *tables[(int)epi][(int)e];
   const GroupedKernel *k = ragged_k ? (cls == STREAM ? nullptr : &t.over_k[direct][cls])
@@ -175,7 +176,7 @@ hipblasStatus_t run_columns(cuMpSGEMM_handle *h, Elem e, bool a_kc, GroupedArgs 
   const uint32_t bytes = bytes_of(e);
   const bool direct = chunks_ok(args.a, a_kc ? args.k : args.m, args.lda, args.stride_a, bytes, a_kc ? 256 : 64) &&
                       chunks_ok(args.b, args.k, args.ldb, 0, bytes, 256) &&
-                      (epi != Epilogue::GATED || chunks_ok(args.up, 16, args.lda, args.stride_a, bytes, 0));
+                      ((epi != Epilogue::GATED && epi != Epilogue::GATED_EXACT) || chunks_ok(args.up, 16, args.lda, args.stride_a, bytes, 0));
   int cls = TILE_128;
   if (bytes == 2 && !direct && !a_kc && args.m < 8) {
     cls = STREAM; // (a line is shorter than the chunks that the tiled kernels read)
@@ -465,7 +466,8 @@ hipblasStatus_t cuMpSGEMM_gemm_gated_f8(cuMpSGEMM_handle_t h, cuMpSGEMM_activati
   args.up = (const char *)up;
   args.scale_up = scale_up;
   args.act = (uint32_t)activation;
-  return run_columns(h, e, true, args, "gemm_gated_f8", Epilogue::GATED);
+  // (f8_kernel.hpp says why results wider than BF16 come from exact sums)
+  return run_columns(h, e, true, args, "gemm_gated_f8", args.out == OUT_BF16 ? Epilogue::GATED : Epilogue::GATED_EXACT);
 }
 
 hipblasStatus_t cuMpSGEMM_gemm_i8(cuMpSGEMM_handle_t h, uint64_t m, uint64_t n, uint64_t k, const int8_t *a, uint64_t lda,
