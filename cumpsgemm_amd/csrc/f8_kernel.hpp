@@ -554,6 +554,7 @@ template <Elem E, Epilogue EPI> void launch_f8_stream(const GroupedArgs &args, u
 // Tiles of 32 tokens wait for memory, and are exact.
 template <Elem E, Epilogue EPI, bool A_KC, bool EXACT> constexpr void f8_entries(GroupedTable &t) {
   t.columns[A_KC][0][TILE_128] = f8_entry<E, A_KC, 128, 128, 64, 64, 2, false, EPI, EXACT>();
+  t.columns[A_KC][0][TILE_NARROW] = f8_entry<E, A_KC, 128, 32, 32, 32, 2, false, EPI, true>();
   if constexpr (!EXACT) t.columns[A_KC][1][TILE_256] = f8_entry<E, A_KC, 256, 256, 128, 64, 2, true, EPI, false>();
   t.columns[A_KC][1][TILE_128] = f8_entry<E, A_KC, 128, 128, 64, 64, 2, true, EPI, EXACT>();
   t.columns[A_KC][1][TILE_NARROW] = f8_entry<E, A_KC, 128, 32, 32, 32, 3, true, EPI, true>();

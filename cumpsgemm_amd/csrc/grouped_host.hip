@@ -401,8 +401,6 @@ hipblasStatus_t cuMpSGEMM_gemm_gated(cuMpSGEMM_handle_t h, hipblasOperation_t op
   args.z[0] = (char *)z_gate;
   args.z[1] = (char *)z_up;
   args.ldz = ldz;
-  args.vec_c = four_at_once(c, m, ldc, 0, args.out) &&
-               (z_gate == nullptr || (four_at_once(z_gate, m, ldz, 0, args.out) && four_at_once(z_up, m, ldz, 0, args.out)));
   return run_columns(h, e, op_A != HIPBLAS_OP_N, args, "gemm_gated", Epilogue::GATED);
 }
 
@@ -429,9 +427,6 @@ hipblasStatus_t cuMpSGEMM_gemm_gated_backward(cuMpSGEMM_handle_t h, hipblasOpera
   args.ldd = ldd;
   args.c = (char *)c;
   args.ldc = ldc;
-  args.vec_c = four_at_once(z_gate, m, ldz, 0, args.out) && four_at_once(z_up, m, ldz, 0, args.out) &&
-               four_at_once(d_gate, m, ldd, 0, args.out) && four_at_once(d_up, m, ldd, 0, args.out) &&
-               (c == nullptr || four_at_once(c, m, ldc, 0, args.out));
   return run_columns(h, e, op_A != HIPBLAS_OP_N, args, "gemm_gated_backward", Epilogue::GATED_BACKWARD);
 }
 

@@ -498,6 +498,41 @@ __device__ inline void store_four(char *c, const f4v_t x, float beta, uint32_t r
   }
 }
 
+// Four rows of a column at any alignment: one access, unless the matrix ends among them.  (Value by value, at sizes that are not
+// multiples of four: 1001 tokens of 5 experts, 515 x 389 in FP16, the gradient ODD_US.)
+template <uint32_t OUT> struct four_of {
+  typedef typename out_type<OUT>::type O;
+  typedef O type __attribute__((ext_vector_type(4)));
+  typedef O anywhere __attribute__((ext_vector_type(4), aligned(sizeof(O))));
+};
+template <uint32_t OUT> __device__ inline void put_four(char *column, const f4v_t x, uint32_t row, uint32_t m) {
+  auto *p = reinterpret_cast<typename out_type<OUT>::type *>(column) + row;
+  const typename four_of<OUT>::type y = __builtin_convertvector(x, typename four_of<OUT>::type);
+  if (row + 4 <= m) {
+    *reinterpret_cast<typename four_of<OUT>::anywhere *>(p) = y;
+  } else {
+#pragma unroll
+    for (int v = 0; v < 3; v++)
+      if (row + v < m) p[v] = y[v];
+  }
+}
+// (values of rows from m on: any; their results are not stored)
+template <uint32_t OUT> __device__ inline typename four_of<OUT>::type take_four(const char *column, uint32_t row, uint32_t m) {
+  const auto *p = reinterpret_cast<const typename out_type<OUT>::type *>(column);
+  if (m >= 4) { // the last four in place of those that stick out, moved to their places
+    const uint32_t at = row + 4 <= m ? row : m - 4;
+    typename four_of<OUT>::type x = *reinterpret_cast<const typename four_of<OUT>::anywhere *>(p + at);
+    if (at != row) {
+      const uint32_t by = row - at;
+      x = by == 1 ? __builtin_shufflevector(x, x, 1, 2, 3, 3) : by == 2 ? __builtin_shufflevector(x, x, 2, 3, 3, 3) : __builtin_shufflevector(x, x, 3, 3, 3, 3);
+    }
+    return x;
+  }
+  typename four_of<OUT>::type x;
+#pragma unroll
+  for (int v = 0; v < 4; v++) x[v] = p[row + v < m ? row + v : m - 1];
+  return x;
+}
 // Rows row .. row + 3 of column col of a gated block: the result, and the projections where they are wanted.
 template <uint32_t OUT, bool EXACT>
 __device__ inline void store_gated(const GroupedArgs &args, const f4v_t gate, const f4v_t up, uint32_t row, uint32_t col) {
@@ -506,46 +541,31 @@ __device__ inline void store_gated(const GroupedArgs &args, const f4v_t gate, co
   float slope;
 #pragma unroll
   for (int v = 0; v < 4; v++) x[v] = activation<EXACT, false>(args.act, gate[v], slope) * up[v];
-  store_four<OUT>(args.c + ((uint64_t)col * args.ldc + row) * BYTES, x, 0.0f, row, args.m, args.vec_c != 0);
+  put_four<OUT>(args.c + (uint64_t)col * args.ldc * BYTES, x, row, args.m);
   if (args.z[0] == nullptr) return;
-  const uint64_t at = ((uint64_t)col * args.ldz + row) * BYTES;
-  store_four<OUT>(args.z[0] + at, gate, 0.0f, row, args.m, args.vec_c != 0);
-  store_four<OUT>(args.z[1] + at, up, 0.0f, row, args.m, args.vec_c != 0);
+  const uint64_t at = (uint64_t)col * args.ldz * BYTES;
+  put_four<OUT>(args.z[0] + at, gate, row, args.m);
+  put_four<OUT>(args.z[1] + at, up, row, args.m);
 }
-// p[0 .. 3], zeros from row m on
-template <uint32_t OUT> __device__ inline f4v_t load_four(const char *c, uint32_t row, uint32_t m, bool vec) {
-  typedef typename out_type<OUT>::type O;
-  typedef O o4_t __attribute__((ext_vector_type(4)));
-  const O *p = reinterpret_cast<const O *>(c);
-  f4v_t x = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (vec) {
-    if (row < m) x = __builtin_convertvector(*reinterpret_cast<const o4_t *>(p), f4v_t);
-  } else {
-#pragma unroll
-    for (int v = 0; v < 4; v++)
-      if (row + v < m) x[v] = (float)p[v];
-  }
-  return x;
-}
-// ... of its gradient: x is that of act(G) * U.  (G and U are read before anything is written: dG and dU may take their place.)
+// ... of its gradient: x is that of act(G) * U.  (G and U were read before anything is written: dG and dU may take their place.)
 template <uint32_t OUT, bool EXACT>
-__device__ inline void store_gradients(const GroupedArgs &args, const f4v_t x, uint32_t row, uint32_t col) {
+__device__ inline void store_gradients(const GroupedArgs &args, const f4v_t x, const typename four_of<OUT>::type gate,
+                                       const typename four_of<OUT>::type up, uint32_t row, uint32_t col) {
   constexpr int BYTES = sizeof(typename out_type<OUT>::type);
-  const bool vec = args.vec_c != 0;
-  const uint64_t from = ((uint64_t)col * args.ldz + row) * BYTES, to = ((uint64_t)col * args.ldd + row) * BYTES;
-  const f4v_t gate = load_four<OUT>(args.z[0] + from, row, args.m, vec), up = load_four<OUT>(args.z[1] + from, row, args.m, vec);
+  const uint64_t to = (uint64_t)col * args.ldd * BYTES;
   f4v_t h, dg, du;
 #pragma unroll
   for (int v = 0; v < 4; v++) {
+    const float u = (float)up[v];
     float slope;
-    const float a = activation<EXACT, true>(args.act, gate[v], slope);
-    h[v] = a * up[v];
-    dg[v] = x[v] * up[v] * slope;
+    const float a = activation<EXACT, true>(args.act, (float)gate[v], slope);
+    h[v] = a * u;
+    dg[v] = x[v] * u * slope;
     du[v] = x[v] * a;
   }
-  store_four<OUT>(args.d[0] + to, dg, 0.0f, row, args.m, vec);
-  store_four<OUT>(args.d[1] + to, du, 0.0f, row, args.m, vec);
-  if (args.c != nullptr) store_four<OUT>(args.c + ((uint64_t)col * args.ldc + row) * BYTES, h, 0.0f, row, args.m, vec);
+  put_four<OUT>(args.d[0] + to, dg, row, args.m);
+  put_four<OUT>(args.d[1] + to, du, row, args.m);
+  if (args.c != nullptr) put_four<OUT>(args.c + (uint64_t)col * args.ldc * BYTES, h, row, args.m);
 }
 
 // A tile's place in memory: what its loops need to know.
@@ -581,8 +601,8 @@ __device__ inline void write_tile(const GroupedArgs &args, const TileWork &w, ch
     else if (Cfg::E == Elem::F16 || (T::BYTES == 1 && args.out == OUT_F16)) f(std::integral_constant<uint32_t, OUT_F16>{});
     else f(std::integral_constant<uint32_t, OUT_BF16>{});
   };
-#pragma unroll
-  for (int j = 0; j < TN; j++) {
+  auto column_of = [&](int j, int r) { return w.n0 + (j * Cfg::WAVES_N + wn) * 16 + r + lane / LANES; };
+  auto put = [&](const int j) { // column block j into LDS
 #pragma unroll
     for (int i = 0; i < TM; i++) {
       f4v_t x;
@@ -592,18 +612,60 @@ __device__ inline void write_tile(const GroupedArgs &args, const TileWork &w, ch
     }
     // (a wave's own writes and reads of LDS are carried out in order)
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
-    const uint32_t col0 = w.n0 + (j * Cfg::WAVES_N + wn) * 16;
-    f4v_t sa = {args.alpha, args.alpha, args.alpha, args.alpha};
-    if constexpr (T::I8) {
+  };
+  if constexpr (Cfg::EPI == Epilogue::GATED_BACKWARD) {
+    // G and U of a whole column block are asked for while the one before is computed.  (Asked for four rows at a time, each
+    // pair waited a memory's round trip for: 16384 tokens of 8 experts, 2048 x 2048 in BF16, 312 us, so BACKWARD_US.)
+    constexpr uint32_t OUT = T::F32 ? OUT_F32 : Cfg::E == Elem::F16 ? OUT_F16 : OUT_BF16;
+    constexpr int BYTES = sizeof(typename out_type<OUT>::type), ROUNDS = 16 / COLS;
+    typename four_of<OUT>::type z[2][ROUNDS][2];
+    auto ask = [&](const int j, const int set) {
 #pragma unroll
-      for (int v = 0; v < 4; v++)
-        sa[v] = args.scale_a[(uint64_t)w.group * args.m + (row + v < args.m ? row + v : args.m - 1)];
+      for (int r = 0; r < ROUNDS; r++) {
+        const uint32_t col = column_of(j, r * COLS);
+        const uint64_t from = (uint64_t)(col < w.n_end ? col : w.n_end - 1) * args.ldz * BYTES;
+#pragma unroll
+        for (int side = 0; side < 2; side++) z[set][r][side] = take_four<OUT>(args.z[side] + from, row, args.m);
+      }
+    };
+    ask(0, 0);
+#pragma unroll
+    for (int j = 0; j < TN; j++) {
+      if (j + 1 < TN) ask(j + 1, (j + 1) % 2);
+      put(j);
+#pragma unroll
+      for (int r = 0; r < ROUNDS; r++) {
+        const uint32_t col = column_of(j, r * COLS);
+        const f4v_t x = *reinterpret_cast<const f4v_t *>(mine + (r * COLS + lane / LANES) * PITCH + lane % LANES * 4);
+        if (col < w.n_end) store_gradients<OUT, T::F32>(args, x, z[j % 2][r][0], z[j % 2][r][1], row, col);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
     }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < TN; j++) {
+    put(j);
+    if constexpr (Cfg::GATED) {
 #pragma unroll 1
-    for (int r = 0; r < 16; r += COLS) {
-      const uint32_t col = col0 + r + lane / LANES;
-      if (col >= w.n_end) continue;
-      if constexpr (Cfg::EPI == Epilogue::STORE) {
+      for (int r = 0; r < 16; r += COLS) {
+        const uint32_t col = column_of(j, r);
+        const int own = lane % LANES * 4;
+        const float *p = mine + (r + lane / LANES) * PITCH + (own >> 4) * 32 + (own & 15);
+        const f4v_t x = *reinterpret_cast<const f4v_t *>(p), y = *reinterpret_cast<const f4v_t *>(p + 16);
+        if (col < w.n_end) typed([&](auto out) { store_gated<out.value, T::F32>(args, x, y, row, col); });
+      }
+    } else {
+      f4v_t sa = {args.alpha, args.alpha, args.alpha, args.alpha};
+      if constexpr (T::I8) {
+#pragma unroll
+        for (int v = 0; v < 4; v++)
+          sa[v] = args.scale_a[(uint64_t)w.group * args.m + (row + v < args.m ? row + v : args.m - 1)];
+      }
+#pragma unroll 1
+      for (int r = 0; r < 16; r += COLS) {
+        const uint32_t col = column_of(j, r);
+        if (col >= w.n_end) continue;
         f4v_t x = *reinterpret_cast<const f4v_t *>(mine + (r + lane / LANES) * PITCH + (lane % LANES) * 4);
         if constexpr (Cfg::RAGGED_K) {
           if (args.splits > 1) {
@@ -618,16 +680,6 @@ __device__ inline void write_tile(const GroupedArgs &args, const TileWork &w, ch
         typed([&](auto out) {
           store_four<out.value>(w.c + at * sizeof(typename out_type<out.value>::type), x, args.beta, row, args.m, args.vec_c != 0);
         });
-      } else {
-        const int own = lane % LANES * 4;
-        const float *p = mine + (r + lane / LANES) * PITCH + (Cfg::GATED ? (own >> 4) * 32 + (own & 15) : own);
-        const f4v_t x = *reinterpret_cast<const f4v_t *>(p);
-        if constexpr (Cfg::GATED) {
-          const f4v_t y = *reinterpret_cast<const f4v_t *>(p + 16);
-          typed([&](auto out) { store_gated<out.value, T::F32>(args, x, y, row, col); });
-        } else {
-          typed([&](auto out) { store_gradients<out.value, T::F32>(args, x, row, col); });
-        }
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");

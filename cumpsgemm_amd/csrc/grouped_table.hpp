@@ -74,6 +74,7 @@ template <Elem E, Epilogue EPI, bool A_KC> constexpr void gated_entries(GroupedT
     t.columns[A_KC][1][TILE_NARROW] = grouped_of<E, A_KC, true, 128, 32, 32, 32, 64, 2, true, false, false, EPI>();
   } else {
     t.columns[A_KC][0][TILE_128] = grouped_of<E, A_KC, true, 128, 128, 64, 64, 128, 2, false, false, false, EPI>();
+    t.columns[A_KC][0][TILE_NARROW] = grouped_of<E, A_KC, true, 128, 32, 32, 32, 128, 2, false, false, false, EPI>();
     t.columns[A_KC][1][TILE_256] = grouped_of<E, A_KC, true, 256, 256, 128, 64, 128, 2, true, false, false, EPI>();
     t.columns[A_KC][1][TILE_128] = grouped_of<E, A_KC, true, 128, 128, 64, 64, 128, 2, true, false, false, EPI>();
     t.columns[A_KC][1][TILE_NARROW] = grouped_of<E, A_KC, true, 128, 32, 32, 32, 128, 4, true, false, false, EPI>();
