@@ -27,6 +27,7 @@ namespace cumpsgemm_amd {
 
 typedef int i8v_t __attribute__((ext_vector_type(8)));
 
+
 // B in E; A is E4M3
 template <Elem E> __device__ inline f4v_t f8_mfma(const i8v_t a, const i8v_t b) {
   // (format 0: E4M3, 1: E5M2; scales of zero: none)
@@ -123,7 +124,7 @@ __device__ inline void multiply_f8_tile(const GroupedArgs &args, const TileWork 
   using LB = grouped_loader<Cfg::E, true, BN, 128, NT>;
   constexpr int UB = (TN * 16 * Cfg::WAVES_N * 8 + NT - 1) / NT; // rounds of loads that B's columns need
   const char *a = w.a, *b = w.b;
-  if constexpr (Cfg::GATED) a = uniform_address(LA::side(wave) ? w.up : w.a);
+  if constexpr (Cfg::GATED) a = uniform_address(w.a + (uint64_t)LA::side(wave) * (uint64_t)(w.up - w.a)); // (no choice of two: it would put w into memory)
   const uint64_t a_step = Cfg::A_KC ? 128 : 128 * args.lda, b_step = 128;
 
   // ---- scales ----
@@ -170,11 +171,14 @@ __device__ inline void multiply_f8_tile(const GroupedArgs &args, const TileWork 
       return out;
     }
   };
-  i8v_t fa[2];
+  // row blocks of A on their way ahead of the one that is multiplied (two, in tiles of 256 rows: level)
+  constexpr int AHEAD = 1, A_RING = 2 * AHEAD;
+  static_assert(TM % A_RING == 0, "a step begins where the ring does");
+  i8v_t fa[A_RING];
   typename std::conditional<Cfg::EXACT, F8Wide, i8v_t>::type fb[TN];
   float now[SIDES][TN], old[SIDES][TN], next_scales[SIDES][TN]; // of this step, the one before, the one behind
   auto read_a = [&](const char *stage, const int g) {
-    fa[g % 2] = frag(stage, wm * Cfg::WM + g % TM * 16, std::integral_constant<bool, Cfg::A_KC>{});
+    fa[g % A_RING] = frag(stage, wm * Cfg::WM + g % TM * 16, std::integral_constant<bool, Cfg::A_KC>{});
   };
   auto read_b = [&](const char *stage, const int j) {
     fb[j] = f8_fragment<Cfg::EXACT, Cfg::E == Elem::E5M2>(frag(stage + Cfg::A_STAGE, (j * Cfg::WAVES_N + wn) * 16, std::true_type{}));
@@ -192,7 +196,8 @@ __device__ inline void multiply_f8_tile(const GroupedArgs &args, const TileWork 
     }
   };
   auto begin = [&](const char *stage) {
-    read_a(stage, 0);
+#pragma unroll
+    for (int g = 0; g < AHEAD; g++) read_a(stage, g);
 #pragma unroll
     for (int j = 0; j < TN; j++) read_b(stage, j);
     read_scales(stage);
@@ -230,10 +235,10 @@ __device__ inline void multiply_f8_tile(const GroupedArgs &args, const TileWork 
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int g = from.value; g < to.value; g++) {
-      if (g + 1 < TM) read_a(stage, g + 1);
-      else if constexpr (HAS_NEXT) read_a(next, 0);
+      if (g + AHEAD < TM) read_a(stage, g + AHEAD);
+      else if constexpr (HAS_NEXT) read_a(next, g + AHEAD - TM);
       beside(g);
-      const auto a_now = f8_fragment<Cfg::EXACT, false>(fa[g % 2]);
+      const auto a_now = f8_fragment<Cfg::EXACT, false>(fa[g % A_RING]);
 #pragma unroll
       for (int j = 0; j < TN; j++) {
         const int q = g * TN + j;
@@ -263,7 +268,7 @@ __device__ inline void multiply_f8_tile(const GroupedArgs &args, const TileWork 
   };
   auto nothing = [](int) {};
   constexpr std::integral_constant<int, 0> first;
-  constexpr std::integral_constant<int, TM - 1> last;
+  constexpr std::integral_constant<int, TM - AHEAD> last;
   constexpr std::integral_constant<int, TM> end;
 
   // ---- K loop ----
@@ -308,7 +313,7 @@ __device__ inline void multiply_f8_tile(const GroupedArgs &args, const TileWork 
       block_sync_lds();
       begin(lds);
     }
-    constexpr int SPREAD = TM / 2 > 1 ? TM / 2 : 1; // a step's loads are spread over half of one
+    constexpr int SPREAD = TM / 2 > AHEAD ? TM / 2 : AHEAD; // a step's loads are spread over half of one
     int at = 0, before = 0; // buffers of steps s and s - 1
     const char *qa = uniform_address(a + block_of(Cfg::NSTAGE) * a_step), *qb = uniform_address(b + block_of(Cfg::NSTAGE) * b_step);
     const char *qs = scale + block_of(Cfg::NSTAGE) * scale_step; // of step s + NSTAGE
@@ -323,7 +328,7 @@ __device__ inline void multiply_f8_tile(const GroupedArgs &args, const TileWork 
         if (rest) {
 #pragma unroll
           for (int l = 0; l < LOADS; l++)
-            if (l * SPREAD / LOADS == g + 1) issue(l, pa, pb, ps, old_stage);
+            if (l * SPREAD / LOADS == g + AHEAD) issue(l, pa, pb, ps, old_stage);
         }
       });
       if (s + Cfg::NSTAGE <= steps) __builtin_amdgcn_s_waitcnt(waitcnt_vm(LOADS * (Cfg::NSTAGE - 2)));
@@ -332,11 +337,11 @@ __device__ inline void multiply_f8_tile(const GroupedArgs &args, const TileWork 
       const uint32_t stage = lds0 + at * Cfg::STAGE;
       const bool more = s + Cfg::NSTAGE < steps;
       // (behind the last step, unused values are read)
-      multiply(here, (const char *)lds + next * Cfg::STAGE, last, end, [&](int) {
+      multiply(here, (const char *)lds + next * Cfg::STAGE, last, end, [&](int g) {
         if (more) {
 #pragma unroll
           for (int l = 0; l < LOADS; l++)
-            if (l * SPREAD / LOADS == 0) issue(l, qa, qb, qs, stage);
+            if (l * SPREAD / LOADS == g - last.value) issue(l, qa, qb, qs, stage);
         }
       });
       qa += a_step;

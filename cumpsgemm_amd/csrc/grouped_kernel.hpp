@@ -702,7 +702,7 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
   const char *a = w.a, *b = w.b;
   uint64_t apart = 0; // from a row of the gate's matrix to the other's
   if constexpr (Cfg::GATED && LA::LINES) apart = (uint64_t)(w.up - w.a);
-  else if constexpr (Cfg::GATED) a = uniform_address(LA::side(wave) ? w.up : w.a);
+  else if constexpr (Cfg::GATED) a = uniform_address(w.a + (uint64_t)LA::side(wave) * (uint64_t)(w.up - w.a)); // (no choice of two: it would put w into memory)
   const uint64_t a_step = (Cfg::A_KC ? (uint64_t)BK : (uint64_t)BK * args.lda) * T::BYTES;
   const uint64_t b_step = (Cfg::B_KC ? (uint64_t)BK : (uint64_t)BK * args.ldb) * T::BYTES;
 

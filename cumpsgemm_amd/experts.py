@@ -140,6 +140,10 @@ class Experts:
             _check(self.handle.quantize_i8(inner, count * out, self.weights, inner, _type(self.weights), q, inner, scale))
         return Int8Experts(self.handle, q, scale)
 
+    def to_f8(self):
+        """The same layer for serving, in 8-bit floating point (E4M3) with a scale for 128 x 128 of each matrix."""
+        return F8Experts(self.handle, *_matrices_to_f8(self.handle, self.weights))
+
 
 class Int8Experts:
     """weights: [experts, features out, features in] 8-bit integers, scale: [experts, features out].  Tokens of no expert as in
@@ -168,6 +172,66 @@ class Int8Experts:
             _check(self.handle.quantize_i8(inner, len(x), grouped, inner, _type(x), q, inner, scale))
             _check(self.handle.gemm_i8(out, len(x), inner, self.weights, inner, out * inner, self.scale, q, inner, scale, y, out,
                                        _type(y), offsets, count))
+        return torch.empty_like(y).index_copy_(0, order, y)
+
+
+def _blocks(size):
+    return -(-size // 128)
+
+
+def _matrices_to_f8(handle, weights):
+    """(E4M3 values, scales [matrices, blocks of rows, blocks of columns]) of [matrices, rows, columns]"""
+    import torch
+    count, rows, cols = weights.shape
+    q = torch.empty(count, rows, cols, device=weights.device, dtype=torch.float8_e4m3fn)
+    scale = torch.empty(count, _blocks(rows), _blocks(cols), device=weights.device, dtype=torch.float32)
+    with _on_current_stream(handle, weights):
+        _check(handle.quantize_f8(cols, rows, weights, cols, rows * cols, _type(weights), 128, q, cols, rows * cols, lib.R_8F_E4M3, scale,
+                                  count))
+    return q, scale
+
+
+def _tokens_to_f8(handle, x):
+    """(E4M3 values, scales [tokens, blocks]); on the stream that the handle has"""
+    import torch
+    n, k = x.shape
+    q = torch.empty(n, k, device=x.device, dtype=torch.float8_e4m3fn)
+    scale = torch.empty(n, _blocks(k), device=x.device, dtype=torch.float32)
+    _check(handle.quantize_f8(k, n, x, k, 0, _type(x), 1, q, k, 0, lib.R_8F_E4M3, scale))
+    return q, scale
+
+
+def _f8_matrices(name, weights, scale):
+    import torch
+    count, out, inner = _sizes(name, weights)
+    _expect(name, weights, (count, out, inner), weights.device, torch.float8_e4m3fn)
+    _expect(f"scale of {name}", scale, (count, _blocks(out), _blocks(inner)), weights.device, torch.float32)
+    return weights.contiguous(), scale.contiguous()
+
+
+class F8Experts:
+    """weights: [experts, features out, features in] in E4M3, scale: [experts, ceil(out / 128), ceil(in / 128)].  Tokens of no expert
+    as in Experts."""
+
+    def __init__(self, handle, weights, scale):
+        self.handle = handle
+        self.weights, self.scale = _f8_matrices("weights", weights, scale)
+
+    def forward(self, x, experts):
+        """x in FP32, FP16 or BF16, a scale taken for each 128 values of a token; y of the same type"""
+        import torch
+        _type(x)
+        count, out, inner = self.weights.shape
+        _expect("x", x, (len(x), inner), self.weights.device)
+        _expect("experts", experts, (len(x),), x.device)
+        order, offsets = group_by_expert(experts, count)
+        grouped = x[order]
+        y = torch.zeros(len(x), out, device=x.device, dtype=x.dtype)  # (the library writes the rows of experts' tokens only)
+        with _on_current_stream(self.handle, self.weights):
+            q, scale = _tokens_to_f8(self.handle, grouped)
+            _check(self.handle.gemm_f8(lib.OP_T, out, len(x), inner, self.weights, inner, out * inner, lib.R_8F_E4M3, self.scale,
+                                       self.scale[0].numel() if count else 0, q, inner, lib.R_8F_E4M3, scale, y, out, _type(y), offsets,
+                                       count))
         return torch.empty_like(y).index_copy_(0, order, y)
 
 
