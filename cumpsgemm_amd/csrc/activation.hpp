@@ -10,6 +10,7 @@
 #pragma once
 #include <cumpsgemm/cumpsgemm_ext.h>
 #include <hip/hip_runtime.h>
+#include <type_traits>
 
 namespace cumpsgemm_amd {
 
@@ -33,26 +34,32 @@ template <bool EXACT> __device__ inline float normal_below(float x, float &bell)
   return x > 0.0f ? 1.0f - tail : tail;
 }
 
-// slope: the derivative, if DERIVATIVE
-template <bool EXACT, bool DERIVATIVE> __device__ inline float activation(uint32_t act, float x, float &slope) {
-  if (act == CUMPSGEMM_SILU) {
-    const float s = sigmoid<EXACT>(x);
-    if (DERIVATIVE) slope = s + x * s * (1.0f - s);
-    return x * s;
-  }
-  if (act == CUMPSGEMM_GELU) {
+// act(x), and its derivative as slope if DERIVATIVE
+template <uint32_t ACT, bool EXACT, bool DERIVATIVE> __device__ inline float activation(float x, float &slope) {
+  if constexpr (ACT == CUMPSGEMM_SILU) {
+    const float s = sigmoid<EXACT>(x), y = x * s;
+    if (DERIVATIVE) slope = fmaf(y, 1.0f - s, s);
+    return y;
+  } else if constexpr (ACT == CUMPSGEMM_GELU) {
     float bell;
     const float p = normal_below<EXACT>(x, bell);
-    if (DERIVATIVE) slope = p + x * 0.39894228f * bell;
+    if (DERIVATIVE) slope = fmaf(x * 0.39894228f, bell, p);
     return x * p;
+  } else if constexpr (ACT == CUMPSGEMM_GELU_TANH) {
+    const float s = sigmoid<EXACT>(1.5957691216f * (x + 0.044715f * x * x * x)), y = x * s;
+    if (DERIVATIVE) slope = fmaf(y * (1.0f - s), 1.5957691216f * (1.0f + 0.134145f * x * x), s);
+    return y;
+  } else {
+    if (DERIVATIVE) slope = x > 0.0f ? 1.0f : 0.0f;
+    return x < 0.0f ? 0.0f : x; // (a NaN stays one)
   }
-  if (act == CUMPSGEMM_GELU_TANH) {
-    const float s = sigmoid<EXACT>(1.5957691216f * (x + 0.044715f * x * x * x));
-    if (DERIVATIVE) slope = s + x * s * (1.0f - s) * (1.5957691216f * (1.0f + 0.134145f * x * x));
-    return x * s;
-  }
-  if (DERIVATIVE) slope = x > 0.0f ? 1.0f : 0.0f;
-  return x < 0.0f ? 0.0f : x; // (a NaN stays one)
+}
+// f(the activation, as a constant)
+template <class F> __device__ inline void with_activation(uint32_t act, F f) {
+  if (act == CUMPSGEMM_SILU) f(std::integral_constant<uint32_t, CUMPSGEMM_SILU>{});
+  else if (act == CUMPSGEMM_GELU) f(std::integral_constant<uint32_t, CUMPSGEMM_GELU>{});
+  else if (act == CUMPSGEMM_GELU_TANH) f(std::integral_constant<uint32_t, CUMPSGEMM_GELU_TANH>{});
+  else f(std::integral_constant<uint32_t, CUMPSGEMM_RELU>{});
 }
 
 } // namespace cumpsgemm_amd

@@ -393,7 +393,14 @@ __device__ inline void multiply_f8_tile(const GroupedArgs &args, const TileWork 
 #pragma unroll
   for (int q = MFMAS - DELAY; q < MFMAS; q++) take(q, now);
 
-  write_tile<Cfg, TN>(args, w, lds, [&](const int j, const int i, const int v) { return acc[j][i][v]; });
+  write_tile<Cfg, TN>(
+      args, w, lds, [&](const int j, const int i, const int v) { return acc[j][i][v]; },
+      [&]() {
+#pragma unroll
+        for (int j = 0; j + 1 < TN; j++)
+#pragma unroll
+          for (int i = 0; i < TM; i++) acc[j][i] = acc[j + 1][i];
+      });
 }
 
 template <class Cfg>
@@ -544,8 +551,13 @@ __global__ __launch_bounds__(kStreamWaves * 64) void f8_stream_kernel(const Grou
 #pragma unroll
     for (int w = 0; w < kStreamWaves; w++) x[side] += sums[side][w][j][r];
   }
-  float y = x[0], slope;
-  if constexpr (EPI == Epilogue::GATED) y = activation<false, false>(args.act, y, slope) * x[SIDES - 1];
+  float y = x[0];
+  if constexpr (EPI == Epilogue::GATED) {
+    with_activation(args.act, [&](auto act) {
+      float slope;
+      y = activation<act.value, false, false>(x[0], slope) * x[SIDES - 1];
+    });
+  }
   const uint64_t at = (uint64_t)(n0 + j) * args.ldc + m0 + r;
   if (args.out == OUT_F32) reinterpret_cast<float *>(args.c)[at] = y;
   else if (args.out == OUT_F16) reinterpret_cast<_Float16 *>(args.c)[at] = (_Float16)y;
@@ -563,6 +575,7 @@ template <Elem E, Epilogue EPI, bool A_KC, bool EXACT> constexpr void f8_entries
   if constexpr (!EXACT) t.columns[A_KC][1][TILE_256] = f8_entry<E, A_KC, 256, 256, 128, 64, 2, true, EPI, false>();
   t.columns[A_KC][1][TILE_128] = f8_entry<E, A_KC, 128, 128, 64, 64, 2, true, EPI, EXACT>();
   t.columns[A_KC][1][TILE_NARROW] = f8_entry<E, A_KC, 128, 32, 32, 32, 3, true, EPI, true>();
+  t.columns[A_KC][1][TILE_64] = f8_entry<E, A_KC, 128, 64, 64, 32, 3, true, EPI, EXACT>();
   if constexpr (A_KC) t.stream[A_KC] = {&launch_f8_stream<E, EPI>, 16, kStreamTokens};
 }
 template <Elem E> constexpr GroupedTable f8_table() {

@@ -62,8 +62,9 @@ struct GroupedKernel {
 enum class Epilogue : int { STORE = 0, GATED = 1, GATED_BACKWARD = 2, GATED_EXACT = 3 };
 
 // Kernels of ragged columns: three tiles of the tiled kernel, from the largest, and the kernel of few tokens to a group
-// (grouped_stream.hpp).  Ragged K: the first two, and one for matrices of fewer than eight 16-bit rows or columns.
-enum KernelClass : int { TILE_256 = 0, TILE_128 = 1, TILE_NARROW = 2, SHORT_LINES = 2, kGroupedClasses = 3, STREAM = 3 };
+// (grouped_stream.hpp).  Gated blocks and 8-bit floating point: a tile of 64 tokens as well, three stages deep.  Ragged K: the first
+// two, and one for matrices of fewer than eight 16-bit rows or columns.
+enum KernelClass : int { TILE_256 = 0, TILE_128 = 1, TILE_NARROW = 2, SHORT_LINES = 2, STREAM = 3, TILE_64 = 4, kGroupedClasses = 5 };
 
 // Ragged K: how the lists of tiles, one for each group and part of its K, are dealt to the eight XCDs.  Each list is cut
 // into 2^log2_shares shares of at most `most` tiles; one after the other goes to the XCDs in turns of eight.

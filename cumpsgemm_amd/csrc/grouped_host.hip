@@ -25,7 +25,7 @@ const GroupedKernel *lookup_grouped(Elem e, bool a_kc, bool ragged_k, bool direc
       {nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, &g_gated_f8_exact_e4m3, &g_gated_f8_exact_e5m2}};
   if (tables[(int)epi][(int)e] == nullptr) return nullptr;
   const GroupedTable &t = *tables[(int)epi][(int)e];
-  const GroupedKernel *k = ragged_k ? (cls == STREAM ? nullptr : &t.over_k[direct][cls])
+  const GroupedKernel *k = ragged_k ? (cls > SHORT_LINES ? nullptr : &t.over_k[direct][cls])
                            : cls == STREAM ? &t.stream[a_kc] : &t.columns[a_kc][direct][cls];
   return k != nullptr && k->launch != nullptr ? k : nullptr;
 }
@@ -122,14 +122,14 @@ struct Cost {
   float least;
 };
 const Cost &cost_of(Elem e, int cls) {
-  static const Cost sixteen[4] = {{4.4f, 1.38f, 2.33f, 1, 64, 0.46f}, {4.0f, 0.58f, 0.75f, 2, 64, 0.67f},
-                                  {4.4f, 0.24f, 0.39f, 2, 64, 1.00f}, {3.4f, 0.90f, 0.96f, 2, 512, 0.41f}};
-  static const Cost eight[4] = {{6.5f, 1.87f, 3.02f, 1, 128, 0.27f}, {5.4f, 0.72f, 0.94f, 2, 128, 0.41f},
-                                {4.7f, 0.24f, 0.42f, 2, 128, 0.87f}, {3.1f, 1.14f, 1.01f, 2, 1024, 0.46f}};
-  static const Cost fp32[4] = {{8.1f, 1.03f, 1.71f, 1, 32, 0.61f}, {5.9f, 0.62f, 0.91f, 1, 32, 0.62f},
-                               {6.1f, 0.45f, 0.49f, 3, 32, 1.00f}, {4.0f, 0.90f, 0.99f, 2, 256, 0.42f}};
-  static const Cost fp32x3[4] = {{11.1f, 1.93f, 2.64f, 1, 32, 0.42f}, {7.2f, 1.06f, 1.40f, 1, 32, 0.57f},
-                                 {5.8f, 0.78f, 0.61f, 2, 32, 0.88f}, {4.1f, 0.89f, 0.98f, 2, 256, 0.43f}};
+  static const Cost sixteen[5] = {{4.4f, 1.38f, 2.33f, 1, 64, 0.46f}, {4.0f, 0.58f, 0.75f, 2, 64, 0.67f},
+                                  {4.4f, 0.24f, 0.39f, 2, 64, 1.00f}, {3.4f, 0.90f, 0.96f, 2, 512, 0.41f}, {4.0f, 0.40f, 0.45f, 2, 64, 0.7f}};
+  static const Cost eight[5] = {{6.5f, 1.87f, 3.02f, 1, 128, 0.27f}, {5.4f, 0.72f, 0.94f, 2, 128, 0.41f},
+                                {4.7f, 0.24f, 0.42f, 2, 128, 0.87f}, {3.1f, 1.14f, 1.01f, 2, 1024, 0.46f}, {5.0f, 0.45f, 0.55f, 2, 128, 0.7f}};
+  static const Cost fp32[5] = {{8.1f, 1.03f, 1.71f, 1, 32, 0.61f}, {5.9f, 0.62f, 0.91f, 1, 32, 0.62f},
+                               {6.1f, 0.45f, 0.49f, 3, 32, 1.00f}, {4.0f, 0.90f, 0.99f, 2, 256, 0.42f}, {6.0f, 0.5f, 0.6f, 2, 32, 0.7f}};
+  static const Cost fp32x3[5] = {{11.1f, 1.93f, 2.64f, 1, 32, 0.42f}, {7.2f, 1.06f, 1.40f, 1, 32, 0.57f},
+                                 {5.8f, 0.78f, 0.61f, 2, 32, 0.88f}, {4.1f, 0.89f, 0.98f, 2, 256, 0.43f}, {6.5f, 0.9f, 0.9f, 2, 32, 0.7f}};
   return ((int)e >= (int)Elem::I8 ? eight : e == Elem::F32_BF16X3 ? fp32x3 : (int)e <= 3 ? fp32 : sixteen)[cls];
 }
 double cost_us(const Cost &c, double workgroups, double steps, double cus, double filled = 1.0) {
@@ -158,7 +158,7 @@ double cost_over_k_us(Elem e, int cls, double tiles, double tile_bytes, double k
 // CUMPSGEMM_FORCE_TILE_CLASS goes before the rule where there is such a kernel.
 bool forced(Elem e, bool a_kc, bool ragged_k, bool direct, int &cls, Epilogue epi = Epilogue::STORE) {
   const int want = tuning().force_cls;
-  if (want < 0 || want > STREAM || (ragged_k && want == SHORT_LINES) || lookup_grouped(e, a_kc, ragged_k, direct, want, epi) == nullptr) return false;
+  if (want < 0 || want >= kGroupedClasses || (ragged_k && want >= SHORT_LINES) || lookup_grouped(e, a_kc, ragged_k, direct, want, epi) == nullptr) return false;
   cls = want;
   return true;
 }
@@ -182,7 +182,7 @@ hipblasStatus_t run_columns(cuMpSGEMM_handle *h, Elem e, bool a_kc, GroupedArgs 
     cls = STREAM; // (a line is shorter than the chunks that the tiled kernels read)
   } else if (!forced(e, a_kc, false, direct, cls, epi)) {
     double best = 0.0;
-    for (int c = TILE_256; c <= STREAM; c++) {
+    for (int c = TILE_256; c < kGroupedClasses; c++) {
       const GroupedKernel *const kern = lookup_grouped(e, a_kc, false, direct, c, epi);
       if (kern == nullptr || most_tiles(args, *kern) > kMostWorkgroups) continue;
       // columns of tiles, the groups' sizes being unknown here: half of each group's last one, or one for each group

@@ -538,9 +538,11 @@ template <uint32_t OUT, bool EXACT>
 __device__ inline void store_gated(const GroupedArgs &args, const f4v_t gate, const f4v_t up, uint32_t row, uint32_t col) {
   constexpr int BYTES = sizeof(typename out_type<OUT>::type);
   f4v_t x;
-  float slope;
+  with_activation(args.act, [&](auto act) {
+    float slope;
 #pragma unroll
-  for (int v = 0; v < 4; v++) x[v] = activation<EXACT, false>(args.act, gate[v], slope) * up[v];
+    for (int v = 0; v < 4; v++) x[v] = activation<act.value, EXACT, false>(gate[v], slope) * up[v];
+  });
   put_four<OUT>(args.c + (uint64_t)col * args.ldc * BYTES, x, row, args.m);
   if (args.z[0] == nullptr) return;
   const uint64_t at = (uint64_t)col * args.ldz * BYTES;
@@ -554,15 +556,17 @@ __device__ inline void store_gradients(const GroupedArgs &args, const f4v_t x, c
   constexpr int BYTES = sizeof(typename out_type<OUT>::type);
   const uint64_t to = (uint64_t)col * args.ldd * BYTES;
   f4v_t h, dg, du;
+  with_activation(args.act, [&](auto act) {
 #pragma unroll
-  for (int v = 0; v < 4; v++) {
-    const float u = (float)up[v];
-    float slope;
-    const float a = activation<EXACT, true>(args.act, (float)gate[v], slope);
-    h[v] = a * u;
-    dg[v] = x[v] * u * slope;
-    du[v] = x[v] * a;
-  }
+    for (int v = 0; v < 4; v++) {
+      const float u = (float)up[v];
+      float slope;
+      const float a = activation<act.value, EXACT, true>((float)gate[v], slope);
+      h[v] = a * u;
+      dg[v] = x[v] * u * slope;
+      du[v] = x[v] * a;
+    }
+  });
   put_four<OUT>(args.d[0] + to, dg, row, args.m);
   put_four<OUT>(args.d[1] + to, du, row, args.m);
   if (args.c != nullptr) put_four<OUT>(args.c + (uint64_t)col * args.ldc * BYTES, h, row, args.m);
@@ -581,10 +585,10 @@ struct TileWork {
 };
 
 // What a tile's sums become.  sum(j, i, v): register v of lane l, MFMA row 4 (l / 16) + v (of C), column l % 16 (token) of
-// column block j and row block i.  One column block after the other passes through LDS, each wave's through a part of its
+// column block j and row block i; shift(): every column block takes the place of the one before it.  One column block after the other passes through LDS, each wave's through a part of its
 // own, so that a wave's store covers the columns' whole rows.
-template <class Cfg, int TN, class Sum>
-__device__ inline void write_tile(const GroupedArgs &args, const TileWork &w, char *lds, Sum sum) {
+template <class Cfg, int TN, class Sum, class Shift>
+__device__ inline void write_tile(const GroupedArgs &args, const TileWork &w, char *lds, Sum sum, Shift shift) {
   using T = typename Cfg::T;
   constexpr int TM = Cfg::TM, BM = Cfg::BM, PITCH = Cfg::PITCH;
   const int tid = threadIdx.x, lane = tid & 63, frow = lane & 15, fg = lane >> 4;
@@ -613,40 +617,48 @@ __device__ inline void write_tile(const GroupedArgs &args, const TileWork &w, ch
     // (a wave's own writes and reads of LDS are carried out in order)
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
   };
+  // Gated blocks: one piece of code for all column blocks, which move through the first one's registers, for the sake of the
+  // instruction cache.  (The gradient's written out for every column block and round, half a megabyte: 16384 tokens of 8 experts,
+  // 2048 x 2048 in BF16, 256 us, so BACKWARD_US.)
+  constexpr int ROUNDS = 16 / COLS;
   if constexpr (Cfg::EPI == Epilogue::GATED_BACKWARD) {
-    // G and U of a whole column block are asked for while the one before is computed.  (Asked for four rows at a time, each
-    // pair waited a memory's round trip for: 16384 tokens of 8 experts, 2048 x 2048 in BF16, 312 us, so BACKWARD_US.)
+    // G and U are asked for AHEAD rounds before they are needed.  (When they are needed, each pair waits a memory's round trip
+    // for: 312 us.)
     constexpr uint32_t OUT = T::F32 ? OUT_F32 : Cfg::E == Elem::F16 ? OUT_F16 : OUT_BF16;
-    constexpr int BYTES = sizeof(typename out_type<OUT>::type), ROUNDS = 16 / COLS;
-    typename four_of<OUT>::type z[2][ROUNDS][2];
-    auto ask = [&](const int j, const int set) {
+    constexpr int BYTES = sizeof(typename out_type<OUT>::type), AHEAD = ROUNDS < 4 ? ROUNDS : 4;
+    typename four_of<OUT>::type z[AHEAD][2];
+    auto ask = [&](const int round, typename four_of<OUT>::type(&to)[2]) { // (of all column blocks)
+      const uint32_t col = column_of(round / ROUNDS, round % ROUNDS * COLS);
+      const uint64_t from = (uint64_t)(col < w.n_end ? col : w.n_end - 1) * args.ldz * BYTES;
 #pragma unroll
-      for (int r = 0; r < ROUNDS; r++) {
-        const uint32_t col = column_of(j, r * COLS);
-        const uint64_t from = (uint64_t)(col < w.n_end ? col : w.n_end - 1) * args.ldz * BYTES;
-#pragma unroll
-        for (int side = 0; side < 2; side++) z[set][r][side] = take_four<OUT>(args.z[side] + from, row, args.m);
-      }
+      for (int side = 0; side < 2; side++) to[side] = take_four<OUT>(args.z[side] + from, row, args.m);
     };
-    ask(0, 0);
 #pragma unroll
+    for (int k = 0; k < AHEAD; k++) ask(k, z[k]);
+#pragma unroll 1
     for (int j = 0; j < TN; j++) {
-      if (j + 1 < TN) ask(j + 1, (j + 1) % 2);
-      put(j);
+      put(0);
+      shift();
+#pragma unroll 1
+      for (int r = 0; r < ROUNDS; r += AHEAD)
 #pragma unroll
-      for (int r = 0; r < ROUNDS; r++) {
-        const uint32_t col = column_of(j, r * COLS);
-        const f4v_t x = *reinterpret_cast<const f4v_t *>(mine + (r * COLS + lane / LANES) * PITCH + lane % LANES * 4);
-        if (col < w.n_end) store_gradients<OUT, T::F32>(args, x, z[j % 2][r][0], z[j % 2][r][1], row, col);
-      }
+        for (int k = 0; k < AHEAD; k++) {
+          const int round = j * ROUNDS + r + k;
+          const uint32_t col = column_of(j, (r + k) * COLS);
+          const f4v_t x = *reinterpret_cast<const f4v_t *>(mine + ((r + k) * COLS + lane / LANES) * PITCH + lane % LANES * 4);
+          const typename four_of<OUT>::type gate = z[k][0], up = z[k][1];
+          if (round + AHEAD < TN * ROUNDS) ask(round + AHEAD, z[k]);
+          if (col < w.n_end) store_gradients<OUT, T::F32>(args, x, gate, up, row, col);
+        }
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
     }
     return;
   }
-#pragma unroll
-  for (int j = 0; j < TN; j++) {
-    put(j);
-    if constexpr (Cfg::GATED) {
+  if constexpr (Cfg::GATED) {
+#pragma unroll 1
+    for (int j = 0; j < TN; j++) {
+      put(0);
+      shift();
 #pragma unroll 1
       for (int r = 0; r < 16; r += COLS) {
         const uint32_t col = column_of(j, r);
@@ -655,7 +667,14 @@ __device__ inline void write_tile(const GroupedArgs &args, const TileWork &w, ch
         const f4v_t x = *reinterpret_cast<const f4v_t *>(p), y = *reinterpret_cast<const f4v_t *>(p + 16);
         if (col < w.n_end) typed([&](auto out) { store_gated<out.value, T::F32>(args, x, y, row, col); });
       }
-    } else {
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < TN; j++) {
+    put(j);
+    {
       f4v_t sa = {args.alpha, args.alpha, args.alpha, args.alpha};
       if constexpr (T::I8) {
 #pragma unroll
@@ -1006,11 +1025,21 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
   }
 
   // ---- results ----
-  write_tile<Cfg, TN>(args, w, lds, [&](const int j, const int i, const int v) {
-    float x = (float)acc[0][j][i][v];
-    if constexpr (T::NACC == 2) x += acc[1][j][i][v] * prec_traits<T::P>::CORR_SCALE;
-    return x;
-  });
+  write_tile<Cfg, TN>(
+      args, w, lds,
+      [&](const int j, const int i, const int v) {
+        float x = (float)acc[0][j][i][v];
+        if constexpr (T::NACC == 2) x += acc[1][j][i][v] * prec_traits<T::P>::CORR_SCALE;
+        return x;
+      },
+      [&]() {
+#pragma unroll
+        for (int s = 0; s < T::NACC; s++)
+#pragma unroll
+          for (int j = 0; j + 1 < TN; j++)
+#pragma unroll
+            for (int i = 0; i < TM; i++) acc[s][j][i] = acc[s][j + 1][i];
+      });
 }
 
 template <class Cfg>

@@ -330,10 +330,11 @@ __global__ __launch_bounds__(kStreamWaves * 64) void grouped_stream_kernel(const
     float y = x[0][at];
     if constexpr (EPI == Epilogue::GATED) {
       const float up = x[SIDES - 1][at];
-      float slope;
+      float slope, a = 0.0f;
+      with_activation(args.act, [&](auto act) { a = activation<act.value, T::F32, false>(y, slope); });
       typed([&](auto o) {
         typedef decltype(o) O;
-        reinterpret_cast<O *>(args.c)[c_at] = (O)(activation<T::F32, false>(args.act, y, slope) * up);
+        reinterpret_cast<O *>(args.c)[c_at] = (O)(a * up);
         if (args.z[0] == nullptr) return;
         reinterpret_cast<O *>(args.z[0])[z_at] = (O)y;
         reinterpret_cast<O *>(args.z[1])[z_at] = (O)up;
@@ -343,8 +344,8 @@ __global__ __launch_bounds__(kStreamWaves * 64) void grouped_stream_kernel(const
         typedef decltype(o) O;
         const float gate = (float)reinterpret_cast<const O *>(args.z[0])[z_at], up = (float)reinterpret_cast<const O *>(args.z[1])[z_at];
         const uint64_t d_at = (uint64_t)col * args.ldd + row;
-        float slope;
-        const float a = activation<T::F32, true>(args.act, gate, slope);
+        float slope = 0.0f, a = 0.0f;
+        with_activation(args.act, [&](auto act) { a = activation<act.value, T::F32, true>(gate, slope); });
         reinterpret_cast<O *>(args.d[0])[d_at] = (O)(y * up * slope);
         reinterpret_cast<O *>(args.d[1])[d_at] = (O)(y * a);
         if (args.c != nullptr) reinterpret_cast<O *>(args.c)[c_at] = (O)(a * up);

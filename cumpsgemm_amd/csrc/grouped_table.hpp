@@ -7,7 +7,7 @@ namespace cumpsgemm_amd {
 
 struct GroupedTable {
   // [A K-contiguous][through registers, direct][tile]; B K-contiguous
-  GroupedKernel columns[2][2][kGroupedClasses];
+  GroupedKernel columns[2][2][kGroupedClasses]; // (not STREAM)
   GroupedKernel over_k[2][kGroupedClasses]; // ragged K, both row-contiguous
   GroupedKernel stream[2];                  // few tokens; [A K-contiguous]
 };
@@ -72,12 +72,14 @@ template <Elem E, Epilogue EPI, bool A_KC> constexpr void gated_entries(GroupedT
     t.columns[A_KC][1][TILE_256] = grouped_of<E, A_KC, true, 256, 128, 64, 64, 64, 2, true, false, false, EPI>();
     t.columns[A_KC][1][TILE_128] = grouped_of<E, A_KC, true, 128, 128, 64, 32, 64, 2, true, false, false, EPI>();
     t.columns[A_KC][1][TILE_NARROW] = grouped_of<E, A_KC, true, 128, 32, 32, 32, 64, 2, true, false, false, EPI>();
+    t.columns[A_KC][1][TILE_64] = grouped_of<E, A_KC, true, 128, 64, 64, 32, 64, 2, true, false, false, EPI>();
   } else {
     t.columns[A_KC][0][TILE_128] = grouped_of<E, A_KC, true, 128, 128, 64, 64, 128, 2, false, false, false, EPI>();
     t.columns[A_KC][0][TILE_NARROW] = grouped_of<E, A_KC, true, 128, 32, 32, 32, 128, 2, false, false, false, EPI>();
     t.columns[A_KC][1][TILE_256] = grouped_of<E, A_KC, true, 256, 256, 128, 64, 128, 2, true, false, false, EPI>();
     t.columns[A_KC][1][TILE_128] = grouped_of<E, A_KC, true, 128, 128, 64, 64, 128, 2, true, false, false, EPI>();
     t.columns[A_KC][1][TILE_NARROW] = grouped_of<E, A_KC, true, 128, 32, 32, 32, 128, 4, true, false, false, EPI>();
+    t.columns[A_KC][1][TILE_64] = grouped_of<E, A_KC, true, 128, 64, 64, 32, 128, 3, true, false, false, EPI>();
   }
   t.stream[A_KC] = stream_entry<E, A_KC, EPI>();
 }

@@ -59,13 +59,16 @@ template <bool E5M2> struct BlockScale {
   float scale, times, peak, inverse;
   __device__ inline BlockScale(uint32_t most) {
     const bool finite = most < 0x7f800000u;
-    scale = finite ? __uint_as_float(most) / M : __uint_as_float(0x7fc00000u);
-    const uint32_t e = most >> 23 > 20 ? most >> 23 : 20; // (2^109 at most, times 57344)
-    const float up = __uint_as_float((256 - e) << 23);    // peak: 4 .. 8, or less if the maximum is below 2^-107
+    const uint32_t e = most >> 23 > 20 ? (most >> 23 < 254 ? most >> 23 : 254) : 20;
+    const float up = __uint_as_float((256 - e) << 23), down = __uint_as_float((e - 2) << 23); // 2^(129 - e) at most 2^109, and its inverse
+    const float big = __uint_as_float(most) * up; // 4 .. 8, or less if the maximum is below 2^-107
+    // big / M: a multiplication and the remainder, as above
+    const float s = big * (1.0f / M);
+    scale = finite ? fmaf(fmaf(-s, M, big), 1.0f / M, s) * down : __uint_as_float(0x7fc00000u);
     const bool some = finite && scale != 0.0f;
     times = some ? up * M : 0.0f;
-    peak = some ? __uint_as_float(most) * up : 1.0f;
-    inverse = 1.0f / peak;
+    peak = some ? big : 1.0f;
+    inverse = __builtin_amdgcn_rcpf(peak);
   }
   __device__ inline float operator()(float x) const {
     const float y = x * times, q = y * inverse;
@@ -99,12 +102,14 @@ __device__ inline void store_eight(uint8_t *q, uint32_t at, uint32_t k, const Ei
   }
 }
 
-// Tokens.  BIG: more units than 32 bits count.
-template <class T, bool E5M2, bool ALIGNED, bool BIG> __global__ __launch_bounds__(kThreads) void quantize_f8_kernel(const QuantizeF8Args args) {
+// Tokens.  BIG: more units than 32 bits count.  AT_ONCE: the blocks of sixteen lanes, read together.
+template <class T, bool E5M2, bool ALIGNED, bool BIG, int AT_ONCE>
+__global__ __launch_bounds__(kThreads) void quantize_f8_kernel(const QuantizeF8Args args) {
   const uint32_t lane = threadIdx.x % kLanes;
-  const uint64_t step = (uint64_t)gridDim.x * (kThreads / kLanes);
-  for (uint64_t unit = (uint64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes; unit < args.units; unit += step) {
-    uint64_t column;
+  constexpr int GROUPS = kThreads / kLanes;
+  const uint64_t step = (uint64_t)gridDim.x * (GROUPS * AT_ONCE);
+  // where a unit lies: its matrix and column, its first value
+  auto place = [&](uint64_t unit, uint64_t &matrix, uint64_t &column, uint32_t &at) {
     uint32_t b;
     if constexpr (BIG) {
       column = unit / args.kb;
@@ -114,22 +119,40 @@ template <class T, bool E5M2, bool ALIGNED, bool BIG> __global__ __launch_bounds
       column = c;
       b = (uint32_t)unit - c * args.kb;
     }
-    uint64_t matrix = 0;
+    matrix = 0;
     if (args.units != (uint64_t)args.kb * args.n) { // (several matrices)
       matrix = column / args.n;
       column -= matrix * args.n;
     }
-    const uint32_t at = b * kBlock + lane * kVec;
-    const Eight<T> x = load_eight<T, ALIGNED>(reinterpret_cast<const T *>(args.x) + matrix * args.stride_x + column * args.ldx, at, args.k);
-    uint32_t most = most_of(x, 0);
+    at = b * kBlock + lane * kVec;
+  };
+  for (uint64_t first = (uint64_t)blockIdx.x * (GROUPS * AT_ONCE) + threadIdx.x / kLanes; first < args.units; first += step) {
+    Eight<T> x[AT_ONCE];
 #pragma unroll
-    for (int d = kLanes / 2; d > 0; d >>= 1) {
-      const uint32_t o = __shfl_xor(most, d, kLanes);
-      most = most > o ? most : o;
+    for (int i = 0; i < AT_ONCE; i++) { // (one beyond the last: that again, not stored)
+      uint64_t matrix, column;
+      uint32_t at;
+      const uint64_t unit = first + i * GROUPS;
+      place(unit < args.units ? unit : args.units - 1, matrix, column, at);
+      x[i] = load_eight<T, ALIGNED>(reinterpret_cast<const T *>(args.x) + matrix * args.stride_x + column * args.ldx, at, args.k);
     }
-    const BlockScale<E5M2> s(most);
-    if (lane == 0) args.scale[unit] = s.scale;
-    store_eight<E5M2, T, ALIGNED>(args.q + matrix * args.stride_q + column * args.ldq, at, args.k, x, s, most < 0x7f800000u);
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; i++) {
+      uint32_t most = most_of(x[i], 0);
+#pragma unroll
+      for (int d = kLanes / 2; d > 0; d >>= 1) {
+        const uint32_t o = __shfl_xor(most, d, kLanes);
+        most = most > o ? most : o;
+      }
+      const uint64_t unit = first + i * GROUPS;
+      if (unit >= args.units) continue; // (the sixteen lanes together)
+      uint64_t matrix, column;
+      uint32_t at;
+      place(unit, matrix, column, at);
+      const BlockScale<E5M2> s(most);
+      if (lane == 0) args.scale[unit] = s.scale;
+      store_eight<E5M2, T, ALIGNED>(args.q + matrix * args.stride_q + column * args.ldq, at, args.k, x[i], s, most < 0x7f800000u);
+    }
   }
 }
 
@@ -172,25 +195,31 @@ template <class T, bool E5M2, bool ALIGNED> __global__ __launch_bounds__(kThread
 
 constexpr uint64_t kMostWorkgroups = 1u << 20; // (a launch has fewer than 2^32 threads; more blocks in turns)
 
-template <class T, bool E5M2, bool ALIGNED> void launch_quantize_f8(const QuantizeF8Args &args, bool matrices, hipStream_t stream) {
+template <class T, bool E5M2, bool ALIGNED> void launch_quantize_f8(const QuantizeF8Args &args, bool matrices, int cus, hipStream_t stream) {
   if (matrices) {
     hipLaunchKernelGGL((quantize_f8_matrix_kernel<T, E5M2, ALIGNED>), dim3((uint32_t)std::min(args.units, kMostWorkgroups)), dim3(kThreads), 0,
                        stream, args);
     return;
   }
-  const uint32_t workgroups = (uint32_t)std::min((args.units + kThreads / kLanes - 1) / (kThreads / kLanes), kMostWorkgroups);
-  if (args.units >> 32) hipLaunchKernelGGL((quantize_f8_kernel<T, E5M2, ALIGNED, true>), dim3(workgroups), dim3(kThreads), 0, stream, args);
-  else hipLaunchKernelGGL((quantize_f8_kernel<T, E5M2, ALIGNED, false>), dim3(workgroups), dim3(kThreads), 0, stream, args);
+  // Four blocks at once keep enough loads under way where there is a workgroup of them for every CU.
+  constexpr uint64_t GROUPS = kThreads / kLanes;
+  auto launch = [&](auto kernel, uint64_t each) {
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)std::min((args.units + GROUPS * each - 1) / (GROUPS * each), kMostWorkgroups)), dim3(kThreads), 0,
+                       stream, args);
+  };
+  if (args.units >> 32) launch(quantize_f8_kernel<T, E5M2, ALIGNED, true, 4>, 4);
+  else if (args.units >= 4 * GROUPS * 4 * (uint64_t)cus) launch(quantize_f8_kernel<T, E5M2, ALIGNED, false, 4>, 4);
+  else launch(quantize_f8_kernel<T, E5M2, ALIGNED, false, 1>, 1);
 }
-template <class T> void launch_quantize_f8(const QuantizeF8Args &args, bool matrices, bool e5m2, hipStream_t stream) {
+template <class T> void launch_quantize_f8(const QuantizeF8Args &args, bool matrices, bool e5m2, int cus, hipStream_t stream) {
   const bool aligned = args.k % kVec == 0 && args.ldx * sizeof(T) % 16 == 0 && args.stride_x * sizeof(T) % 16 == 0 && args.ldq % kVec == 0 &&
                        args.stride_q % kVec == 0 && (uintptr_t)args.x % 16 == 0 && (uintptr_t)args.q % kVec == 0;
   if (e5m2) {
-    if (aligned) launch_quantize_f8<T, true, true>(args, matrices, stream);
-    else launch_quantize_f8<T, true, false>(args, matrices, stream);
+    if (aligned) launch_quantize_f8<T, true, true>(args, matrices, cus, stream);
+    else launch_quantize_f8<T, true, false>(args, matrices, cus, stream);
   } else {
-    if (aligned) launch_quantize_f8<T, false, true>(args, matrices, stream);
-    else launch_quantize_f8<T, false, false>(args, matrices, stream);
+    if (aligned) launch_quantize_f8<T, false, true>(args, matrices, cus, stream);
+    else launch_quantize_f8<T, false, false>(args, matrices, cus, stream);
   }
 }
 } // namespace
@@ -213,8 +242,8 @@ extern "C" hipblasStatus_t cuMpSGEMM_quantize_f8(cuMpSGEMM_handle_t h, uint64_t 
   args.units = (uint64_t)args.kb * args.nb * batch_count;
   ProfileScope prof(h, "quantize_f8");
   const bool matrices = block_n != 1, e5m2 = type_q == HIP_R_8F_E5M2;
-  if (type_x == HIP_R_32F) launch_quantize_f8<float>(args, matrices, e5m2, h->stream);
-  else if (type_x == HIP_R_16F) launch_quantize_f8<_Float16>(args, matrices, e5m2, h->stream);
-  else launch_quantize_f8<__bf16>(args, matrices, e5m2, h->stream);
+  if (type_x == HIP_R_32F) launch_quantize_f8<float>(args, matrices, e5m2, h->num_cus, h->stream);
+  else if (type_x == HIP_R_16F) launch_quantize_f8<_Float16>(args, matrices, e5m2, h->num_cus, h->stream);
+  else launch_quantize_f8<__bf16>(args, matrices, e5m2, h->num_cus, h->stream);
   return hipGetLastError() == hipSuccess ? HIPBLAS_STATUS_SUCCESS : HIPBLAS_STATUS_EXECUTION_FAILED;
 }
