@@ -120,20 +120,71 @@ struct Cost {
   float fixed, alone, each;
   int slots, step; // workgroups to a CU; K-values of a step (the kernel of few tokens: of its eight waves)
   float least;
+  float tail; // a tile's first loads and write-out, in steps (0: in the others)
 };
 const Cost &cost_of(Elem e, int cls) {
-  static const Cost sixteen[5] = {{4.4f, 1.38f, 2.33f, 1, 64, 0.46f}, {4.0f, 0.58f, 0.75f, 2, 64, 0.67f},
-                                  {4.4f, 0.24f, 0.39f, 2, 64, 1.00f}, {3.4f, 0.90f, 0.96f, 2, 512, 0.41f}, {4.0f, 0.40f, 0.45f, 2, 64, 0.7f}};
-  static const Cost eight[5] = {{6.5f, 1.87f, 3.02f, 1, 128, 0.27f}, {5.4f, 0.72f, 0.94f, 2, 128, 0.41f},
-                                {4.7f, 0.24f, 0.42f, 2, 128, 0.87f}, {3.1f, 1.14f, 1.01f, 2, 1024, 0.46f}, {5.0f, 0.45f, 0.55f, 2, 128, 0.7f}};
-  static const Cost fp32[5] = {{8.1f, 1.03f, 1.71f, 1, 32, 0.61f}, {5.9f, 0.62f, 0.91f, 1, 32, 0.62f},
-                               {6.1f, 0.45f, 0.49f, 3, 32, 1.00f}, {4.0f, 0.90f, 0.99f, 2, 256, 0.42f}, {6.0f, 0.5f, 0.6f, 2, 32, 0.7f}};
-  static const Cost fp32x3[5] = {{11.1f, 1.93f, 2.64f, 1, 32, 0.42f}, {7.2f, 1.06f, 1.40f, 1, 32, 0.57f},
-                                 {5.8f, 0.78f, 0.61f, 2, 32, 0.88f}, {4.1f, 0.89f, 0.98f, 2, 256, 0.43f}, {6.5f, 0.9f, 0.9f, 2, 32, 0.7f}};
-  return ((int)e >= (int)Elem::I8 ? eight : e == Elem::F32_BF16X3 ? fp32x3 : (int)e <= 3 ? fp32 : sixteen)[cls];
+  static const Cost sixteen[4] = {{4.4f, 1.38f, 2.33f, 1, 64, 0.46f}, {4.0f, 0.58f, 0.75f, 2, 64, 0.67f},
+                                  {4.4f, 0.24f, 0.39f, 2, 64, 1.00f}, {3.4f, 0.90f, 0.96f, 2, 512, 0.41f}};
+  static const Cost eight[4] = {{6.5f, 1.87f, 3.02f, 1, 128, 0.27f}, {5.4f, 0.72f, 0.94f, 2, 128, 0.41f},
+                                {4.7f, 0.24f, 0.42f, 2, 128, 0.87f}, {3.1f, 1.14f, 1.01f, 2, 1024, 0.46f}};
+  static const Cost fp32[4] = {{8.1f, 1.03f, 1.71f, 1, 32, 0.61f}, {5.9f, 0.62f, 0.91f, 1, 32, 0.62f},
+                               {6.1f, 0.45f, 0.49f, 3, 32, 1.00f}, {4.0f, 0.90f, 0.99f, 2, 256, 0.42f}};
+  static const Cost fp32x3[4] = {{11.1f, 1.93f, 2.64f, 1, 32, 0.42f}, {7.2f, 1.06f, 1.40f, 1, 32, 0.57f},
+                                 {5.8f, 0.78f, 0.61f, 2, 32, 0.88f}, {4.1f, 0.89f, 0.98f, 2, 256, 0.43f}};
+  return (e == Elem::I8 ? eight : e == Elem::F32_BF16X3 ? fp32x3 : (int)e <= 3 ? fp32 : sixteen)[cls];
+}
+// Gated blocks, their gradients and 8-bit floating point, in the same terms, with what their larger epilogues cost, and apart for
+// operands that go straight to LDS and for others (_any): fitted to 200 calls of each kind (and 100 of any alignment; sizes as
+// above, m to 4096, k to 4096 in FP8 and 2048 else, 1 - 16384 tokens) with every kernel in turn.  On 100 other calls each the choice
+// loses 3.4 % (gated, 16 bits), 3.5 (gradient), 4.1 and 3.3 (gated FP32: FP16TCEC, TF32TCEC), 1.9 and 1.9 (gradients), 5.9 (FP8), 4.1
+// and 2.7 (gated FP8, exact sums), of any alignment 1.5, 3.0, 4.6 (FP8) and 2.2 (gated FP8) against the best kernel for each; by the
+// figures of the plain products 24 % for gated blocks of any alignment, 5 - 10 % for the others.
+const Cost &gated_cost_of(Elem e, int cls, Epilogue epi, bool direct) {
+  static const Cost gated16[5] = {{2.4f, 1.45f, 2.05f, 1, 64, 0.38f, 5.5f}, {5.7f, 0.52f, 0.71f, 2, 64, 0.51f, 2.1f},
+                                  {6.3f, 0.14f, 0.29f, 2, 64, 0.95f, 2.8f}, {5.7f, 1.18f, 0.82f, 2, 512, 0.82f, 0.4f},
+                                  {6.0f, 0.25f, 0.41f, 2, 64, 0.79f, 2.4f}};
+  static const Cost backward16[5] = {{0.6f, 1.60f, 1.96f, 1, 64, 0.25f, 19.8f}, {6.1f, 0.66f, 0.67f, 2, 64, 0.26f, 12.0f},
+                                     {7.6f, 0.17f, 0.27f, 2, 64, 0.72f, 5.9f}, {7.6f, 0.90f, 0.33f, 2, 512, 0.61f, 0.8f},
+                                     {7.3f, 0.33f, 0.41f, 2, 64, 0.45f, 7.3f}};
+  static const Cost gated16_any[5] = {{}, {6.2f, 0.86f, 1.02f, 2, 64, 0.47f, 2.2f}, {5.4f, 0.47f, 0.55f, 2, 64, 0.93f, 2.2f},
+                                      {3.5f, 6.33f, 2.82f, 2, 512, 0.83f, 0.2f}, {}};
+  static const Cost backward16_any[5] = {{}, {5.8f, 1.03f, 1.03f, 2, 64, 0.27f, 11.2f}, {6.7f, 0.40f, 0.47f, 2, 64, 0.72f, 4.4f},
+                                         {7.3f, 1.62f, 1.37f, 2, 512, 0.74f, 0.1f}, {}};
+  static const Cost gated32[5] = {{1.3f, 1.18f, 1.61f, 1, 32, 0.55f, 6.7f}, {3.3f, 0.63f, 0.84f, 1, 32, 0.65f, 6.5f},
+                                  {5.4f, 0.43f, 0.46f, 2, 32, 0.95f, 1.4f}, {6.3f, 0.96f, 1.17f, 2, 256, 0.74f, 0.2f},
+                                  {5.8f, 0.43f, 0.57f, 2, 32, 0.84f, 2.2f}};
+  static const Cost gated32x3[5] = {{2.1f, 2.23f, 2.63f, 1, 32, 0.44f, 3.3f}, {3.9f, 1.12f, 1.46f, 1, 32, 0.63f, 2.7f},
+                                    {5.3f, 0.67f, 0.62f, 2, 32, 0.90f, 0.8f}, {6.2f, 0.92f, 1.13f, 2, 256, 0.77f, 0.5f},
+                                    {6.1f, 0.76f, 0.83f, 2, 32, 0.70f, 0.9f}};
+  static const Cost backward32[5] = {{0.4f, 1.52f, 1.98f, 1, 32, 0.49f, 9.7f}, {0.8f, 0.84f, 1.03f, 1, 32, 0.60f, 11.5f},
+                                     {5.5f, 0.66f, 0.62f, 2, 32, 0.78f, 2.1f}, {7.7f, 0.58f, 0.46f, 2, 256, 0.71f, 0.4f},
+                                     {3.7f, 0.73f, 0.68f, 2, 32, 0.67f, 7.1f}};
+  static const Cost backward32x3[5] = {{0.5f, 2.37f, 2.92f, 1, 32, 0.42f, 7.5f}, {1.0f, 1.27f, 1.47f, 1, 32, 0.58f, 8.2f},
+                                       {4.2f, 0.90f, 0.67f, 2, 32, 0.77f, 4.1f}, {6.1f, 1.05f, 0.48f, 2, 256, 0.83f, 0.9f},
+                                       {5.0f, 0.97f, 0.87f, 2, 32, 0.65f, 5.0f}};
+  static const Cost f8[5] = {{1.5f, 1.51f, 1.90f, 1, 128, 0.39f, 6.9f}, {4.8f, 0.74f, 0.74f, 2, 128, 0.45f, 2.6f},
+                             {4.3f, 0.51f, 0.44f, 2, 128, 0.74f, 2.8f}, {5.1f, 1.80f, 0.59f, 2, 1024, 0.74f, 0.4f},
+                             {5.0f, 0.46f, 0.46f, 2, 128, 0.62f, 2.9f}};
+  static const Cost f8_any[5] = {{}, {3.0f, 1.92f, 1.31f, 2, 128, 0.50f, 3.3f}, {3.2f, 1.32f, 0.88f, 2, 128, 0.82f, 1.8f},
+                                 {2.6f, 7.52f, 2.24f, 2, 1024, 0.78f, 0.1f}, {}};
+  static const Cost gated_f8[5] = {{3.7f, 1.41f, 1.81f, 1, 128, 0.34f, 6.2f}, {6.6f, 0.54f, 0.72f, 2, 128, 0.43f, 2.0f},
+                                   {5.9f, 0.32f, 0.39f, 2, 128, 0.80f, 2.9f}, {6.3f, 1.11f, 0.99f, 2, 1024, 0.75f, 0.9f},
+                                   {6.3f, 0.32f, 0.42f, 2, 128, 0.69f, 2.7f}};
+  static const Cost gated_f8_exact[5] = {{}, {5.9f, 1.15f, 1.05f, 2, 128, 0.34f, 1.8f}, {5.9f, 0.37f, 0.41f, 2, 128, 0.72f, 2.6f},
+                                         {5.9f, 1.88f, 1.11f, 2, 1024, 0.67f, 0.6f}, {5.8f, 0.60f, 0.61f, 2, 128, 0.60f, 2.1f}};
+  static const Cost gated_f8_any[5] = {{}, {5.1f, 1.95f, 1.37f, 2, 128, 0.50f, 1.9f}, {4.5f, 1.12f, 0.75f, 2, 128, 0.87f, 2.1f},
+                                       {5.5f, 3.26f, 2.28f, 2, 1024, 0.69f, 0.9f}, {}};
+  if (e == Elem::E4M3 || e == Elem::E5M2) {
+    if (epi == Epilogue::STORE) return (direct ? f8 : f8_any)[cls];
+    return (!direct ? gated_f8_any : epi == Epilogue::GATED ? gated_f8 : gated_f8_exact)[cls];
+  }
+  const bool forward = epi == Epilogue::GATED;
+  if (e == Elem::F32_BF16X3) return (forward ? gated32x3 : backward32x3)[cls];
+  if ((int)e <= 3) return (forward ? gated32 : backward32)[cls];
+  return (forward ? direct ? gated16 : gated16_any : direct ? backward16 : backward16_any)[cls];
 }
 double cost_us(const Cost &c, double workgroups, double steps, double cus, double filled = 1.0) {
-  return c.fixed + steps * (c.least + (1.0 - c.least) * filled) * std::max<double>(c.alone, c.each * (workgroups / cus + (workgroups > cus * c.slots ? 0.2 * c.slots : 0.0)));
+  return c.fixed + (steps + c.tail) * (c.least + (1.0 - c.least) * filled) * std::max<double>(c.alone, c.each * (workgroups / cus + (workgroups > cus * c.slots ? 0.2 * c.slots : 0.0)));
 }
 // For products over K (342 calls, 1 - 64 groups of 16 - 16384 tokens, results of 256^2 - 4096 x 2048, K in 1 - 16 parts, both
 // tiles; BF16, FP16TCEC and TF32TCEC, aligned), whose groups often have a few steps only: every round of tiles also costs
@@ -189,7 +240,8 @@ hipblasStatus_t run_columns(cuMpSGEMM_handle *h, Elem e, bool a_kc, GroupedArgs 
       const double some = std::min(args.n, args.groups), each = (double)args.n / args.groups;
       const double columns = args.groups == 1 ? (args.n + kern->bn - 1) / kern->bn
                              : each < kern->bn / 2 ? some : (double)args.n / kern->bn + 0.5 * some;
-      const Cost &cost = cost_of(e, c);
+      const bool plain = epi == Epilogue::STORE && e != Elem::E4M3 && e != Elem::E5M2;
+      const Cost &cost = plain ? cost_of(e, c) : gated_cost_of(e, c, epi, direct);
       // (the kernel of few tokens: in workgroups of 16 rows, as fitted with op T; where rows are contiguous it has 64 in one,
       // and this is too high)
       const double rows = c == STREAM ? (args.m + 15) / 16 : (args.m + kern->bm - 1) / kern->bm;
