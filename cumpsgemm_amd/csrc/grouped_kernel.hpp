@@ -499,17 +499,20 @@ __device__ inline void store_four(char *c, const f4v_t x, float beta, uint32_t r
 }
 
 // Four rows of a column at any alignment: one access, unless the matrix ends among them.  (Value by value, at sizes that are not
-// multiples of four: 1001 tokens of 5 experts, 515 x 389 in FP16, the gradient ODD_US.)
+// multiples of four: 1001 tokens of 5 experts, 515 x 389 in FP16, the
+// gradient 38 us, so 12.6.)
 template <uint32_t OUT> struct four_of {
   typedef typename out_type<OUT>::type O;
   typedef O type __attribute__((ext_vector_type(4)));
   typedef O anywhere __attribute__((ext_vector_type(4), aligned(sizeof(O))));
 };
-template <uint32_t OUT> __device__ inline void put_four(char *column, const f4v_t x, uint32_t row, uint32_t m) {
+// LATER: values that no kernel soon reads, past the caches.
+template <uint32_t OUT, bool LATER = false> __device__ inline void put_four(char *column, const f4v_t x, uint32_t row, uint32_t m) {
   auto *p = reinterpret_cast<typename out_type<OUT>::type *>(column) + row;
   const typename four_of<OUT>::type y = __builtin_convertvector(x, typename four_of<OUT>::type);
   if (row + 4 <= m) {
-    *reinterpret_cast<typename four_of<OUT>::anywhere *>(p) = y;
+    if constexpr (LATER) __builtin_nontemporal_store(y, reinterpret_cast<typename four_of<OUT>::anywhere *>(p));
+    else *reinterpret_cast<typename four_of<OUT>::anywhere *>(p) = y;
   } else {
 #pragma unroll
     for (int v = 0; v < 3; v++)
@@ -521,7 +524,8 @@ template <uint32_t OUT> __device__ inline typename four_of<OUT>::type take_four(
   const auto *p = reinterpret_cast<const typename out_type<OUT>::type *>(column);
   if (m >= 4) { // the last four in place of those that stick out, moved to their places
     const uint32_t at = row + 4 <= m ? row : m - 4;
-    typename four_of<OUT>::type x = *reinterpret_cast<const typename four_of<OUT>::anywhere *>(p + at);
+    // (read once here: past the caches, 2 - 4 % in the figure below)
+    typename four_of<OUT>::type x = __builtin_nontemporal_load(reinterpret_cast<const typename four_of<OUT>::anywhere *>(p + at));
     if (at != row) {
       const uint32_t by = row - at;
       x = by == 1 ? __builtin_shufflevector(x, x, 1, 2, 3, 3) : by == 2 ? __builtin_shufflevector(x, x, 2, 3, 3, 3) : __builtin_shufflevector(x, x, 3, 3, 3, 3);
@@ -546,8 +550,10 @@ __device__ inline void store_gated(const GroupedArgs &args, const f4v_t gate, co
   put_four<OUT>(args.c + (uint64_t)col * args.ldc * BYTES, x, row, args.m);
   if (args.z[0] == nullptr) return;
   const uint64_t at = (uint64_t)col * args.ldz * BYTES;
-  put_four<OUT>(args.z[0] + at, gate, row, args.m);
-  put_four<OUT>(args.z[1] + at, up, row, args.m);
+  // (the projections are for the gradient, much later: 16384 tokens of 8 experts, 2048 x 2048 in BF16, 300 us, so 284; the result
+  // as well: level here, and the product behind it 5 % slower where the caches hold it)
+  put_four<OUT, true>(args.z[0] + at, gate, row, args.m);
+  put_four<OUT, true>(args.z[1] + at, up, row, args.m);
 }
 // ... of its gradient: x is that of act(G) * U.  (G and U were read before anything is written: dG and dU may take their place.)
 template <uint32_t OUT, bool EXACT>
@@ -619,7 +625,7 @@ __device__ inline void write_tile(const GroupedArgs &args, const TileWork &w, ch
   };
   // Gated blocks: one piece of code for all column blocks, which move through the first one's registers, for the sake of the
   // instruction cache.  (The gradient's written out for every column block and round, half a megabyte: 16384 tokens of 8 experts,
-  // 2048 x 2048 in BF16, 256 us, so BACKWARD_US.)
+  // 2048 x 2048 in BF16, 256 us, so 213.)
   constexpr int ROUNDS = 16 / COLS;
   if constexpr (Cfg::EPI == Epilogue::GATED_BACKWARD) {
     // G and U are asked for AHEAD rounds before they are needed.  (When they are needed, each pair waits a memory's round trip
