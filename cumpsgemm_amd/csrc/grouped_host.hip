@@ -225,7 +225,7 @@ uint64_t most_tiles(const GroupedArgs &args, const GroupedKernel &k) {
 hipblasStatus_t run_columns(cuMpSGEMM_handle *h, Elem e, bool a_kc, GroupedArgs &args, const char *label,
                             Epilogue epi = Epilogue::STORE) {
   const uint32_t bytes = bytes_of(e);
-  const bool direct = chunks_ok(args.a, a_kc ? args.k : args.m, args.lda, args.stride_a, bytes, a_kc ? 256 : 64) &&
+  const bool direct = chunks_ok(args.a, a_kc ? args.k : args.m, args.lda, args.stride_a, bytes, a_kc ? 256 : bytes == 1 ? 128 : 64) &&
                       chunks_ok(args.b, args.k, args.ldb, 0, bytes, 256) &&
                       ((epi != Epilogue::GATED && epi != Epilogue::GATED_EXACT) || chunks_ok(args.up, 16, args.lda, args.stride_a, bytes, 0));
   int cls = TILE_128;

@@ -89,7 +89,8 @@ const void *cuMpSGEMM_get_workspace_pointer(cuMpSGEMM_handle_t handle);
  * _PERSISTENT_MAX_STEPS, _MAX_WORKSPACE_BYTES) are read from the environment
  * once per process (the products of experts' layers below look at
  * _FORCE_TILE_CLASS, 0 - 3: tiles of 256 and 128 rows, of 32 tokens, the kernel
- * of few tokens, and over K at _FORCE_KSPLIT); this reads them again and publishes the new set as one
+ * of few tokens, 4 in gated blocks and 8-bit floating point: of 64 tokens, and over
+ * K at _FORCE_KSPLIT); this reads them again and publishes the new set as one
  * immutable snapshot.  Safe to call while other threads run GEMMs: a call in
  * flight goes on with the values it has already looked up and may take later
  * ones from the new set.  For tests and experiments.  The reference has no

@@ -201,3 +201,40 @@ def test_offsets_past_32_bits(cg, handle):
     assert handle.gemm_f8(cg.OP_T, m, n, k, wq, k, m * k, cg.R_8F_E4M3, ws, 1, q, 2 * ld, cg.R_8F_E4M3, s, yv[0], ld, cg.R_16BF, off, 2) == 0
     # (E4M3's roundings, 2^-4 of each value at most, are independent over 128 products)
     assert float((yv[0][rows].double() - g).norm() / g.norm()) <= 0.08
+
+
+@pytest.mark.parametrize("op", ["T", "N"])
+@pytest.mark.parametrize("cls", ["1", "3"])
+def test_leading_dimensions_beyond_32_bits_of_a_tile(cg, handle, op, cls, monkeypatch):
+    """FP32 and FP8 matrices whose tiles span more bytes than the kernels' 32-bit offsets reach."""
+    monkeypatch.setenv("CUMPSGEMM_FORCE_TILE_CLASS", cls)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    m, k, n = (40, 48, 20) if op == "T" else (48, 40, 20)
+    rows, cols = (m, k) if op == "T" else (k, m)
+    ld = (1 << 21) + 64 if op == "T" else (1 << 23) + 64  # a step's rows: 256 of K-contiguous ones, 64 lines else
+    buf = torch.empty(2 * rows * ld, device="cuda")
+    w = torch.as_strided(buf, (2, rows, cols), (rows * ld, ld, 1))
+    w.copy_(torch.randn(2, rows, cols, generator=g, device="cuda") * k ** -0.5)
+    x = torch.randn(n, k, generator=g, device="cuda")
+    y, z = torch.empty(n, m, device="cuda"), torch.empty(2, n, m, device="cuda")
+    o = cg.OP_T if op == "T" else cg.OP_N
+    assert handle.gemm_gated(o, cg.SILU, m, n, k, buf, w[1], ld, 0, x, k, y, m, z[0], z[1], m, None, 1, cg.TF32TCEC, cg.R_32F) == 0
+    wide = w.double() if op == "T" else w.double().transpose(1, 2)
+    a, b = (x.double() @ t.t().contiguous() for t in wide)
+    for got, want in ((z[0], a), (z[1], b), (y, a * torch.sigmoid(a) * b)):
+        assert relative(got, want) <= 2.0 ** -20
+    d = torch.empty(2, n, m, device="cuda")
+    assert handle.gemm_gated_backward(o, cg.SILU, m, n, k, buf, ld, 0, x, k, z[0], z[1], m, d[0], d[1], m, None, 0, None, 1, cg.TF32TCEC, cg.R_32F) == 0
+    s = torch.sigmoid(z[0].double())
+    assert relative(d[1], a * z[0].double() * s) <= 2.0 ** -20
+    del buf, w
+    ld8 = (1 << 23) + 64 if op == "T" else (1 << 24) + 64
+    q = torch.empty(rows * ld8, device="cuda", dtype=torch.uint8)
+    v = torch.as_strided(q, (rows, cols), (ld8, 1))
+    v.copy_(torch.randn(rows, cols, generator=g, device="cuda").to(torch.float8_e4m3fn).view(torch.uint8))
+    xq = x.to(torch.float8_e4m3fn)
+    ws, xs = torch.ones(1, device="cuda"), torch.ones(n, device="cuda")
+    assert handle.gemm_f8(o, m, n, k, q, ld8, 0, cg.R_8F_E4M3, ws, 0, xq, k, cg.R_8F_E4M3, xs, y, m, cg.R_32F) == 0
+    wide = v.contiguous().view(torch.float8_e4m3fn).float().double()
+    want = xq.float().double() @ (wide.t().contiguous() if op == "T" else wide)
+    assert relative(y, want) <= 2.0 ** -13
