@@ -14,19 +14,34 @@
 
 namespace cumpsgemm_amd {
 
-// EXACT: for FP32 results.  Otherwise the exponential and the reciprocal are the hardware's own, off by a few 2^-23 |x|, which
-// a rounding to 16 bits does not show.
+// EXACT: for FP32 results, off by a few 2^-24.  Otherwise the exponential and the reciprocal are the hardware's own, off by a
+// few 2^-23 |x|, which a rounding to 16 bits does not show.
+// e^x for x up to 88 (from there on: e^88), 0 below -150
+template <bool EXACT> __device__ inline float exponential(float x) {
+  if constexpr (!EXACT) return __expf(x);
+  constexpr float log2e = 1.44269504f, rest = 1.92596299e-8f, ln2 = 0.693147181f;
+  x = fminf(fmaxf(x, -150.0f), 88.0f);
+  // (x log2 e in two parts, the second of which the hardware's 2^t does not see)
+  const float t = x * log2e, more = fmaf(x, rest, fmaf(x, log2e, -t));
+  const float y = __builtin_amdgcn_exp2f(t);
+  return fmaf(y, more * ln2, y);
+}
+// 1 / x, x from 1 to e^88 + 1
+template <bool EXACT> __device__ inline float reciprocal(float x) {
+  const float r = __builtin_amdgcn_rcpf(x);
+  return EXACT ? fmaf(fmaf(-x, r, 1.0f), r, r) : r;
+}
 template <bool EXACT> __device__ inline float sigmoid(float x) {
-  if constexpr (EXACT) return 1.0f / (1.0f + expf(-x));
-  else return __builtin_amdgcn_rcpf(1.0f + __expf(-x));
+  const float s = reciprocal<EXACT>(1.0f + exponential<EXACT>(-x));
+  return EXACT && x < -88.0f ? 0.0f : s; // (6e-39 from there on otherwise, times an x of -1e38)
 }
 
 // P, and e^(-x^2 / 2)
 template <bool EXACT> __device__ inline float normal_below(float x, float &bell) {
   constexpr float c[10] = {0.101554129f, 0.101553861f, 0.0949720355f, 0.081958194f, 0.0614630061f,
-                             0.0532569567f, -0.0143161425f, 0.0717105734f, -0.0709835375f, 0.0188309427f};
-  const float u = 1.0f + 0.25455844f * fabsf(x), t = EXACT ? 1.0f / u : __builtin_amdgcn_rcpf(u);
-  bell = EXACT ? expf(-0.5f * x * x) : __expf(-0.5f * x * x);
+                           0.0532569567f, -0.0143161425f, 0.0717105734f, -0.0709835375f, 0.0188309427f};
+  const float t = reciprocal<EXACT>(1.0f + 0.25455844f * fminf(fabsf(x), 1e30f));
+  bell = exponential<EXACT>(-0.5f * x * x);
   float p = c[9];
 #pragma unroll
   for (int i = 8; i >= 0; i--) p = fmaf(p, t, c[i]);
@@ -47,7 +62,9 @@ template <uint32_t ACT, bool EXACT, bool DERIVATIVE> __device__ inline float act
     return x * p;
   } else if constexpr (ACT == CUMPSGEMM_GELU_TANH) {
     const float s = sigmoid<EXACT>(1.5957691216f * (x + 0.044715f * x * x * x)), y = x * s;
-    if (DERIVATIVE) slope = fmaf(y * (1.0f - s), 1.5957691216f * (1.0f + 0.134145f * x * x), s);
+    // (y (1 - s) is 0 long before 1000, and stays so where x^2 is infinite)
+    const float near = fminf(fmaxf(x, -1000.0f), 1000.0f);
+    if (DERIVATIVE) slope = fmaf(y * (1.0f - s), 1.5957691216f * (1.0f + 0.134145f * near * near), s);
     return y;
   } else {
     if (DERIVATIVE) slope = x > 0.0f ? 1.0f : 0.0f;

@@ -266,6 +266,20 @@ def test_extreme_projections(cg, handle, act):
     assert bool(torch.isnan(d1[0, 11]))
 
 
+@pytest.mark.parametrize("kind", ["TF32TCEC", "bf16"])
+@pytest.mark.parametrize("act", ACTS)
+def test_gradients_far_out(cg, handle, act, kind):
+    """From 200 on an activation is G or 0 and its slope 1 or 0, also where squares and cubes of G are infinite."""
+    dt = dtype_of(kind)
+    z = torch.tensor([200.0, -200.0, 1e4, -1e4, 1e18, -1e18, 1e20, -1e20, 1e38, -1e38], device="cuda").to(dt)[None].contiguous()
+    m = z.shape[1]
+    w, one, x = torch.ones(1, m, 1, device="cuda", dtype=dt), torch.ones_like(z), torch.ones(1, 1, device="cuda", dtype=dt)
+    d = torch.full((3, 1, m), 7.0, device="cuda", dtype=dt)
+    assert handle.gemm_gated_backward(cg.OP_T, getattr(cg, act), m, 1, 1, w, 1, m, x, 1, z, one, m, d[0], d[1], m, d[2], m, None, 1,
+                                      mode_of(cg, kind), type_code(cg, dt)) == 0
+    assert torch.equal(d[0], (z > 0).to(dt)) and torch.equal(d[1], z.clamp(min=0)) and torch.equal(d[2], d[1])
+
+
 def test_the_gradient_is_that_of_differences(cg, handle):
     """d_gate and d_up against central differences of the block's result, in FP32: a step of 2^-6 in G leaves a third derivative,
     at most 1.2 for SiLU, and two results that are off by 2^-21 each."""
