@@ -22,6 +22,12 @@
 // (2870 TOP/s) and 27 beside that, a tile's first loads, its write-out and the launch: at K = 4096 123, 2230 TOP/s.  FP16TCEC,
 // 4096 tokens of 8, 2048 x 1024: 78 with uneven experts in 128 x 128 tiles, 60 with even ones (256 x 128 tiles: 54, zeros 44);
 // 28 % MFMAs, and beside them as many clocks of LDS reads, which the schedule does not hide whole.
+// Gated blocks have a tile's BM rows from two matrices, sixteen rows of each in turn, so that a lane holds G and U of the same rows and
+// tokens and act(G) * U needs no second product.  BF16, 16384 tokens of 8 experts, 2048 x 2048: 280 with uneven experts and G and U
+// kept (981 TFLOP/s), as long as the plain product of both matrices, 287.  Their gradients: 204 - 216, the plain product 153, which
+// the 268 MB more that pass in the epilogue, 52 at a copy's rate, do not overlap with.  FP32: 4096 tokens to 14 of 16 experts, 1024 x
+// 1024, in FP16TCEC 91 (the plain product 82, with even experts 52), gradients in TF32TCEC 95 (68 - 80, 47): rounds of tiles that
+// uneven experts do not fill.
 #pragma once
 #include "activation.hpp"
 #include "gemm_kernel.hpp"
@@ -499,8 +505,7 @@ __device__ inline void store_four(char *c, const f4v_t x, float beta, uint32_t r
 }
 
 // Four rows of a column at any alignment: one access, unless the matrix ends among them.  (Value by value, at sizes that are not
-// multiples of four: 1001 tokens of 5 experts, 515 x 389 in FP16, the
-// gradient 38 us, so 12.6.)
+// multiples of four: 1001 tokens of 5 experts, 515 x 389 in FP16, the gradient 38 us, so 14.)
 template <uint32_t OUT> struct four_of {
   typedef typename out_type<OUT>::type O;
   typedef O type __attribute__((ext_vector_type(4)));
@@ -591,8 +596,8 @@ struct TileWork {
 };
 
 // What a tile's sums become.  sum(j, i, v): register v of lane l, MFMA row 4 (l / 16) + v (of C), column l % 16 (token) of
-// column block j and row block i; shift(): every column block takes the place of the one before it.  One column block after the other passes through LDS, each wave's through a part of its
-// own, so that a wave's store covers the columns' whole rows.
+// column block j and row block i; shift(): every column block takes the place of the one before it.  One column block after the
+// other passes through LDS, each wave's through a part of its own, so that a wave's store covers the columns' whole rows.
 template <class Cfg, int TN, class Sum, class Shift>
 __device__ inline void write_tile(const GroupedArgs &args, const TileWork &w, char *lds, Sum sum, Shift shift) {
   using T = typename Cfg::T;
