@@ -274,6 +274,17 @@ def test_quantize(cg, handle, dtype, f8, block_n):
             assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("k", [520, 515])
+@pytest.mark.parametrize("dtype", OUTS, ids=str)
+def test_quantize_many(cg, handle, dtype, k):
+    """So many tokens that a thread has several blocks, an odd number of them: as a thousand tokens at a time."""
+    x = (randn(1, 1, 9001, k) * 10.0 ** randn(2, 1, 9001, 1)).to(dtype)
+    got, s = quantised(cg, handle, x, "e4m3", 1)
+    for at in range(0, 9001, 1000):
+        part, t = quantised(cg, handle, x[:, at:at + 1000].contiguous(), "e4m3", 1)
+        assert torch.equal(got[:, at:at + 1000], part) and torch.equal(s[:, at:at + 1000], t)
+
+
 @pytest.mark.parametrize("block_n", [1, 128])
 @pytest.mark.parametrize("f8", F8)
 def test_quantize_extremes(cg, handle, f8, block_n):
