@@ -166,7 +166,7 @@ def test_larger_tiles(cg, handle, f8, op):
             run_gated(cg, handle, "SILU", m, k, sizes, f8, out)
 
 
-@pytest.mark.parametrize("cls", [0, 1, 2, 3])
+@pytest.mark.parametrize("cls", [0, 1, 2, 3, 4])
 @pytest.mark.parametrize("op", ["T", "N"])
 @pytest.mark.parametrize("f8", F8)
 def test_every_tile(cg, handle, f8, op, cls, monkeypatch):

@@ -189,7 +189,7 @@ def test_larger_tiles(cg, handle, kind, op):
         run_backward(cg, handle, kind, op, act, m, k, sizes)
 
 
-@pytest.mark.parametrize("cls", [0, 1, 2, 3])
+@pytest.mark.parametrize("cls", [0, 1, 2, 3, 4])
 @pytest.mark.parametrize("op", ["T", "N"])
 @pytest.mark.parametrize("kind", KINDS)
 def test_every_tile(cg, handle, kind, op, cls, monkeypatch):
