@@ -366,14 +366,28 @@ __device__ inline void multiply_f8_tile(const GroupedArgs &args, const TileWork 
     float rs = 0.0f;
     uint64_t apart = 0;
     if constexpr (Cfg::GATED && LA::LINES) apart = (uint64_t)(w.up - w.a);
+    uint64_t offa[LA::U], offb[UB];
+#pragma unroll
+    for (int u = 0; u < LA::U; u++) offa[u] = LA::offset(tid + u * NT, args.lda, w.rows_a, apart);
+#pragma unroll
+    for (int u = 0; u < UB; u++) offb[u] = LB::offset(tid + u * NT, args.ldb, w.rows_b);
+    const bool short_lines = !Cfg::A_KC && (args.m < (uint32_t)T::CHUNK || args.lda < (uint64_t)T::CHUNK);
     auto ask = [&](int s) {
       const int have = (int)w.klen - s * 128;
       const char *pa = a + (uint64_t)s * a_step, *pb = b + (uint64_t)s * b_step;
+      // (a step that is whole, and not the matrix's last lines, whose chunks must not be read beyond its end)
+      if (have >= (Cfg::A_KC ? 128 : 129) && !short_lines) {
 #pragma unroll
-      for (int u = 0; u < LA::U; u++)
-        LA::fetch_tail(ra, u, pa, args.lda, w.rows_a, have, Cfg::A_KC ? w.safe_a : w.safe_a - s * 128, tid, apart);
+        for (int u = 0; u < LA::U; u++) LA::template fetch<false, false>(ra, u, pa, args.lda, offa[u], w.rows_a, 0, tid);
 #pragma unroll
-      for (int u = 0; u < UB; u++) LB::fetch_tail(rb, u, pb, args.ldb, w.rows_b, have, w.safe_b, tid);
+        for (int u = 0; u < UB; u++) LB::template fetch<false, false>(rb, u, pb, args.ldb, offb[u], w.rows_b, 0, tid);
+      } else {
+#pragma unroll
+        for (int u = 0; u < LA::U; u++)
+          LA::fetch_tail(ra, u, pa, args.lda, w.rows_a, have, Cfg::A_KC ? w.safe_a : w.safe_a - s * 128, tid, apart);
+#pragma unroll
+        for (int u = 0; u < UB; u++) LB::fetch_tail(rb, u, pb, args.ldb, w.rows_b, have, w.safe_b, tid);
+      }
       rs = *reinterpret_cast<const float *>(scale + (uint64_t)s * scale_step);
     };
     auto put = [&](char *stage) {
