@@ -366,17 +366,22 @@ __device__ inline void multiply_f8_tile(const GroupedArgs &args, const TileWork 
     float rs = 0.0f;
     uint64_t apart = 0;
     if constexpr (Cfg::GATED && LA::LINES) apart = (uint64_t)(w.up - w.a);
+    // PLAIN: whole steps without the checks that the last one needs.  (128 x 128 tiles with exact sums have no registers for the
+    // offsets.  4225 tokens of 8 experts, 1024 x 1016: 21.0 us, so 16.4.)
+    constexpr bool PLAIN = !Cfg::EXACT || BN < 128;
     uint64_t offa[LA::U], offb[UB];
+    if constexpr (PLAIN) {
 #pragma unroll
-    for (int u = 0; u < LA::U; u++) offa[u] = LA::offset(tid + u * NT, args.lda, w.rows_a, apart);
+      for (int u = 0; u < LA::U; u++) offa[u] = LA::offset(tid + u * NT, args.lda, w.rows_a, apart);
 #pragma unroll
-    for (int u = 0; u < UB; u++) offb[u] = LB::offset(tid + u * NT, args.ldb, w.rows_b);
+      for (int u = 0; u < UB; u++) offb[u] = LB::offset(tid + u * NT, args.ldb, w.rows_b);
+    }
     const bool short_lines = !Cfg::A_KC && (args.m < (uint32_t)T::CHUNK || args.lda < (uint64_t)T::CHUNK);
     auto ask = [&](int s) {
       const int have = (int)w.klen - s * 128;
       const char *pa = a + (uint64_t)s * a_step, *pb = b + (uint64_t)s * b_step;
-      // (a step that is whole, and not the matrix's last lines, whose chunks must not be read beyond its end)
-      if (have >= (Cfg::A_KC ? 128 : 129) && !short_lines) {
+      // (not the matrix's last lines, whose chunks must not be read beyond its end)
+      if (PLAIN && have >= (Cfg::A_KC ? 128 : 129) && !short_lines) {
 #pragma unroll
         for (int u = 0; u < LA::U; u++) LA::template fetch<false, false>(ra, u, pa, args.lda, offa[u], w.rows_a, 0, tid);
 #pragma unroll

@@ -349,6 +349,7 @@ template <Elem E, bool KC, int ROWS, int ROW_BYTES, int NT, bool GATED = false> 
 
   struct Regs {
     typename std::conditional<T::F32, f8_t, u4_t>::type v[U];
+    uint32_t more[U]; // (fetch_words)
   };
 
   // memory -> registers, unit u of a whole step.  off: the unit's offset() from the uniform base, in 32 bits if FAST.
@@ -386,6 +387,18 @@ template <Elem E, bool KC, int ROWS, int ROW_BYTES, int NT, bool GATED = false> 
         fetch_tail(r, u, base, ld, rows, 1 << 30, safe, tid, apart);
       }
     }
+  }
+
+  // ... at any alignment, as the aligned words that hold it: what lies beside its values is dropped by put_words.  off: counted
+  // from a base that is a multiple of four.  (For the lines of a gated block's two matrices, where an access that begins inside a
+  // word costs most: 1001 tokens of 5 experts, 515 x 389 in FP16 16.9 us, so 11.9, 2055 x 2049 67, so 54; lines that are whole
+  // words, for which the kernel keeps the plain loads, 1 - 3 % longer for the choice.  Rows along K, and FP8: level or slower.)
+  __device__ static inline void fetch_words(Regs &r, int u, const char *base, uint64_t off, int tid) {
+    if (!active(tid)) return;
+    typedef uint32_t u4w_t __attribute__((ext_vector_type(4), aligned(4)));
+    const u4w_t x = *reinterpret_cast<const u4w_t *>(base + (off & ~(uint64_t)3));
+    r.v[u] = u4_t{x.x, x.y, x.z, x.w};
+    r.more[u] = *reinterpret_cast<const uint32_t *>(base + ((off + 15) & ~(uint64_t)3)); // (the word of its last byte)
   }
 
   // ... any step: `left` K-values (one at least) from its first to the end.  Zeros come in the place of K-values beyond
@@ -463,6 +476,15 @@ template <Elem E, bool KC, int ROWS, int ROW_BYTES, int NT, bool GATED = false> 
     } else {
       *reinterpret_cast<u4_t *>(lds_op + id * 16) = r.v[u];
     }
+  }
+  // ... of what fetch_words has read
+  __device__ static inline void put_words(const Regs &r, int u, uint64_t off, char *lds_op, int tid) {
+    if (!active(tid)) return;
+    const uint32_t by = ((uint32_t)off & 3) * 8;
+    const u4_t x = r.v[u];
+    *reinterpret_cast<u4_t *>(lds_op + (tid + u * NT) * 16) =
+        u4_t{__builtin_amdgcn_alignbit(x.y, x.x, by), __builtin_amdgcn_alignbit(x.z, x.y, by), __builtin_amdgcn_alignbit(x.w, x.z, by),
+             __builtin_amdgcn_alignbit(r.more[u], x.w, by)};
   }
 };
 
@@ -973,14 +995,31 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
     constexpr std::integral_constant<int, BLOCKS - AHEAD_A> last;
     typename LA::Regs ra[SETS];
     typename LB::Regs rb[SETS];
+    // WORDS: lines of two matrices in turn, pieces of 32 bytes; in words if one of them is not made of such
+    constexpr bool WORDS = !T::F32 && !Cfg::DIRECT && Cfg::GATED && LA::LINES;
+    const uint32_t low_a = (uint32_t)(uintptr_t)a & 3;
+    const bool words = WORDS && ((low_a | (uint32_t)apart | (uint32_t)args.lda * T::BYTES) & 3) != 0;
+    if constexpr (WORDS) {
+#pragma unroll
+      for (int u = 0; u < LA::U; u++) offa[u] += low_a;
+    }
     auto put = [&](int l, const int set, char *stage) {
       if (l < LA::U) LA::put(ra[set], l, stage, tid);
       else LB::put(rb[set], l - LA::U, stage + Cfg::A_STAGE, tid);
     };
+    auto put_whole = [&](int l, const int set, char *stage) { // (of a whole step)
+      if constexpr (WORDS) {
+        if (words && l < LA::U) return LA::put_words(ra[set], l, offa[l], stage, tid);
+      }
+      put(l, set, stage);
+    };
     auto fetch = [&](int l, const int set, const char *pa, const char *pb, int64_t k0) { // (k0: the step's first K-value)
       constexpr bool FAST = Cfg::DIRECT, CAREFUL = Cfg::CAREFUL;
+      if constexpr (WORDS) {
+        if (words && l < LA::U) return LA::fetch_words(ra[set], l, pa - low_a, offa[l], tid);
+      }
       if (l < LA::U)
-        LA::template fetch<FAST, CAREFUL>(ra[set], l, pa, args.lda, offa[l], w.rows_a, Cfg::A_KC ? w.safe_a : w.safe_a - k0, tid, apart);
+        LA::template fetch<FAST, CAREFUL>(ra[set], l, WORDS ? pa - low_a : pa, args.lda, offa[l], w.rows_a, Cfg::A_KC ? w.safe_a : w.safe_a - k0, tid, apart);
       else
         LB::template fetch<FAST, CAREFUL>(rb[set], l - LA::U, pb, args.ldb, offb[l - LA::U], w.rows_b, Cfg::B_KC ? w.safe_b : w.safe_b - k0, tid);
     };
@@ -1002,8 +1041,13 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
         ask(0, 0);
       }
       if (SETS > 1 && steps > 1) ask(1, SETS - 1);
+      if (partial) {
 #pragma unroll
-      for (int l = 0; l < LOADS; l++) put(l, 0, lds);
+        for (int l = 0; l < LOADS; l++) put(l, 0, lds);
+      } else {
+#pragma unroll
+        for (int l = 0; l < LOADS; l++) put_whole(l, 0, lds);
+      }
       if (steps > SETS) ask(SETS, 0);
       block_sync_lds();
       if (EARLY) begin(lds);
@@ -1017,7 +1061,7 @@ __device__ inline void multiply_tile(const GroupedArgs &args, const TileWork &w,
       char *stage = lds + ((s + 1) & 1) * Cfg::STAGE;
       auto beside = [&](int g) {
         share(g, EARLY ? last.value : BLOCKS, [&](int l) {
-          put(l, set, stage);
+          put_whole(l, set, stage);
           fetch(l, set, pa, pb, (int64_t)(far - partial) * BK);
         });
       };
