@@ -177,6 +177,19 @@ def test_every_tile(cg, handle, f8, op, cls, monkeypatch):
             run_gated(cg, handle, "SILU", m, k, sizes, f8, torch.bfloat16)
 
 
+@pytest.mark.parametrize("cls", [1, 2])
+@pytest.mark.parametrize("op", ["T", "N"])
+def test_any_alignment_over_many_steps(cg, handle, op, cls, monkeypatch):
+    """Steps that are whole and the last one, lines shorter and a little longer than a chunk."""
+    monkeypatch.setenv("CUMPSGEMM_FORCE_TILE_CLASS", str(cls))
+    for m, k, sizes in ((301, 1021, [130, 0, 257]), (7, 520, [40]), (16, 385, [5, 60]), (17, 384, [70]), (130, 640, [33, 1])):
+        run(cg, handle, op, m, k, sizes, "e4m3", torch.bfloat16, (1, 3, 5, 7), extra=2)
+        run(cg, handle, op, m, k, sizes, "e5m2", torch.float32)
+        if op == "T":
+            for out in OUTS:
+                run_gated(cg, handle, "SILU", m, k, sizes, "e4m3", out, (1, 3, 5, 7))
+
+
 @pytest.mark.parametrize("pads", [(16, 32, 8, 5), (1, 3, 5, 7), (16, 0, 4, 0)])
 @pytest.mark.parametrize("op", ["T", "N"])
 def test_strides(cg, handle, op, pads):

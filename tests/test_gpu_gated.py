@@ -200,6 +200,16 @@ def test_every_tile(cg, handle, kind, op, cls, monkeypatch):
         run_backward(cg, handle, kind, op, act, m, k, sizes)
 
 
+@pytest.mark.parametrize("cls", [1, 2])
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_lines_that_begin_inside_words(cg, handle, kind, cls, monkeypatch):
+    """Matrices stored along their rows, of odd and even lengths and distances, over many steps."""
+    monkeypatch.setenv("CUMPSGEMM_FORCE_TILE_CLASS", str(cls))
+    for m, k, sizes, pad in ((301, 1003, [130, 0, 257], 0), (300, 704, [40, 1], 1), (129, 577, [33], 2), (8, 321, [5, 60], 0), (15, 640, [70], 0)):
+        for layout in ("separate", "stacked", "reversed", "interleaved"):
+            run_forward(cg, handle, kind, "N", "SILU", m, k, sizes, layout=layout, pads=(pad, 0, 0, 0))
+
+
 @pytest.mark.parametrize("layout", ["separate", "stacked", "reversed", "interleaved"])
 @pytest.mark.parametrize("op", ["T", "N"])
 @pytest.mark.parametrize("kind", ["FP16TCEC", "f16", "bf16"])
