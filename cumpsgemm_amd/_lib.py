@@ -22,6 +22,8 @@ STATUS_SUCCESS, STATUS_INVALID_VALUE = 0, 3
 R_32F, R_16F, R_8I, R_16BF, R_8F_E4M3, R_8F_E5M2 = 0, 2, 3, 14, 28, 29
 # cuMpSGEMM_activation_t
 SILU, GELU, GELU_TANH, RELU = range(4)
+# cuMpSGEMM_f8_sums_t
+F8_SUMS_FP32, F8_SUMS_FAST = range(2)
 
 _u64 = ctypes.c_uint64
 _u32 = ctypes.c_uint
@@ -135,6 +137,7 @@ def _declare(L):
     f8_tail = [_ptr, _u64, _int, _ptr, _ptr, _u64, _int, _ptr, _u64]
     L.cuMpSGEMM_gemm_f8.argtypes = [_ptr, _int] + gemm_tail + [_ptr, _u64, _u64, _int, _ptr, _u64] + f8_tail
     L.cuMpSGEMM_gemm_gated_f8.argtypes = [_ptr, _int] + gemm_tail + [_ptr, _ptr, _u64, _u64, _int, _ptr, _ptr, _u64] + f8_tail
+    L.cuMpSGEMM_set_f8_sums.argtypes = [_ptr, _int]
     L.cuMpSGEMM_quantize_f8.argtypes = [_ptr, _u64, _u64, _ptr, _u64, _u64, _int, _u64, _ptr, _u64, _u64, _int, _ptr, _u64]
     L.cuMpSGEMM_get_workspace_size.argtypes = [_ptr]
     L.cuMpSGEMM_get_workspace_size.restype = ctypes.c_size_t
@@ -404,6 +407,10 @@ class Handle:
                                                      _dptr(c), ldc, _dptr(offsets), groups, int(mode), int(type))
 
     # ---- 8-bit floating point ----
+    def set_f8_sums(self, sums):
+        """F8_SUMS_FP32 (a new handle's) or F8_SUMS_FAST, for the products of 8-bit floating point from here on."""
+        return self._L.cuMpSGEMM_set_f8_sums(self._h, int(sums))
+
     def gemm_f8(self, op_a, m, n, k, a, lda, stridea, type_a, scale_a, stridescale, b, ldb, type_b, scale_b, c, ldc,
                 type_c=R_32F, offsets=None, groups=1):
         """FP8 with a scale for 128 x 128 of a and for 128 values of each token (column of b); grouped with offsets."""

@@ -12,21 +12,24 @@
 // Products of random values come out 2e-5 of their norm from exact, a hundredth of what a result in BF16 is rounded by, a
 // tenth of FP16's.  (v_mfma_f32_16x16x32_fp8_fp8, at half the rate, gives the same bits.)
 // EXACT kernels take BF16 MFMAs instead, to which FP8 converts without rounding: products are exact, sums FP32, at half the
-// rate and with a conversion of every fragment.  That is for the kernels that wait for memory anyway, and for gated blocks whose
-// result is wider than BF16: it is FP8 again in the layer behind, where a value that was near half way between two of E4M3's
-// comes out a whole step away, and 2e-5 more before makes 4e-4 to 1e-3 of that layer's result (FP16's own rounding: 2e-4).
+// rate and with a conversion of every fragment.  They serve every call, unless the handle was told FAST sums: then the FP8 MFMAs
+// are taken where they are faster, but for few tokens, which wait for memory anyway, and for gated blocks whose result is wider
+// than BF16.  Such a result is FP8 again in the layer behind, where a value that was near half way between two of E4M3's comes
+// out a whole step away, and 2e-5 more before makes 4e-4 to 1e-3 of that layer's result (FP16's own rounding: 2e-4; in BF16 the
+// block is 2.1e-3 from FP64 with FAST sums, 1.7e-3 with exact ones).
 //
 // LDS images: rows of 128 bytes as for 8-bit integers.  Operands whose rows, not K, are contiguous (A of op N): 128 lines of
 // BM bytes, read by ds_read_b64_tr_b8, which takes eight lines of sixteen rows and hands each lane one row's eight K-values.
 // The 16-byte pieces of a line are exchanged so that the eight lines that each of two quarters of a wave reads at a time cover
 // all banks.  Behind the operands come the step's scales: one for each token, and those of the rows.
 //
-// What it spends its time on (us).  8192 tokens, 4096 x 4096, 256 x 256 tiles: 130 - 136, up to 2110 TFLOP/s (this card's best FP8
+// What it spends its time on (us).  8192 tokens, 4096 x 4096, exact sums, 128 x 128 tiles: 245 - 262, 1050 - 1120 TFLOP/s, nearly
+// the BF16 rate of this card's library on random values (1205), of half the bytes; FAST, 256 x 256 tiles: 123 - 136, up to 2230 TFLOP/s (this card's best FP8
 // product of that size, with one scale for each matrix, takes 99 to 112).  An MFMA with its four multiply-adds takes 37 clocks, the
 // MFMA alone 32.  Of a wave's time MFMAs are 56 % and waits 33; no LDS read meets another's bank; on zeros, which leave the clock
 // higher, a fifth less.  128 x 256 and 256 x 128 tiles in three buffers were slower, two 128 x 128 workgroups on a CU too where 256 x
 // 256 tiles fill the chip.  64 tokens to 40 of 64 experts, a gated block of 2 x 1024 x 2048: reading the matrices, 36 (4.7 TB/s) in
-// tiles of 64 tokens, 39 by the kernel of few tokens.  One token of 4096 x 4096: 5.8, the launch and a memory's round trip for every
+// tiles of 64 tokens (exact or FAST), 39 by the kernel of few tokens.  One token of 4096 x 4096: 5.8, the launch and a memory's round trip for every
 // four of a wave's steps.  1531 tokens to 7 of 8 experts, 2048 x 1536, the matrices read along their rows: 17, a tile's twelve steps
 // with no other workgroup beside it.
 #pragma once
@@ -595,9 +598,13 @@ template <Elem E, Epilogue EPI> void launch_f8_stream(const GroupedArgs &args, u
 }
 
 // ---- tables ----
-// Tiles of 32 tokens wait for memory, and are exact.
+// Tiles of 32 tokens wait for memory, and are exact.  Exact sums have no 256 x 256 tile (its fragments in BF16 leave too few
+// registers, and with fewer results under way it was 2 - 9 % faster at best: 8192 tokens, 4096 x 4096 240 us for 262), and for lines
+// of any alignment no 128 x 128 one, which spills, but one of 64 tokens, which rows of any alignment have as well (1531 tokens, 2047 x
+// 1535 25.6 us for 32.5; 8192, 4095 x 4095 446 for 333).
 template <Elem E, Epilogue EPI, bool A_KC, bool EXACT> constexpr void f8_entries(GroupedTable &t) {
-  t.columns[A_KC][0][TILE_128] = f8_entry<E, A_KC, 128, 128, 64, 64, 2, false, EPI, EXACT>();
+  if constexpr (A_KC || !EXACT) t.columns[A_KC][0][TILE_128] = f8_entry<E, A_KC, 128, 128, 64, 64, 2, false, EPI, EXACT>();
+  if constexpr (EXACT) t.columns[A_KC][0][TILE_64] = f8_entry<E, A_KC, 128, 64, 64, 32, 2, false, EPI, true>();
   t.columns[A_KC][0][TILE_NARROW] = f8_entry<E, A_KC, 128, 32, 32, 32, 2, false, EPI, true>();
   if constexpr (!EXACT) t.columns[A_KC][1][TILE_256] = f8_entry<E, A_KC, 256, 256, 128, 64, 2, true, EPI, false>();
   t.columns[A_KC][1][TILE_128] = f8_entry<E, A_KC, 128, 128, 64, 64, 2, true, EPI, EXACT>();
@@ -605,10 +612,10 @@ template <Elem E, Epilogue EPI, bool A_KC, bool EXACT> constexpr void f8_entries
   t.columns[A_KC][1][TILE_64] = f8_entry<E, A_KC, 128, 64, 64, 32, 3, true, EPI, EXACT>();
   if constexpr (A_KC) t.stream[A_KC] = {&launch_f8_stream<E, EPI>, 16, kStreamTokens};
 }
-template <Elem E> constexpr GroupedTable f8_table() {
+template <Elem E, bool EXACT> constexpr GroupedTable f8_table() {
   GroupedTable t{};
-  f8_entries<E, Epilogue::STORE, false, false>(t);
-  f8_entries<E, Epilogue::STORE, true, false>(t);
+  f8_entries<E, Epilogue::STORE, false, EXACT>(t);
+  f8_entries<E, Epilogue::STORE, true, EXACT>(t);
   return t;
 }
 template <Elem E, bool EXACT> constexpr GroupedTable gated_f8_table() {
@@ -618,7 +625,8 @@ template <Elem E, bool EXACT> constexpr GroupedTable gated_f8_table() {
 }
 
 #define CUMPSGEMM_F8(kind, E)                                        \
-  GroupedTable g_f8_##kind = f8_table<E>();                          \
+  GroupedTable g_f8_##kind = f8_table<E, false>();                   \
+  GroupedTable g_f8_exact_##kind = f8_table<E, true>();              \
   GroupedTable g_gated_f8_##kind = gated_f8_table<E, false>();       \
   GroupedTable g_gated_f8_exact_##kind = gated_f8_table<E, true>();
 

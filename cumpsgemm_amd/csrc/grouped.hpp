@@ -57,9 +57,9 @@ struct GroupedKernel {
   int bm, bn;
 };
 
-// What becomes of the sums: C as they are, a gated block's result, or its gradient.  (GATED_EXACT: the kernels of GATED for 8-bit
-// floating point whose sums are exact, f8_kernel.hpp.)
-enum class Epilogue : int { STORE = 0, GATED = 1, GATED_BACKWARD = 2, GATED_EXACT = 3 };
+// What becomes of the sums: C as they are, a gated block's result, or its gradient.  (STORE_EXACT, GATED_EXACT: the kernels of STORE
+// and GATED for 8-bit floating point whose products are exact and summed in FP32, f8_kernel.hpp.)
+enum class Epilogue : int { STORE = 0, GATED = 1, GATED_BACKWARD = 2, GATED_EXACT = 3, STORE_EXACT = 4 };
 
 // Kernels of ragged columns: three tiles of the tiled kernel, from the largest, and the kernel of few tokens to a group
 // (grouped_stream.hpp).  Gated blocks and 8-bit floating point: a tile of 64 tokens as well, three stages deep.  Ragged K: the first

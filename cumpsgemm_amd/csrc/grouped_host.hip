@@ -11,18 +11,20 @@ extern GroupedTable g_grouped_f32_fp16tcec, g_grouped_f32_fp16tc, g_grouped_f32_
 extern GroupedTable g_gated_f32_fp16tcec, g_gated_f32_fp16tc, g_gated_f32_bf16x3, g_gated_f32_bf16x2, g_gated_f16, g_gated_bf16;
 extern GroupedTable g_gated_backward_f32_fp16tcec, g_gated_backward_f32_fp16tc, g_gated_backward_f32_bf16x3,
     g_gated_backward_f32_bf16x2, g_gated_backward_f16, g_gated_backward_bf16;
-extern GroupedTable g_f8_e4m3, g_f8_e5m2, g_gated_f8_e4m3, g_gated_f8_e5m2, g_gated_f8_exact_e4m3, g_gated_f8_exact_e5m2;
+extern GroupedTable g_f8_e4m3, g_f8_e5m2, g_f8_exact_e4m3, g_f8_exact_e5m2, g_gated_f8_e4m3, g_gated_f8_e5m2, g_gated_f8_exact_e4m3,
+    g_gated_f8_exact_e5m2;
 
 // direct: the operands can take the shorter way into LDS (grouped_kernel.hpp); the kernel of few tokens takes any
 const GroupedKernel *lookup_grouped(Elem e, bool a_kc, bool ragged_k, bool direct, int cls, Epilogue epi = Epilogue::STORE) {
-  static const GroupedTable *const tables[4][kNumElems] = {
+  static const GroupedTable *const tables[5][kNumElems] = {
       {&g_grouped_f32_fp16tcec, &g_grouped_f32_fp16tc, &g_grouped_f32_bf16x3, &g_grouped_f32_bf16x2, &g_grouped_f16,
        &g_grouped_bf16, &g_grouped_i8, &g_f8_e4m3, &g_f8_e5m2},
       {&g_gated_f32_fp16tcec, &g_gated_f32_fp16tc, &g_gated_f32_bf16x3, &g_gated_f32_bf16x2, &g_gated_f16, &g_gated_bf16,
        nullptr, &g_gated_f8_e4m3, &g_gated_f8_e5m2},
       {&g_gated_backward_f32_fp16tcec, &g_gated_backward_f32_fp16tc, &g_gated_backward_f32_bf16x3, &g_gated_backward_f32_bf16x2,
        &g_gated_backward_f16, &g_gated_backward_bf16},
-      {nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, &g_gated_f8_exact_e4m3, &g_gated_f8_exact_e5m2}};
+      {nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, &g_gated_f8_exact_e4m3, &g_gated_f8_exact_e5m2},
+      {nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, &g_f8_exact_e4m3, &g_f8_exact_e5m2}};
   if (tables[(int)epi][(int)e] == nullptr) return nullptr;
   const GroupedTable &t = *tables[(int)epi][(int)e];
   const GroupedKernel *k = ragged_k ? (cls > SHORT_LINES ? nullptr : &t.over_k[direct][cls])
@@ -133,12 +135,12 @@ const Cost &cost_of(Elem e, int cls) {
                                  {5.8f, 0.78f, 0.61f, 2, 32, 0.88f}, {4.1f, 0.89f, 0.98f, 2, 256, 0.43f}};
   return (e == Elem::I8 ? eight : e == Elem::F32_BF16X3 ? fp32x3 : (int)e <= 3 ? fp32 : sixteen)[cls];
 }
-// Gated blocks, their gradients and 8-bit floating point, in the same terms, with what their larger epilogues cost, and apart for
+// Gated blocks, their gradients and 8-bit floating point (exact sums, and the FAST ones), in the same terms, with what their larger epilogues cost, and apart for
 // operands that go straight to LDS and for others (_any): fitted to 200 calls of each kind (and 100 of any alignment; sizes as
 // above, m to 4096, k to 4096 in FP8 and 2048 else, 1 - 16384 tokens) with every kernel in turn.  On 100 other calls each the choice
-// loses 3.4 % (gated, 16 bits), 3.5 (gradient), 4.1 and 3.3 (gated FP32: FP16TCEC, TF32TCEC), 1.9 and 1.9 (gradients), 5.9 (FP8), 4.1
-// and 2.7 (gated FP8, exact sums), of any alignment 1.5, 3.0, 4.6 (FP8) and 2.2 (gated FP8) against the best kernel for each; by the
-// figures of the plain products 24 % for gated blocks of any alignment, 5 - 10 % for the others.
+// loses 3.4 % (gated, 16 bits), 3.5 (gradient), 4.1 and 3.3 (gated FP32: FP16TCEC, TF32TCEC), 1.9 and 1.9 (gradients), 1.3 (FP8) and 3.3
+// (gated FP8), of any alignment 1.5, 3.0, 1.4 (FP8) and 2.4 (gated FP8), with FAST sums 5.9, 4.1, 4.6 and 2.2, against the best kernel for
+// each; by the figures of the plain products 24 % for gated blocks of any alignment, 5 - 10 % for the others.
 const Cost &gated_cost_of(Elem e, int cls, Epilogue epi, bool direct) {
   static const Cost gated16[5] = {{2.4f, 1.45f, 2.05f, 1, 64, 0.38f, 5.5f}, {5.7f, 0.52f, 0.71f, 2, 64, 0.51f, 2.1f},
                                   {6.3f, 0.14f, 0.29f, 2, 64, 0.95f, 2.8f}, {5.7f, 1.18f, 0.82f, 2, 512, 0.82f, 0.4f},
@@ -167,16 +169,24 @@ const Cost &gated_cost_of(Elem e, int cls, Epilogue epi, bool direct) {
                              {5.0f, 0.46f, 0.46f, 2, 128, 0.62f, 2.9f}};
   static const Cost f8_any[5] = {{}, {3.0f, 1.92f, 1.31f, 2, 128, 0.50f, 3.3f}, {3.2f, 1.32f, 0.88f, 2, 128, 0.82f, 1.8f},
                                  {2.6f, 7.52f, 2.24f, 2, 1024, 0.78f, 0.1f}, {}};
+  static const Cost f8_exact[5] = {{}, {4.6f, 1.17f, 1.11f, 2, 128, 0.44f, 1.5f}, {4.6f, 0.46f, 0.45f, 2, 128, 0.76f, 2.4f},
+                                   {4.9f, 0.86f, 0.61f, 2, 1024, 0.56f, 2.1f}, {4.2f, 0.74f, 0.69f, 2, 128, 0.70f, 1.7f}};
+  static const Cost f8_exact_any[5] = {{}, {4.5f, 2.68f, 1.65f, 2, 128, 0.44f, 1.2f}, {3.3f, 0.99f, 0.65f, 2, 128, 0.86f, 2.5f},
+                                       {4.7f, 2.85f, 2.54f, 2, 1024, 0.66f, 0.1f}, {4.1f, 1.29f, 0.92f, 2, 128, 0.64f, 1.9f}};
   static const Cost gated_f8[5] = {{3.7f, 1.41f, 1.81f, 1, 128, 0.34f, 6.2f}, {6.6f, 0.54f, 0.72f, 2, 128, 0.43f, 2.0f},
                                    {5.9f, 0.32f, 0.39f, 2, 128, 0.80f, 2.9f}, {6.3f, 1.11f, 0.99f, 2, 1024, 0.75f, 0.9f},
                                    {6.3f, 0.32f, 0.42f, 2, 128, 0.69f, 2.7f}};
-  static const Cost gated_f8_exact[5] = {{}, {5.9f, 1.15f, 1.05f, 2, 128, 0.34f, 1.8f}, {5.9f, 0.37f, 0.41f, 2, 128, 0.72f, 2.6f},
-                                         {5.9f, 1.88f, 1.11f, 2, 1024, 0.67f, 0.6f}, {5.8f, 0.60f, 0.61f, 2, 128, 0.60f, 2.1f}};
+  static const Cost gated_f8_exact[5] = {{}, {6.8f, 0.95f, 1.03f, 2, 128, 0.32f, 1.4f}, {6.1f, 0.36f, 0.41f, 2, 128, 0.69f, 2.6f},
+                                         {6.9f, 1.14f, 1.10f, 2, 1024, 0.53f, 0.7f}, {6.2f, 0.57f, 0.62f, 2, 128, 0.57f, 1.8f}};
+  static const Cost gated_f8_exact_any[5] = {{}, {4.6f, 2.24f, 1.53f, 2, 128, 0.47f, 2.1f}, {5.2f, 0.99f, 0.75f, 2, 128, 0.76f, 1.9f},
+                                             {2.7f, 4.36f, 2.55f, 2, 1024, 0.95f, 0.6f}, {5.2f, 1.31f, 0.98f, 2, 128, 0.61f, 2.0f}};
   static const Cost gated_f8_any[5] = {{}, {5.1f, 1.95f, 1.37f, 2, 128, 0.50f, 1.9f}, {4.5f, 1.12f, 0.75f, 2, 128, 0.87f, 2.1f},
                                        {5.5f, 3.26f, 2.28f, 2, 1024, 0.69f, 0.9f}, {}};
   if (e == Elem::E4M3 || e == Elem::E5M2) {
     if (epi == Epilogue::STORE) return (direct ? f8 : f8_any)[cls];
-    return (!direct ? gated_f8_any : epi == Epilogue::GATED ? gated_f8 : gated_f8_exact)[cls];
+    if (epi == Epilogue::STORE_EXACT) return (direct ? f8_exact : f8_exact_any)[cls];
+    if (epi == Epilogue::GATED) return (direct ? gated_f8 : gated_f8_any)[cls];
+    return (direct ? gated_f8_exact : gated_f8_exact_any)[cls];
   }
   const bool forward = epi == Epilogue::GATED;
   if (e == Elem::F32_BF16X3) return (forward ? gated32x3 : backward32x3)[cls];
@@ -494,7 +504,7 @@ hipblasStatus_t cuMpSGEMM_gemm_f8(cuMpSGEMM_handle_t h, hipblasOperation_t op_A,
   const hipblasStatus_t st = f8_arguments(h, m, n, k, a_kc, a, lda, stridea, type_a, scale_a, stridescale, b, ldb, type_b, scale_b, c,
                                           ldc, type_c, offsets, group_count, e, nothing, args);
   if (st != HIPBLAS_STATUS_SUCCESS || nothing) return st;
-  return run_columns(h, e, a_kc, args, "gemm_f8");
+  return run_columns(h, e, a_kc, args, "gemm_f8", h->f8_sums == CUMPSGEMM_F8_SUMS_FAST ? Epilogue::STORE : Epilogue::STORE_EXACT);
 }
 
 hipblasStatus_t cuMpSGEMM_gemm_gated_f8(cuMpSGEMM_handle_t h, cuMpSGEMM_activation_t activation, uint64_t m, uint64_t n, uint64_t k,
@@ -513,8 +523,15 @@ hipblasStatus_t cuMpSGEMM_gemm_gated_f8(cuMpSGEMM_handle_t h, cuMpSGEMM_activati
   args.up = (const char *)up;
   args.scale_up = scale_up;
   args.act = (uint32_t)activation;
-  // (f8_kernel.hpp says why results wider than BF16 come from exact sums)
-  return run_columns(h, e, true, args, "gemm_gated_f8", args.out == OUT_BF16 ? Epilogue::GATED : Epilogue::GATED_EXACT);
+  // (f8_kernel.hpp says why results wider than BF16 come from exact sums in any case)
+  return run_columns(h, e, true, args, "gemm_gated_f8",
+                     h->f8_sums == CUMPSGEMM_F8_SUMS_FAST && args.out == OUT_BF16 ? Epilogue::GATED : Epilogue::GATED_EXACT);
+}
+
+hipblasStatus_t cuMpSGEMM_set_f8_sums(cuMpSGEMM_handle_t h, cuMpSGEMM_f8_sums_t sums) {
+  if (h == nullptr || (sums != CUMPSGEMM_F8_SUMS_FP32 && sums != CUMPSGEMM_F8_SUMS_FAST)) return HIPBLAS_STATUS_INVALID_VALUE;
+  h->f8_sums = sums;
+  return HIPBLAS_STATUS_SUCCESS;
 }
 
 hipblasStatus_t cuMpSGEMM_gemm_i8(cuMpSGEMM_handle_t h, uint64_t m, uint64_t n, uint64_t k, const int8_t *a, uint64_t lda,

@@ -129,6 +129,8 @@ struct cuMpSGEMM_handle {
   // here), so replays of the graph keep reading and writing memory they own.
   bool pack_ws_captured = false;
   std::vector<void *> retired_ws;
+  int f8_sums = 0; // cuMpSGEMM_f8_sums_t
+
   // Set for the duration of one call by the entry point that allocates
   // nothing: the planes go to this caller-independent buffer (a static device
   // array), the pre-split path is taken whatever the shape rules say, and no
