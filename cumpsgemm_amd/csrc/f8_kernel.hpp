@@ -585,7 +585,8 @@ __global__ __launch_bounds__(kStreamWaves * 64) void f8_stream_kernel(const Grou
   if constexpr (EPI == Epilogue::GATED) {
     with_activation(args.act, [&](auto act) {
       float slope;
-      y = activation<act.value, false, false>(x[0], slope) * x[SIDES - 1];
+      const float a = args.out == OUT_F32 ? activation<act.value, true, false>(x[0], slope) : activation<act.value, false, false>(x[0], slope);
+      y = a * x[SIDES - 1];
     });
   }
   const uint64_t at = (uint64_t)(n0 + j) * args.ldc + m0 + r;

@@ -709,7 +709,8 @@ __device__ inline void write_tile(const GroupedArgs &args, const TileWork &w, ch
           for (int k = 0; k < AT_ONCE; k++) {
             const uint32_t col = column_of(j, (r + k) * COLS);
             if (col >= w.n_end) continue;
-            if constexpr (Cfg::GATED) store_gated<out.value, T::F32>(args, x[k], y[k], row, col);
+            // (8-bit values can have results in FP32)
+            if constexpr (Cfg::GATED) store_gated<out.value, T::F32 || (T::F8 && out.value == OUT_F32)>(args, x[k], y[k], row, col);
             else put_four<out.value>(w.c + (uint64_t)col * args.ldc * sizeof(typename out_type<out.value>::type), x[k], row, args.m);
           }
         });
