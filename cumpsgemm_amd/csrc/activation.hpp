@@ -6,7 +6,8 @@
 //   RELU       x where x > 0                               1 where x > 0
 // P of a negative x is e^(-x^2 / 2) times a function that falls slowly, t times a polynomial in t = 1 / (1 + 0.36 |x| / sqrt 2),
 // fitted to 3.5e-8 of erfc's values over all |x|; P(x) = 1 - P(-x).  So it keeps its significant bits for negative x, and its
-// derivative has the same exponential.  At minus infinity SiLU and both GELUs are 0 times infinity, NaN, as their formulas say.
+// derivative has the same exponential.  At the infinities, where the formulas have 0 times infinity, all of them have their limits: a
+// projection that FP16 could only store as an infinity has a gradient like any other far out.  (NaN stays NaN.)
 #pragma once
 #include <cumpsgemm/cumpsgemm_ext.h>
 #include <hip/hip_runtime.h>
@@ -51,20 +52,23 @@ template <bool EXACT> __device__ inline float normal_below(float x, float &bell)
 
 // act(x), and its derivative as slope if DERIVATIVE
 template <uint32_t ACT, bool EXACT, bool DERIVATIVE> __device__ inline float activation(float x, float &slope) {
+  // (values that minus infinity and infinity are taken as, where the other factor is 0; unlike fmaxf and fminf these keep a NaN)
+  constexpr float least = -3.4028235e38f, far = 1000.0f;
+  if constexpr (ACT != CUMPSGEMM_RELU) x = __builtin_elementwise_maximum(x, least);
   if constexpr (ACT == CUMPSGEMM_SILU) {
     const float s = sigmoid<EXACT>(x), y = x * s;
-    if (DERIVATIVE) slope = fmaf(y, 1.0f - s, s);
+    if (DERIVATIVE) slope = fmaf(__builtin_elementwise_minimum(y, far), 1.0f - s, s);
     return y;
   } else if constexpr (ACT == CUMPSGEMM_GELU) {
     float bell;
     const float p = normal_below<EXACT>(x, bell);
-    if (DERIVATIVE) slope = fmaf(x * 0.39894228f, bell, p);
+    if (DERIVATIVE) slope = fmaf(__builtin_elementwise_minimum(x, far) * 0.39894228f, bell, p);
     return x * p;
   } else if constexpr (ACT == CUMPSGEMM_GELU_TANH) {
     const float s = sigmoid<EXACT>(1.5957691216f * (x + 0.044715f * x * x * x)), y = x * s;
-    // (y (1 - s) is 0 long before 1000, and stays so where x^2 is infinite)
-    const float near = fminf(fmaxf(x, -1000.0f), 1000.0f);
-    if (DERIVATIVE) slope = fmaf(y * (1.0f - s), 1.5957691216f * (1.0f + 0.134145f * near * near), s);
+    // (y (1 - s) is 0 long before `far`, and stays so where x^2 is infinite)
+    const float near = fminf(fmaxf(x, -far), far);
+    if (DERIVATIVE) slope = fmaf(__builtin_elementwise_minimum(y, far) * (1.0f - s), 1.5957691216f * (1.0f + 0.134145f * near * near), s);
     return y;
   } else {
     if (DERIVATIVE) slope = x > 0.0f ? 1.0f : 0.0f;
