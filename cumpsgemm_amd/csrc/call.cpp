@@ -432,7 +432,8 @@ PyObject *quantize_f8(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
 // the addresses of the functions, in the order of `Functions` (`GroupedFunctions`, `GatedFunctions`)
 PyObject *bind_to(void *to, PyObject *const *args, Py_ssize_t n, const Py_ssize_t want) {
   if (!count_is(n, want)) return nullptr;
-  void *p[kFunctions > kGroupedFunctions ? kFunctions : kGroupedFunctions];
+  void *p[kFunctions];
+  static_assert(kGroupedFunctions <= kFunctions && kGatedFunctions <= kFunctions, "room for each of the three");
   for (Py_ssize_t i = 0; i < want; i++) {
     p[i] = PyLong_AsVoidPtr(args[i]);
     if (p[i] == nullptr) {
