@@ -296,8 +296,6 @@ hipblasStatus_t f8_arguments(cuMpSGEMM_handle *h, uint64_t m, uint64_t n, uint64
   args.ldb = ldb;
   args.ldc = ldc;
   args.stride_a = stridea;
-  args.alpha = 1.0f;
-  args.vec_c = four_at_once(c, m, ldc, 0, args.out);
   args.scale_a = scale_a;
   args.scale_b = scale_b;
   args.stride_scale = stridescale;
@@ -328,7 +326,6 @@ hipblasStatus_t gated_arguments(cuMpSGEMM_handle *h, hipblasOperation_t op_A, cu
   args.lda = lda;
   args.ldb = ldb;
   args.stride_a = stridea;
-  args.alpha = 1.0f;
   args.act = (uint32_t)activation;
   return HIPBLAS_STATUS_SUCCESS;
 }
