@@ -2,12 +2,12 @@
 //
 //   C[i, j] = sum_b scale_a[i / 128, b] scale_b[b, j] sum_{l in block b of 128} A[l, i] B[l, j]
 //
-// The tiles, their loads and the write-out are those of grouped_kernel.hpp; a step is one block of K, 128 bytes of a row, and
-// one v_mfma_f32_16x16x128_f8f6f4 deep.  Such an MFMA starts from zero, and its four sums a lane are multiplied with the
-// block's scales and added in FP32 by vector instructions, beside the MFMAs that follow it.  (It cannot go on with the sums of
-// the block before: those have other scales.)
+// The tiles, their loads and the write-out are those of grouped_kernel.hpp; a step is one block of K, 128 bytes of a row: four
+// v_mfma_f32_16x16x32_bf16 deep, of fragments that are converted to BF16, or (FAST, below) one v_mfma_f32_16x16x128_f8f6f4.  Their
+// sums start from zero, and a lane's four are multiplied with the block's scales and added in FP32 by vector instructions, beside
+// the MFMAs that follow.  (They cannot go on with the sums of the block before: those have other scales.)
 //
-// What the matrix cores keep, measured with single products: products of eight K-values (two registers of a lane) are cut to
+// What the FP8 MFMAs keep, measured with single products: products of eight K-values (two registers of a lane) are cut to
 // multiples of 2^-13 of the largest one's power of two, then the sixteen such sums of a block are added in FP32, cut to 2^-23.
 // Products of random values come out 2e-5 of their norm from exact, a hundredth of what a result in BF16 is rounded by, a
 // tenth of FP16's.  (v_mfma_f32_16x16x32_fp8_fp8, at half the rate, gives the same bits.)
@@ -23,14 +23,15 @@
 // The 16-byte pieces of a line are exchanged so that the eight lines that each of two quarters of a wave reads at a time cover
 // all banks.  Behind the operands come the step's scales: one for each token, and those of the rows.
 //
-// What it spends its time on (us).  8192 tokens, 4096 x 4096, exact sums, 128 x 128 tiles: 245 - 262, 1050 - 1120 TFLOP/s, nearly
-// the BF16 rate of this card's library on random values (1205), of half the bytes; FAST, 256 x 256 tiles: 123 - 136, up to 2230 TFLOP/s (this card's best FP8
-// product of that size, with one scale for each matrix, takes 99 to 112).  An MFMA with its four multiply-adds takes 37 clocks, the
-// MFMA alone 32.  Of a wave's time MFMAs are 56 % and waits 33; no LDS read meets another's bank; on zeros, which leave the clock
-// higher, a fifth less.  128 x 256 and 256 x 128 tiles in three buffers were slower, two 128 x 128 workgroups on a CU too where 256 x
-// 256 tiles fill the chip.  64 tokens to 40 of 64 experts, a gated block of 2 x 1024 x 2048: reading the matrices, 36 (4.7 TB/s) in
-// tiles of 64 tokens (exact or FAST), 39 by the kernel of few tokens.  One token of 4096 x 4096: 5.8, the launch and a memory's round trip for every
-// four of a wave's steps.  1531 tokens to 7 of 8 experts, 2048 x 1536, the matrices read along their rows: 17, a tile's twelve steps
+// What it spends its time on (us).  8192 tokens, 4096 x 4096, exact sums, 128 x 128 tiles: 245 - 275, up to 1120 TFLOP/s (the
+// library's product of that size in BF16: 198): 192 vector instructions, two thirds of them conversions, beside the 64 MFMAs of a
+// wave's step, and the clock.  FAST, 256 x 256 tiles: 123 - 136, up to 2230 TFLOP/s (this card's best FP8 product of that size, with
+// one scale for each matrix, takes 99 to 112).  An FP8 MFMA with its four multiply-adds takes 37 clocks, the MFMA alone 32; of a wave's
+// time MFMAs are 56 % and waits 33; no LDS read meets another's bank; on zeros, which leave the clock higher, a fifth less.  128 x 256
+// and 256 x 128 tiles in three buffers were slower, two 128 x 128 workgroups on a CU too where 256 x 256 tiles fill the chip.  64
+// tokens to 40 of 64 experts, a gated block of 2 x 1024 x 2048: reading the matrices, 35 (4.8 TB/s) in tiles of 32 tokens (FAST: of
+// 64, 36), 39 by the kernel of few tokens.  One token of 4096 x 4096: 6, the launch and a memory's round trip for every four of a
+// wave's steps.  1531 tokens to 7 of 8 experts, 2048 x 1536, the matrices read along their rows: 22, FAST 17, a tile's twelve steps
 // with no other workgroup beside it.
 #pragma once
 #include "grouped_table.hpp"

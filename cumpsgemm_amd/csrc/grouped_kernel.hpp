@@ -23,11 +23,11 @@
 // 4096 tokens of 8, 2048 x 1024: 78 with uneven experts in 128 x 128 tiles, 60 with even ones (256 x 128 tiles: 54, zeros 44);
 // 28 % MFMAs, and beside them as many clocks of LDS reads, which the schedule does not hide whole.
 // Gated blocks have a tile's BM rows from two matrices, sixteen rows of each in turn, so that a lane holds G and U of the same rows and
-// tokens and act(G) * U needs no second product.  BF16, 16384 tokens of 8 experts, 2048 x 2048: 280 with uneven experts and G and U
-// kept (981 TFLOP/s), as long as the plain product of both matrices, 287.  Their gradients: 204 - 216, the plain product 153, which
+// tokens and act(G) * U needs no second product.  BF16, 16384 tokens of 8 experts, 2048 x 2048: 274 - 288 with uneven experts and G and
+// U kept (up to 1000 TFLOP/s), as long as the plain product of both matrices, 287.  Their gradients: 212 - 224, the plain product 153, which
 // the 268 MB more that pass in the epilogue, 52 at a copy's rate, do not overlap with.  FP32: 4096 tokens to 14 of 16 experts, 1024 x
-// 1024, in FP16TCEC 91 (the plain product 82, with even experts 52), gradients in TF32TCEC 95 (68 - 80, 47): rounds of tiles that
-// uneven experts do not fill.
+// 1024, in FP16TCEC 88 - 92 (the plain product 82, with even experts 52), gradients in TF32TCEC 95 - 97 (68 - 80, 47): rounds of
+// tiles that uneven experts do not fill, and short steps with one workgroup on a CU.
 #pragma once
 #include "activation.hpp"
 #include "gemm_kernel.hpp"

@@ -245,9 +245,11 @@ hipblasStatus_t cuMpSGEMM_gemm_gated(cuMpSGEMM_handle_t handle, hipblasOperation
 /* Its gradient, on top of the product that brings the gradient to it:
  *   D[:, j] = op(A_g) B[:, j]             (the layer behind: A its matrix, B the gradients of its results)
  *   d_gate = D * U * act'(G),  d_up = D * act(G),  C = act(G) * U
- * G = z_gate and U = z_up as cuMpSGEMM_gemm_gated left them.  D is kept in FP32
- * and not stored.  C, the block's result again, is what the gradient of A needs;
- * NULL: not wanted.  d_gate and d_up (m x n, ldd) may be z_gate and z_up
+ * G = z_gate and U = z_up as cuMpSGEMM_gemm_gated left them: in 16 bits rounded,
+ * beyond FP16's range infinite (with the value and slope that large numbers
+ * have).  D is kept in FP32 and not stored.  C, the block's result again, is what
+ * the gradient of A needs; it comes from the rounded G and U, and so is not bit by
+ * bit the one that gemm_gated made of its FP32 sums.  NULL: not wanted.  d_gate and d_up (m x n, ldd) may be z_gate and z_up
  * themselves, with ldd = ldz; apart from that nothing may overlap.  (At 0 the
  * derivative of RELU is 0.) */
 hipblasStatus_t cuMpSGEMM_gemm_gated_backward(cuMpSGEMM_handle_t handle, hipblasOperation_t op_A,
@@ -300,8 +302,8 @@ hipblasStatus_t cuMpSGEMM_gemm_gated_f8(cuMpSGEMM_handle_t handle, cuMpSGEMM_act
  *     product of random values, whatever type_c is.  Calls and tiles of few tokens
  *     keep FP32 sums, so that a token's result depends by that much on how many
  *     others its call has.  So do gated blocks with FP32 or FP16 results; with BF16
- *     results, quantised again, such a block and the product behind it are a fifth
- *     further from exact (2.1e-3 in place of 1.7e-3). */
+ *     results, quantised again, such a block and the product behind it are further
+ *     from exact (2.15e-3 of the norm in place of 1.67e-3). */
 typedef enum { CUMPSGEMM_F8_SUMS_FP32 = 0, CUMPSGEMM_F8_SUMS_FAST = 1 } cuMpSGEMM_f8_sums_t;
 hipblasStatus_t cuMpSGEMM_set_f8_sums(cuMpSGEMM_handle_t handle, cuMpSGEMM_f8_sums_t sums);
 /* batch_count matrices of n columns, k values each, of type_x = HIP_R_32F, _16F or
