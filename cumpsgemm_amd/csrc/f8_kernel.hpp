@@ -476,7 +476,7 @@ template <class Cfg> void launch_f8(const GroupedArgs &args, uint32_t workgroups
 template <Elem E, bool A_KC, int BM, int BN, int WM, int WN, int NSTAGE, bool DIRECT, Epilogue EPI, bool EXACT>
 constexpr GroupedKernel f8_entry() {
   using Cfg = F8Cfg<E, A_KC, BM, BN, WM, WN, NSTAGE, DIRECT, EPI, EXACT>;
-  return {&launch_f8<Cfg>, Cfg::ROWS_OUT, Cfg::BN};
+  return {&launch_f8<Cfg>, Cfg::ROWS_OUT, Cfg::BN, Cfg::NT};
 }
 
 // ---- few tokens: the matrices are read once, straight into MFMA fragments (grouped_stream.hpp) ----
@@ -612,7 +612,7 @@ template <Elem E, Epilogue EPI, bool A_KC, bool EXACT> constexpr void f8_entries
   t.columns[A_KC][1][TILE_128] = f8_entry<E, A_KC, 128, 128, 64, 64, 2, true, EPI, EXACT>();
   t.columns[A_KC][1][TILE_NARROW] = f8_entry<E, A_KC, 128, 32, 32, 32, 3, true, EPI, true>();
   t.columns[A_KC][1][TILE_64] = f8_entry<E, A_KC, 128, 64, 64, 32, 3, true, EPI, EXACT>();
-  if constexpr (A_KC) t.stream[A_KC] = {&launch_f8_stream<E, EPI>, 16, kStreamTokens};
+  if constexpr (A_KC) t.stream[A_KC] = {&launch_f8_stream<E, EPI>, 16, kStreamTokens, kStreamWaves * 64};
 }
 template <Elem E, bool EXACT> constexpr GroupedTable f8_table() {
   GroupedTable t{};

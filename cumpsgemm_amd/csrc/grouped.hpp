@@ -55,6 +55,7 @@ struct GroupedArgs {
 struct GroupedKernel {
   void (*launch)(const GroupedArgs &, uint32_t workgroups, hipStream_t);
   int bm, bn;
+  int threads; // of a workgroup
 };
 
 // What becomes of the sums: C as they are, a gated block's result, or its gradient.  (STORE_EXACT, GATED_EXACT: the kernels of STORE

@@ -231,6 +231,8 @@ uint64_t most_tiles(const GroupedArgs &args, const GroupedKernel &k) {
   return columns * ((args.m + k.bm - 1) / k.bm);
 }
 
+uint64_t most_workgroups(const GroupedKernel &k) { return 0xffffffffull / k.threads; } // (a launch has fewer than 2^32 threads)
+
 // Ragged columns: B and C have args.n columns in args.groups groups.
 hipblasStatus_t run_columns(cuMpSGEMM_handle *h, Elem e, bool a_kc, GroupedArgs &args, const char *label,
                             Epilogue epi = Epilogue::STORE) {
@@ -238,14 +240,14 @@ hipblasStatus_t run_columns(cuMpSGEMM_handle *h, Elem e, bool a_kc, GroupedArgs 
   const bool direct = chunks_ok(args.a, a_kc ? args.k : args.m, args.lda, args.stride_a, bytes, a_kc ? 256 : bytes == 1 ? 128 : 64) &&
                       chunks_ok(args.b, args.k, args.ldb, 0, bytes, 256) &&
                       ((epi != Epilogue::GATED && epi != Epilogue::GATED_EXACT) || chunks_ok(args.up, 16, args.lda, args.stride_a, bytes, 0));
-  int cls = TILE_128;
+  int cls = -1; // (none: more tiles than a launch has, of all of them)
   if (bytes == 2 && !direct && !a_kc && args.m < 8) {
     cls = STREAM; // (a line is shorter than the chunks that the tiled kernels read)
   } else if (!forced(e, a_kc, false, direct, cls, epi)) {
     double best = 0.0;
     for (int c = TILE_256; c < kGroupedClasses; c++) {
       const GroupedKernel *const kern = lookup_grouped(e, a_kc, false, direct, c, epi);
-      if (kern == nullptr || most_tiles(args, *kern) > kMostWorkgroups) continue;
+      if (kern == nullptr || most_tiles(args, *kern) > most_workgroups(*kern)) continue;
       // columns of tiles, the groups' sizes being unknown here: half of each group's last one, or one for each group
       const double some = std::min(args.n, args.groups), each = (double)args.n / args.groups;
       const double columns = args.groups == 1 ? (args.n + kern->bn - 1) / kern->bn
@@ -260,10 +262,11 @@ hipblasStatus_t run_columns(cuMpSGEMM_handle *h, Elem e, bool a_kc, GroupedArgs 
       if (best == 0.0 || us < best) best = us, cls = c;
     }
   }
+  if (cls < 0) return HIPBLAS_STATUS_INVALID_VALUE;
   const GroupedKernel *k = lookup_grouped(e, a_kc, false, direct, cls, epi);
   if (k == nullptr) return HIPBLAS_STATUS_INTERNAL_ERROR;
   const uint64_t workgroups = most_tiles(args, *k);
-  if (workgroups > kMostWorkgroups) return HIPBLAS_STATUS_INVALID_VALUE;
+  if (workgroups > most_workgroups(*k)) return HIPBLAS_STATUS_INVALID_VALUE;
   ProfileScope prof(h, label);
   k->launch(args, (uint32_t)workgroups, h->stream);
   return launched();

@@ -1184,6 +1184,6 @@ template <class Cfg> void launch_grouped(const GroupedArgs &args, uint32_t workg
   allow_dynamic_lds(reinterpret_cast<const void *>(&grouped_kernel<Cfg>), Cfg::LDS_BYTES, done);
   hipLaunchKernelGGL(grouped_kernel<Cfg>, dim3(workgroups), dim3(Cfg::NT), Cfg::LDS_BYTES, stream, args);
 }
-template <class Cfg> constexpr GroupedKernel grouped_entry() { return {&launch_grouped<Cfg>, Cfg::ROWS_OUT, Cfg::BN}; }
+template <class Cfg> constexpr GroupedKernel grouped_entry() { return {&launch_grouped<Cfg>, Cfg::ROWS_OUT, Cfg::BN, Cfg::NT}; }
 
 } // namespace cumpsgemm_amd

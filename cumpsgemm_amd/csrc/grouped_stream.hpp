@@ -366,7 +366,7 @@ template <Elem E, bool A_KC, Epilogue EPI> void launch_grouped_stream(const Grou
   hipLaunchKernelGGL((grouped_stream_kernel<E, A_KC, EPI>), dim3(workgroups), dim3(kStreamWaves * 64), 0, stream, args);
 }
 template <Elem E, bool A_KC, Epilogue EPI = Epilogue::STORE> constexpr GroupedKernel stream_entry() {
-  return {&launch_grouped_stream<E, A_KC, EPI>, StreamCfg<E, A_KC>::ROWS, kStreamTokens};
+  return {&launch_grouped_stream<E, A_KC, EPI>, StreamCfg<E, A_KC>::ROWS, kStreamTokens, kStreamWaves * 64};
 }
 
 } // namespace cumpsgemm_amd

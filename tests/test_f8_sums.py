@@ -50,3 +50,18 @@ def test_additions_are_among_the_mfmas(kernels):  # noqa: F811
                 longest = max(longest, row)
             assert longest <= 3, (name, longest)
     assert loops > 20
+
+
+@pytest.mark.parametrize("ld", [0, 1, 16])
+@pytest.mark.parametrize("op", [cg.OP_T, cg.OP_N])
+@pytest.mark.parametrize("sums", [0, 1])
+def test_more_tiles_than_a_launch_has_are_refused(sums, op, ld):
+    """As an invalid value, whichever tiles the operands and sums can take; nothing is launched."""
+    memory = ctypes.create_string_buffer(4096)
+    h = cg.Handle.__new__(cg.Handle)
+    h._L, h._h, h._addr, h.close = _lib.lib(), ctypes.c_void_p(ctypes.addressof(memory)), ctypes.addressof(memory), lambda: None
+    assert h.set_f8_sums(sums) == 0
+    most, p = (1 << 31) - 16, 0x1000
+    a = dict(m=most, n=most, k=160, stridea=0, type_a=cg.R_8F_E4M3, stridescale=0, b=p, ldb=160 + ld, type_b=cg.R_8F_E4M3, scale_b=p, c=p, ldc=most)
+    assert h.gemm_f8(op_a=op, a=p, lda=(160 if op == cg.OP_T else most) + ld, scale_a=p, **a) == cg.STATUS_INVALID_VALUE
+    assert h.gemm_gated_f8(activation=cg.SILU, gate=p, up=p, lda=160 + ld, scale_gate=p, scale_up=p, **a) == cg.STATUS_INVALID_VALUE
