@@ -6,7 +6,6 @@ FP64, rounded once to its type.  Sums that cut the eight products to multiples o
 import pytest
 import torch
 
-import test_gpu_f8
 from test_gpu_f8 import F8, OUTS, blocks, code, run, run_gated
 from test_gpu_grouped import offsets_of, spans, type_code
 
@@ -161,4 +160,39 @@ def test_the_choice_is_the_handles(cg, fast, monkeypatch):
     other.close()
     assert fast.set_f8_sums(cg.F8_SUMS_FP32) == 0
     assert torch.equal(product(cg, fast, *shape, torch.float32)[0], want.float())
-    assert test_gpu_f8.unit(512) > 2.0 ** -11  # (what the other tests allow is for FAST)
+
+
+def test_a_graph_keeps_the_sums_it_was_captured_with(cg, torch_gpu, monkeypatch):
+    """Two graphs of one handle, one with each; replayed in turn after the setting has changed, with eager calls between them."""
+    monkeypatch.setenv("CUMPSGEMM_FORCE_TILE_CLASS", "1")
+    m, k, n = 256, 512, 300
+    ((w, ws, wide),), (x, xs, tokens) = operands(5, m, n, k, 1, "T", "e4m3")
+    want = (tokens @ wide[0].t().contiguous()).float()
+    h, side = cg.Handle(), torch.cuda.Stream()
+    h.set_stream(side)
+
+    def call(c):
+        assert h.gemm_f8(cg.OP_T, m, n, k, w, k, 0, cg.R_8F_E4M3, ws, 0, x, k, cg.R_8F_E4M3, xs, c, m, cg.R_32F) == 0
+    graphs, eager = [], torch.empty(n, m, device="cuda")
+    torch.cuda.synchronize()
+    for sums in (cg.F8_SUMS_FAST, cg.F8_SUMS_FP32):
+        assert h.set_f8_sums(sums) == 0
+        with torch.cuda.stream(side):
+            call(eager)
+        torch.cuda.synchronize()
+        graph, c = torch.cuda.CUDAGraph(), torch.empty(n, m, device="cuda")
+        with torch.cuda.graph(graph, stream=side):
+            call(c)
+        graphs.append((graph, c, eager.clone()))
+    assert torch.equal(graphs[1][2], want) and not torch.equal(graphs[0][2], want)
+    for _ in range(3):
+        for graph, c, result in graphs:
+            c.fill_(7.0)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            with torch.cuda.stream(side):
+                call(eager)
+            torch.cuda.synchronize()
+            assert torch.equal(c, result) and torch.equal(eager, want)
+    h.close()
